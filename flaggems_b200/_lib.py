@@ -6,6 +6,7 @@ operator of the package fails loudly (there is no CPU or eager fallback).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import threading
@@ -14,9 +15,11 @@ from pathlib import Path
 import torch
 
 FG_F32, FG_F16, FG_BF16 = 0, 1, 2
+FG_E4M3, FG_E5M2 = 3, 4   # types of an 8-bit KV cache
 ABI_VERSION = 2
 
 _DTYPE_CODE = {torch.float32: FG_F32, torch.float16: FG_F16, torch.bfloat16: FG_BF16}
+FP8_CODE = {torch.float8_e4m3fn: FG_E4M3, torch.float8_e5m2: FG_E5M2}
 
 _LIB = None
 _LIB_LOCK = threading.Lock()
@@ -74,6 +77,17 @@ class AttnParams(C.Structure):
     )
 
 
+class AttnCacheParams(C.Structure):
+    _fields_ = (
+        [("base", AttnParams)]
+        + [(n, C.c_void_p) for n in ("k_scale", "v_scale")]
+        + [(n, C.c_int64) for n in (
+            "k_scale_batch_stride", "k_scale_head_stride", "v_scale_batch_stride", "v_scale_head_stride",
+            "sink_tokens", "block_table_cols")]
+        + [(n, C.c_int32) for n in ("cache_dtype", "reserved")]
+    )
+
+
 class GemmPlan(C.Structure):
     _fields_ = ([(n, C.c_int32) for n in ("tile_m", "tile_n", "grid", "group_m")]
                 + [(n, C.c_int64) for n in ("tiles_m", "tiles_n", "full_units", "num_units")])
@@ -119,6 +133,8 @@ SIGNATURES = {
     "fg_rotary_embedding": (C.c_int, [C.POINTER(RopeParams), _P]),
     "fg_reshape_and_cache_flash": (C.c_int, [_P, _P, _P, _P, _P] + [_I64] * 10 + [C.c_int, _P]),
     "fg_reshape_and_cache": (C.c_int, [_P, _P, _P, _P, _P] + [_I64] * 8 + [C.c_int, _P]),
+    "fg_reshape_and_cache_flash_fp8": (C.c_int, [_P] * 7 + [_I64] * 12 + [C.c_int, C.c_int, _P]),
+    "fg_gather_cache_flash": (C.c_int, [_P] * 9 + [_I64] * 15 + [C.c_int, C.c_int, _P]),
     "fg_gemm": (C.c_int, [C.POINTER(GemmParams), _P]),
     "fg_gemm_batched": (C.c_int, [C.POINTER(GemmParams)] + [_I64] * 5 + [_P]),
     "fg_gemm_uses_tcgen05": (C.c_int, [C.POINTER(GemmParams)]),
@@ -130,6 +146,9 @@ SIGNATURES = {
     "fg_flash_attn_path": (C.c_int, [C.POINTER(AttnParams)]),
     "fg_flash_attn_decode_static": (C.c_int, [C.POINTER(AttnParams), _P]),
     "fg_flash_attn_decode_static_capacity": (C.c_int64, []),
+    "fg_flash_attn_cache": (C.c_int, [C.POINTER(AttnCacheParams), _P]),
+    "fg_flash_attn_cache_workspace_bytes": (_I64, [C.POINTER(AttnCacheParams)]),
+    "fg_flash_attn_cache_path": (C.c_int, [C.POINTER(AttnCacheParams)]),
     "fg_scheduler_plan": (C.c_int, [C.POINTER(SchedulerParams), C.POINTER(SchedulerPlan)]),
     "fg_get_scheduler_metadata": (C.c_int, [C.POINTER(SchedulerParams), _P, _P]),
 }
@@ -195,6 +214,20 @@ def require_cuda(*tensors) -> torch.device:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is current; free when it already is."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def call(device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``device``, with that device current."""
+    with on_device(device):
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
 
 
 def ptr(t) -> int | None:

@@ -1,0 +1,182 @@
+// fg_flash_attn_cache: argument validation, choice of the kernel family and of the split over the keys.
+#include "attn_cache_common.cuh"
+
+namespace fg {
+
+int* device_status_ptr();
+
+namespace {
+
+enum { kPathGeneric = 0 };
+
+struct Plan {
+  int path;
+  int splits, tiles_per_split;
+};
+
+// Keys that one sequence can have visible to one row tile: everything, or window and first tokens.
+int64_t most_keys(const fg_attn_cache_params* p, int64_t tokens) {
+  const fg_attn_params& b = p->base;
+  if (b.window_left < 0 || b.window_left >= b.max_seqlen_k) return b.max_seqlen_k;
+  const int64_t right = b.causal ? 0 : (b.window_right < 0 ? b.max_seqlen_k : b.window_right);
+  const int64_t keys = b.window_left + 1 + right + tokens + p->sink_tokens + 3 * 128;   // ends of the tile runs
+  return keys < b.max_seqlen_k ? keys : b.max_seqlen_k;
+}
+
+// `ctas` row tiles without a split, `tiles` K/V tiles each at most: enough splits to fill `want` CTAs, of at least `least`
+// tiles each.
+void split_plan(int64_t ctas, int64_t tiles, int64_t want, int64_t least, Plan* plan) {
+  int64_t splits = ctas > 0 ? (want + ctas - 1) / ctas : 1;
+  if (splits > tiles / least) splits = tiles / least;
+  if (splits < 1) splits = 1;
+  if (splits > 4096) splits = 4096;
+  int64_t per = (tiles + splits - 1) / splits;
+  if (per < 1) per = 1;
+  plan->tiles_per_split = (int)per;
+  plan->splits = (int)((tiles + per - 1) / per);
+  if (plan->splits < 1) plan->splits = 1;
+}
+
+Plan make_plan(const fg_attn_cache_params* p, int sms) {
+  const fg_attn_params& b = p->base;
+  Plan plan;
+  const int64_t group = b.num_heads / b.num_heads_k;
+  plan.path = kPathGeneric;
+  const int64_t mb = (b.max_seqlen_q * group + 63) / 64;
+  const int64_t tiles = (most_keys(p, 64 / group + 1) + 63) / 64;
+  split_plan(mb * b.num_heads_k * b.batch, tiles, (int64_t)sms * 2, 4, &plan);
+  return plan;
+}
+
+int64_t plan_bytes(const fg_attn_params& b, const Plan& plan) {
+  return plan.splits > 1 ? (int64_t)plan.splits * b.total_q * b.num_heads * (b.head_dim + 1) * 4 : 0;
+}
+
+bool sizes_ok(const fg_attn_cache_params* p) {
+  const fg_attn_params& b = p->base;
+  return b.batch >= 0 && b.total_q >= 0 && b.num_heads > 0 && b.num_heads_k > 0 && b.num_heads % b.num_heads_k == 0 &&
+         b.head_dim > 0 && b.head_dim <= 256 && b.head_dim % 8 == 0 && b.max_seqlen_q >= 0 && b.max_seqlen_k >= 0 &&
+         b.max_seqlen_q <= 2147483647LL / 64 && b.max_seqlen_k <= 2147483647LL / 64 && p->sink_tokens >= 0;
+}
+
+}  // namespace
+}  // namespace fg
+
+extern "C" int fg_flash_attn_cache_path(const fg_attn_cache_params* p) {
+  using namespace fg;
+  return p && sizes_ok(p) ? make_plan(p, num_sms()).path : 0;
+}
+
+extern "C" int64_t fg_flash_attn_cache_workspace_bytes(const fg_attn_cache_params* p) {
+  using namespace fg;
+  if (p == nullptr || !sizes_ok(p)) return 0;
+  return plan_bytes(p->base, make_plan(p, num_sms()));
+}
+
+extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) {
+  using namespace fg;
+  FG_REQUIRE_HEALTHY("flash_attn_cache");
+  FG_REQUIRE(p != nullptr, "flash_attn_cache: null params");
+  const fg_attn_params& b = p->base;
+  FG_REQUIRE(b.dtype == FG_F16 || b.dtype == FG_BF16, "FlashAttention only support fp16 and bf16 data type");
+  FG_REQUIRE(p->cache_dtype == b.dtype || is_fp8(p->cache_dtype),
+             "flash_attn_cache: the cache must hold the type of the queries or an 8-bit type");
+  FG_REQUIRE(is_fp8(p->cache_dtype) || (p->k_scale == nullptr && p->v_scale == nullptr),
+             "flash_attn_cache: scales belong to an 8-bit cache");
+  FG_REQUIRE(b.batch >= 0 && b.total_q >= 0, "flash_attn_cache: negative size");
+  FG_REQUIRE(b.num_heads > 0 && b.num_heads_k > 0, "flash_attn_cache: head counts must be positive");
+  FG_REQUIRE(b.num_heads % b.num_heads_k == 0, "Number of heads in key/value must divide number of heads in query");
+  FG_REQUIRE(b.head_dim > 0 && b.head_dim <= 256, "FlashAttention forward only supports head dimension at most 256");
+  FG_REQUIRE(b.head_dim % 8 == 0, "head_size must be a multiple of 8");
+  FG_REQUIRE(p->sink_tokens >= 0, "flash_attn_cache: sink_tokens must not be negative");
+  FG_REQUIRE(b.max_seqlen_q >= 0 && b.max_seqlen_k >= 0, "flash_attn_cache: negative max_seqlen");
+  FG_REQUIRE(sizes_ok(p) && b.total_q <= 2147483647LL, "flash_attn_cache: sequence too long");
+  FG_REQUIRE(b.alibi_slopes == nullptr, "flash_attn_cache: ALiBi is not supported over an 8-bit cache or with sink_tokens");
+  FG_REQUIRE((b.q_batch_stride | b.k_batch_stride | b.v_batch_stride | b.o_batch_stride) == 0,
+             "flash_attn_cache: batch strides are not supported");
+  FG_REQUIRE(b.softcap >= 0.0, "flash_attn_cache: softcap must be >= 0");
+  if (b.batch == 0 || b.total_q == 0 || b.max_seqlen_q == 0) return FG_OK;
+  FG_REQUIRE(b.batch <= 65535 && b.num_heads_k <= 65535, "flash_attn_cache: batch or heads above 65535");
+  FG_REQUIRE(b.q && b.k && b.v && b.out, "flash_attn_cache: null tensor");
+  FG_REQUIRE(b.cu_seqlens_q != nullptr, "flash_attn_cache: cu_seqlens_q is required");
+  const bool paged = b.block_table != nullptr;
+  if (paged) {
+    FG_REQUIRE(b.seqused_k != nullptr, "seqused_k must be provided if block_table is provided");
+    FG_REQUIRE(b.block_size > 0 && b.num_blocks > 0, "flash_attn_cache: paged KV needs block_size and num_blocks");
+    FG_REQUIRE(b.block_size <= 2147483647LL && b.num_blocks <= 2147483647LL, "flash_attn_cache: cache too large");
+    FG_REQUIRE(p->block_table_cols > 0 && p->block_table_cols <= 2147483647LL, "flash_attn_cache: block_table has no columns");
+  } else {
+    FG_REQUIRE(b.cu_seqlens_k != nullptr, "cu_seqlens_k or seqused_k must be provided");
+    FG_REQUIRE(b.total_k >= 0, "flash_attn_cache: negative total_k");
+  }
+  FG_REQUIRE(aligned16(b.q) && aligned16(b.k) && aligned16(b.v) && aligned16(b.out),
+             "flash_attn_cache: tensors must be 16-byte aligned");
+  FG_REQUIRE(b.q_row_stride % 8 == 0 && b.q_head_stride % 8 == 0 && b.k_row_stride % 8 == 0 && b.k_head_stride % 8 == 0 &&
+                 b.v_row_stride % 8 == 0 && b.v_head_stride % 8 == 0 && b.o_row_stride % 8 == 0 &&
+                 b.o_head_stride % 8 == 0 && (!paged || (b.k_block_stride % 8 == 0 && b.v_block_stride % 8 == 0)),
+             "flash_attn_cache: strides must be multiples of 8 elements");
+
+  CacheAttnArgs c;
+  AttnArgs& a = c.a;
+  a.q = b.q; a.k = b.k; a.v = b.v; a.out = b.out; a.lse = b.lse;
+  a.cu_q = b.cu_seqlens_q; a.cu_k = b.cu_seqlens_k; a.seqused_k = b.seqused_k;
+  a.block_table = b.block_table; a.alibi = nullptr;
+  a.q_rs = b.q_row_stride; a.q_hs = b.q_head_stride;
+  a.k_rs = b.k_row_stride; a.k_hs = b.k_head_stride; a.k_bs = b.k_block_stride;
+  a.v_rs = b.v_row_stride; a.v_hs = b.v_head_stride; a.v_bs = b.v_block_stride;
+  a.o_rs = b.o_row_stride; a.o_hs = b.o_head_stride;
+  a.bt_stride = b.block_table_stride; a.alibi_bs = 0;
+  a.total_q = b.total_q; a.total_k = b.total_k;
+  a.q_batch = a.k_batch = a.v_batch = a.o_batch = 0;
+  a.batch_strided = 0;
+  a.batch = (int)b.batch; a.H = (int)b.num_heads; a.Hk = (int)b.num_heads_k;
+  a.group = a.H / a.Hk; a.D = (int)b.head_dim;
+  a.max_q = (int)b.max_seqlen_q; a.max_k = (int)b.max_seqlen_k;
+  a.block_size = (int)b.block_size; a.num_blocks = (int)b.num_blocks;
+  a.paged = paged;
+  a.has_alibi = 0;
+  a.causal = b.causal != 0;
+  int64_t wl = b.window_left, wr = b.window_right;
+  if (a.causal) wr = 0;
+  if (wl >= b.max_seqlen_k) wl = -1;
+  if (wr >= b.max_seqlen_k) wr = -1;
+  a.wl = (int)(wl < 0 ? -1 : wl);
+  a.wr = (int)(wr < 0 ? -1 : wr);
+  a.local = a.wl >= 0 || (!a.causal && a.wr >= 0);
+  a.has_softcap = b.softcap > 0.0;
+  const double LOG2E = 1.4426950408889634074;
+  a.scale = (float)(a.has_softcap ? b.softcap : b.softmax_scale);
+  a.softcap_pre = a.has_softcap ? (float)(b.softmax_scale / b.softcap) : 0.f;
+  a.scale_log2 = (float)((a.has_softcap ? b.softcap : b.softmax_scale) * LOG2E);
+  a.status = device_status_ptr();
+  c.k_scale = p->k_scale; c.v_scale = p->v_scale;
+  c.ks_batch = p->k_scale_batch_stride; c.ks_head = p->k_scale_head_stride;
+  c.vs_batch = p->v_scale_batch_stride; c.vs_head = p->v_scale_head_stride;
+  c.sinks = a.wl < 0 ? 0 : (int)(p->sink_tokens < b.max_seqlen_k ? p->sink_tokens : b.max_seqlen_k);
+  c.table_cols = (int)p->block_table_cols;
+
+  Plan plan = make_plan(p, num_sms());
+  a.ws_o = nullptr;
+  a.ws_lse = nullptr;
+  if (plan.splits > 1) {
+    const int64_t need = plan_bytes(b, plan);
+    if (b.workspace == nullptr) {
+      plan.splits = 1;
+    } else {
+      FG_REQUIRE(b.workspace_bytes >= need, "flash_attn_cache: workspace of %lld bytes, %lld needed",
+                 (long long)b.workspace_bytes, (long long)need);
+      FG_REQUIRE(aligned16(b.workspace), "flash_attn_cache: workspace must be 16-byte aligned");
+      a.ws_o = reinterpret_cast<float*>(b.workspace);
+      a.ws_lse = a.ws_o + (int64_t)plan.splits * b.total_q * b.num_heads * b.head_dim;
+    }
+  }
+  a.num_splits = plan.splits;
+  c.tiles_per_split = plan.tiles_per_split;
+  const int kind = p->cache_dtype == FG_E4M3 ? kCacheE4M3 : p->cache_dtype == FG_E5M2 ? kCacheE5M2 : kCache16;
+  cudaStream_t st = (cudaStream_t)stream;
+  FG_REQUIRE((b.max_seqlen_q * a.group + 63) / 64 * plan.splits <= 2147483647LL, "flash_attn_cache: too many row tiles");
+  FG_REQUIRE(b.total_q * b.num_heads <= 2147483647LL * 4, "flash_attn_cache: too many rows");
+  const int rc = attn_cache_generic(c, b.dtype, kind, st);
+  if (rc != FG_OK || a.num_splits == 1) return rc;
+  return attn_cache_combine(c, b.dtype, st);
+}

@@ -1,0 +1,105 @@
+// Shared definitions of the attention over an 8-bit or windowed cache (fg_flash_attn_cache).
+//
+//   S_ij = scale * k_scale * q_i . c_j,   O_i = v_scale * sum_j softmax(S)_ij cv_j
+//
+// over the keys j that query i sees: j < k_len, j <= p_i + wr (causal: wr = 0), and j >= p_i - wl or j < sinks, with
+// p_i = i + k_len - q_len.  The scales factor out of both products, so the kernels multiply what the cache holds.
+//
+// The 8-bit types are subsets of fp16 and the products run in fp16 with fp32 accumulators: exact for K and V, and for
+// fp16 queries.  A bf16 query row is multiplied by a power of two that brings its largest value to [2^14, 2^15): its
+// 8-bit significands stay exact down to 2^-31 of the row's largest, and the power is taken out of the scores in fp32.
+// Probabilities are rounded to fp16 (2^-12), four times finer than bf16 would be; their sum is taken before that.
+//
+// `group` query heads share a KV head.  The rows of a tile are (token, head of the group) pairs, head fastest, so that
+// every K/V byte is fetched once for all of them.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "attn_common.cuh"
+#include "fp8.cuh"
+
+namespace fg {
+
+struct CacheAttnArgs {
+  AttnArgs a;
+  const float *k_scale, *v_scale;          // null: 1
+  int64_t ks_batch, ks_head, vs_batch, vs_head;
+  int sinks;
+  int table_cols;                          // entries of a block table row
+  int tiles_per_split;                     // K/V tiles of one split
+};
+
+__device__ __forceinline__ float cache_scale(const float* s, int64_t batch_stride, int64_t head_stride, int b, int hk) {
+  return s ? s[b * batch_stride + hk * head_stride] : 1.f;
+}
+
+// Row of the paged store (elements) of token `tok`; page numbers are clamped into the table and the cache, so that a
+// wrong table entry or length cannot fault.
+__device__ __forceinline__ int cache_page(const CacheAttnArgs& c, const int32_t* bt_row, int pg) {
+  const int page = bt_row[min(pg, c.table_cols - 1)];
+  return max(0, min(page, c.a.num_blocks - 1));
+}
+__device__ __forceinline__ int64_t cache_row(const CacheAttnArgs& c, const int32_t* bt_row, int k_begin, int tok, int64_t rs,
+                                             int64_t bs) {
+  if (c.a.paged) {
+    const int pg = tok / c.a.block_size;
+    return (int64_t)cache_page(c, bt_row, pg) * bs + (int64_t)(tok - pg * c.a.block_size) * rs;
+  }
+  return (int64_t)(k_begin + tok) * rs;
+}
+
+// K/V tiles of BN keys that the queries at positions [p_first, p_last] see any key of: `sink` tiles from the start of
+// the sequence, then the tiles [win, win + n - sink).
+struct TileSpan {
+  int sink, win, n;
+  __device__ __forceinline__ int tile(int i) const { return i < sink ? i : win + i - sink; }
+};
+template <int BN>
+__device__ __forceinline__ TileSpan tile_span(const CacheAttnArgs& c, int k_len, int p_first, int p_last) {
+  const AttnArgs& a = c.a;
+  int hi = k_len;                               // keys [0, hi) at most
+  if (a.causal || a.wr >= 0) hi = min(hi, p_last + (a.causal ? 0 : a.wr) + 1);
+  TileSpan t;
+  if (hi <= 0) {
+    t.sink = t.win = t.n = 0;
+    return t;
+  }
+  const int lo = a.wl >= 0 ? max(0, min(hi, p_first - a.wl)) : 0;
+  t.win = lo / BN;
+  t.sink = min((min(c.sinks, hi) + BN - 1) / BN, t.win);
+  t.n = t.sink + (hi + BN - 1) / BN - t.win;
+  return t;
+}
+
+// What one row sees: columns [lo, hi) and [0, sinks).
+struct RowMask {
+  int lo, hi, sinks;
+  __device__ __forceinline__ bool dead(int col) const { return col >= hi || (col < lo && col >= sinks); }
+};
+__device__ __forceinline__ RowMask row_mask(const CacheAttnArgs& c, int k_len, int p) {
+  const AttnArgs& a = c.a;
+  RowMask m;
+  m.hi = k_len;
+  if (a.causal || a.wr >= 0) m.hi = min(m.hi, p + (a.causal ? 0 : a.wr) + 1);
+  m.lo = a.wl >= 0 ? max(0, p - a.wl) : 0;
+  m.sinks = c.sinks;
+  return m;
+}
+
+// Power of two (as a float) that takes a row whose largest magnitude is `top` to [2^14, 2^15), and its inverse.
+__device__ __forceinline__ void row_power(float top, float& up, float& down) {
+  const int e = (int)((__float_as_uint(top) >> 23) & 0xff);   // biased exponent; 0 for zero and subnormals
+  if (e == 0xff || top == 0.f) {                               // infinity or NaN: left alone, they stay what they are
+    up = down = 1.f;
+    return;
+  }
+  const int k = min(14 - (max(e, 1) - 127), 112);
+  up = __int_as_float((127 + k) << 23);
+  down = __int_as_float((127 - k) << 23);
+}
+
+// Kernel families of fg_flash_attn_cache.
+int attn_cache_generic(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
+int attn_cache_combine(const CacheAttnArgs& c, int dtype, cudaStream_t st);
+
+}  // namespace fg

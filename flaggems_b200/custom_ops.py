@@ -25,6 +25,11 @@ SCHEMAS = {
     "reshape_and_cache_flash":
         "reshape_and_cache_flash(Tensor key, Tensor value, Tensor(a!) key_cache, Tensor(b!) value_cache, "
         "Tensor slot_mapping, str kv_cache_dtype, Tensor? k_scale=None, Tensor? v_scale=None) -> ()",
+    # no counterpart in the reference's extension
+    "gather_cache_flash":
+        "gather_cache_flash(Tensor key_cache, Tensor value_cache, Tensor(a!) key, Tensor(b!) value, "
+        "Tensor block_table, Tensor cu_seqlens, str kv_cache_dtype, Tensor? k_scale=None, Tensor? v_scale=None, "
+        "Tensor? seq_starts=None) -> ()",
     "flash_attn_varlen_func":
         "flash_attn_varlen_func(Tensor q, Tensor k, Tensor v, SymInt max_seqlen_q, Tensor cu_seqlens_q, "
         "SymInt max_seqlen_k, Tensor? cu_seqlens_k=None, Tensor? seqused_k=None, Tensor? q_v=None, "
@@ -60,6 +65,12 @@ def _reshape_and_cache_flash(key, value, key_cache, value_cache, slot_mapping, k
                                   k_scale, v_scale)
 
 
+def _gather_cache_flash(key_cache, value_cache, key, value, block_table, cu_seqlens, kv_cache_dtype, k_scale=None,
+                        v_scale=None, seq_starts=None):
+    fused.gather_cache_flash(key_cache, value_cache, key, value, block_table, cu_seqlens, kv_cache_dtype, k_scale,
+                             v_scale, seq_starts)
+
+
 def _flash_attn_varlen_func(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seqlens_k=None,
                             seqused_k=None, q_v=None, dropout_p=0.0, softmax_scale=None, causal=False,
                             window_size=None, softcap=0.0, alibi_slopes=None, deterministic=False,
@@ -78,6 +89,7 @@ _IMPLS = {
     "rotary_embedding_inplace": _rotary_embedding_inplace,
     "rotary_embedding": _rotary_embedding,
     "reshape_and_cache_flash": _reshape_and_cache_flash,
+    "gather_cache_flash": _gather_cache_flash,
     "flash_attn_varlen_func": _flash_attn_varlen_func,
     "mm": ops.mm,
     "addmm": ops.addmm,

@@ -25,6 +25,7 @@ __all__ = [
     "silu_and_mul_out", "gelu_and_mul",
     "reshape_and_cache_flash",
     "reshape_and_cache",
+    "gather_cache_flash",
 ]
 
 
@@ -235,6 +236,129 @@ def silu_and_mul_out(A, B, out):
 
 
 # ---------------------------------------------------------------------------
+# the 8-bit paged cache (the reference accepts its arguments and has none)
+# ---------------------------------------------------------------------------
+_FP8_NAMES = {"fp8": torch.float8_e4m3fn, "fp8_e4m3": torch.float8_e4m3fn, "fp8_e5m2": torch.float8_e5m2}
+
+
+def _head_scale(what, scale, num_heads, dev):
+    """``(pointer, elements between heads)`` of a K or V scale: None, one element, or one for each head."""
+    if scale is None:
+        return None, 0
+    if scale.dtype != torch.float32:
+        raise RuntimeError(f"{what} must be float32, got {scale.dtype}")
+    if scale.device != dev:
+        raise RuntimeError(f"{what} is on {scale.device}, the cache on {dev}")
+    if scale.numel() == 1:
+        return scale.data_ptr(), 0
+    if scale.dim() != 1 or scale.shape[0] != num_heads:
+        raise RuntimeError(f"{what} must have one element or one for each of the {num_heads} heads, "
+                           f"got shape {tuple(scale.shape)}")
+    return scale.data_ptr(), scale.stride(0)
+
+
+def _check_cache_pair(op, key_cache, value_cache, kv_cache_dtype):
+    """Shapes and strides of a pair of 4-D caches; with an 8-bit ``kv_cache_dtype`` also their dtype."""
+    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape:
+        raise RuntimeError(f"{op}: the caches must be two [num_blocks, block_size, num_heads, head_size] tensors")
+    if key_cache.stride() != value_cache.stride():
+        raise RuntimeError(f"{op}: key_cache and value_cache must have equal strides")
+    if key_cache.stride(3) != 1:
+        raise RuntimeError(f"{op}: head_size must be the unit-stride dimension")
+    if key_cache.dtype != value_cache.dtype:
+        raise RuntimeError(f"{op}: the caches must share a dtype")
+    want = _FP8_NAMES.get(kv_cache_dtype)
+    if want is not None and key_cache.dtype not in (want, torch.uint8):
+        raise RuntimeError(f"{op}: kv_cache_dtype {kv_cache_dtype!r} needs caches of {want} or uint8, "
+                           f"got {key_cache.dtype}")
+    return want
+
+
+def _check_rows(op, key, value, num_heads, head_size):
+    if key.dim() != 3 or key.shape != value.shape or key.dtype != value.dtype:
+        raise RuntimeError(f"{op}: key and value must be two [num_tokens, num_heads, head_size] tensors of one dtype")
+    if key.shape[1] != num_heads or key.shape[2] != head_size:
+        raise RuntimeError(f"{op}: key and value of shape {tuple(key.shape)} do not fit caches of {num_heads} heads of "
+                           f"{head_size}")
+    for t in (key, value):
+        st = t.stride()
+        if st[2] != 1 and head_size > 1 or st[1] != head_size and num_heads > 1:
+            raise RuntimeError(f"{op}: key/value heads must be densely packed per token")
+
+
+def _write_fp8(key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale):
+    op = "reshape_and_cache_flash"
+    dev = _lib.require_cuda(key, value, key_cache, value_cache, slot_mapping)
+    want = _check_cache_pair(op, key_cache, value_cache, kv_cache_dtype)
+    num_blocks, block_size, num_heads, head_size = key_cache.shape
+    _check_rows(op, key, value, num_heads, head_size)
+    if slot_mapping.dim() != 1 or slot_mapping.shape[0] > key.shape[0]:
+        raise RuntimeError(f"{op}: slot_mapping must have one dimension and no more entries than key has tokens")
+    ks, ksh = _head_scale("k_scale", k_scale, num_heads, dev)
+    vs, vsh = _head_scale("v_scale", v_scale, num_heads, dev)
+    if slot_mapping.dtype != torch.int64:
+        slot_mapping = slot_mapping.to(torch.int64)
+    slot_mapping = slot_mapping.contiguous()
+    cst = key_cache.stride()
+    _lib.call(dev, _lib.load().fg_reshape_and_cache_flash_fp8,
+              key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(),
+              ks, vs, ksh, vsh, slot_mapping.shape[0], num_heads, head_size, block_size, num_blocks,
+              key.stride(0), value.stride(0), cst[0], cst[1], cst[2], _lib.dtype_code(key.dtype), _lib.FP8_CODE[want])
+    return None
+
+
+def gather_cache_flash(
+    key_cache,     # [num_blocks, block_size, num_heads, head_size]
+    value_cache,   # [num_blocks, block_size, num_heads, head_size]
+    key,           # [num_tokens, num_heads, head_size], written
+    value,         # [num_tokens, num_heads, head_size], written
+    block_table,   # int32 [batch, max_blocks]
+    cu_seqlens,    # int32 [batch + 1]
+    kv_cache_dtype="auto",
+    k_scale=None,
+    v_scale=None,
+    seq_starts=None,   # int32 [batch]
+):
+    """Read cached K/V rows back, packed: rows ``cu_seqlens[b] .. cu_seqlens[b + 1]`` of ``key`` and
+    ``value`` become the cached tokens ``seq_starts[b], seq_starts[b] + 1, ...`` of sequence ``b``
+    (from 0 without ``seq_starts``).  The counterpart of ``reshape_and_cache_flash``.
+
+    ``kv_cache_dtype`` ``"auto"``: a copy, the outputs have the caches' dtype.  ``"fp8"`` /
+    ``"fp8_e4m3"`` / ``"fp8_e5m2"``: caches of that type (or uint8), the outputs are float32,
+    float16 or bfloat16 and hold ``cache * scale`` rounded once; scales as for
+    ``reshape_and_cache_flash``.  Rows outside the sequences are left as they were.
+    Returns ``(key, value)``."""
+    op = "gather_cache_flash"
+    logger.debug("GEMS GATHER_CACHE_FLASH")
+    dev = _lib.require_cuda(key_cache, value_cache, key, value, block_table, cu_seqlens, seq_starts)
+    if kv_cache_dtype != "auto" and kv_cache_dtype not in _FP8_NAMES:
+        raise RuntimeError(f"{op}: unknown kv_cache_dtype {kv_cache_dtype!r}")
+    want = _check_cache_pair(op, key_cache, value_cache, kv_cache_dtype)
+    num_blocks, block_size, num_heads, head_size = key_cache.shape
+    _check_rows(op, key, value, num_heads, head_size)
+    if want is None and key.dtype != key_cache.dtype:
+        raise RuntimeError(f"{op}: key/value and the caches must share a dtype")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        raise RuntimeError(f"{op}: block_table must be int32 [batch, max_blocks] with unit column stride")
+    batch = block_table.shape[0]
+    for name, t, n in (("cu_seqlens", cu_seqlens, batch + 1), ("seq_starts", seq_starts, batch)):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous()):
+            raise RuntimeError(f"{op}: {name} must be int32 of shape ({n},) and contiguous")
+    if key.shape[0] > 1 and (key.stride(0) < num_heads * head_size or value.stride(0) < num_heads * head_size):
+        raise RuntimeError(f"{op}: key/value must not have internal overlap")
+    ks, ksh = _head_scale("k_scale", k_scale if want else None, num_heads, dev)
+    vs, vsh = _head_scale("v_scale", v_scale if want else None, num_heads, dev)
+    cst = key_cache.stride()
+    code = _lib.dtype_code(key.dtype)
+    _lib.call(dev, _lib.load().fg_gather_cache_flash,
+              key_cache.data_ptr(), value_cache.data_ptr(), key.data_ptr(), value.data_ptr(), block_table.data_ptr(),
+              cu_seqlens.data_ptr(), _lib.ptr(seq_starts), ks, vs, ksh, vsh, key.shape[0], batch, num_heads, head_size,
+              block_size, num_blocks, block_table.stride(0), block_table.shape[1], key.stride(0), value.stride(0),
+              cst[0], cst[1], cst[2], code, _lib.FP8_CODE[want] if want else code)
+    return key, value
+
+
+# ---------------------------------------------------------------------------
 # reshape_and_cache_flash  (src/flag_gems/fused/reshape_and_cache_flash.py:61-112)
 # ---------------------------------------------------------------------------
 def reshape_and_cache_flash(
@@ -249,9 +373,16 @@ def reshape_and_cache_flash(
 ):
     """Scatter new K/V tokens into the paged cache: ``cache[slot // bs, slot % bs] = key[tok]``.
 
-    ``kv_cache_dtype``, ``k_scale`` and ``v_scale`` are accepted and ignored, as in the
-    reference (no fp8 cache).  Negative slots are skipped.  Returns None."""
+    Caches of the dtype of key and value are copied into, whatever ``kv_cache_dtype``,
+    ``k_scale`` and ``v_scale`` say (the reference ignores them).  With ``kv_cache_dtype``
+    ``"fp8"`` / ``"fp8_e4m3"`` or ``"fp8_e5m2"`` and caches of that 8-bit type (or uint8) the
+    16- or 32-bit rows are quantised as they are written: ``cache = RN8(key / k_scale)``,
+    saturated at the type's largest value, NaN kept.  ``k_scale`` / ``v_scale`` are float32
+    tensors of one element or one for each head; None is 1.  Negative slots are skipped.
+    Returns None."""
     logger.debug("GEMS RESHAPE_AND_CACHE_FLASH")
+    if key_cache.element_size() == 1 and key.element_size() > 1 and kv_cache_dtype in _FP8_NAMES:
+        return _write_fp8(key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale)
     dev = _lib.require_cuda(key, value, key_cache, value_cache, slot_mapping)
     num_tokens = slot_mapping.size(0)
     num_heads, head_size = key.size(1), key.size(2)

@@ -308,6 +308,7 @@ def flash_attn_varlen_func(
     v_descale=None,
     num_splits: int = 0,
     fa_version: int = 2,
+    sink_tokens: int = 0,
 ):
     """FlashAttention-2 forward over variable-length sequences (vLLM-compatible signature).
 
@@ -317,6 +318,14 @@ def flash_attn_varlen_func(
     ``cu_seqlens_k`` (the reference accepts the paged form only, flash_api.py:272).
     The causal mask is aligned to the bottom-right corner; rows that see no key
     produce zeros.  Returns ``out`` or ``(out, softmax_lse)`` with lse ``(nheads, total_q)``.
+
+    k and v may be held in ``torch.float8_e4m3fn`` or ``torch.float8_e5m2`` (as
+    ``reshape_and_cache_flash`` writes them); a cached value then stands for itself times
+    ``k_descale`` / ``v_descale``: float32 tensors of one element, ``(nheads_k,)`` or
+    ``(batch, nheads_k)``, None is 1.  They are ignored for 16-bit K/V, as in the reference.
+    With a left window, the first ``sink_tokens`` keys of each sequence stay visible beside
+    it (the causal mask still holds).  Neither goes with ALiBi.  Rows of ``q`` outside the
+    sequences leave ``out`` as it was in these forms.
     """
     logger.debug("GEMS FLASH_ATTN_VARLEN_FUNC")
     assert cu_seqlens_k is not None or seqused_k is not None, "cu_seqlens_k or seqused_k must be provided"
@@ -342,6 +351,12 @@ def flash_attn_varlen_func(
         raise RuntimeError("flash_attn_varlen_func: q_v is not supported")
     if return_attn_probs:
         raise RuntimeError("flash_attn_varlen_func: return_attn_probs needs dropout, which is not supported")
+    if sink_tokens < 0:
+        raise RuntimeError("flash_attn_varlen_func: sink_tokens must not be negative")
+    if k.dtype in _lib.FP8_CODE or (sink_tokens > 0 and real_window_size[0] >= 0):
+        return _flash_attn_cache(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seqlens_k, seqused_k,
+                                 softmax_scale, causal, real_window_size, softcap, alibi_slopes, block_table,
+                                 return_softmax_lse, out, k_descale, v_descale, sink_tokens)
     dev = _lib.require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, seqused_k, block_table, alibi_slopes, out)
     q, k, v = [maybe_contiguous(x) for x in (q, k, v)]
     max_seqlen_q = max_seqlen_q.item() if hasattr(max_seqlen_q, "item") else max_seqlen_q
@@ -421,6 +436,104 @@ def flash_attn_varlen_func(
             ws = _workspace(dev, nbytes)
             p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
         _lib.check(lib.fg_flash_attn_varlen(C.byref(p), _lib.stream_ptr(dev)))
+    return (out, lse) if return_softmax_lse else out
+
+
+def _descale(what, scale, batch, heads, dev):
+    """``(pointer, batch stride, head stride)`` of a K or V scale."""
+    if scale is None:
+        return None, 0, 0
+    if scale.dtype != torch.float32:
+        raise RuntimeError(f"flash_attn_varlen_func: {what} must be float32, got {scale.dtype}")
+    if scale.device != dev:
+        raise RuntimeError(f"flash_attn_varlen_func: {what} is on {scale.device}, the cache on {dev}")
+    if scale.numel() == 1:
+        return scale.data_ptr(), 0, 0
+    if scale.shape == (heads,):
+        return scale.data_ptr(), 0, scale.stride(0)
+    if scale.shape == (batch, heads):
+        return scale.data_ptr(), scale.stride(0), scale.stride(1)
+    raise RuntimeError(f"flash_attn_varlen_func: {what} must have one element or the shape ({heads},) or "
+                       f"({batch}, {heads}), got {tuple(scale.shape)}")
+
+
+def _flash_attn_cache(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seqlens_k, seqused_k, softmax_scale, causal,
+                      window, softcap, alibi_slopes, block_table, return_softmax_lse, out, k_descale, v_descale,
+                      sink_tokens):
+    """The forms of ``flash_attn_varlen_func`` with 8-bit K/V or with first tokens that stay visible under a window."""
+    dev = _lib.require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, seqused_k, block_table, alibi_slopes, out)
+    if alibi_slopes is not None:
+        raise RuntimeError("flash_attn_varlen_func: ALiBi is not supported with 8-bit K/V or sink_tokens")
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    max_seqlen_q, max_seqlen_k = int(max_seqlen_q), int(max_seqlen_k)
+    fp8 = _lib.FP8_CODE.get(k.dtype)
+    assert q.dtype in (torch.float16, torch.bfloat16), "FlashAttention only support fp16 and bf16 data type"
+    assert k.dtype == v.dtype and (fp8 is not None or k.dtype == q.dtype)
+    assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous()
+    total_q, num_heads, head_size = q.shape
+    batch = cu_seqlens_q.numel() - 1
+    paged = block_table is not None
+    assert k.shape == v.shape and k.stride() == v.stride() and k.dim() == (4 if paged else 3)
+    kst = k.stride()
+    num_heads_k = k.shape[-2]
+    assert k.shape[-1] == head_size and kst[-1] == 1
+    assert head_size <= 256, "FlashAttention forward only supports head dimension at most 256"
+    assert head_size % 8 == 0, "head_size must be a multiple of 8, this is ensured by padding!"
+    assert num_heads % num_heads_k == 0, "Number of heads in key/value must divide number of heads in query"
+    if seqused_k is not None:
+        assert seqused_k.dtype == torch.int32 and seqused_k.is_contiguous() and seqused_k.shape == (batch,)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        assert out.stride(-1) == 1 and out.dtype == q.dtype and out.shape == q.shape
+    lse = torch.empty((num_heads, total_q), dtype=torch.float32, device=dev) if return_softmax_lse else None
+
+    p = _lib.AttnCacheParams()
+    b = p.base
+    b.q, b.k, b.v, b.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    if lse is not None:
+        b.lse = lse.data_ptr()
+    b.cu_seqlens_q = cu_seqlens_q.data_ptr()
+    if seqused_k is not None:
+        b.seqused_k = seqused_k.data_ptr()
+    b.q_row_stride, b.q_head_stride, _ = q.stride()
+    b.o_row_stride, b.o_head_stride, _ = out.stride()
+    if paged:
+        assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
+        assert block_table.shape[0] == batch
+        b.block_table, b.block_table_stride = block_table.data_ptr(), block_table.stride(0)
+        p.block_table_cols = block_table.shape[1]
+        b.num_blocks, b.block_size = k.shape[0], k.shape[1]
+        b.k_block_stride, b.k_row_stride, b.k_head_stride, _ = kst
+        b.v_block_stride, b.v_row_stride, b.v_head_stride, _ = kst
+    else:
+        assert cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.is_contiguous() and cu_seqlens_k.shape == (batch + 1,)
+        b.cu_seqlens_k, b.total_k = cu_seqlens_k.data_ptr(), k.shape[0]
+        b.k_row_stride, b.k_head_stride, _ = kst
+        b.v_row_stride, b.v_head_stride, _ = kst
+    b.total_q, b.batch, b.num_heads, b.num_heads_k, b.head_dim = total_q, batch, num_heads, num_heads_k, head_size
+    b.max_seqlen_q, b.max_seqlen_k = max_seqlen_q, max_seqlen_k
+    b.window_left, b.window_right = window
+    b.softmax_scale, b.softcap = softmax_scale, softcap
+    b.causal = 1 if causal else 0
+    b.dtype = _lib.dtype_code(q.dtype)
+    p.sink_tokens = sink_tokens
+    if fp8 is None:
+        p.cache_dtype = b.dtype
+    else:
+        p.cache_dtype = fp8
+        p.k_scale, p.k_scale_batch_stride, p.k_scale_head_stride = _descale("k_descale", k_descale, batch, num_heads_k, dev)
+        p.v_scale, p.v_scale_batch_stride, p.v_scale_head_stride = _descale("v_descale", v_descale, batch, num_heads_k, dev)
+    lib = _lib.load()
+    ref = C.byref(p)
+    with _lib.on_device(dev):
+        nbytes = lib.fg_flash_attn_cache_workspace_bytes(ref)
+        if nbytes > 0:
+            # a buffer of the call's own: the allocator keeps it from other streams, and a captured graph keeps its own
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            b.workspace, b.workspace_bytes = ws.data_ptr(), nbytes
+        _lib.check(lib.fg_flash_attn_cache(ref, _lib.stream_ptr(dev)))
     return (out, lse) if return_softmax_lse else out
 
 

@@ -131,7 +131,9 @@ def custom_gems_flash_attention_impl_forward(
     output_block_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """``FlashAttentionImpl.forward``: write the new K/V tokens into the paged cache, then
-    run varlen attention over the cache (patch_vllm_all.py:142-241)."""
+    run varlen attention over the cache (patch_vllm_all.py:142-241).  8-bit caches
+    (``kv_cache_dtype`` ``fp8``, ``fp8_e4m3``, ``fp8_e5m2``; the reference refuses them) are
+    quantised with ``layer._k_scale`` / ``_v_scale`` and read with the same scales."""
     assert output is not None, "Output tensor must be provided."
     if output_scale is not None or output_block_scale is not None:
         raise NotImplementedError("fused output quantization is not yet supported for FlashAttentionImpl")
@@ -139,11 +141,19 @@ def custom_gems_flash_attention_impl_forward(
         return output
     num_actual_tokens = attn_metadata.num_actual_tokens
     key_cache, value_cache = kv_cache.unbind(0)
+    fp8 = self.kv_cache_dtype.startswith("fp8")
+    if fp8 and (self.kv_cache_dtype not in fused._FP8_NAMES or kv_cache.element_size() != 1):
+        raise NotImplementedError(f"kv_cache_dtype {self.kv_cache_dtype} with a cache of {kv_cache.dtype} is not supported "
+                                  "for FlashAttentionImpl")
     fused.reshape_and_cache_flash(key, value, key_cache, value_cache, attn_metadata.slot_mapping,
                                   self.kv_cache_dtype, getattr(layer, "_k_scale", None),
                                   getattr(layer, "_v_scale", None))
-    if self.kv_cache_dtype.startswith("fp8"):
-        raise NotImplementedError("FP8 quantization is not yet supported for FlashAttentionImpl")
+    k_descale = v_descale = None
+    if fp8:
+        # vLLM allocates 8-bit caches as uint8; the scales of the write are those of the read
+        cache_dtype = fused._FP8_NAMES[self.kv_cache_dtype]
+        key_cache, value_cache = key_cache.view(cache_dtype), value_cache.view(cache_dtype)
+        k_descale, v_descale = getattr(layer, "_k_scale", None), getattr(layer, "_v_scale", None)
     local_md = getattr(attn_metadata, "local_attn_metadata", None)
     use_local_attn = getattr(self, "use_irope", False) and local_md is not None
     if getattr(attn_metadata, "use_cascade", False) and not use_local_attn:
@@ -176,6 +186,8 @@ def custom_gems_flash_attention_impl_forward(
         block_table=block_table,
         softcap=self.logits_soft_cap,
         fa_version=2,
+        k_descale=k_descale,
+        v_descale=v_descale,
     )
     return output
 

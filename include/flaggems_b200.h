@@ -30,6 +30,9 @@ extern "C" {
 /* dtype codes for floating-point tensors */
 enum { FG_F32 = 0, FG_F16 = 1, FG_BF16 = 2 };
 
+/* dtype codes of the 8-bit types a KV cache may be held in (fp8 e4m3 without infinities, e5m2) */
+enum { FG_E4M3 = 3, FG_E5M2 = 4 };
+
 /* error codes */
 enum {
   FG_OK = 0,
@@ -361,6 +364,73 @@ FG_API int fg_flash_attn_path(const fg_attn_params* p);
  * ---------------------------------------------------------------------- */
 FG_API int fg_flash_attn_decode_static(const fg_attn_params* p, void* stream);
 FG_API int64_t fg_flash_attn_decode_static_capacity(void);
+
+/* ------------------------------------------------------------------------
+ * The 8-bit paged KV cache.  The reference accepts kv_cache_dtype / k_scale / v_scale and k_descale / v_descale and
+ * ignores them (src/flag_gems/fused/reshape_and_cache_flash.py:61-112, src/flag_gems/ops/attention.py:1118-1287); here a
+ * cache of FG_E4M3 or FG_E5M2 elements is written, read back and attended over.  A cached value c stands for
+ * c * scale, with one fp32 scale for K and one for V, or one of each per KV head (device memory; NULL = 1; a
+ * head's scale is *_scale_stride elements behind the previous head's, 0 = one for all).
+ *
+ * fg_reshape_and_cache_flash_fp8: as fg_reshape_and_cache_flash, with key / value of `dtype` (FG_F32, FG_F16, FG_BF16) and
+ * the caches of `cache_dtype`: cache = RN8(RN32(x / scale)), to nearest even, saturated at the type's largest finite
+ * value (infinities too); NaN stays NaN.  Slots < 0 or beyond the cache are skipped.  When two tokens name one slot,
+ * which of them it holds is not defined.
+ *
+ * fg_gather_cache_flash: rows [cu_seqlens[b], cu_seqlens[b+1]) of key / value [num_rows, H, D] (dense heads, row
+ * strides given) become the cached tokens seq_starts[b], seq_starts[b] + 1, ... of sequence b (seq_starts NULL = 0):
+ * RN(fp32(c) * scale) in `dtype`, or a byte copy when cache_dtype == dtype.  Rows outside [cu_seqlens[0],
+ * cu_seqlens[batch]) are left as they were.  Page numbers are clamped into the cache, positions into the
+ * block_table_cols pages of a table row.
+ * ---------------------------------------------------------------------- */
+FG_API int fg_reshape_and_cache_flash_fp8(const void* key, const void* value, void* key_cache, void* value_cache,
+                                          const int64_t* slot_mapping, const float* k_scale, const float* v_scale,
+                                          int64_t k_scale_stride, int64_t v_scale_stride, int64_t num_tokens,
+                                          int64_t num_heads, int64_t head_size, int64_t block_size,
+                                          int64_t num_blocks, int64_t key_stride, int64_t value_stride,
+                                          int64_t cache_block_stride, int64_t cache_row_stride,
+                                          int64_t cache_head_stride, int dtype, int cache_dtype, void* stream);
+FG_API int fg_gather_cache_flash(const void* key_cache, const void* value_cache, void* key, void* value,
+                                 const int32_t* block_table, const int32_t* cu_seqlens, const int32_t* seq_starts,
+                                 const float* k_scale, const float* v_scale, int64_t k_scale_stride,
+                                 int64_t v_scale_stride, int64_t num_rows, int64_t batch, int64_t num_heads,
+                                 int64_t head_size, int64_t block_size, int64_t num_blocks,
+                                 int64_t block_table_stride, int64_t block_table_cols, int64_t key_stride,
+                                 int64_t value_stride, int64_t cache_block_stride, int64_t cache_row_stride,
+                                 int64_t cache_head_stride, int dtype, int cache_dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * flash_attn_cache: flash_attn_varlen over an 8-bit cache, or with a sliding window whose sequences keep their first
+ * `sink_tokens` keys visible.  No counterpart in the reference.
+ *
+ * `base` as for fg_flash_attn_varlen, without ALiBi and batch strides; q and out are of base.dtype, K/V of cache_dtype
+ * (base.dtype, FG_E4M3 or FG_E5M2; strides in elements of the cache, multiples of 8).  Key j is visible to the query
+ * at position p of its sequence (p = i + k_len - q_len) iff j < k_len, j <= p + window_right (causal: j <= p), and
+ * j >= p - window_left or j < sink_tokens.  Rows with no visible key produce 0 and an LSE of +inf; rows of q outside
+ * [cu_seqlens_q[0], cu_seqlens_q[batch]) leave out and lse as they were.  K/V that no query of a 64-key tile's
+ * readers sees take no part, whatever they hold (freed pages under a window); a NaN or infinity in a V row that
+ * some query of a tile sees can reach the others of that tile.
+ * k_scale / v_scale: what a cached value is multiplied by, batch and head strides in elements (0 = shared), NULL = 1;
+ * they must be NULL for a 16-bit cache.
+ * workspace: at least fg_flash_attn_cache_workspace_bytes(p) bytes of 16-byte aligned device memory that no other call in
+ * flight uses, or NULL to forbid splitting the keys over CTAs.  Two captured graphs that may run at the same time
+ * need workspaces of their own.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  fg_attn_params base;
+  const float* k_scale; /* may be NULL */
+  const float* v_scale; /* may be NULL */
+  int64_t k_scale_batch_stride, k_scale_head_stride;
+  int64_t v_scale_batch_stride, v_scale_head_stride;
+  int64_t sink_tokens;
+  int64_t block_table_cols; /* entries of a block table row (paged form) */
+  int32_t cache_dtype;
+  int32_t reserved;
+} fg_attn_cache_params;
+FG_API int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream);
+FG_API int64_t fg_flash_attn_cache_workspace_bytes(const fg_attn_cache_params* p);
+/* Which kernel family fg_flash_attn_cache picks: 0 general (mma.sync).  Pure host logic. */
+FG_API int fg_flash_attn_cache_path(const fg_attn_cache_params* p);
 
 /* ------------------------------------------------------------------------
  * get_scheduler_metadata: split-KV scheduling vector of a FlashAttention-3 style

@@ -1,0 +1,160 @@
+"""Host side of the 8-bit and windowed cache: structure layout, refusals before any CUDA call, path and workspace rules,
+and a restatement of the tile runs that the attention kernels walk."""
+import ctypes
+
+import pytest
+import torch
+
+from flaggems_b200 import _lib, fused
+
+
+def params(**kw):
+    p = _lib.AttnCacheParams()
+    b = p.base
+    b.q = b.k = b.v = b.out = b.cu_seqlens_q = b.seqused_k = b.block_table = 0x10000
+    b.q_row_stride, b.q_head_stride, b.o_row_stride, b.o_head_stride = 1024, 128, 1024, 128
+    b.k_block_stride = b.v_block_stride = 16 * 256
+    b.k_row_stride = b.v_row_stride = 256
+    b.k_head_stride = b.v_head_stride = 128
+    b.total_q, b.batch, b.num_heads, b.num_heads_k, b.head_dim = 4, 4, 8, 2, 128
+    b.max_seqlen_q, b.max_seqlen_k, b.block_size, b.num_blocks = 1, 1000, 16, 100
+    b.window_left = b.window_right = -1
+    b.softmax_scale, b.causal, b.dtype = 0.1, 1, _lib.FG_BF16
+    p.block_table_cols, p.cache_dtype = 63, _lib.FG_E4M3
+    for name, v in kw.items():
+        setattr(p if hasattr(p, name) else b, name, v)
+    return p
+
+
+def test_struct_size():
+    assert ctypes.sizeof(_lib.AttnCacheParams) == ctypes.sizeof(_lib.AttnParams) + 2 * 8 + 6 * 8 + 2 * 4
+
+
+@pytest.mark.parametrize("match, kw", [
+    ("fp16 and bf16", dict(dtype=_lib.FG_F32)), ("8-bit type", dict(cache_dtype=_lib.FG_F16)), ("8-bit type", dict(cache_dtype=9)),
+    ("scales belong", dict(cache_dtype=_lib.FG_BF16, k_scale=0x10000)), ("negative size", dict(batch=-1)),
+    ("must divide", dict(num_heads=7)), ("at most 256", dict(head_dim=264)), ("multiple of 8", dict(head_dim=124)),
+    ("sink_tokens", dict(sink_tokens=-1)), ("ALiBi", dict(alibi_slopes=0x10000)), ("batch strides", dict(q_batch_stride=8)),
+    ("softcap", dict(softcap=-1.0)), ("65535", dict(batch=70000, total_q=70000)), ("null tensor", dict(k=None)),
+    ("cu_seqlens_q", dict(cu_seqlens_q=None)), ("seqused_k", dict(seqused_k=None)), ("block_size", dict(block_size=0)),
+    ("no columns", dict(block_table_cols=0)), ("16-byte", dict(q=0x10008)), ("multiples of 8", dict(k_row_stride=252)),
+    ("too long", dict(max_seqlen_k=2 ** 31)), ("cu_seqlens_k", dict(block_table=None)), ("positive", dict(num_heads_k=0))])
+def test_attention_refuses_on_the_host(match, kw):
+    lib = _lib.load()
+    rc = lib.fg_flash_attn_cache(ctypes.byref(params(**kw)), None)
+    assert rc < 0
+    with pytest.raises(RuntimeError, match=match):
+        _lib.check(rc)
+
+
+def test_nothing_to_do_is_no_call():
+    lib = _lib.load()
+    for kw in (dict(batch=0), dict(total_q=0), dict(max_seqlen_q=0)):
+        assert lib.fg_flash_attn_cache(ctypes.byref(params(**kw)), None) == 0
+
+
+def test_small_workspace_is_refused():
+    lib = _lib.load()
+    p = params(max_seqlen_k=60000, batch=1, total_q=1)
+    need = lib.fg_flash_attn_cache_workspace_bytes(ctypes.byref(p))
+    assert need > 0 and need % (8 * 129 * 4) == 0
+    p.base.workspace, p.base.workspace_bytes = 0x10000, need - 4
+    with pytest.raises(RuntimeError, match="workspace of"):
+        _lib.check(lib.fg_flash_attn_cache(ctypes.byref(p), None))
+    p.base.workspace, p.base.workspace_bytes = 0x10004, need
+    with pytest.raises(RuntimeError, match="aligned"):
+        _lib.check(lib.fg_flash_attn_cache(ctypes.byref(p), None))
+
+
+def test_workspace_goes_by_what_is_visible():
+    """A window bounds the keys that are split, however long the context."""
+    need = lambda **kw: _lib.load().fg_flash_attn_cache_workspace_bytes(ctypes.byref(params(**kw)))
+    long, windowed = need(max_seqlen_k=10 ** 6), need(max_seqlen_k=10 ** 6, window_left=1023, sink_tokens=4)
+    assert 0 < windowed < long and windowed == need(max_seqlen_k=10 ** 5, window_left=1023, sink_tokens=4)
+
+
+@pytest.mark.parametrize("match, kw", [("no 8-bit", dict(cache_dtype=_lib.FG_F16)), ("negative", dict(num_tokens=-1)),
+                                       ("block_size", dict(block_size=0)), ("null pointer", dict(key=None)),
+                                       ("unknown dtype", dict(dtype=7))])
+def test_write_refuses_on_the_host(match, kw):
+    a = dict(key=0x10000, value=0x10000, kc=0x10000, vc=0x10000, slots=0x10000, ks=None, vs=None, ksh=0, vsh=0, num_tokens=2,
+             heads=2, dim=64, block_size=16, blocks=4, kst=128, vst=128, cb=2048, cr=128, ch=64, dtype=_lib.FG_BF16,
+             cache_dtype=_lib.FG_E4M3)
+    a.update(kw)
+    with pytest.raises(RuntimeError, match=match):
+        _lib.check(_lib.load().fg_reshape_and_cache_flash_fp8(*a.values(), None))
+
+
+@pytest.mark.parametrize("match, kw", [("hold the type", dict(cache_dtype=_lib.FG_F16)), ("negative", dict(rows=-1)),
+                                       ("empty cache", dict(blocks=0)), ("no columns", dict(cols=0)), ("null pointer", dict(cu=None)),
+                                       ("unknown dtype", dict(dtype=7, cache_dtype=_lib.FG_E5M2))])
+def test_gather_refuses_on_the_host(match, kw):
+    a = dict(kc=0x10000, vc=0x10000, key=0x10000, value=0x10000, table=0x10000, cu=0x10000, starts=None, ks=None, vs=None, ksh=0,
+             vsh=0, rows=2, batch=1, heads=2, dim=64, block_size=16, blocks=4, tst=4, cols=4, kst=128, vst=128, cb=2048, cr=128,
+             ch=64, dtype=_lib.FG_BF16, cache_dtype=_lib.FG_E4M3)
+    a.update(kw)
+    with pytest.raises(RuntimeError, match=match):
+        _lib.check(_lib.load().fg_gather_cache_flash(*a.values(), None))
+
+
+def test_cpu_tensors_are_refused():
+    kc = torch.zeros((2, 8, 1, 16), dtype=torch.float8_e4m3fn)
+    x = torch.zeros((2, 1, 16), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        fused.reshape_and_cache_flash(x, x, kc, kc, torch.arange(2), "fp8", None, None)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        fused.gather_cache_flash(kc, kc, x, x, torch.zeros((1, 1), dtype=torch.int32), torch.zeros(2, dtype=torch.int32), "fp8")
+
+
+def span(k_len, p_first, p_last, wl, wr, sinks, bn):
+    """The tile runs of attn_cache_common.cuh, restated: tile numbers in the order they are walked."""
+    hi = min(k_len, p_last + wr + 1) if wr >= 0 else k_len
+    if hi <= 0:
+        return []
+    lo = max(0, min(hi, p_first - wl)) if wl >= 0 else 0
+    win = lo // bn
+    sink = min(-(-min(sinks, hi) // bn), win)
+    n = sink + -(-hi // bn) - win
+    return [i if i < sink else win + i - sink for i in range(n)]
+
+
+@pytest.mark.parametrize("bn", [4, 8])
+def test_tile_runs_cover_what_is_visible_once(bn):
+    for k_len in (0, 1, 3, 8, 9, 23, 40):
+        for q_len in (1, 2, 7, 12):
+            for wl in (-1, 0, 2, 9, 30):
+                for wr in (-1, 0, 3):
+                    for sinks in (0, 1, 5, 17, 50):
+                        first, last = k_len - q_len, k_len - 1
+                        tiles = span(k_len, first, last, wl, wr, sinks if wl >= 0 else 0, bn)
+                        assert len(set(tiles)) == len(tiles) and all(0 <= t < -(-k_len // bn) for t in tiles)
+                        seen = {j // bn for p in range(first, last + 1) for j in range(k_len)
+                                if (wr < 0 or j <= p + wr) and (wl < 0 or j >= p - wl or j < sinks)}
+                        assert seen <= set(tiles)
+                        if wl >= 0:
+                            assert all(t * bn < sinks or t >= max(0, first - wl) // bn for t in tiles)
+
+
+def gathered_row(row, cu, starts, table, page, num_blocks):
+    """(block, row of the block) that packed row `row` is read from, as the gather kernel finds it; None: not in a sequence."""
+    batch, cols = len(table), len(table[0])
+    if row < cu[0] or row >= cu[batch]:
+        return None
+    lo, hi = 0, batch
+    while hi - lo > 1:
+        mid = (lo + hi) // 2
+        lo, hi = (mid, hi) if cu[mid] <= row else (lo, mid)
+    pos = max(0, row - cu[lo] + (starts[lo] if starts else 0))
+    pg = pos // page
+    return min(max(table[lo][min(pg, cols - 1)], 0), num_blocks - 1), pos - pg * page
+
+
+def test_gather_stays_inside_the_cache():
+    """Page numbers outside the cache, positions behind the table and before the sequence, decreasing starts."""
+    for cu in ([0, 200, 300], [3, 3, 300], [0, 250, 100], [5, 0, 300]):
+        for starts in (None, [-7, 10 ** 9]):
+            for row in range(310):
+                got = gathered_row(row, cu, starts, [[0, 10 ** 6, 2], [-5, 1, 3]], 16, 4)
+                assert got is None or (0 <= got[0] < 4 and 0 <= got[1] < 16)
+    assert gathered_row(21, [0, 5, 40], [0, 3], [[9, 9], [2, 1]], 16, 4) == (1, 3)
+    assert gathered_row(4, [0, 5, 5, 40], None, [[1], [2], [3]], 16, 4) == (1, 4)
