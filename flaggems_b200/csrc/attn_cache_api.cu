@@ -1,4 +1,6 @@
 // fg_flash_attn_cache: argument validation, choice of the kernel family and of the split over the keys.
+#include <initializer_list>
+
 #include "attn_cache_common.cuh"
 
 namespace fg {
@@ -7,7 +9,7 @@ int* device_status_ptr();
 
 namespace {
 
-enum { kPathGeneric = 0 };
+enum { kPathGeneric = 0, kPathDecode = 2 };
 
 struct Plan {
   int path;
@@ -37,10 +39,35 @@ void split_plan(int64_t ctas, int64_t tiles, int64_t want, int64_t least, Plan* 
   if (plan->splits < 1) plan->splits = 1;
 }
 
+// Whether TMA can fetch the cache: strides in multiples of 16 bytes, and pages that tile a K/V tile.
+bool tma_ready(const fg_attn_cache_params* p) {
+  const fg_attn_params& b = p->base;
+  const int64_t es = is_fp8(p->cache_dtype) ? 1 : 2;
+  for (int64_t st : {b.k_row_stride, b.k_head_stride, b.v_row_stride, b.v_head_stride})
+    if (st <= 0 || (st * es) % 16 != 0 || st * es >= (1ll << 40)) return false;
+  if (b.block_table == nullptr) return true;
+  for (int64_t st : {b.k_block_stride, b.v_block_stride})
+    if (st <= 0 || (st * es) % 16 != 0 || st * es >= (1ll << 40)) return false;
+  return b.block_size >= 8 && (b.block_size & (b.block_size - 1)) == 0;
+}
+
 Plan make_plan(const fg_attn_cache_params* p, int sms) {
   const fg_attn_params& b = p->base;
   Plan plan;
   const int64_t group = b.num_heads / b.num_heads_k;
+  if (b.max_seqlen_q * group <= 16 && tma_ready(p)) {
+    // Enough CTAs to balance contexts of very different length over all SMs (two resident each), but no range shorter
+    // than 256 keys.
+    plan.path = kPathDecode;
+    const int64_t bn = is_fp8(p->cache_dtype) ? 128 : 64;
+    const int64_t keys = most_keys(p, b.max_seqlen_q), ctas = b.num_heads_k * b.batch;
+    int64_t chunk = 1024;
+    while (chunk > 256 && ctas * ((keys + chunk - 1) / chunk) < (int64_t)sms * 2 * 8) chunk >>= 1;
+    plan.tiles_per_split = (int)(chunk / bn);
+    plan.splits = (int)((keys + chunk - 1) / chunk);
+    if (plan.splits < 1) plan.splits = 1;
+    return plan;
+  }
   plan.path = kPathGeneric;
   const int64_t mb = (b.max_seqlen_q * group + 63) / 64;
   const int64_t tiles = (most_keys(p, 64 / group + 1) + 63) / 64;
@@ -176,7 +203,7 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   cudaStream_t st = (cudaStream_t)stream;
   FG_REQUIRE((b.max_seqlen_q * a.group + 63) / 64 * plan.splits <= 2147483647LL, "flash_attn_cache: too many row tiles");
   FG_REQUIRE(b.total_q * b.num_heads <= 2147483647LL * 4, "flash_attn_cache: too many rows");
-  const int rc = attn_cache_generic(c, b.dtype, kind, st);
+  const int rc = plan.path == kPathDecode ? attn_cache_decode(c, b.dtype, kind, st) : attn_cache_generic(c, b.dtype, kind, st);
   if (rc != FG_OK || a.num_splits == 1) return rc;
   return attn_cache_combine(c, b.dtype, st);
 }

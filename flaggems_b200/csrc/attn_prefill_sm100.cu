@@ -151,9 +151,6 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-__device__ __forceinline__ void fence_proxy_async_smem() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
 
 template <bool kBf16>   // element type of Q/K/V/P/out: bf16 or fp16 (a compile-time choice keeps the
                         // per-pair conversions of the softmax loop free of selects)

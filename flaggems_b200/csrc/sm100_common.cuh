@@ -94,6 +94,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// Makes this thread's shared-memory writes visible to what TMA and the tensor cores do afterwards.
+__device__ __forceinline__ void fence_proxy_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
 // ---- TMA --------------------------------------------------------------------
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
@@ -275,5 +280,8 @@ __host__ __device__ __forceinline__ uint32_t umma_idesc_f16(bool bf16, bool a_mn
 // dims/strides are innermost first; strides (bytes) are given for dims 1..rank-1.
 int encode_tmap_16bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
                       const uint64_t* strides_bytes, const uint32_t* box);
+// The same over 8-bit elements; 64-byte swizzle when the box is 64 elements wide, else 128-byte.
+int encode_tmap_8bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                     const uint32_t* box);
 
 }  // namespace fg
