@@ -9,7 +9,7 @@ int* device_status_ptr();
 
 namespace {
 
-enum { kPathGeneric = 0, kPathDecode = 2 };
+enum { kPathGeneric = 0, kPathChunk = 1, kPathDecode = 2 };
 
 struct Plan {
   int path;
@@ -66,6 +66,17 @@ Plan make_plan(const fg_attn_cache_params* p, int sms) {
     plan.tiles_per_split = (int)(chunk / bn);
     plan.splits = (int)((keys + chunk - 1) / chunk);
     if (plan.splits < 1) plan.splits = 1;
+    return plan;
+  }
+  if (b.head_dim == 128 && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 && tma_ready(p) && b.q_head_stride > 0 &&
+      b.q_row_stride > 0) {
+    plan.path = kPathChunk;
+    const int64_t tokens = 128 / group;                        // of a Q tile; two tiles a CTA when there are more
+    const int64_t per_cta = b.max_seqlen_q > tokens ? 2 * tokens : tokens;
+    const int64_t mb = (b.max_seqlen_q + per_cta - 1) / per_cta;
+    const int64_t tiles = (most_keys(p, per_cta) + 127) / 128;
+    split_plan(mb * b.num_heads_k * b.batch, tiles, (int64_t)sms * 2, 8, &plan);
+    if (mb * b.num_heads_k * b.batch >= sms) plan.splits = 1;
     return plan;
   }
   plan.path = kPathGeneric;
@@ -203,7 +214,9 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   cudaStream_t st = (cudaStream_t)stream;
   FG_REQUIRE((b.max_seqlen_q * a.group + 63) / 64 * plan.splits <= 2147483647LL, "flash_attn_cache: too many row tiles");
   FG_REQUIRE(b.total_q * b.num_heads <= 2147483647LL * 4, "flash_attn_cache: too many rows");
-  const int rc = plan.path == kPathDecode ? attn_cache_decode(c, b.dtype, kind, st) : attn_cache_generic(c, b.dtype, kind, st);
+  const int rc = plan.path == kPathDecode  ? attn_cache_decode(c, b.dtype, kind, st)
+                 : plan.path == kPathChunk ? attn_cache_chunk(c, b.dtype, kind, st)
+                                           : attn_cache_generic(c, b.dtype, kind, st);
   if (rc != FG_OK || a.num_splits == 1) return rc;
   return attn_cache_combine(c, b.dtype, st);
 }

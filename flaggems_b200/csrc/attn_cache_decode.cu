@@ -121,7 +121,9 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   auto wwait = [&](uint64_t* bar, uint32_t parity) -> bool {
     int r = 1;
     if (lane == 0) r = mbar_wait(bar, parity, abort_flag, a.status, kStatusAttnTimeout) ? 1 : 0;
-    return __shfl_sync(0xffffffffu, r, 0) != 0;
+    r = __shfl_sync(0xffffffffu, r, 0);
+    __syncwarp();   // what lane 0 has seen arrive is there for the others
+    return r != 0;
   };
 
   if (warp == 0) {

@@ -429,8 +429,8 @@ typedef struct {
 } fg_attn_cache_params;
 FG_API int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream);
 FG_API int64_t fg_flash_attn_cache_workspace_bytes(const fg_attn_cache_params* p);
-/* Which kernel family fg_flash_attn_cache picks: 0 general (mma.sync), 2 TMA-fed kernel for at most
- * 16 query rows per sequence and KV head.  Pure host logic. */
+/* Which kernel family fg_flash_attn_cache picks: 0 general (mma.sync), 1 tcgen05 (head dim 128), 2 TMA-fed
+ * kernel for at most 16 query rows per sequence and KV head.  Pure host logic. */
 FG_API int fg_flash_attn_cache_path(const fg_attn_cache_params* p);
 
 /* ------------------------------------------------------------------------
