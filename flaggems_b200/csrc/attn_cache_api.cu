@@ -9,7 +9,7 @@ int* device_status_ptr();
 
 namespace {
 
-enum { kPathGeneric = 0, kPathChunk = 1, kPathDecode = 2 };
+enum { kPathGeneric = 0, kPathChunk = 1, kPathDecode = 2, kPathDecodeSm100 = 3 };
 
 struct Plan {
   int path;
@@ -58,8 +58,8 @@ Plan make_plan(const fg_attn_cache_params* p, int sms) {
   if (b.max_seqlen_q * group <= 16 && tma_ready(p)) {
     // Enough CTAs to balance contexts of very different length over all SMs (two resident each), but no range shorter
     // than 256 keys.
-    plan.path = kPathDecode;
-    const int64_t bn = is_fp8(p->cache_dtype) ? 128 : 64;
+    plan.path = b.head_dim == 128 && b.softcap == 0.0 ? kPathDecodeSm100 : kPathDecode;
+    const int64_t bn = plan.path == kPathDecodeSm100 || is_fp8(p->cache_dtype) ? 128 : 64;
     const int64_t keys = most_keys(p, b.max_seqlen_q), ctas = b.num_heads_k * b.batch;
     int64_t chunk = 1024;
     while (chunk > 256 && ctas * ((keys + chunk - 1) / chunk) < (int64_t)sms * 2 * 8) chunk >>= 1;
@@ -214,9 +214,10 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   cudaStream_t st = (cudaStream_t)stream;
   FG_REQUIRE((b.max_seqlen_q * a.group + 63) / 64 * plan.splits <= 2147483647LL, "flash_attn_cache: too many row tiles");
   FG_REQUIRE(b.total_q * b.num_heads <= 2147483647LL * 4, "flash_attn_cache: too many rows");
-  const int rc = plan.path == kPathDecode  ? attn_cache_decode(c, b.dtype, kind, st)
-                 : plan.path == kPathChunk ? attn_cache_chunk(c, b.dtype, kind, st)
-                                           : attn_cache_generic(c, b.dtype, kind, st);
+  const int rc = plan.path == kPathDecodeSm100 ? attn_cache_decode_sm100(c, b.dtype, kind, st)
+                 : plan.path == kPathDecode    ? attn_cache_decode(c, b.dtype, kind, st)
+                 : plan.path == kPathChunk     ? attn_cache_chunk(c, b.dtype, kind, st)
+                                               : attn_cache_generic(c, b.dtype, kind, st);
   if (rc != FG_OK || a.num_splits == 1) return rc;
   return attn_cache_combine(c, b.dtype, st);
 }

@@ -237,6 +237,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// D[tmem] (+)= A[smem desc] * B[smem desc], 8-bit floating point inputs (each operand of its own type), fp32 accumulate.
+__device__ __forceinline__ void mma_f8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // ---- UMMA descriptors ---------------------------------------------------------
 // Shared-memory matrix descriptor, 128-byte swizzle, sm_100 format:
 //   bits [0,14)  start address >> 4        bits [16,30) leading byte offset >> 4
@@ -266,6 +275,21 @@ __host__ __device__ __forceinline__ uint32_t umma_idesc_f16(bool bf16, bool a_mn
   d |= 1u << 4;
   d |= (bf16 ? 1u : 0u) << 7;
   d |= (bf16 ? 1u : 0u) << 10;
+  d |= (a_mn_major ? 1u : 0u) << 15;
+  d |= (b_mn_major ? 1u : 0u) << 16;
+  d |= (uint32_t)(N >> 3) << 17;
+  d |= (uint32_t)(M >> 4) << 24;
+  return d;
+}
+
+// Instruction descriptor for kind::f8f6f4 with fp32 accumulation: formats 0 = E4M3, 1 = E5M2, else as above.  The 8-bit
+// types may be MN-major too; a 128-byte row of the 128-byte swizzle then holds 128 MN elements of one k.
+__host__ __device__ __forceinline__ uint32_t umma_idesc_f8(bool a_e5m2, bool b_e5m2, bool a_mn_major, bool b_mn_major,
+                                                           int M, int N) {
+  uint32_t d = 0;
+  d |= 1u << 4;
+  d |= (a_e5m2 ? 1u : 0u) << 7;
+  d |= (b_e5m2 ? 1u : 0u) << 10;
   d |= (a_mn_major ? 1u : 0u) << 15;
   d |= (b_mn_major ? 1u : 0u) << 16;
   d |= (uint32_t)(N >> 3) << 17;
