@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -88,6 +89,13 @@ class AttnCacheParams(C.Structure):
     )
 
 
+# The parameter blocks of the cache operators in the order of the header, packed in one call: setting fifty fields of a
+# Structure one by one costs more host time than the launch.  Null pointers are 0.
+CACHE_WRITE = struct.Struct("=7Q12q2i")
+CACHE_GATHER = struct.Struct("=9Q15q2i")
+ATTN_CACHE = struct.Struct("=11Q29q2d4i2Q6q2i")
+
+
 class GemmPlan(C.Structure):
     _fields_ = ([(n, C.c_int32) for n in ("tile_m", "tile_n", "grid", "group_m")]
                 + [(n, C.c_int64) for n in ("tiles_m", "tiles_n", "full_units", "num_units")])
@@ -133,8 +141,8 @@ SIGNATURES = {
     "fg_rotary_embedding": (C.c_int, [C.POINTER(RopeParams), _P]),
     "fg_reshape_and_cache_flash": (C.c_int, [_P, _P, _P, _P, _P] + [_I64] * 10 + [C.c_int, _P]),
     "fg_reshape_and_cache": (C.c_int, [_P, _P, _P, _P, _P] + [_I64] * 8 + [C.c_int, _P]),
-    "fg_reshape_and_cache_flash_fp8": (C.c_int, [_P] * 7 + [_I64] * 12 + [C.c_int, C.c_int, _P]),
-    "fg_gather_cache_flash": (C.c_int, [_P] * 9 + [_I64] * 15 + [C.c_int, C.c_int, _P]),
+    "fg_reshape_and_cache_flash_fp8": (C.c_int, [_P, _P]),   # packed by CACHE_WRITE
+    "fg_gather_cache_flash": (C.c_int, [_P, _P]),            # packed by CACHE_GATHER
     "fg_gemm": (C.c_int, [C.POINTER(GemmParams), _P]),
     "fg_gemm_batched": (C.c_int, [C.POINTER(GemmParams)] + [_I64] * 5 + [_P]),
     "fg_gemm_uses_tcgen05": (C.c_int, [C.POINTER(GemmParams)]),
@@ -146,9 +154,10 @@ SIGNATURES = {
     "fg_flash_attn_path": (C.c_int, [C.POINTER(AttnParams)]),
     "fg_flash_attn_decode_static": (C.c_int, [C.POINTER(AttnParams), _P]),
     "fg_flash_attn_decode_static_capacity": (C.c_int64, []),
-    "fg_flash_attn_cache": (C.c_int, [C.POINTER(AttnCacheParams), _P]),
-    "fg_flash_attn_cache_workspace_bytes": (_I64, [C.POINTER(AttnCacheParams)]),
-    "fg_flash_attn_cache_path": (C.c_int, [C.POINTER(AttnCacheParams)]),
+    # AttnCacheParams, or the same bytes packed by ATTN_CACHE
+    "fg_flash_attn_cache": (C.c_int, [_P, _P]),
+    "fg_flash_attn_cache_workspace_bytes": (_I64, [_P]),
+    "fg_flash_attn_cache_path": (C.c_int, [_P]),
     "fg_scheduler_plan": (C.c_int, [C.POINTER(SchedulerParams), C.POINTER(SchedulerPlan)]),
     "fg_get_scheduler_metadata": (C.c_int, [C.POINTER(SchedulerParams), _P, _P]),
 }
@@ -217,6 +226,8 @@ def stream_ptr(device: torch.device) -> int:
 
 
 _HERE = contextlib.nullcontext()
+# the stream handle without a torch.cuda.Stream object around it
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def on_device(device: torch.device):
@@ -226,8 +237,14 @@ def on_device(device: torch.device):
 
 def call(device: torch.device, fn, *args) -> None:
     """``fn(*args, stream)`` on the current stream of ``device``, with that device current."""
-    with on_device(device):
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc < 0:
+        check(rc)
 
 
 def ptr(t) -> int | None:

@@ -14,6 +14,7 @@ enum { kPathGeneric = 0, kPathChunk = 1, kPathDecode = 2, kPathDecodeSm100 = 3 }
 struct Plan {
   int path;
   int splits, tiles_per_split;
+  int64_t bytes;       // of workspace
 };
 
 // Keys that one sequence can have visible to one row tile: everything, or window and first tokens.
@@ -51,25 +52,31 @@ bool tma_ready(const fg_attn_cache_params* p) {
   return b.block_size >= 8 && (b.block_size & (b.block_size - 1)) == 0;
 }
 
-Plan make_plan(const fg_attn_cache_params* p, int sms) {
+// `workspace`: whether the caller has any.
+Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
   const fg_attn_params& b = p->base;
   Plan plan;
   const int64_t group = b.num_heads / b.num_heads_k;
-  if (b.max_seqlen_q * group <= 16 && tma_ready(p)) {
+  const bool tma = tma_ready(p);
+  if (b.max_seqlen_q * group <= 16 && tma && b.head_dim == 128 && b.softcap == 0.0 && workspace) {
+    plan.path = kPathDecodeSm100;      // cuts the keys itself, on the device
+    plan.splits = plan.tiles_per_split = 1;
+    plan.bytes = attn_cache_decode_sm100_bytes(b.max_seqlen_q * group, sms);
+    return plan;
+  }
+  if (b.max_seqlen_q * group <= 16 && tma) {
     // Enough CTAs to balance contexts of very different length over all SMs (two resident each), but no range shorter
     // than 256 keys.
-    plan.path = b.head_dim == 128 && b.softcap == 0.0 ? kPathDecodeSm100 : kPathDecode;
-    const int64_t bn = plan.path == kPathDecodeSm100 || is_fp8(p->cache_dtype) ? 128 : 64;
+    plan.path = kPathDecode;
+    const int64_t bn = is_fp8(p->cache_dtype) ? 128 : 64;
     const int64_t keys = most_keys(p, b.max_seqlen_q), ctas = b.num_heads_k * b.batch;
     int64_t chunk = 1024;
     while (chunk > 256 && ctas * ((keys + chunk - 1) / chunk) < (int64_t)sms * 2 * 8) chunk >>= 1;
     plan.tiles_per_split = (int)(chunk / bn);
     plan.splits = (int)((keys + chunk - 1) / chunk);
     if (plan.splits < 1) plan.splits = 1;
-    return plan;
-  }
-  if (b.head_dim == 128 && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 && tma_ready(p) && b.q_head_stride > 0 &&
-      b.q_row_stride > 0) {
+  } else if (b.head_dim == 128 && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 && tma && b.q_head_stride > 0 &&
+             b.q_row_stride > 0) {
     plan.path = kPathChunk;
     const int64_t tokens = 128 / group;                        // of a Q tile; two tiles a CTA when there are more
     const int64_t per_cta = b.max_seqlen_q > tokens ? 2 * tokens : tokens;
@@ -77,17 +84,15 @@ Plan make_plan(const fg_attn_cache_params* p, int sms) {
     const int64_t tiles = (most_keys(p, per_cta) + 127) / 128;
     split_plan(mb * b.num_heads_k * b.batch, tiles, (int64_t)sms * 2, 8, &plan);
     if (mb * b.num_heads_k * b.batch >= sms) plan.splits = 1;
-    return plan;
+  } else {
+    plan.path = kPathGeneric;
+    const int64_t mb = (b.max_seqlen_q * group + 63) / 64;
+    const int64_t tiles = (most_keys(p, 64 / group + 1) + 63) / 64;
+    split_plan(mb * b.num_heads_k * b.batch, tiles, (int64_t)sms * 2, 4, &plan);
   }
-  plan.path = kPathGeneric;
-  const int64_t mb = (b.max_seqlen_q * group + 63) / 64;
-  const int64_t tiles = (most_keys(p, 64 / group + 1) + 63) / 64;
-  split_plan(mb * b.num_heads_k * b.batch, tiles, (int64_t)sms * 2, 4, &plan);
+  if (!workspace) plan.splits = 1;
+  plan.bytes = plan.splits > 1 ? (int64_t)plan.splits * b.total_q * b.num_heads * (b.head_dim + 1) * 4 : 0;
   return plan;
-}
-
-int64_t plan_bytes(const fg_attn_params& b, const Plan& plan) {
-  return plan.splits > 1 ? (int64_t)plan.splits * b.total_q * b.num_heads * (b.head_dim + 1) * 4 : 0;
 }
 
 bool sizes_ok(const fg_attn_cache_params* p) {
@@ -102,13 +107,13 @@ bool sizes_ok(const fg_attn_cache_params* p) {
 
 extern "C" int fg_flash_attn_cache_path(const fg_attn_cache_params* p) {
   using namespace fg;
-  return p && sizes_ok(p) ? make_plan(p, num_sms()).path : 0;
+  return p && sizes_ok(p) ? make_plan(p, num_sms(), true).path : 0;
 }
 
 extern "C" int64_t fg_flash_attn_cache_workspace_bytes(const fg_attn_cache_params* p) {
   using namespace fg;
   if (p == nullptr || !sizes_ok(p)) return 0;
-  return plan_bytes(p->base, make_plan(p, num_sms()));
+  return make_plan(p, num_sms(), true).bytes;
 }
 
 extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) {
@@ -193,20 +198,15 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   c.sinks = a.wl < 0 ? 0 : (int)(p->sink_tokens < b.max_seqlen_k ? p->sink_tokens : b.max_seqlen_k);
   c.table_cols = (int)p->block_table_cols;
 
-  Plan plan = make_plan(p, num_sms());
+  const Plan plan = make_plan(p, num_sms(), b.workspace != nullptr);
   a.ws_o = nullptr;
   a.ws_lse = nullptr;
-  if (plan.splits > 1) {
-    const int64_t need = plan_bytes(b, plan);
-    if (b.workspace == nullptr) {
-      plan.splits = 1;
-    } else {
-      FG_REQUIRE(b.workspace_bytes >= need, "flash_attn_cache: workspace of %lld bytes, %lld needed",
-                 (long long)b.workspace_bytes, (long long)need);
-      FG_REQUIRE(aligned16(b.workspace), "flash_attn_cache: workspace must be 16-byte aligned");
-      a.ws_o = reinterpret_cast<float*>(b.workspace);
-      a.ws_lse = a.ws_o + (int64_t)plan.splits * b.total_q * b.num_heads * b.head_dim;
-    }
+  if (plan.bytes > 0) {
+    FG_REQUIRE(b.workspace_bytes >= plan.bytes, "flash_attn_cache: workspace of %lld bytes, %lld needed",
+               (long long)b.workspace_bytes, (long long)plan.bytes);
+    FG_REQUIRE(aligned16(b.workspace), "flash_attn_cache: workspace must be 16-byte aligned");
+    a.ws_o = reinterpret_cast<float*>(b.workspace);
+    a.ws_lse = a.ws_o + (int64_t)plan.splits * b.total_q * b.num_heads * b.head_dim;   // split forms only
   }
   a.num_splits = plan.splits;
   c.tiles_per_split = plan.tiles_per_split;
@@ -214,6 +214,8 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   cudaStream_t st = (cudaStream_t)stream;
   FG_REQUIRE((b.max_seqlen_q * a.group + 63) / 64 * plan.splits <= 2147483647LL, "flash_attn_cache: too many row tiles");
   FG_REQUIRE(b.total_q * b.num_heads <= 2147483647LL * 4, "flash_attn_cache: too many rows");
+  FG_REQUIRE(b.batch * b.num_heads_k <= 2147483647LL && b.batch * b.num_heads_k * (b.max_seqlen_k / 128 + 1) <= (1ll << 37),
+             "flash_attn_cache: too many sequences and heads");
   const int rc = plan.path == kPathDecodeSm100 ? attn_cache_decode_sm100(c, b.dtype, kind, st)
                  : plan.path == kPathDecode    ? attn_cache_decode(c, b.dtype, kind, st)
                  : plan.path == kPathChunk     ? attn_cache_chunk(c, b.dtype, kind, st)

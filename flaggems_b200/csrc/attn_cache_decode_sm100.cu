@@ -22,6 +22,14 @@
 //
 //   warps 0-3   softmax and output        warp 4   TMA producer (K and V tiles of 128 keys alternate in one ring)
 //   warp 5      issues the products: scores of the next tile before P V of the current one
+//
+// The kernel is persistent.  An item is one (sequence, KV head).  A team of CTAs walks the same sequences, each for a KV head of
+// its own, so that the heads' pieces of a cached row, which lie side by side in memory, are fetched at about the same time.
+// The K/V tiles of all sequences, laid end to end, are cut into equal runs, one per team, whatever the lengths (each CTA sums
+// the tile counts up once at its start).  The ring, the tensor
+// memory and the barriers carry on from item to item: the producer runs ahead into the next one, and the softmax warps
+// prepare the next item's Q while they work on the current one.  An item inside one run is written out at once; the
+// parts of an item that runs cut are joined by a second kernel, in order.
 #include "attn_cache_common.cuh"
 #include "sm100_common.cuh"
 
@@ -33,7 +41,7 @@ constexpr int TMA_WARP = 4, MMA_WARP = 5;
 constexpr float kRaise = 4.0f;               // log2 units
 constexpr float kPScale = 2048.0f;           // of P before it is split (8-bit caches)
 
-constexpr int up16(int n) { return (n + 15) / 16 * 16; }
+constexpr int up(int n, int to) { return (n + to - 1) / to * to; }
 
 // T: query type; KIND: cache; RP: query rows, rounded up to 4, 8 or 16
 template <typename T, int KIND, int RP>
@@ -42,21 +50,83 @@ struct Cfg {
   static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   static constexpr int PQ = !k8 ? 1 : (kBf16 ? 2 : 3);        // pieces of Q
   static constexpr int PP = k8 ? 4 : (kBf16 ? 2 : 1);         // pieces of P
-  static constexpr int NS = up16(RP * PQ), NP = up16(RP * PP);   // columns of the two products
+  static constexpr int NS = up(RP * PQ, 16), NP = up(RP * PP, 16);   // columns of the two products
+  // Rows of Q and P that shared memory holds: whole 8-row swizzle groups.  Where the product has 8 columns more, it reads
+  // whatever follows there; nothing uses those columns.
+  static constexpr int QR = up(RP * PQ, 8), PR = up(RP * PP, 8);
   static constexpr int TILE = BN * HD * (k8 ? 1 : 2);         // bytes of a K or V tile
-  static constexpr int SLOTS = k8 ? (RP == 16 ? 5 : 6) : 3;   // 80 to 96 KB: two CTAs an SM (one for RP 16, 16 bit)
-  static constexpr int QB = NS * HD * (k8 ? 1 : 2);           // bytes of Q
-  static constexpr int PB = NP * BN * (k8 ? 1 : 2);           // bytes of one P buffer
+  static constexpr int SLOTS = k8 && RP == 16 ? 5 : 6;
+  static constexpr int QB = QR * HD * (k8 ? 1 : 2);           // bytes of one Q buffer
+  static constexpr int PB = PR * BN * (k8 ? 1 : 2);           // bytes of one P buffer
   static constexpr int SCOL = NS <= 32 ? 32 : 64;             // TMEM columns of one score buffer
   static constexpr int OCOL = 2 * SCOL;
   static constexpr int TCOLS = OCOL + NP <= 128 ? 128 : 256;
-  static constexpr int SMEM = SLOTS * TILE + QB + 2 * PB + 1024 + 256 + 2 * 4 * 16 * 4;
+  static constexpr int SMEM = SLOTS * TILE + 2 * QB + 2 * PB + 1024 + 1024;
+  static constexpr int CTAS = k8 ? 2 : 1;                     // per SM: 160 to 192 KB of tiles on their way in either form
+};
+
+// What a CTA leaves for the joining kernel: the item whose start it holds but not its end (or -1), and whether the item it
+// began in the middle of ends in it.
+struct PartRecord {
+  int tail_item, head_ends;
 };
 
 struct DecodeArgs {
   CacheAttnArgs c;
   int page_rows, pages_per_tile;
+  float* part_o;        // [2 * CTAs][RP][128]: head part, tail part of each CTA
+  float* part_lse;      // [2 * CTAs][RP]
+  PartRecord* record;   // [CTAs]
+  int team;             // CTAs of a team: a divisor of the KV heads
 };
+
+// Fewest tiles that a run is worth starting a CTA for.
+constexpr int kMinRun = 4;
+
+// One item's part of a CTA's run.
+struct Segment {
+  int b, hk, lo, hi, n;         // K/V tiles [lo, hi) of the item's n; hk goes up in steps of the team
+  int left;                     // tiles of the run from lo on
+  int rows, shift;
+  SeqInfo s;
+  TileSpan span;
+};
+template <int RP>
+__device__ __forceinline__ int item_tiles(const CacheAttnArgs& c, const SeqInfo& s, TileSpan& span) {
+  const int rows = min(s.q_len * c.a.group, RP);
+  if (rows < 1) return 0;
+  const int shift = s.k_len - s.q_len;
+  span = tile_span<BN>(c, s.k_len, shift, (rows - 1) / c.a.group + shift);
+  return max(span.n, 1);        // nothing visible: one tile, all of it masked, gives the zeros
+}
+template <int RP>
+__device__ __forceinline__ void fill_segment(const CacheAttnArgs& c, Segment& g, int lo) {
+  g.s = seq_info(c.a, g.b);
+  g.n = item_tiles<RP>(c, g.s, g.span);
+  g.rows = min(g.s.q_len * c.a.group, RP);
+  g.shift = g.s.k_len - g.s.q_len;
+  g.lo = lo;
+  g.hi = min(g.n, lo + g.left);
+}
+// The part after `g`; false when the run ends with g.
+template <int RP>
+__device__ __forceinline__ bool next_segment(const CacheAttnArgs& c, int team, const Segment& g, Segment& to) {
+  to = g;
+  to.left = g.left - (g.hi - g.lo);
+  if (to.left <= 0) return false;
+  to.hk += team;
+  if (to.hk < c.a.Hk) {
+    to.lo = 0;
+    to.hi = min(to.n, to.left);
+    return true;
+  }
+  to.hk -= c.a.Hk;
+  do {
+    if (++to.b >= c.a.batch) return false;
+    fill_segment<RP>(c, to, 0);
+  } while (to.n == 0);
+  return true;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -81,62 +151,90 @@ __device__ __forceinline__ uint16_t f16x2_to_e5m2x2(uint32_t h) {
 }
 
 template <typename T, int KIND, int RP>
-__global__ void __launch_bounds__(NUM_THREADS, 2)
+__global__ void __launch_bounds__(NUM_THREADS, Cfg<T, KIND, RP>::CTAS)
 attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                                  const __grid_constant__ DecodeArgs da) {
   using namespace sm100;
   using C = Cfg<T, KIND, RP>;
   const CacheAttnArgs& c = da.c;
   const AttnArgs& a = c.a;
-  const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
-  const SeqInfo s = seq_info(a, b);
-  const int group = a.group;
-  const int rows = min(s.q_len * group, RP);
-  if (rows < 1) return;
-  __shared__ int s_drain;
-  if (threadIdx.x == 0) s_drain = *reinterpret_cast<volatile int*>(a.status);
-  __syncthreads();
-  if (s_drain != 0) return;   // a wait gave up on this device: finish the launch quickly
-  const int shift = s.k_len - s.q_len;
-  const int t_last = (rows - 1) / group;
-  const TileSpan span = tile_span<BN>(c, s.k_len, shift, t_last + shift);
-  const int i_begin = split * c.tiles_per_split;
-  const int n_tiles = (a.num_splits > 1 ? min(span.n, i_begin + c.tiles_per_split) : span.n) - i_begin;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t q0 = s.q_begin;
-
-  if (n_tiles <= 0) {  // nothing visible in this range: contributes nothing
-    if (tid < rows) {
-      const int64_t qtok = q0 + tid / group;
-      const int h = hk * group + tid % group;
-      if (a.num_splits > 1)
-        a.ws_lse[((int64_t)split * a.H + h) * a.total_q + qtok] = -INFINITY;
-      else if (a.lse)
-        a.lse[(int64_t)h * a.total_q + qtok] = INFINITY;
-    }
-    if (a.num_splits == 1)
-      for (int i = tid; i < rows * HD; i += NUM_THREADS) {
-        const int r = i / HD;
-        reinterpret_cast<T*>(a.out)[(q0 + r / group) * a.o_rs + (int64_t)(hk * group + r % group) * a.o_hs + i - r * HD] =
-            Cvt<T>::from_f32(0.f);
-      }
-    return;
-  }
+  const int group = a.group;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sP = smem + C::SLOTS * C::TILE;                        // [2 buffers]
-  uint8_t* sQ = sP + 2 * C::PB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sQ + C::QB);       // [SLOTS]
+  uint8_t* sQ = smem + C::SLOTS * C::TILE;                        // [2 buffers]: items alternate
+  uint8_t* sP = sQ + 2 * C::QB;                                   // [2 buffers]: tiles alternate
+  uint8_t* rest = sP + 2 * C::PB;                                 // 1024 bytes
+  uint64_t* full = reinterpret_cast<uint64_t*>(rest);             // [SLOTS]
   uint64_t* empty = full + C::SLOTS;
   uint64_t* s_full = empty + C::SLOTS;   // [2] scores of a tile have landed
   uint64_t* s_free = s_full + 2;         // [2] ... and have been read into registers
   uint64_t* p_ready = s_free + 2;        // [2]
   uint64_t* o_done = p_ready + 2;        // [2] P V of even / odd tiles
-  uint64_t* q_ready = o_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 1);
+  uint64_t* q_ready = o_done + 2;        // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* sRed = reinterpret_cast<float*>(sQ + C::QB + 256);       // [4 warps][16] maxima, then as many sums
+  float* sMax = reinterpret_cast<float*>(rest + 256);               // [4 warps][16]
+  float* sSum = sMax + 64;                                        // [4 warps][16]
+  float* sDown = sSum + 64;                                       // [2 buffers][16]
+
+  __shared__ int s_drain;
+  __shared__ int64_t s_sum[NUM_THREADS / 32], s_off;
+  __shared__ int s_b;
+  // ---- this team's run: tiles [begin, begin + left) of the tiles that each of its members has
+  const int rounds = a.Hk / da.team, teams = gridDim.x / da.team;
+  if (tid == 0) s_drain = *reinterpret_cast<volatile int*>(a.status);
+  int64_t total = 0;
+  for (int b = tid; b < a.batch; b += NUM_THREADS) {
+    TileSpan span;
+    total += item_tiles<RP>(c, seq_info(a, b), span);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) s_sum[warp] = total;
+  __syncthreads();
+  if (s_drain != 0) return;   // a wait gave up on this device: finish the launch quickly
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < NUM_THREADS / 32; ++i) total += s_sum[i];
+  total *= rounds;
+  int64_t run = (total + teams - 1) / teams;
+  if (run < kMinRun) run = kMinRun;
+  const int64_t begin = run * (blockIdx.x / da.team);   // the CTAs behind the last whole team begin behind the end
+  if (begin >= total) {
+    if (tid == 0) da.record[blockIdx.x] = PartRecord{-1, 1};
+    return;
+  }
+  // the sequence that holds tile `begin`
+  int64_t before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += NUM_THREADS) {
+    int64_t mine = 0;
+    if (b0 + tid < a.batch) {
+      TileSpan span;
+      mine = (int64_t)item_tiles<RP>(c, seq_info(a, b0 + tid), span) * rounds;
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    int64_t base = before;
+#pragma unroll
+    for (int i = 0; i < NUM_THREADS / 32; ++i) {
+      if (i < warp) base += s_sum[i];
+      before += s_sum[i];
+    }
+    if (mine > 0 && base + incl - mine <= begin && begin < base + incl) {
+      s_b = b0 + tid;
+      s_off = begin - (base + incl - mine);
+    }
+    if (before > begin) break;
+  }
 
   if (tid == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
@@ -148,8 +246,8 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
       mbar_init(&s_free[i], 4);
       mbar_init(&p_ready[i], 4);
       mbar_init(&o_done[i], 1);
+      mbar_init(&q_ready[i], 4);
     }
-    mbar_init(q_ready, 4);
     *abort_flag = 0;
     mbar_fence_init();
     prefetch_tmap(&tmap_k);
@@ -163,6 +261,14 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  Segment seg;
+  seg.b = s_b;
+  seg.left = (int)(min(total, begin + run) - begin);
+  fill_segment<RP>(c, seg, 0);
+  seg.hk = (int)(s_off / seg.n);
+  seg.lo = (int)(s_off - (int64_t)seg.hk * seg.n);
+  seg.hk = seg.hk * da.team + blockIdx.x % da.team;
+  seg.hi = min(seg.n, seg.lo + seg.left);
   auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
     return mbar_wait(bar, parity, abort_flag, a.status, kStatusAttnTimeout);
   };
@@ -177,44 +283,50 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
 
   if (warp == TMA_WARP) {
     // ================================ producer ====================================
-    const int32_t* bt_row = a.paged ? a.block_table + (int64_t)b * a.bt_stride : nullptr;
-    const int last_page = a.paged ? max(0, (s.k_len - 1) / a.block_size) : 0;
-    auto lookup = [&](int t, int& page, int& row) {
+    auto lookup = [&](const Segment& g, int t, int& page, int& row) {
+      const int tok = g.span.tile(t) * BN + lane * da.page_rows;
       page = 0;
-      row = 0;
-      if (t >= n_tiles) return;
-      const int tok = span.tile(i_begin + t) * BN + lane * da.page_rows;
-      if (!a.paged) {
-        row = s.k_begin + tok;
-      } else if (lane < da.pages_per_tile) {
+      row = g.s.k_begin + tok;
+      if (a.paged && lane < da.pages_per_tile) {
         const int pg = tok / a.block_size;
         row = tok - pg * a.block_size;
-        page = cache_page(c, bt_row, min(pg, last_page));  // past the sequence: any valid page (those keys are masked)
+        // past the sequence: any valid page (those keys are masked)
+        page = cache_page(c, a.block_table + (int64_t)g.b * a.bt_stride, min(pg, max(0, (g.s.k_len - 1) / a.block_size)));
       }
     };
     int page, row;
-    lookup(0, page, row);
+    lookup(seg, seg.lo, page, row);
+    uint32_t n = 0;   // ring items so far
     bool ok = true;
-    for (int t = 0; t < n_tiles && ok; ++t) {
-      int npage, nrow;
-      lookup(t + 1, npage, nrow);  // the table entry of the next tile is in flight while this one is issued
-      for (int which = 0; which < 2; ++which) {
-        const int n = 2 * t + which, slot = n % C::SLOTS;
-        if (!wwait(&empty[slot], ((n / C::SLOTS) & 1) ^ 1)) {
-          ok = false;
-          break;
+    while (ok) {
+      Segment next;
+      const bool more = next_segment<RP>(c, da.team, seg, next);
+      for (int t = seg.lo; t < seg.hi && ok; ++t) {
+        int npage = 0, nrow = 0;   // the table entry of the next tile is in flight while this one is issued
+        if (t + 1 < seg.hi)
+          lookup(seg, t + 1, npage, nrow);
+        else if (more)
+          lookup(next, next.lo, npage, nrow);
+        for (int which = 0; which < 2; ++which, ++n) {
+          const uint32_t slot = n % C::SLOTS;
+          if (!wwait(&empty[slot], ((n / C::SLOTS) & 1) ^ 1)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_expect_tx(&full[slot], C::TILE);
+          __syncwarp();
+          if (lane < da.pages_per_tile) {
+            uint8_t* dst = smem + slot * C::TILE + lane * da.page_rows * 128;
+            const CUtensorMap* tm = which ? &tmap_v : &tmap_k;
+            tma_load_4d(dst, tm, &full[slot], 0, seg.hk, row, page);
+            if constexpr (!C::k8) tma_load_4d(dst + C::TILE / 2, tm, &full[slot], 64, seg.hk, row, page);
+          }
         }
-        if (lane == 0) mbar_expect_tx(&full[slot], C::TILE);
-        __syncwarp();
-        if (lane < da.pages_per_tile) {
-          uint8_t* dst = smem + slot * C::TILE + lane * da.page_rows * 128;
-          const CUtensorMap* tm = which ? &tmap_v : &tmap_k;
-          tma_load_4d(dst, tm, &full[slot], 0, hk, row, page);
-          if constexpr (!C::k8) tma_load_4d(dst + C::TILE / 2, tm, &full[slot], 64, hk, row, page);
-        }
+        page = npage;
+        row = nrow;
       }
-      page = npage;
-      row = nrow;
+      if (!more) break;
+      seg = next;
     }
   } else if (warp == MMA_WARP) {
     // ================================ products ====================================
@@ -223,73 +335,105 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
                                   : umma_idesc_f16(C::kBf16, false, false, BN, C::NS);
       const uint32_t id_o = C::k8 ? umma_idesc_f8(KIND == kCacheE5M2, true, true, false, HD, C::NP)
                                   : umma_idesc_f16(C::kBf16, true, false, HD, C::NP);
-      const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ), 0, 1024);
-      auto scores = [&](int t) -> bool {
-        const int n = 2 * t, slot = n % C::SLOTS;
+      // tile g of the run (tiles and ring items count on through all items); `item`: the how-manieth
+      auto scores = [&](uint32_t g, bool first, uint32_t item) -> bool {
+        const uint32_t n = 2 * g, slot = n % C::SLOTS;
+        if (first && !wait1(&q_ready[item & 1], (item >> 1) & 1)) return false;
         if (!wait1(&full[slot], (n / C::SLOTS) & 1)) return false;
-        if (t >= 2 && !wait1(&s_free[t & 1], ((t - 2) >> 1) & 1)) return false;   // scores two tiles back are read
+        if (g >= 2 && !wait1(&s_free[g & 1], ((g - 2) >> 1) & 1)) return false;   // scores two tiles back are read
         tc_fence_after();
         const uint64_t k_desc = umma_desc_sw128(smem_u32(smem + slot * C::TILE), 0, 1024);
-        const uint32_t d = tmem_base + (t & 1) * C::SCOL;
+        const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ + (item & 1) * C::QB), 0, 1024);
+        const uint32_t d = tmem_base + (g & 1) * C::SCOL;
         if constexpr (C::k8) {
 #pragma unroll
           for (int k = 0; k < HD / 32; ++k) mma_f8_ss(d, k_desc + k * 2, q_desc + k * 2, id_s, k != 0);
         } else {
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k)
-            mma_f16_ss(d, k_desc + (k >> 2) * (C::TILE / 2 / 16) + (k & 3) * 2, q_desc + (k >> 2) * (C::NS * 128 / 16) + (k & 3) * 2,
+            mma_f16_ss(d, k_desc + (k >> 2) * (C::TILE / 2 / 16) + (k & 3) * 2, q_desc + (k >> 2) * (C::QR * 128 / 16) + (k & 3) * 2,
                        id_s, k != 0);
         }
-        tc_commit(&s_full[t & 1]);
+        tc_commit(&s_full[g & 1]);
         tc_commit(&empty[slot]);
         return true;
       };
-      bool ok = wait1(q_ready, 0) && scores(0);
-      for (int t = 0; t < n_tiles && ok; ++t) {
-        if (t + 1 < n_tiles && !scores(t + 1)) break;
-        const int n = 2 * t + 1, slot = n % C::SLOTS;
-        if (!wait1(&full[slot], (n / C::SLOTS) & 1) || !wait1(&p_ready[t & 1], (t >> 1) & 1)) break;
-        tc_fence_after();
-        const uint64_t v_desc = umma_desc_sw128(smem_u32(smem + slot * C::TILE), C::k8 ? C::TILE : C::TILE / 2, 1024);
-        const uint64_t p_desc = umma_desc_sw128(smem_u32(sP + (t & 1) * C::PB), 0, 1024);
-        const uint32_t d = tmem_base + C::OCOL;
-        if constexpr (C::k8) {
+      Segment ahead = seg;                 // where the scores are, one tile ahead of P V
+      int at = seg.lo;
+      uint32_t ahead_item = 0, g = 0;
+      bool ok = scores(0, true, 0), left = true;
+      while (ok && left) {
+        for (int t = seg.lo; t < seg.hi && ok; ++t, ++g) {
+          bool first = false, more = true;
+          if (++at >= ahead.hi) {
+            Segment to;
+            more = next_segment<RP>(c, da.team, ahead, to);
+            ahead = to;
+            at = to.lo;
+            first = true;
+            ++ahead_item;
+          }
+          if (more && !scores(g + 1, first, ahead_item)) {
+            ok = false;
+            break;
+          }
+          const uint32_t n = 2 * g + 1, slot = n % C::SLOTS;
+          if (!wait1(&full[slot], (n / C::SLOTS) & 1) || !wait1(&p_ready[g & 1], (g >> 1) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t v_desc = umma_desc_sw128(smem_u32(smem + slot * C::TILE), C::k8 ? C::TILE : C::TILE / 2, 1024);
+          const uint64_t p_desc = umma_desc_sw128(smem_u32(sP + (g & 1) * C::PB), 0, 1024);
+          const uint32_t d = tmem_base + C::OCOL;
+          const bool add = t > seg.lo;     // the first tile of an item overwrites
+          if constexpr (C::k8) {
 #pragma unroll
-          for (int k = 0; k < BN / 32; ++k) mma_f8_ss(d, v_desc + k * (4096 >> 4), p_desc + k * 2, id_o, t > 0 || k > 0);
-        } else {
+            for (int k = 0; k < BN / 32; ++k) mma_f8_ss(d, v_desc + k * (4096 >> 4), p_desc + k * 2, id_o, add || k > 0);
+          } else {
 #pragma unroll
-          for (int k = 0; k < BN / 16; ++k)
-            mma_f16_ss(d, v_desc + k * (2048 >> 4), p_desc + (k >> 2) * (C::NP * 128 / 16) + (k & 3) * 2, id_o, t > 0 || k > 0);
+            for (int k = 0; k < BN / 16; ++k)
+              mma_f16_ss(d, v_desc + k * (2048 >> 4), p_desc + (k >> 2) * (C::PR * 128 / 16) + (k & 3) * 2, id_o, add || k > 0);
+          }
+          tc_commit(&o_done[g & 1]);
+          tc_commit(&empty[slot]);
         }
-        tc_commit(&o_done[t & 1]);
-        tc_commit(&empty[slot]);
+        Segment to;
+        left = next_segment<RP>(c, da.team, seg, to);
+        seg = to;
       }
     }
   } else {
     // ================================ softmax / output =============================
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
-    // ---- Q, split into pieces: 128 / RP threads a row, RP values each
-    float pre[RP];           // takes a sum of columns to the scores
-    {
-      constexpr int TPR = 128 / RP;
-      const int r = tid / TPR, d0 = (tid % TPR) * RP;
-      const bool live = r < rows;
-      const int tok = live ? r / group : 0;
-      const T* q = reinterpret_cast<const T*>(a.q) + (q0 + tok) * a.q_rs + (int64_t)(hk * group + (live ? r - tok * group : 0)) * a.q_hs + d0;
-      uint32_t w[RP / 2];
+    // ---- an item's Q: 128 / RP threads a row, RP values each, loaded ahead and then split into pieces
+    constexpr int TPR = 128 / RP;
+    const int q_row = tid / TPR, d0 = (tid % TPR) * RP;
+    uint32_t qw[RP / 2];
+    float ksc = 1.f, vsc = 1.f;
+    auto load_q = [&](const Segment& g) {
+      const bool live = q_row < g.rows;
+      const int tok = live ? q_row / group : 0;
+      const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(g.s.q_begin + tok) * a.q_rs +
+                   (int64_t)(g.hk * group + (live ? q_row - tok * group : 0)) * a.q_hs + d0;
 #pragma unroll
       for (int i = 0; i < RP / 4; ++i) {
         const uint2 u = live ? *reinterpret_cast<const uint2*>(q + i * 4) : make_uint2(0, 0);
-        w[2 * i] = u.x;
-        w[2 * i + 1] = u.y;
+        qw[2 * i] = u.x;
+        qw[2 * i + 1] = u.y;
       }
+      ksc = cache_scale(c.k_scale, c.ks_batch, c.ks_head, g.b, g.hk);
+      vsc = cache_scale(c.v_scale, c.vs_batch, c.vs_head, g.b, g.hk);
+    };
+    auto store_q = [&](uint32_t item) {
+      uint8_t* buf = sQ + (item & 1) * C::QB;
       float down = 1.f;
       if constexpr (C::k8) {
         float x[RP], top = 0.f;
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < RP / 2; ++i) {
-          const float2 f = Pair<T>::unpack(w[i]);
+          const float2 f = Pair<T>::unpack(qw[i]);
           x[2 * i] = f.x;
           x[2 * i + 1] = f.y;
           top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
@@ -308,8 +452,8 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
         for (int i = 0; i < RP; ++i) x[i] *= up;
 #pragma unroll
         for (int p = 0; p < C::PQ; ++p) {
-          const int n = p * RP + r;
-          uint8_t* dst = sQ + n * 128 + (((d0 >> 4) ^ (n & 7)) << 4) + (d0 & 15);
+          const int n = p * RP + q_row;
+          uint8_t* dst = buf + n * 128 + (((d0 >> 4) ^ (n & 7)) << 4) + (d0 & 15);
 #pragma unroll
           for (int i = 0; i < RP / 4; ++i) {
             const uint16_t e0 = f32x2_to_fp8x2<kCacheE4M3>(x[4 * i], x[4 * i + 1]);
@@ -323,214 +467,226 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             *reinterpret_cast<uint32_t*>(dst + i * 4) = e0 | ((uint32_t)e1 << 16);
           }
         }
-        // the columns behind the pieces
-        for (int i = tid; i < (C::NS - C::PQ * RP) * 8; i += 128)
-          *reinterpret_cast<uint4*>(sQ + C::PQ * RP * 128 + i * 16) = make_uint4(0, 0, 0, 0);
       } else {
 #pragma unroll
         for (int i = 0; i < RP / 4; ++i) {
           const int d = d0 + i * 4;
-          *reinterpret_cast<uint2*>(sQ + (d >> 6) * (C::NS * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 7) * 2) =
-              make_uint2(w[2 * i], w[2 * i + 1]);
+          *reinterpret_cast<uint2*>(buf + (d >> 6) * (C::QR * 128) + q_row * 128 + ((((d & 63) >> 3) ^ (q_row & 7)) << 4) +
+                                    (d & 7) * 2) = make_uint2(qw[2 * i], qw[2 * i + 1]);
         }
-        // the columns behind the pieces, of Q (both halves of the dims) and of P (both buffers, both halves of the keys)
-        for (int i = tid; i < (C::NS - RP) * 8; i += 128)
-          for (int hf = 0; hf < 2; ++hf)
-            *reinterpret_cast<uint4*>(sQ + hf * (C::NS * 128) + RP * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-        for (int i = tid; i < (C::NP - C::PP * RP) * 8; i += 128)
-          for (int part = 0; part < 4; ++part)
-            *reinterpret_cast<uint4*>(sP + part * (C::NP * 128) + C::PP * RP * 128 + i * 16) = make_uint4(0, 0, 0, 0);
       }
-      // every thread needs every row's power: through the reduction scratch
-      if (tid % TPR == 0) sRed[r] = down;
+      if (tid % TPR == 0) sDown[(item & 1) * 16 + q_row] = down;
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_ready);
-      softmax_sync();
-      const float ksc = cache_scale(c.k_scale, c.ks_batch, c.ks_head, b, hk) * a.scale_log2;
-#pragma unroll
-      for (int i = 0; i < RP; ++i) pre[i] = sRed[i] * ksc;
-    }
-    const RowMask first = row_mask(c, s.k_len, shift), last = row_mask(c, s.k_len, t_last + shift);
-    float m_ref[RP], l_run[RP];
-#pragma unroll
-    for (int r = 0; r < RP; ++r) {
-      m_ref[r] = -INFINITY;
-      l_run[r] = 0.f;
-    }
-    // A wait that gave up does not end the loop: the barriers below need every warp.
-    bool ok = true;
-    for (int t = 0; t < n_tiles; ++t) {
-      ok = ok && wwait(&s_full[t & 1], (t >> 1) & 1);
-      tc_fence_after();
-      float x[RP];
-      {
-        uint32_t col[C::NS];
-#pragma unroll
-        for (int q = 0; q < C::NS / 16; ++q)
-          tmem_ld16(tmem_base + lane_addr + (t & 1) * C::SCOL + q * 16, *reinterpret_cast<uint32_t(*)[16]>(&col[q * 16]));
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t & 1]);
-#pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          float v = __uint_as_float(col[r]);
-#pragma unroll
-          for (int p = 1; p < C::PQ; ++p) v += __uint_as_float(col[p * RP + r]);
-          x[r] = v * pre[r];
-        }
-      }
-      const int j0 = span.tile(i_begin + t) * BN;
-      const int n_v = 2 * t + 1, v_slot = n_v % C::SLOTS;
-      if (j0 + BN > first.hi || (j0 < last.lo && j0 + BN > c.sinks)) {
-        const int col = j0 + tid;
-        int tok = 0, in = 0;
-#pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          if (row_mask(c, s.k_len, tok + shift).dead(col)) x[r] = -INFINITY;
-          if (++in == group) {
-            in = 0;
-            ++tok;
-          }
-        }
-        // a V row that no query row sees must not reach the product
-        ok = ok && wwait(&full[v_slot], (n_v / C::SLOTS) & 1);
-        if (ok && (col >= last.hi || (col < first.lo && col >= c.sinks))) {
-          uint8_t* v = smem + v_slot * C::TILE + tid * 128;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
-          if constexpr (!C::k8) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + C::TILE / 2 + i * 16) = make_uint4(0, 0, 0, 0);
-          }
-        }
-      }
-      bool raise = false;
-#pragma unroll
-      for (int r = 0; r < RP; ++r) raise = raise || x[r] > m_ref[r] + kRaise;
-      if (softmax_any(raise)) {
-        // exact maxima of the tile, shared by the four warps
-#pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float m = warp_max(x[r]);
-          if (lane == 0) sRed[warp * 16 + r] = m;
-        }
-        softmax_sync();
-        float f[RP];
-#pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float m = fmaxf(fmaxf(fmaxf(sRed[r], sRed[16 + r]), fmaxf(sRed[32 + r], sRed[48 + r])), m_ref[r]);
-          f[r] = m == -INFINITY ? 1.f : ex2(m_ref[r] - m);
-          m_ref[r] = m;
-          l_run[r] *= f[r];
-        }
-        if (t > 0) {
-          ok = ok && wwait(&o_done[(t - 1) & 1], ((t - 1) >> 1) & 1);   // every product so far has landed
-          tc_fence_after();
-#pragma unroll
-          for (int q = 0; q < C::NP / 16; ++q) {
-            uint32_t o[16];
-            tmem_ld16(tmem_base + lane_addr + C::OCOL + q * 16, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (q * 16 + e < C::PP * RP) o[e] = __float_as_uint(__uint_as_float(o[e]) * f[(q * 16 + e) % RP]);
-            tmem_st16(tmem_base + lane_addr + C::OCOL + q * 16, o);
-          }
-          tmem_st_wait();
-          tc_fence_before();
-        }
-      }
-      if (t >= 2) ok = ok && wwait(&o_done[t & 1], ((t - 2) >> 1) & 1);   // the P buffer has been read
-      uint8_t* buf = sP + (t & 1) * C::PB;
-#pragma unroll
-      for (int r = 0; r < RP; r += 2) {
-        const float p0 = ex2(x[r] - (m_ref[r] == -INFINITY ? 0.f : m_ref[r]));
-        const float p1 = ex2(x[r + 1] - (m_ref[r + 1] == -INFINITY ? 0.f : m_ref[r + 1]));
-        l_run[r] += p0;
-        l_run[r + 1] += p1;
-        if constexpr (C::k8) {
-          uint32_t h = Pair<__half>::pack(p0 * kPScale, p1 * kPScale);
-          const int at = tid & 15, ch = tid >> 4;
-#pragma unroll
-          for (int p = 0; p < C::PP; ++p) {
-            const uint16_t e = f16x2_to_e5m2x2(h);
-            const uint32_t back = fp8x2_to_f16x2<kCacheE5M2>(e);
-            const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&back));
-            h = *reinterpret_cast<const uint32_t*>(&d);
-            const int n = p * RP + r;
-            buf[n * 128 + ((ch ^ (n & 7)) << 4) + at] = (uint8_t)(e & 0xff);
-            buf[(n + 1) * 128 + ((ch ^ ((n + 1) & 7)) << 4) + at] = (uint8_t)(e >> 8);
-          }
-        } else {
-          const int at = (tid & 7) * 2, ch = (tid & 63) >> 3;
-          uint8_t* half = buf + (tid >> 6) * (C::NP * 128);
-          float y0 = p0, y1 = p1;
-#pragma unroll
-          for (int p = 0; p < C::PP; ++p) {
-            const uint32_t e = Pair<T>::pack(y0, y1);
-            const float2 back = Pair<T>::unpack(e);
-            y0 -= back.x;
-            y1 -= back.y;
-            const int n = p * RP + r;
-            *reinterpret_cast<uint16_t*>(half + n * 128 + ((ch ^ (n & 7)) << 4) + at) = (uint16_t)(e & 0xffff);
-            *reinterpret_cast<uint16_t*>(half + (n + 1) * 128 + ((ch ^ ((n + 1) & 7)) << 4) + at) = (uint16_t)(e >> 16);
-          }
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[t & 1]);
-    }
-
-    // ---- sums over the keys (threads), then one output dim a thread
-    softmax_sync();          // the scratch of the maxima has been read
-#pragma unroll
-    for (int r = 0; r < RP; ++r) {
-      const float l = warp_sum(l_run[r]);
-      if (lane == 0) sRed[warp * 16 + r] = l;
-    }
+      if (lane == 0) mbar_arrive(&q_ready[item & 1]);
+    };
+    load_q(seg);
+    store_q(0);
     softmax_sync();
-    ok = ok && wwait(&o_done[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1);
-    tc_fence_after();
-    if (ok) {
+    PartRecord rec{-1, 1};
+    uint32_t g = 0;            // tiles so far
+    // A wait that gave up does not end the loops: the barriers below need every warp.
+    bool ok = true;
+    for (uint32_t item = 0;; ++item) {
+      float pre[RP];           // takes a sum of columns to the scores
+#pragma unroll
+      for (int i = 0; i < RP; ++i) pre[i] = sDown[(item & 1) * 16 + i] * (ksc * a.scale_log2);
+      const float v_scale = vsc;
+      Segment next;
+      const bool more = next_segment<RP>(c, da.team, seg, next);
+      if (more) load_q(next);
+      const int k_len = seg.s.k_len, shift = seg.shift;
+      const RowMask first = row_mask(c, k_len, shift), last = row_mask(c, k_len, (seg.rows - 1) / group + shift);
+      float m_ref[RP], l_run[RP];
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        m_ref[r] = -INFINITY;
+        l_run[r] = 0.f;
+      }
+      for (int t = seg.lo; t < seg.hi; ++t, ++g) {
+        ok = ok && wwait(&s_full[g & 1], (g >> 1) & 1);
+        tc_fence_after();
+        float x[RP];
+        {
+          uint32_t col[C::NS];
+#pragma unroll
+          for (int q = 0; q < C::NS / 16; ++q)
+            tmem_ld16(tmem_base + lane_addr + (g & 1) * C::SCOL + q * 16, *reinterpret_cast<uint32_t(*)[16]>(&col[q * 16]));
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[g & 1]);
+#pragma unroll
+          for (int r = 0; r < RP; ++r) {
+            float v = __uint_as_float(col[r]);
+#pragma unroll
+            for (int p = 1; p < C::PQ; ++p) v += __uint_as_float(col[p * RP + r]);
+            x[r] = v * pre[r];
+          }
+        }
+        const int j0 = seg.span.tile(t) * BN;
+        if (j0 + BN > first.hi || (j0 < last.lo && j0 + BN > c.sinks)) {
+          const int col = j0 + tid;
+          int tok = 0, in = 0;
+#pragma unroll
+          for (int r = 0; r < RP; ++r) {
+            if (row_mask(c, k_len, tok + shift).dead(col)) x[r] = -INFINITY;
+            if (++in == group) {
+              in = 0;
+              ++tok;
+            }
+          }
+          // a V row that no query row sees must not reach the product
+          const uint32_t n_v = 2 * g + 1, v_slot = n_v % C::SLOTS;
+          ok = ok && wwait(&full[v_slot], (n_v / C::SLOTS) & 1);
+          if (ok && (col >= last.hi || (col < first.lo && col >= c.sinks))) {
+            uint8_t* v = smem + v_slot * C::TILE + tid * 128;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
+            if constexpr (!C::k8) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + C::TILE / 2 + i * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+        }
+        bool raise = false;
+#pragma unroll
+        for (int r = 0; r < RP; ++r) raise = raise || x[r] > m_ref[r] + kRaise;
+        if (softmax_any(raise)) {
+          // exact maxima of the tile, shared by the four warps
+#pragma unroll
+          for (int r = 0; r < RP; ++r) {
+            const float m = warp_max(x[r]);
+            if (lane == 0) sMax[warp * 16 + r] = m;
+          }
+          softmax_sync();
+          float f[RP];
+#pragma unroll
+          for (int r = 0; r < RP; ++r) {
+            const float m = fmaxf(fmaxf(fmaxf(sMax[r], sMax[16 + r]), fmaxf(sMax[32 + r], sMax[48 + r])), m_ref[r]);
+            f[r] = m == -INFINITY ? 1.f : ex2(m_ref[r] - m);
+            m_ref[r] = m;
+            l_run[r] *= f[r];
+          }
+          if (t > seg.lo) {
+            ok = ok && wwait(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);   // every product so far has landed
+            tc_fence_after();
+#pragma unroll
+            for (int q = 0; q < C::NP / 16; ++q) {
+              uint32_t o[16];
+              tmem_ld16(tmem_base + lane_addr + C::OCOL + q * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (q * 16 + e < C::PP * RP) o[e] = __float_as_uint(__uint_as_float(o[e]) * f[(q * 16 + e) % RP]);
+              tmem_st16(tmem_base + lane_addr + C::OCOL + q * 16, o);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+          }
+        }
+        if (g >= 2) ok = ok && wwait(&o_done[g & 1], ((g - 2) >> 1) & 1);   // the P buffer has been read
+        uint8_t* buf = sP + (g & 1) * C::PB;
+#pragma unroll
+        for (int r = 0; r < RP; r += 2) {
+          const float p0 = ex2(x[r] - (m_ref[r] == -INFINITY ? 0.f : m_ref[r]));
+          const float p1 = ex2(x[r + 1] - (m_ref[r + 1] == -INFINITY ? 0.f : m_ref[r + 1]));
+          l_run[r] += p0;
+          l_run[r + 1] += p1;
+          if constexpr (C::k8) {
+            uint32_t h = Pair<__half>::pack(p0 * kPScale, p1 * kPScale);
+            const int at = tid & 15, ch = tid >> 4;
+#pragma unroll
+            for (int p = 0; p < C::PP; ++p) {
+              const uint16_t e = f16x2_to_e5m2x2(h);
+              const uint32_t back = fp8x2_to_f16x2<kCacheE5M2>(e);
+              const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&back));
+              h = *reinterpret_cast<const uint32_t*>(&d);
+              const int n = p * RP + r;
+              buf[n * 128 + ((ch ^ (n & 7)) << 4) + at] = (uint8_t)(e & 0xff);
+              buf[(n + 1) * 128 + ((ch ^ ((n + 1) & 7)) << 4) + at] = (uint8_t)(e >> 8);
+            }
+          } else {
+            const int at = (tid & 7) * 2, ch = (tid & 63) >> 3;
+            uint8_t* half = buf + (tid >> 6) * (C::PR * 128);
+            float y0 = p0, y1 = p1;
+#pragma unroll
+            for (int p = 0; p < C::PP; ++p) {
+              const uint32_t e = Pair<T>::pack(y0, y1);
+              const float2 back = Pair<T>::unpack(e);
+              y0 -= back.x;
+              y1 -= back.y;
+              const int n = p * RP + r;
+              *reinterpret_cast<uint16_t*>(half + n * 128 + ((ch ^ (n & 7)) << 4) + at) = (uint16_t)(e & 0xffff);
+              *reinterpret_cast<uint16_t*>(half + (n + 1) * 128 + ((ch ^ ((n + 1) & 7)) << 4) + at) = (uint16_t)(e >> 16);
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[g & 1]);
+        // the next item's Q, into the buffer whose item's scores have all landed
+        if (t == seg.lo && more) store_q(item + 1);
+      }
+
+      // ---- sums over the keys (threads), then one output dim a thread
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        const float l = warp_sum(l_run[r]);
+        if (lane == 0) sSum[warp * 16 + r] = l;
+      }
+      softmax_sync();
+      ok = ok && wwait(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
+      tc_fence_after();
       uint32_t o[C::NP];
 #pragma unroll
       for (int q = 0; q < C::NP / 16; ++q)
         tmem_ld16(tmem_base + lane_addr + C::OCOL + q * 16, *reinterpret_cast<uint32_t(*)[16]>(&o[q * 16]));
       tmem_ld_wait();
-      const float vsc = cache_scale(c.v_scale, c.vs_batch, c.vs_head, b, hk);
-      int tok = 0, in = 0;
+      tc_fence_before();   // the next item's first product overwrites O after its P, which this thread has yet to store
+      const bool whole = seg.lo == 0 && seg.hi == seg.n;
+      const int part = 2 * blockIdx.x + (seg.lo == 0 ? 1 : 0);
+      if (!whole) {
+        if (seg.lo == 0)
+          rec.tail_item = seg.b * a.Hk + seg.hk;
+        else
+          rec.head_ends = seg.hi == seg.n;
+      }
+      if (ok) {
+        int tok = 0, in = 0;
 #pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        if (r < rows) {
-          float v = __uint_as_float(o[r]);
+        for (int r = 0; r < RP; ++r) {
+          if (r < seg.rows) {
+            float v = __uint_as_float(o[r]);
 #pragma unroll
-          for (int p = 1; p < C::PP; ++p) v += __uint_as_float(o[p * RP + r]);
-          const float l = (sRed[r] + sRed[16 + r]) + (sRed[32 + r] + sRed[48 + r]);
-          // a NaN sum stays one: only a row that saw nothing is set to zero
-          v = l == 0.f ? 0.f : v * (C::k8 ? 1.f / kPScale : 1.f) * (vsc / l);
-          const int64_t qtok = q0 + tok;
-          const int h = hk * group + in;
-          if (a.num_splits > 1)
-            a.ws_o[(((int64_t)split * a.total_q + qtok) * a.H + h) * HD + tid] = v;
-          else
-            reinterpret_cast<T*>(a.out)[qtok * a.o_rs + (int64_t)h * a.o_hs + tid] = Cvt<T>::from_f32(v);
-          if (tid == 0) {
-            const float lse2 = l == 0.f ? -INFINITY : m_ref[r] + log2f(l);
-            if (a.num_splits > 1)
-              a.ws_lse[((int64_t)split * a.H + h) * a.total_q + qtok] = lse2;
-            else if (a.lse)
-              a.lse[(int64_t)h * a.total_q + qtok] = l == 0.f ? INFINITY : lse2 * 0.6931471805599453f;
+            for (int p = 1; p < C::PP; ++p) v += __uint_as_float(o[p * RP + r]);
+            const float l = (sSum[r] + sSum[16 + r]) + (sSum[32 + r] + sSum[48 + r]);
+            // a NaN sum stays one: only a row that saw nothing is set to zero
+            v = l == 0.f ? 0.f : v * (C::k8 ? 1.f / kPScale : 1.f) * (v_scale / l);
+            const int64_t qtok = seg.s.q_begin + tok;
+            const int h = seg.hk * group + in;
+            if (whole)
+              reinterpret_cast<T*>(a.out)[qtok * a.o_rs + (int64_t)h * a.o_hs + tid] = Cvt<T>::from_f32(v);
+            else
+              da.part_o[((int64_t)part * RP + r) * HD + tid] = v;
+            if (tid == 0) {
+              const float lse2 = l == 0.f ? -INFINITY : m_ref[r] + log2f(l);
+              if (!whole)
+                da.part_lse[part * RP + r] = lse2;
+              else if (a.lse)
+                a.lse[(int64_t)h * a.total_q + qtok] = l == 0.f ? INFINITY : lse2 * 0.6931471805599453f;
+            }
+          }
+          if (++in == group) {
+            in = 0;
+            ++tok;
           }
         }
-        if (++in == group) {
-          in = 0;
-          ++tok;
-        }
       }
+      if (!more) break;
+      seg = next;
     }
+    if (tid == 0) da.record[blockIdx.x] = rec;
   }
 
   // ================================ teardown ======================================
@@ -546,10 +702,55 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   }
 }
 
+// Joins the parts of the items that runs cut.  Block (i, r) does row r of the item whose start, but not end, CTA i holds: its
+// tail part, then the head parts of the same member of the teams after it, up to the one the item ends in.  Four groups of 128 threads take
+// every fourth part; their sums are added in a fixed order.
+template <typename T, int RP>
+__global__ void __launch_bounds__(512) attn_cache_join_kernel(DecodeArgs da, int ctas) {
+  const AttnArgs& a = da.c.a;
+  __shared__ float s_acc[3][HD], s_w[4], s_max[16];
+  const int i = blockIdx.x, r = blockIdx.y;
+  if (*reinterpret_cast<volatile int*>(a.status) != 0) return;   // the parts and the records may be missing
+  const int item = da.record[i].tail_item;
+  if (item < 0) return;
+  const int b = item / a.Hk, hk = item - b * a.Hk;
+  const SeqInfo s = seq_info(a, b);
+  if (r >= min(s.q_len * a.group, RP)) return;
+  const int grp = threadIdx.x >> 7, d = threadIdx.x & 127;
+  int n = 2;                              // parts
+  while (i + n * da.team < ctas && !da.record[i + (n - 1) * da.team].head_ends) ++n;
+  auto slot = [&](int k) { return (int64_t)(k == 0 ? 2 * i + 1 : 2 * (i + k * da.team)) * RP + r; };
+  float m = -INFINITY;
+  for (int k = threadIdx.x; k < n; k += 512) m = fmaxf(m, da.part_lse[slot(k)]);
+  m = warp_max(m);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 16; ++k) m = fmaxf(m, s_max[k]);
+  const float ms = m == -INFINITY ? 0.f : m;
+  float acc = 0.f, wsum = 0.f;
+  for (int k = grp; k < n; k += 4) {
+    const float w = exp2f(da.part_lse[slot(k)] - ms);
+    wsum += w;
+    if (w != 0.f) acc += w * da.part_o[slot(k) * HD + d];   // NaN goes on
+  }
+  if (grp > 0) s_acc[grp - 1][d] = acc;
+  if (d == 0) s_w[grp] = wsum;
+  __syncthreads();
+  if (grp > 0) return;
+  acc = ((acc + s_acc[0][d]) + (s_acc[1][d] + s_acc[2][d]));
+  wsum = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]);
+  const int64_t qtok = s.q_begin + r / a.group;
+  const int h = hk * a.group + r % a.group;
+  reinterpret_cast<T*>(a.out)[qtok * a.o_rs + (int64_t)h * a.o_hs + d] = Cvt<T>::from_f32(wsum == 0.f ? 0.f : acc / wsum);
+  if (a.lse && d == 0)
+    a.lse[(int64_t)h * a.total_q + qtok] = wsum == 0.f ? INFINITY : (m + log2f(wsum)) * 0.6931471805599453f;
+}
+
 template <typename T, int KIND, int RP>
 int launch(DecodeArgs& da, cudaStream_t st) {
   using C = Cfg<T, KIND, RP>;
-  static_assert(!C::k8 && RP == 16 ? C::SMEM <= 232448 : 2 * (C::SMEM + 1024) <= 233472, "CTAs an SM");
+  static_assert(C::SMEM <= 232448 && C::CTAS * (C::SMEM + 1024) <= 233472, "CTAs an SM");
   const AttnArgs& a = da.c.a;
   constexpr int ES = C::k8 ? 1 : 2;
   da.page_rows = a.paged && a.block_size < BN ? a.block_size : BN;
@@ -574,9 +775,17 @@ int launch(DecodeArgs& da, cudaStream_t st) {
                                     C::SMEM));
     attr_dev = dev;
   }
-  dim3 grid(a.num_splits, a.Hk, a.batch);
-  attn_cache_decode_tcgen05_kernel<T, KIND, RP><<<grid, NUM_THREADS, C::SMEM, st>>>(maps[0], maps[1], da);
+  const int ctas = C::CTAS * num_sms();
+  da.team = 1;
+  for (int t = 2; t <= 16; ++t)
+    if (a.Hk % t == 0) da.team = t;
+  da.part_o = a.ws_o;
+  da.part_lse = a.ws_o + (int64_t)2 * ctas * RP * HD;
+  da.record = reinterpret_cast<PartRecord*>(da.part_lse + 2 * ctas * RP);
+  attn_cache_decode_tcgen05_kernel<T, KIND, RP><<<ctas, NUM_THREADS, C::SMEM, st>>>(maps[0], maps[1], da);
   FG_CHECK_LAUNCH("attn_cache_decode_tcgen05_kernel");
+  attn_cache_join_kernel<T, RP><<<dim3(ctas, a.max_q * a.group), 512, 0, st>>>(da, ctas);
+  FG_CHECK_LAUNCH("attn_cache_join_kernel");
   return FG_OK;
 }
 
@@ -596,6 +805,12 @@ int launch_kind(DecodeArgs& da, int kind, cudaStream_t st) {
 }
 
 }  // namespace
+
+// Bytes of workspace for `rows` query rows of a sequence and KV head: a head and a tail part, and a record, for each CTA.
+int64_t attn_cache_decode_sm100_bytes(int64_t rows, int sms) {
+  const int64_t rp = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+  return 2 * (int64_t)sms * (2 * rp * (HD + 1) * 4 + (int64_t)sizeof(PartRecord));
+}
 
 int attn_cache_decode_sm100(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st) {
   DecodeArgs da;

@@ -286,78 +286,65 @@ int launch_gather(const GatherArgs& a, bool vec, cudaStream_t st) {
 }  // namespace
 }  // namespace fg
 
-extern "C" int fg_reshape_and_cache_flash_fp8(const void* key, const void* value, void* key_cache, void* value_cache,
-                                              const int64_t* slot_mapping, const float* k_scale, const float* v_scale,
-                                              int64_t k_scale_stride, int64_t v_scale_stride, int64_t num_tokens,
-                                              int64_t num_heads, int64_t head_size, int64_t block_size,
-                                              int64_t num_blocks, int64_t key_stride, int64_t value_stride,
-                                              int64_t cache_block_stride, int64_t cache_row_stride,
-                                              int64_t cache_head_stride, int dtype, int cache_dtype, void* stream) {
+extern "C" int fg_reshape_and_cache_flash_fp8(const fg_cache_write_params* p, void* stream) {
   using namespace fg;
   FG_REQUIRE_HEALTHY("reshape_and_cache_flash");
-  FG_REQUIRE(num_tokens >= 0 && num_heads >= 0 && head_size >= 0, "reshape_and_cache_flash: negative size");
-  FG_REQUIRE(block_size > 0 && num_blocks >= 0, "reshape_and_cache_flash: block_size must be positive");
-  FG_REQUIRE(is_fp8(cache_dtype), "reshape_and_cache_flash: cache dtype code %d is no 8-bit type", cache_dtype);
-  if (num_tokens == 0 || num_heads * head_size == 0) return FG_OK;
-  FG_REQUIRE(key && value && key_cache && value_cache && slot_mapping, "reshape_and_cache_flash: null pointer");
+  FG_REQUIRE(p != nullptr, "reshape_and_cache_flash: null params");
+  FG_REQUIRE(p->num_tokens >= 0 && p->num_heads >= 0 && p->head_size >= 0, "reshape_and_cache_flash: negative size");
+  FG_REQUIRE(p->block_size > 0 && p->num_blocks >= 0, "reshape_and_cache_flash: block_size must be positive");
+  FG_REQUIRE(is_fp8(p->cache_dtype), "reshape_and_cache_flash: cache dtype code %d is no 8-bit type", p->cache_dtype);
+  if (p->num_tokens == 0 || p->num_heads * p->head_size == 0) return FG_OK;
+  FG_REQUIRE(p->key && p->value && p->key_cache && p->value_cache && p->slot_mapping,
+             "reshape_and_cache_flash: null pointer");
   QuantArgs a;
-  a.key = (const char*)key; a.value = (const char*)value;
-  a.kc = (uint8_t*)key_cache; a.vc = (uint8_t*)value_cache;
-  a.slots = slot_mapping; a.k_scale = k_scale; a.v_scale = v_scale;
-  a.ksh = k_scale_stride; a.vsh = v_scale_stride;
-  a.T = num_tokens; a.H = num_heads; a.D = head_size; a.BS = block_size; a.NB = num_blocks;
-  a.ks = key_stride; a.vs = value_stride;
-  a.cbs = cache_block_stride; a.crs = cache_row_stride; a.chs = cache_head_stride;
-  const int es = dtype_size(dtype);
-  const bool vec = head_size % 16 == 0 && (key_stride * es) % 16 == 0 && (value_stride * es) % 16 == 0 &&
-                   cache_block_stride % 16 == 0 && cache_row_stride % 16 == 0 && cache_head_stride % 16 == 0 &&
-                   aligned16(key) && aligned16(value) && aligned16(key_cache) && aligned16(value_cache) &&
-                   num_tokens * num_heads * (head_size / 16) * 2 < 4000000000LL &&
-                   num_blocks * block_size < 4000000000LL;
+  a.key = (const char*)p->key; a.value = (const char*)p->value;
+  a.kc = (uint8_t*)p->key_cache; a.vc = (uint8_t*)p->value_cache;
+  a.slots = p->slot_mapping; a.k_scale = p->k_scale; a.v_scale = p->v_scale;
+  a.ksh = p->k_scale_stride; a.vsh = p->v_scale_stride;
+  a.T = p->num_tokens; a.H = p->num_heads; a.D = p->head_size; a.BS = p->block_size; a.NB = p->num_blocks;
+  a.ks = p->key_stride; a.vs = p->value_stride;
+  a.cbs = p->cache_block_stride; a.crs = p->cache_row_stride; a.chs = p->cache_head_stride;
+  const int es = dtype_size(p->dtype);
+  const bool vec = a.D % 16 == 0 && (a.ks * es) % 16 == 0 && (a.vs * es) % 16 == 0 && a.cbs % 16 == 0 && a.crs % 16 == 0 &&
+                   a.chs % 16 == 0 && aligned16(a.key) && aligned16(a.value) && aligned16(a.kc) && aligned16(a.vc) &&
+                   a.T * a.H * (a.D / 16) * 2 < 4000000000LL && a.NB * a.BS < 4000000000LL;
   cudaStream_t st = (cudaStream_t)stream;
-  FG_DISPATCH_FLOAT(dtype, T, {
-    return cache_dtype == FG_E4M3 ? launch_quant<T, kCacheE4M3>(a, vec, st) : launch_quant<T, kCacheE5M2>(a, vec, st);
+  FG_DISPATCH_FLOAT(p->dtype, T, {
+    return p->cache_dtype == FG_E4M3 ? launch_quant<T, kCacheE4M3>(a, vec, st) : launch_quant<T, kCacheE5M2>(a, vec, st);
   });
   return FG_OK;
 }
 
-extern "C" int fg_gather_cache_flash(const void* key_cache, const void* value_cache, void* key, void* value,
-                                     const int32_t* block_table, const int32_t* cu_seqlens, const int32_t* seq_starts,
-                                     const float* k_scale, const float* v_scale, int64_t k_scale_stride,
-                                     int64_t v_scale_stride, int64_t num_rows, int64_t batch, int64_t num_heads,
-                                     int64_t head_size, int64_t block_size, int64_t num_blocks,
-                                     int64_t block_table_stride, int64_t block_table_cols, int64_t key_stride,
-                                     int64_t value_stride, int64_t cache_block_stride, int64_t cache_row_stride,
-                                     int64_t cache_head_stride, int dtype, int cache_dtype, void* stream) {
+extern "C" int fg_gather_cache_flash(const fg_cache_gather_params* p, void* stream) {
   using namespace fg;
   FG_REQUIRE_HEALTHY("gather_cache_flash");
-  FG_REQUIRE(num_rows >= 0 && batch >= 0 && num_heads >= 0 && head_size >= 0, "gather_cache_flash: negative size");
-  FG_REQUIRE(is_fp8(cache_dtype) || cache_dtype == dtype,
+  FG_REQUIRE(p != nullptr, "gather_cache_flash: null params");
+  FG_REQUIRE(p->num_rows >= 0 && p->batch >= 0 && p->num_heads >= 0 && p->head_size >= 0,
+             "gather_cache_flash: negative size");
+  FG_REQUIRE(is_fp8(p->cache_dtype) || p->cache_dtype == p->dtype,
              "gather_cache_flash: a cache that is not 8-bit must hold the type of the output");
-  if (num_rows == 0 || batch == 0 || num_heads * head_size == 0) return FG_OK;
-  FG_REQUIRE(block_size > 0 && num_blocks > 0, "gather_cache_flash: empty cache");
-  FG_REQUIRE(block_table_cols > 0, "gather_cache_flash: block_table has no columns");
-  FG_REQUIRE(key && value && key_cache && value_cache && block_table && cu_seqlens, "gather_cache_flash: null pointer");
+  if (p->num_rows == 0 || p->batch == 0 || p->num_heads * p->head_size == 0) return FG_OK;
+  FG_REQUIRE(p->block_size > 0 && p->num_blocks > 0, "gather_cache_flash: empty cache");
+  FG_REQUIRE(p->block_table_cols > 0, "gather_cache_flash: block_table has no columns");
+  FG_REQUIRE(p->key && p->value && p->key_cache && p->value_cache && p->block_table && p->cu_seqlens,
+             "gather_cache_flash: null pointer");
   GatherArgs a;
-  a.kc = (const uint8_t*)key_cache; a.vc = (const uint8_t*)value_cache;
-  a.key = (char*)key; a.value = (char*)value;
-  a.table = block_table; a.cu = cu_seqlens; a.starts = seq_starts;
-  a.k_scale = k_scale; a.v_scale = v_scale; a.ksh = k_scale_stride; a.vsh = v_scale_stride;
-  a.rows = num_rows; a.H = num_heads; a.D = head_size; a.BS = block_size; a.NB = num_blocks; a.B = batch;
-  a.table_stride = block_table_stride; a.table_cols = block_table_cols;
-  a.ks = key_stride; a.vs = value_stride;
-  a.cbs = cache_block_stride; a.crs = cache_row_stride; a.chs = cache_head_stride;
-  const int es = dtype_size(dtype), ec = is_fp8(cache_dtype) ? 1 : es;
-  const int pe = 16 / ec;
-  const bool vec = head_size % pe == 0 && (key_stride * es) % 16 == 0 && (value_stride * es) % 16 == 0 &&
-                   (cache_block_stride * ec) % 16 == 0 && (cache_row_stride * ec) % 16 == 0 &&
-                   (cache_head_stride * ec) % 16 == 0 && aligned16(key) && aligned16(value) && aligned16(key_cache) &&
-                   aligned16(value_cache) && num_heads * head_size < 100000000LL &&
-                   num_rows < 2147483647LL * kGatherRows;
+  a.kc = (const uint8_t*)p->key_cache; a.vc = (const uint8_t*)p->value_cache;
+  a.key = (char*)p->key; a.value = (char*)p->value;
+  a.table = p->block_table; a.cu = p->cu_seqlens; a.starts = p->seq_starts;
+  a.k_scale = p->k_scale; a.v_scale = p->v_scale; a.ksh = p->k_scale_stride; a.vsh = p->v_scale_stride;
+  a.rows = p->num_rows; a.H = p->num_heads; a.D = p->head_size; a.BS = p->block_size; a.NB = p->num_blocks; a.B = p->batch;
+  a.table_stride = p->block_table_stride; a.table_cols = p->block_table_cols;
+  a.ks = p->key_stride; a.vs = p->value_stride;
+  a.cbs = p->cache_block_stride; a.crs = p->cache_row_stride; a.chs = p->cache_head_stride;
+  const int es = dtype_size(p->dtype), ec = is_fp8(p->cache_dtype) ? 1 : es;
+  const bool vec = a.D % (16 / ec) == 0 && (a.ks * es) % 16 == 0 && (a.vs * es) % 16 == 0 && (a.cbs * ec) % 16 == 0 &&
+                   (a.crs * ec) % 16 == 0 && (a.chs * ec) % 16 == 0 && aligned16(a.key) && aligned16(a.value) &&
+                   aligned16(a.kc) && aligned16(a.vc) && a.H * a.D < 100000000LL && a.rows < 2147483647LL * kGatherRows;
   cudaStream_t st = (cudaStream_t)stream;
-  FG_DISPATCH_FLOAT(dtype, T, {
-    if (cache_dtype == FG_E4M3) return launch_gather<T, kCacheE4M3>(a, vec, st);
-    if (cache_dtype == FG_E5M2) return launch_gather<T, kCacheE5M2>(a, vec, st);
+  FG_DISPATCH_FLOAT(p->dtype, T, {
+    if (p->cache_dtype == FG_E4M3) return launch_gather<T, kCacheE4M3>(a, vec, st);
+    if (p->cache_dtype == FG_E5M2) return launch_gather<T, kCacheE5M2>(a, vec, st);
     return launch_gather<T, kCache16>(a, vec, st);
   });
   return FG_OK;

@@ -244,7 +244,7 @@ _FP8_NAMES = {"fp8": torch.float8_e4m3fn, "fp8_e4m3": torch.float8_e4m3fn, "fp8_
 def _head_scale(what, scale, num_heads, dev):
     """``(pointer, elements between heads)`` of a K or V scale: None, one element, or one for each head."""
     if scale is None:
-        return None, 0
+        return 0, 0
     if scale.dtype != torch.float32:
         raise RuntimeError(f"{what} must be float32, got {scale.dtype}")
     if scale.device != dev:
@@ -258,52 +258,50 @@ def _head_scale(what, scale, num_heads, dev):
 
 
 def _check_cache_pair(op, key_cache, value_cache, kv_cache_dtype):
-    """Shapes and strides of a pair of 4-D caches; with an 8-bit ``kv_cache_dtype`` also their dtype."""
-    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape:
+    """Shape, strides and (with an 8-bit ``kv_cache_dtype``) element type of a pair of 4-D caches."""
+    shape, strides, dtype = key_cache.shape, key_cache.stride(), key_cache.dtype
+    if len(shape) != 4 or shape != value_cache.shape:
         raise RuntimeError(f"{op}: the caches must be two [num_blocks, block_size, num_heads, head_size] tensors")
-    if key_cache.stride() != value_cache.stride():
+    if strides != value_cache.stride():
         raise RuntimeError(f"{op}: key_cache and value_cache must have equal strides")
-    if key_cache.stride(3) != 1:
+    if strides[3] != 1:
         raise RuntimeError(f"{op}: head_size must be the unit-stride dimension")
-    if key_cache.dtype != value_cache.dtype:
+    if dtype != value_cache.dtype:
         raise RuntimeError(f"{op}: the caches must share a dtype")
     want = _FP8_NAMES.get(kv_cache_dtype)
-    if want is not None and key_cache.dtype not in (want, torch.uint8):
-        raise RuntimeError(f"{op}: kv_cache_dtype {kv_cache_dtype!r} needs caches of {want} or uint8, "
-                           f"got {key_cache.dtype}")
-    return want
+    if want is not None and dtype != want and dtype != torch.uint8:
+        raise RuntimeError(f"{op}: kv_cache_dtype {kv_cache_dtype!r} needs caches of {want} or uint8, got {dtype}")
+    return shape, strides, want
 
 
 def _check_rows(op, key, value, num_heads, head_size):
-    if key.dim() != 3 or key.shape != value.shape or key.dtype != value.dtype:
+    """Token strides of key and value rows that fit caches of ``num_heads`` heads."""
+    shape, ks, vs = key.shape, key.stride(), value.stride()
+    if len(shape) != 3 or shape != value.shape or key.dtype != value.dtype:
         raise RuntimeError(f"{op}: key and value must be two [num_tokens, num_heads, head_size] tensors of one dtype")
-    if key.shape[1] != num_heads or key.shape[2] != head_size:
-        raise RuntimeError(f"{op}: key and value of shape {tuple(key.shape)} do not fit caches of {num_heads} heads of "
-                           f"{head_size}")
-    for t in (key, value):
-        st = t.stride()
-        if st[2] != 1 and head_size > 1 or st[1] != head_size and num_heads > 1:
-            raise RuntimeError(f"{op}: key/value heads must be densely packed per token")
+    if shape[1] != num_heads or shape[2] != head_size:
+        raise RuntimeError(f"{op}: key and value of shape {tuple(shape)} do not fit caches of {num_heads} heads of {head_size}")
+    if (ks[2] != 1 or vs[2] != 1) and head_size > 1 or (ks[1] != head_size or vs[1] != head_size) and num_heads > 1:
+        raise RuntimeError(f"{op}: key/value heads must be densely packed per token")
+    return shape[0], ks[0], vs[0]
 
 
 def _write_fp8(key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale):
     op = "reshape_and_cache_flash"
     dev = _lib.require_cuda(key, value, key_cache, value_cache, slot_mapping)
-    want = _check_cache_pair(op, key_cache, value_cache, kv_cache_dtype)
-    num_blocks, block_size, num_heads, head_size = key_cache.shape
-    _check_rows(op, key, value, num_heads, head_size)
-    if slot_mapping.dim() != 1 or slot_mapping.shape[0] > key.shape[0]:
+    (num_blocks, block_size, num_heads, head_size), cst, want = _check_cache_pair(op, key_cache, value_cache, kv_cache_dtype)
+    rows, kst, vst = _check_rows(op, key, value, num_heads, head_size)
+    tokens = slot_mapping.numel()
+    if slot_mapping.dim() != 1 or tokens > rows:
         raise RuntimeError(f"{op}: slot_mapping must have one dimension and no more entries than key has tokens")
     ks, ksh = _head_scale("k_scale", k_scale, num_heads, dev)
     vs, vsh = _head_scale("v_scale", v_scale, num_heads, dev)
-    if slot_mapping.dtype != torch.int64:
-        slot_mapping = slot_mapping.to(torch.int64)
-    slot_mapping = slot_mapping.contiguous()
-    cst = key_cache.stride()
-    _lib.call(dev, _lib.load().fg_reshape_and_cache_flash_fp8,
-              key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(),
-              ks, vs, ksh, vsh, slot_mapping.shape[0], num_heads, head_size, block_size, num_blocks,
-              key.stride(0), value.stride(0), cst[0], cst[1], cst[2], _lib.dtype_code(key.dtype), _lib.FP8_CODE[want])
+    if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.to(torch.int64).contiguous()
+    _lib.call(dev, _lib.load().fg_reshape_and_cache_flash_fp8, _lib.CACHE_WRITE.pack(
+        key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(), ks, vs,
+        ksh, vsh, tokens, num_heads, head_size, block_size, num_blocks, kst, vst, cst[0], cst[1], cst[2],
+        _lib.dtype_code(key.dtype), _lib.FP8_CODE[want]))
     return None
 
 
@@ -333,28 +331,29 @@ def gather_cache_flash(
     dev = _lib.require_cuda(key_cache, value_cache, key, value, block_table, cu_seqlens, seq_starts)
     if kv_cache_dtype != "auto" and kv_cache_dtype not in _FP8_NAMES:
         raise RuntimeError(f"{op}: unknown kv_cache_dtype {kv_cache_dtype!r}")
-    want = _check_cache_pair(op, key_cache, value_cache, kv_cache_dtype)
-    num_blocks, block_size, num_heads, head_size = key_cache.shape
-    _check_rows(op, key, value, num_heads, head_size)
+    (num_blocks, block_size, num_heads, head_size), cst, want = _check_cache_pair(op, key_cache, value_cache, kv_cache_dtype)
+    rows, kst, vst = _check_rows(op, key, value, num_heads, head_size)
     if want is None and key.dtype != key_cache.dtype:
         raise RuntimeError(f"{op}: key/value and the caches must share a dtype")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+    table, tst = block_table.shape, block_table.stride()
+    if len(table) != 2 or block_table.dtype != torch.int32 or tst[1] != 1:
         raise RuntimeError(f"{op}: block_table must be int32 [batch, max_blocks] with unit column stride")
-    batch = block_table.shape[0]
+    batch = table[0]
     for name, t, n in (("cu_seqlens", cu_seqlens, batch + 1), ("seq_starts", seq_starts, batch)):
         if t is not None and (t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous()):
             raise RuntimeError(f"{op}: {name} must be int32 of shape ({n},) and contiguous")
-    if key.shape[0] > 1 and (key.stride(0) < num_heads * head_size or value.stride(0) < num_heads * head_size):
+    if rows > 1 and (kst < num_heads * head_size or vst < num_heads * head_size):
         raise RuntimeError(f"{op}: key/value must not have internal overlap")
-    ks, ksh = _head_scale("k_scale", k_scale if want else None, num_heads, dev)
-    vs, vsh = _head_scale("v_scale", v_scale if want else None, num_heads, dev)
-    cst = key_cache.stride()
     code = _lib.dtype_code(key.dtype)
-    _lib.call(dev, _lib.load().fg_gather_cache_flash,
-              key_cache.data_ptr(), value_cache.data_ptr(), key.data_ptr(), value.data_ptr(), block_table.data_ptr(),
-              cu_seqlens.data_ptr(), _lib.ptr(seq_starts), ks, vs, ksh, vsh, key.shape[0], batch, num_heads, head_size,
-              block_size, num_blocks, block_table.stride(0), block_table.shape[1], key.stride(0), value.stride(0),
-              cst[0], cst[1], cst[2], code, _lib.FP8_CODE[want] if want else code)
+    ks = ksh = vs = vsh = 0
+    if want is not None:
+        ks, ksh = _head_scale("k_scale", k_scale, num_heads, dev)
+        vs, vsh = _head_scale("v_scale", v_scale, num_heads, dev)
+    _lib.call(dev, _lib.load().fg_gather_cache_flash, _lib.CACHE_GATHER.pack(
+        key_cache.data_ptr(), value_cache.data_ptr(), key.data_ptr(), value.data_ptr(), block_table.data_ptr(),
+        cu_seqlens.data_ptr(), 0 if seq_starts is None else seq_starts.data_ptr(), ks, vs, ksh, vsh, rows, batch, num_heads,
+        head_size, block_size, num_blocks, tst[0], table[1], kst, vst, cst[0], cst[1], cst[2], code,
+        code if want is None else _lib.FP8_CODE[want]))
     return key, value
 
 

@@ -442,7 +442,7 @@ def flash_attn_varlen_func(
 def _descale(what, scale, batch, heads, dev):
     """``(pointer, batch stride, head stride)`` of a K or V scale."""
     if scale is None:
-        return None, 0, 0
+        return 0, 0, 0
     if scale.dtype != torch.float32:
         raise RuntimeError(f"flash_attn_varlen_func: {what} must be float32, got {scale.dtype}")
     if scale.device != dev:
@@ -467,73 +467,63 @@ def _flash_attn_cache(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seql
     if q.stride(-1) != 1:
         q = q.contiguous()
     max_seqlen_q, max_seqlen_k = int(max_seqlen_q), int(max_seqlen_k)
-    fp8 = _lib.FP8_CODE.get(k.dtype)
-    assert q.dtype in (torch.float16, torch.bfloat16), "FlashAttention only support fp16 and bf16 data type"
-    assert k.dtype == v.dtype and (fp8 is not None or k.dtype == q.dtype)
+    dtype, cache_dtype, shape = q.dtype, k.dtype, k.shape
+    fp8 = _lib.FP8_CODE.get(cache_dtype)
+    assert dtype in (torch.float16, torch.bfloat16), "FlashAttention only support fp16 and bf16 data type"
+    assert cache_dtype == v.dtype and (fp8 is not None or cache_dtype == dtype)
     assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous()
     total_q, num_heads, head_size = q.shape
     batch = cu_seqlens_q.numel() - 1
     paged = block_table is not None
-    assert k.shape == v.shape and k.stride() == v.stride() and k.dim() == (4 if paged else 3)
     kst = k.stride()
-    num_heads_k = k.shape[-2]
-    assert k.shape[-1] == head_size and kst[-1] == 1
+    assert shape == v.shape and kst == v.stride() and len(shape) == (4 if paged else 3)
+    num_heads_k = shape[-2]
+    assert shape[-1] == head_size and kst[-1] == 1
     assert head_size <= 256, "FlashAttention forward only supports head dimension at most 256"
     assert head_size % 8 == 0, "head_size must be a multiple of 8, this is ensured by padding!"
     assert num_heads % num_heads_k == 0, "Number of heads in key/value must divide number of heads in query"
+    used = cu_k = table = table_stride = table_cols = num_blocks = block_size = total_k = block_stride = 0
     if seqused_k is not None:
         assert seqused_k.dtype == torch.int32 and seqused_k.is_contiguous() and seqused_k.shape == (batch,)
+        used = seqused_k.data_ptr()
     if out is None:
         out = torch.empty_like(q)
     else:
-        assert out.stride(-1) == 1 and out.dtype == q.dtype and out.shape == q.shape
+        assert out.stride(-1) == 1 and out.dtype == dtype and out.shape == q.shape
     lse = torch.empty((num_heads, total_q), dtype=torch.float32, device=dev) if return_softmax_lse else None
-
-    p = _lib.AttnCacheParams()
-    b = p.base
-    b.q, b.k, b.v, b.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    if lse is not None:
-        b.lse = lse.data_ptr()
-    b.cu_seqlens_q = cu_seqlens_q.data_ptr()
-    if seqused_k is not None:
-        b.seqused_k = seqused_k.data_ptr()
-    b.q_row_stride, b.q_head_stride, _ = q.stride()
-    b.o_row_stride, b.o_head_stride, _ = out.stride()
     if paged:
         assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
         assert block_table.shape[0] == batch
-        b.block_table, b.block_table_stride = block_table.data_ptr(), block_table.stride(0)
-        p.block_table_cols = block_table.shape[1]
-        b.num_blocks, b.block_size = k.shape[0], k.shape[1]
-        b.k_block_stride, b.k_row_stride, b.k_head_stride, _ = kst
-        b.v_block_stride, b.v_row_stride, b.v_head_stride, _ = kst
+        table, table_stride, table_cols = block_table.data_ptr(), block_table.stride(0), block_table.shape[1]
+        num_blocks, block_size = shape[0], shape[1]
+        block_stride, row_stride, head_stride, _ = kst
     else:
         assert cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.is_contiguous() and cu_seqlens_k.shape == (batch + 1,)
-        b.cu_seqlens_k, b.total_k = cu_seqlens_k.data_ptr(), k.shape[0]
-        b.k_row_stride, b.k_head_stride, _ = kst
-        b.v_row_stride, b.v_head_stride, _ = kst
-    b.total_q, b.batch, b.num_heads, b.num_heads_k, b.head_dim = total_q, batch, num_heads, num_heads_k, head_size
-    b.max_seqlen_q, b.max_seqlen_k = max_seqlen_q, max_seqlen_k
-    b.window_left, b.window_right = window
-    b.softmax_scale, b.softcap = softmax_scale, softcap
-    b.causal = 1 if causal else 0
-    b.dtype = _lib.dtype_code(q.dtype)
-    p.sink_tokens = sink_tokens
-    if fp8 is None:
-        p.cache_dtype = b.dtype
-    else:
-        p.cache_dtype = fp8
-        p.k_scale, p.k_scale_batch_stride, p.k_scale_head_stride = _descale("k_descale", k_descale, batch, num_heads_k, dev)
-        p.v_scale, p.v_scale_batch_stride, p.v_scale_head_stride = _descale("v_descale", v_descale, batch, num_heads_k, dev)
+        cu_k, total_k = cu_seqlens_k.data_ptr(), shape[0]
+        row_stride, head_stride, _ = kst
+    ks = ksb = ksh = vs = vsb = vsh = 0
+    code = _lib.dtype_code(dtype)
+    if fp8 is not None:
+        ks, ksb, ksh = _descale("k_descale", k_descale, batch, num_heads_k, dev)
+        vs, vsb, vsh = _descale("v_descale", v_descale, batch, num_heads_k, dev)
+    qst, ost = q.stride(), out.stride()
+    # before and behind the workspace, in the order of AttnCacheParams
+    head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            cu_seqlens_q.data_ptr(), cu_k, used, table, 0)
+    tail = (qst[0], qst[1], row_stride, head_stride, block_stride, row_stride, head_stride, block_stride, ost[0], ost[1],
+            table_stride, 0, total_q, batch, num_heads, num_heads_k, head_size, max_seqlen_q, max_seqlen_k, block_size,
+            num_blocks, window[0], window[1], total_k, 0, 0, 0, 0, softmax_scale, softcap, 1 if causal else 0, code, 0, 0,
+            ks, vs, ksb, ksh, vsb, vsh, sink_tokens, table_cols, code if fp8 is None else fp8, 0)
     lib = _lib.load()
-    ref = C.byref(p)
+    pack = _lib.ATTN_CACHE.pack
     with _lib.on_device(dev):
-        nbytes = lib.fg_flash_attn_cache_workspace_bytes(ref)
+        params = pack(*head, 0, 0, *tail)
+        nbytes = lib.fg_flash_attn_cache_workspace_bytes(params)
         if nbytes > 0:
             # a buffer of the call's own: the allocator keeps it from other streams, and a captured graph keeps its own
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            b.workspace, b.workspace_bytes = ws.data_ptr(), nbytes
-        _lib.check(lib.fg_flash_attn_cache(ref, _lib.stream_ptr(dev)))
+            params = pack(*head, ws.data_ptr(), nbytes, *tail)
+        _lib.call(dev, lib.fg_flash_attn_cache, params)
     return (out, lse) if return_softmax_lse else out
 
 

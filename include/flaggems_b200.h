@@ -383,21 +383,40 @@ FG_API int64_t fg_flash_attn_decode_static_capacity(void);
  * cu_seqlens[batch]) are left as they were.  Page numbers are clamped into the cache, positions into the
  * block_table_cols pages of a table row.
  * ---------------------------------------------------------------------- */
-FG_API int fg_reshape_and_cache_flash_fp8(const void* key, const void* value, void* key_cache, void* value_cache,
-                                          const int64_t* slot_mapping, const float* k_scale, const float* v_scale,
-                                          int64_t k_scale_stride, int64_t v_scale_stride, int64_t num_tokens,
-                                          int64_t num_heads, int64_t head_size, int64_t block_size,
-                                          int64_t num_blocks, int64_t key_stride, int64_t value_stride,
-                                          int64_t cache_block_stride, int64_t cache_row_stride,
-                                          int64_t cache_head_stride, int dtype, int cache_dtype, void* stream);
-FG_API int fg_gather_cache_flash(const void* key_cache, const void* value_cache, void* key, void* value,
-                                 const int32_t* block_table, const int32_t* cu_seqlens, const int32_t* seq_starts,
-                                 const float* k_scale, const float* v_scale, int64_t k_scale_stride,
-                                 int64_t v_scale_stride, int64_t num_rows, int64_t batch, int64_t num_heads,
-                                 int64_t head_size, int64_t block_size, int64_t num_blocks,
-                                 int64_t block_table_stride, int64_t block_table_cols, int64_t key_stride,
-                                 int64_t value_stride, int64_t cache_block_stride, int64_t cache_row_stride,
-                                 int64_t cache_head_stride, int dtype, int cache_dtype, void* stream);
+typedef struct {
+  const void* key; /* [num_tokens, num_heads, head_size], dense heads */
+  const void* value;
+  void* key_cache; /* [num_blocks, block_size, num_heads, head_size] */
+  void* value_cache;
+  const int64_t* slot_mapping; /* [num_tokens] */
+  const float* k_scale;
+  const float* v_scale;
+  int64_t k_scale_stride, v_scale_stride;
+  int64_t num_tokens, num_heads, head_size, block_size, num_blocks;
+  int64_t key_stride, value_stride;
+  int64_t cache_block_stride, cache_row_stride, cache_head_stride;
+  int32_t dtype, cache_dtype;
+} fg_cache_write_params;
+FG_API int fg_reshape_and_cache_flash_fp8(const fg_cache_write_params* p, void* stream);
+
+typedef struct {
+  const void* key_cache;
+  const void* value_cache;
+  void* key; /* [num_rows, num_heads, head_size], dense heads */
+  void* value;
+  const int32_t* block_table; /* [batch, block_table_cols] */
+  const int32_t* cu_seqlens;  /* [batch + 1] */
+  const int32_t* seq_starts;  /* [batch] or NULL */
+  const float* k_scale;
+  const float* v_scale;
+  int64_t k_scale_stride, v_scale_stride;
+  int64_t num_rows, batch, num_heads, head_size, block_size, num_blocks;
+  int64_t block_table_stride, block_table_cols;
+  int64_t key_stride, value_stride;
+  int64_t cache_block_stride, cache_row_stride, cache_head_stride;
+  int32_t dtype, cache_dtype;
+} fg_cache_gather_params;
+FG_API int fg_gather_cache_flash(const fg_cache_gather_params* p, void* stream);
 
 /* ------------------------------------------------------------------------
  * flash_attn_cache: flash_attn_varlen over an 8-bit cache, or with a sliding window whose sequences keep their first
@@ -429,8 +448,9 @@ typedef struct {
 } fg_attn_cache_params;
 FG_API int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream);
 FG_API int64_t fg_flash_attn_cache_workspace_bytes(const fg_attn_cache_params* p);
-/* Which kernel family fg_flash_attn_cache picks: 0 general (mma.sync), 1 tcgen05 (head dim 128), 2 TMA-fed
- * kernel for at most 16 query rows per sequence and KV head.  Pure host logic. */
+/* Which kernel family fg_flash_attn_cache picks: 0 general (mma.sync), 1 tcgen05 (head dim 128); for at most
+ * 16 query rows per sequence and KV head 2 TMA-fed (mma.sync), 3 tcgen05 (head dim 128, with a workspace).  Pure host
+ * logic. */
 FG_API int fg_flash_attn_cache_path(const fg_attn_cache_params* p);
 
 /* ------------------------------------------------------------------------

@@ -1,6 +1,8 @@
 """Host side of the 8-bit and windowed cache: structure layout, refusals before any CUDA call, path and workspace rules,
 and a restatement of the tile runs that the attention kernels walk."""
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -26,8 +28,20 @@ def params(**kw):
     return p
 
 
-def test_struct_size():
+def test_parameter_blocks():
+    """The packed blocks have the header's layout: every field of the attention block lands where the Structure has it."""
     assert ctypes.sizeof(_lib.AttnCacheParams) == ctypes.sizeof(_lib.AttnParams) + 2 * 8 + 6 * 8 + 2 * 4
+    assert _lib.ATTN_CACHE.size == ctypes.sizeof(_lib.AttnCacheParams)
+    values = [i + 1 for i in range(40)] + [0.5, 0.25] + list(range(43, 47)) + list(range(47, 57))
+    p = _lib.AttnCacheParams.from_buffer_copy(_lib.ATTN_CACHE.pack(*values))
+    got = [getattr(p.base, n) for n, _ in _lib.AttnParams._fields_] + [getattr(p, n) for n, _ in p._fields_[1:]]
+    assert got == values
+    for fmt, name in ((_lib.CACHE_WRITE, "fg_cache_write_params"), (_lib.CACHE_GATHER, "fg_cache_gather_params")):
+        header = (Path(__file__).resolve().parent.parent / "include" / "flaggems_b200.h").read_text()
+        body = re.search(r"typedef struct \{([^}]*)\} " + name, header).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        kinds = [("Q" if "*" in d else "i" if "int32_t" in d else "q") * (d.count(",") + 1) for d in body.split(";") if d.strip()]
+        assert "".join(kinds) == "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([Qqi])", fmt.format))
 
 
 @pytest.mark.parametrize("match, kw", [
@@ -55,9 +69,9 @@ def test_nothing_to_do_is_no_call():
 
 def test_small_workspace_is_refused():
     lib = _lib.load()
-    p = params(max_seqlen_k=60000, batch=1, total_q=1)
+    p = params(max_seqlen_k=60000, batch=1, total_q=1, head_dim=64)
     need = lib.fg_flash_attn_cache_workspace_bytes(ctypes.byref(p))
-    assert need > 0 and need % (8 * 129 * 4) == 0
+    assert need > 0 and need % (8 * 65 * 4) == 0
     p.base.workspace, p.base.workspace_bytes = 0x10000, need - 4
     with pytest.raises(RuntimeError, match="workspace of"):
         _lib.check(lib.fg_flash_attn_cache(ctypes.byref(p), None))
@@ -69,8 +83,20 @@ def test_small_workspace_is_refused():
 def test_workspace_goes_by_what_is_visible():
     """A window bounds the keys that are split, however long the context."""
     need = lambda **kw: _lib.load().fg_flash_attn_cache_workspace_bytes(ctypes.byref(params(**kw)))
-    long, windowed = need(max_seqlen_k=10 ** 6), need(max_seqlen_k=10 ** 6, window_left=1023, sink_tokens=4)
-    assert 0 < windowed < long and windowed == need(max_seqlen_k=10 ** 5, window_left=1023, sink_tokens=4)
+    for size in (dict(head_dim=64), dict(head_dim=256, max_seqlen_q=30, total_q=100), dict(max_seqlen_q=30, total_q=100)):
+        long, windowed = need(max_seqlen_k=10 ** 6, **size), need(max_seqlen_k=10 ** 6, window_left=2047, sink_tokens=4, **size)
+        assert 0 < windowed < long and windowed == need(max_seqlen_k=10 ** 5, window_left=2047, sink_tokens=4, **size)
+    assert need(max_seqlen_k=10 ** 6) == need(max_seqlen_k=10)        # head parts and tail parts of a fixed number of CTAs
+
+
+def test_path_by_sizes():
+    path = lambda **kw: _lib.load().fg_flash_attn_cache_path(ctypes.byref(params(**kw)))
+    assert path() == 3 and path(max_seqlen_q=4, total_q=16) == 3      # 4 tokens of a group of 4: 16 rows
+    assert path(max_seqlen_q=5, total_q=20) == 1 and path(max_seqlen_q=3000, total_q=9000) == 1
+    assert path(head_dim=64) == 2 and path(softcap=5.0) == 2 and path(head_dim=64, max_seqlen_q=5, total_q=20) == 0
+    assert path(block_size=24) == 0 and path(block_size=4) == 0 and path(k_row_stride=264) == 0   # pages or strides TMA cannot take
+    assert path(cache_dtype=_lib.FG_BF16, k_row_stride=264, sink_tokens=1, window_left=7) == 3    # 528 bytes are fine
+    assert path(num_heads=400, num_heads_k=2) == 0                    # a group of 200
 
 
 @pytest.mark.parametrize("match, kw", [("no 8-bit", dict(cache_dtype=_lib.FG_F16)), ("negative", dict(num_tokens=-1)),
@@ -81,8 +107,9 @@ def test_write_refuses_on_the_host(match, kw):
              heads=2, dim=64, block_size=16, blocks=4, kst=128, vst=128, cb=2048, cr=128, ch=64, dtype=_lib.FG_BF16,
              cache_dtype=_lib.FG_E4M3)
     a.update(kw)
+    a = [0 if v is None else v for v in a.values()]
     with pytest.raises(RuntimeError, match=match):
-        _lib.check(_lib.load().fg_reshape_and_cache_flash_fp8(*a.values(), None))
+        _lib.check(_lib.load().fg_reshape_and_cache_flash_fp8(_lib.CACHE_WRITE.pack(*a), None))
 
 
 @pytest.mark.parametrize("match, kw", [("hold the type", dict(cache_dtype=_lib.FG_F16)), ("negative", dict(rows=-1)),
@@ -93,8 +120,9 @@ def test_gather_refuses_on_the_host(match, kw):
              vsh=0, rows=2, batch=1, heads=2, dim=64, block_size=16, blocks=4, tst=4, cols=4, kst=128, vst=128, cb=2048, cr=128,
              ch=64, dtype=_lib.FG_BF16, cache_dtype=_lib.FG_E4M3)
     a.update(kw)
+    a = [0 if v is None else v for v in a.values()]
     with pytest.raises(RuntimeError, match=match):
-        _lib.check(_lib.load().fg_gather_cache_flash(*a.values(), None))
+        _lib.check(_lib.load().fg_gather_cache_flash(_lib.CACHE_GATHER.pack(*a), None))
 
 
 def test_cpu_tensors_are_refused():
@@ -131,7 +159,7 @@ def test_tile_runs_cover_what_is_visible_once(bn):
                         seen = {j // bn for p in range(first, last + 1) for j in range(k_len)
                                 if (wr < 0 or j <= p + wr) and (wl < 0 or j >= p - wl or j < sinks)}
                         assert seen <= set(tiles)
-                        if wl >= 0:
+                        if wl >= 0:   # no tile outside the window's and the first tokens' own runs
                             assert all(t * bn < sinks or t >= max(0, first - wl) // bn for t in tiles)
 
 
