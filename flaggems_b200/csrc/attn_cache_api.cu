@@ -58,7 +58,8 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
   Plan plan;
   const int64_t group = b.num_heads / b.num_heads_k;
   const bool tma = tma_ready(p);
-  if (b.max_seqlen_q * group <= 16 && tma && b.head_dim == 128 && b.softcap == 0.0 && workspace) {
+  if (b.max_seqlen_q * group <= 16 && tma && b.head_dim == 128 && b.softcap == 0.0 && workspace &&
+      b.batch * b.num_heads_k * (b.max_seqlen_k / 128 + 1) <= 2147483647LL) {
     plan.path = kPathDecodeSm100;      // cuts the keys itself, on the device
     plan.splits = plan.tiles_per_split = 1;
     plan.bytes = attn_cache_decode_sm100_bytes(b.max_seqlen_q * group, sms);
@@ -214,8 +215,6 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   cudaStream_t st = (cudaStream_t)stream;
   FG_REQUIRE((b.max_seqlen_q * a.group + 63) / 64 * plan.splits <= 2147483647LL, "flash_attn_cache: too many row tiles");
   FG_REQUIRE(b.total_q * b.num_heads <= 2147483647LL * 4, "flash_attn_cache: too many rows");
-  FG_REQUIRE(b.batch * b.num_heads_k <= 2147483647LL && b.batch * b.num_heads_k * (b.max_seqlen_k / 128 + 1) <= (1ll << 37),
-             "flash_attn_cache: too many sequences and heads");
   const int rc = plan.path == kPathDecodeSm100 ? attn_cache_decode_sm100(c, b.dtype, kind, st)
                  : plan.path == kPathDecode    ? attn_cache_decode(c, b.dtype, kind, st)
                  : plan.path == kPathChunk     ? attn_cache_chunk(c, b.dtype, kind, st)

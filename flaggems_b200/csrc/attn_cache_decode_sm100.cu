@@ -20,8 +20,11 @@
 // The running maximum is shared by the CTA and raised only when a score exceeds it by more than 4 (log2 units); the warps
 // agree on that with one barrier reduction a tile.  Only a raise needs the exact maximum and rescales O in TMEM.
 //
-//   warps 0-3   softmax and output        warp 4   TMA producer (K and V tiles of 128 keys alternate in one ring)
-//   warp 5      issues the products: scores of the next tile before P V of the current one
+//   warps 0-3   softmax and output
+//   warps 4, 5  TMA producers of K and of V tiles (128 keys), each with a ring of its own.  A page of 16 keys is one box, and a
+//               warp issues one in about 95 clocks (lanes in turn; 125 when one lane issues them all): with one warp for both
+//               rings the issue bounded the kernel (256 sequences: 521 us by one lane, 412 us by eight)
+//   warp 6      issues the products: scores of the next tile before P V of the current one when its keys are there
 //
 // The kernel is persistent.  An item is one (sequence, KV head).  A team of CTAs walks the same sequences, each for a KV head of
 // its own, so that the heads' pieces of a cached row, which lie side by side in memory, are fetched at about the same time.
@@ -36,10 +39,12 @@
 namespace fg {
 namespace {
 
-constexpr int BN = 128, HD = 128, NUM_THREADS = 192;
-constexpr int TMA_WARP = 4, MMA_WARP = 5;
+constexpr int BN = 128, HD = 128, NUM_THREADS = 224;
+constexpr int TMA_WARP = 4, MMA_WARP = 6;
 constexpr float kRaise = 4.0f;               // log2 units
 constexpr float kPScale = 2048.0f;           // of P before it is split (8-bit caches)
+
+constexpr int kInfo = 32;                    // sequences of a run whose lengths are kept in shared memory
 
 constexpr int up(int n, int to) { return (n + to - 1) / to * to; }
 
@@ -55,20 +60,21 @@ struct Cfg {
   // whatever follows there; nothing uses those columns.
   static constexpr int QR = up(RP * PQ, 8), PR = up(RP * PP, 8);
   static constexpr int TILE = BN * HD * (k8 ? 1 : 2);         // bytes of a K or V tile
-  static constexpr int SLOTS = k8 && RP == 16 ? 5 : 6;
+  // One CTA an SM, or two where 128 registers a thread are enough; 192 KB of tiles on their way in either form.
+  static constexpr int CTAS = k8 && RP == 4 ? 2 : 1;
+  static constexpr int SLOTS = k8 ? 6 / CTAS : 3;             // tiles of each ring
   static constexpr int QB = QR * HD * (k8 ? 1 : 2);           // bytes of one Q buffer
   static constexpr int PB = PR * BN * (k8 ? 1 : 2);           // bytes of one P buffer
   static constexpr int SCOL = NS <= 32 ? 32 : 64;             // TMEM columns of one score buffer
   static constexpr int OCOL = 2 * SCOL;
   static constexpr int TCOLS = OCOL + NP <= 128 ? 128 : 256;
-  static constexpr int SMEM = SLOTS * TILE + 2 * QB + 2 * PB + 1024 + 1024;
-  static constexpr int CTAS = k8 ? 2 : 1;                     // per SM: 160 to 192 KB of tiles on their way in either form
+  static constexpr int SMEM = 2 * SLOTS * TILE + 2 * QB + 2 * PB + 1024 + 1024 + kInfo * 16;
 };
 
-// What a CTA leaves for the joining kernel: the item whose start it holds but not its end (or -1), and whether the item it
-// began in the middle of ends in it.
+// What a CTA leaves for the joining kernel: the item whose start it holds but not its end (or -1), in how many parts the item
+// is, and its first query token and rows.
 struct PartRecord {
-  int tail_item, head_ends;
+  int item, parts, q_begin, rows;
 };
 
 struct DecodeArgs {
@@ -77,7 +83,7 @@ struct DecodeArgs {
   float* part_o;        // [2 * CTAs][RP][128]: head part, tail part of each CTA
   float* part_lse;      // [2 * CTAs][RP]
   PartRecord* record;   // [CTAs]
-  int team;             // CTAs of a team: a divisor of the KV heads
+  int team, rounds;     // CTAs of a team, a divisor of the KV heads; KV heads of each member
 };
 
 // Fewest tiles that a run is worth starting a CTA for.
@@ -99,9 +105,14 @@ __device__ __forceinline__ int item_tiles(const CacheAttnArgs& c, const SeqInfo&
   span = tile_span<BN>(c, s.k_len, shift, (rows - 1) / c.a.group + shift);
   return max(span.n, 1);        // nothing visible: one tile, all of it masked, gives the zeros
 }
+// Lengths of the sequences [b0, b0 + n) as the CTA found them at its start; the others come from global memory.
+struct InfoTable {
+  const SeqInfo* info;
+  int b0, n;
+};
 template <int RP>
-__device__ __forceinline__ void fill_segment(const CacheAttnArgs& c, Segment& g, int lo) {
-  g.s = seq_info(c.a, g.b);
+__device__ __forceinline__ void fill_segment(const CacheAttnArgs& c, const InfoTable& table, Segment& g, int lo) {
+  g.s = (unsigned)(g.b - table.b0) < (unsigned)table.n ? table.info[g.b - table.b0] : seq_info(c.a, g.b);
   g.n = item_tiles<RP>(c, g.s, g.span);
   g.rows = min(g.s.q_len * c.a.group, RP);
   g.shift = g.s.k_len - g.s.q_len;
@@ -110,7 +121,8 @@ __device__ __forceinline__ void fill_segment(const CacheAttnArgs& c, Segment& g,
 }
 // The part after `g`; false when the run ends with g.
 template <int RP>
-__device__ __forceinline__ bool next_segment(const CacheAttnArgs& c, int team, const Segment& g, Segment& to) {
+__device__ __forceinline__ bool next_segment(const CacheAttnArgs& c, const InfoTable& table, int team, const Segment& g,
+                                             Segment& to) {
   to = g;
   to.left = g.left - (g.hi - g.lo);
   if (to.left <= 0) return false;
@@ -123,7 +135,7 @@ __device__ __forceinline__ bool next_segment(const CacheAttnArgs& c, int team, c
   to.hk -= c.a.Hk;
   do {
     if (++to.b >= c.a.batch) return false;
-    fill_segment<RP>(c, to, 0);
+    fill_segment<RP>(c, table, to, 0);
   } while (to.n == 0);
   return true;
 }
@@ -163,83 +175,43 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem + C::SLOTS * C::TILE;                        // [2 buffers]: items alternate
+  uint8_t* sK = smem;                                             // [KS]
+  uint8_t* sV = sK + C::SLOTS * C::TILE;                             // [VS]
+  uint8_t* sQ = sV + C::SLOTS * C::TILE;                             // [2 buffers]: items alternate
   uint8_t* sP = sQ + 2 * C::QB;                                   // [2 buffers]: tiles alternate
   uint8_t* rest = sP + 2 * C::PB;                                 // 1024 bytes
-  uint64_t* full = reinterpret_cast<uint64_t*>(rest);             // [SLOTS]
-  uint64_t* empty = full + C::SLOTS;
-  uint64_t* s_full = empty + C::SLOTS;   // [2] scores of a tile have landed
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(rest);           // [KS]
+  uint64_t* k_empty = k_full + C::SLOTS;
+  uint64_t* v_full = k_empty + C::SLOTS;    // [VS]
+  uint64_t* v_empty = v_full + C::SLOTS;
+  uint64_t* s_full = v_empty + C::SLOTS;    // [2] scores of a tile have landed
   uint64_t* s_free = s_full + 2;         // [2] ... and have been read into registers
   uint64_t* p_ready = s_free + 2;        // [2]
   uint64_t* o_done = p_ready + 2;        // [2] P V of even / odd tiles
   uint64_t* q_ready = o_done + 2;        // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* sMax = reinterpret_cast<float*>(rest + 256);               // [4 warps][16]
+  float* sMax = reinterpret_cast<float*>(rest + 256);             // [4 warps][16]
   float* sSum = sMax + 64;                                        // [4 warps][16]
   float* sDown = sSum + 64;                                       // [2 buffers][16]
+  SeqInfo* sInfo = reinterpret_cast<SeqInfo*>(rest + 1024);       // [kInfo]
 
   __shared__ int s_drain;
-  __shared__ int64_t s_sum[NUM_THREADS / 32], s_off;
-  __shared__ int s_b;
+  __shared__ int s_sum[NUM_THREADS / 32], s_off, s_b;
   // ---- this team's run: tiles [begin, begin + left) of the tiles that each of its members has
-  const int rounds = a.Hk / da.team, teams = gridDim.x / da.team;
-  if (tid == 0) s_drain = *reinterpret_cast<volatile int*>(a.status);
-  int64_t total = 0;
-  for (int b = tid; b < a.batch; b += NUM_THREADS) {
-    TileSpan span;
-    total += item_tiles<RP>(c, seq_info(a, b), span);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) s_sum[warp] = total;
-  __syncthreads();
-  if (s_drain != 0) return;   // a wait gave up on this device: finish the launch quickly
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < NUM_THREADS / 32; ++i) total += s_sum[i];
-  total *= rounds;
-  int64_t run = (total + teams - 1) / teams;
-  if (run < kMinRun) run = kMinRun;
-  const int64_t begin = run * (blockIdx.x / da.team);   // the CTAs behind the last whole team begin behind the end
-  if (begin >= total) {
-    if (tid == 0) da.record[blockIdx.x] = PartRecord{-1, 1};
-    return;
-  }
-  // the sequence that holds tile `begin`
-  int64_t before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += NUM_THREADS) {
-    int64_t mine = 0;
-    if (b0 + tid < a.batch) {
-      TileSpan span;
-      mine = (int64_t)item_tiles<RP>(c, seq_info(a, b0 + tid), span) * rounds;
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    __syncthreads();
-    if (lane == 31) s_sum[warp] = incl;
-    __syncthreads();
-    int64_t base = before;
-#pragma unroll
-    for (int i = 0; i < NUM_THREADS / 32; ++i) {
-      if (i < warp) base += s_sum[i];
-      before += s_sum[i];
-    }
-    if (mine > 0 && base + incl - mine <= begin && begin < base + incl) {
-      s_b = b0 + tid;
-      s_off = begin - (base + incl - mine);
-    }
-    if (before > begin) break;
-  }
-
+  const int rounds = da.rounds, cta = blockIdx.y * gridDim.x + blockIdx.x;   // block (member, team)
+  TileSpan span;
+  SeqInfo mine_info{0, 0, 0, 0};          // of sequence tid, for batches of at most a thread each
+  if (tid < a.batch) mine_info = seq_info(a, tid);
   if (tid == 0) {
+    s_drain = *reinterpret_cast<volatile int*>(a.status);
     for (int i = 0; i < C::SLOTS; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < C::SLOTS; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -253,6 +225,55 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
   }
+  int mine = tid < a.batch ? item_tiles<RP>(c, mine_info, span) * rounds : 0;
+  int total = mine;
+  for (int b = tid + NUM_THREADS; b < a.batch; b += NUM_THREADS)
+    total += item_tiles<RP>(c, seq_info(a, b), span) * rounds;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) s_sum[warp] = total;
+  __syncthreads();
+  if (s_drain != 0) return;   // a wait gave up on this device: finish the launch quickly
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < NUM_THREADS / 32; ++i) total += s_sum[i];
+  const int run = max((total + (int)gridDim.y - 1) / (int)gridDim.y, kMinRun);
+  const int64_t begin = (int64_t)run * blockIdx.y;
+  if (begin >= total) {
+    if (tid == 0) da.record[cta] = PartRecord{-1, 0, 0, 0};
+    return;
+  }
+  // the sequence that holds tile `begin`
+  int before = 0, b0 = 0;
+  for (;; b0 += NUM_THREADS) {
+    if (b0 > 0) {
+      mine = 0;
+      if (b0 + tid < a.batch) {
+        mine_info = seq_info(a, b0 + tid);
+        mine = item_tiles<RP>(c, mine_info, span) * rounds;
+      }
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    int base = before;
+#pragma unroll
+    for (int i = 0; i < NUM_THREADS / 32; ++i) {
+      if (i < warp) base += s_sum[i];
+      before += s_sum[i];
+    }
+    if (mine > 0 && base + incl - mine <= begin && begin < base + incl) {
+      s_b = b0 + tid;
+      s_off = (int)begin - (base + incl - mine);
+    }
+    if (before > begin) break;
+  }
   if (warp == MMA_WARP) {
     tmem_alloc(tmem_slot, C::TCOLS);
     tmem_relinquish();
@@ -261,13 +282,17 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  const InfoTable table{sInfo, s_b, min(min(kInfo, a.batch - s_b), b0 + NUM_THREADS - s_b)};
+  if ((unsigned)(b0 + tid - table.b0) < (unsigned)table.n) sInfo[b0 + tid - table.b0] = mine_info;
+  __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;");   // the joining kernel may be set up: it waits for this one's end
   Segment seg;
   seg.b = s_b;
-  seg.left = (int)(min(total, begin + run) - begin);
-  fill_segment<RP>(c, seg, 0);
-  seg.hk = (int)(s_off / seg.n);
-  seg.lo = (int)(s_off - (int64_t)seg.hk * seg.n);
-  seg.hk = seg.hk * da.team + blockIdx.x % da.team;
+  seg.left = min(total - (int)begin, run);
+  fill_segment<RP>(c, table, seg, 0);
+  const int round = rounds > 1 ? s_off / seg.n : 0;
+  seg.hk = round * gridDim.x + blockIdx.x;
+  seg.lo = s_off - round * seg.n;
   seg.hi = min(seg.n, seg.lo + seg.left);
   auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
     return mbar_wait(bar, parity, abort_flag, a.status, kStatusAttnTimeout);
@@ -281,46 +306,53 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
     return r != 0;
   };
 
-  if (warp == TMA_WARP) {
-    // ================================ producer ====================================
+  if (warp == TMA_WARP || warp == TMA_WARP + 1) {
+    // ================================ producers of K and of V =====================
+    const bool is_v = warp != TMA_WARP;
+    const CUtensorMap* tm = is_v ? &tmap_v : &tmap_k;
+    uint8_t* ring = is_v ? sV : sK;
+    uint64_t* full = is_v ? v_full : k_full;
+    uint64_t* empty = is_v ? v_empty : k_empty;
+    // Lane i holds the place of the i-th page of a tile, or -1 where no query row sees any of its keys: such a page is not
+    // fetched (its scores are masked and its V rows zeroed).
     auto lookup = [&](const Segment& g, int t, int& page, int& row) {
       const int tok = g.span.tile(t) * BN + lane * da.page_rows;
-      page = 0;
+      const RowMask first = row_mask(c, g.s.k_len, g.shift), last = row_mask(c, g.s.k_len, (g.rows - 1) / group + g.shift);
+      page = -1;
       row = g.s.k_begin + tok;
-      if (a.paged && lane < da.pages_per_tile) {
+      if (lane >= da.pages_per_tile || tok >= last.hi || (tok + da.page_rows <= first.lo && tok >= c.sinks)) return;
+      page = 0;
+      if (a.paged) {
         const int pg = tok / a.block_size;
         row = tok - pg * a.block_size;
-        // past the sequence: any valid page (those keys are masked)
-        page = cache_page(c, a.block_table + (int64_t)g.b * a.bt_stride, min(pg, max(0, (g.s.k_len - 1) / a.block_size)));
+        page = cache_page(c, a.block_table + (int64_t)g.b * a.bt_stride, pg);
       }
     };
     int page, row;
     lookup(seg, seg.lo, page, row);
-    uint32_t n = 0;   // ring items so far
+    uint32_t g = 0;    // tiles so far
     bool ok = true;
     while (ok) {
       Segment next;
-      const bool more = next_segment<RP>(c, da.team, seg, next);
-      for (int t = seg.lo; t < seg.hi && ok; ++t) {
-        int npage = 0, nrow = 0;   // the table entry of the next tile is in flight while this one is issued
+      const bool more = next_segment<RP>(c, table, gridDim.x, seg, next);
+      for (int t = seg.lo; t < seg.hi && ok; ++t, ++g) {
+        int npage = -1, nrow = 0;   // the table entry of the next tile is in flight while this one is issued
         if (t + 1 < seg.hi)
           lookup(seg, t + 1, npage, nrow);
         else if (more)
           lookup(next, next.lo, npage, nrow);
-        for (int which = 0; which < 2; ++which, ++n) {
-          const uint32_t slot = n % C::SLOTS;
-          if (!wwait(&empty[slot], ((n / C::SLOTS) & 1) ^ 1)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) mbar_expect_tx(&full[slot], C::TILE);
-          __syncwarp();
-          if (lane < da.pages_per_tile) {
-            uint8_t* dst = smem + slot * C::TILE + lane * da.page_rows * 128;
-            const CUtensorMap* tm = which ? &tmap_v : &tmap_k;
-            tma_load_4d(dst, tm, &full[slot], 0, seg.hk, row, page);
-            if constexpr (!C::k8) tma_load_4d(dst + C::TILE / 2, tm, &full[slot], 64, seg.hk, row, page);
-          }
+        const uint32_t slot = g % C::SLOTS;
+        if (!wwait(&empty[slot], ((g / C::SLOTS) & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        const int pages = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) mbar_expect_tx(&full[slot], pages * da.page_rows * (C::TILE / BN));
+        __syncwarp();
+        if (page >= 0) {
+          uint8_t* dst = ring + slot * C::TILE + lane * da.page_rows * 128;
+          tma_load_4d(dst, tm, &full[slot], 0, seg.hk, row, page);
+          if constexpr (!C::k8) tma_load_4d(dst + C::TILE / 2, tm, &full[slot], 64, seg.hk, row, page);
         }
         page = npage;
         row = nrow;
@@ -335,14 +367,18 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
                                   : umma_idesc_f16(C::kBf16, false, false, BN, C::NS);
       const uint32_t id_o = C::k8 ? umma_idesc_f8(KIND == kCacheE5M2, true, true, false, HD, C::NP)
                                   : umma_idesc_f16(C::kBf16, true, false, HD, C::NP);
-      // tile g of the run (tiles and ring items count on through all items); `item`: the how-manieth
+      // scores of tile g of the run (tiles count on through all items); `item`: the how-manieth
+      auto scores_ready = [&](uint32_t g, bool first, uint32_t item) -> bool {   // without waiting
+        return (!first || mbar_test(&q_ready[item & 1], (item >> 1) & 1)) && mbar_test(&k_full[g % C::SLOTS], (g / C::SLOTS) & 1) &&
+               (g < 2 || mbar_test(&s_free[g & 1], ((g - 2) >> 1) & 1));
+      };
       auto scores = [&](uint32_t g, bool first, uint32_t item) -> bool {
-        const uint32_t n = 2 * g, slot = n % C::SLOTS;
+        const uint32_t slot = g % C::SLOTS;
         if (first && !wait1(&q_ready[item & 1], (item >> 1) & 1)) return false;
-        if (!wait1(&full[slot], (n / C::SLOTS) & 1)) return false;
+        if (!wait1(&k_full[slot], (g / C::SLOTS) & 1)) return false;
         if (g >= 2 && !wait1(&s_free[g & 1], ((g - 2) >> 1) & 1)) return false;   // scores two tiles back are read
         tc_fence_after();
-        const uint64_t k_desc = umma_desc_sw128(smem_u32(smem + slot * C::TILE), 0, 1024);
+        const uint64_t k_desc = umma_desc_sw128(smem_u32(sK + slot * C::TILE), 0, 1024);
         const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ + (item & 1) * C::QB), 0, 1024);
         const uint32_t d = tmem_base + (g & 1) * C::SCOL;
         if constexpr (C::k8) {
@@ -355,7 +391,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
                        id_s, k != 0);
         }
         tc_commit(&s_full[g & 1]);
-        tc_commit(&empty[slot]);
+        tc_commit(&k_empty[slot]);
         return true;
       };
       Segment ahead = seg;                 // where the scores are, one tile ahead of P V
@@ -367,23 +403,25 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
           bool first = false, more = true;
           if (++at >= ahead.hi) {
             Segment to;
-            more = next_segment<RP>(c, da.team, ahead, to);
+            more = next_segment<RP>(c, table, gridDim.x, ahead, to);
             ahead = to;
             at = to.lo;
             first = true;
             ++ahead_item;
           }
-          if (more && !scores(g + 1, first, ahead_item)) {
+          // the next tile's scores first, so that the softmax warps find them -- unless its keys have yet to arrive
+          const bool early = more && scores_ready(g + 1, first, ahead_item);
+          if (early && !scores(g + 1, first, ahead_item)) {
             ok = false;
             break;
           }
-          const uint32_t n = 2 * g + 1, slot = n % C::SLOTS;
-          if (!wait1(&full[slot], (n / C::SLOTS) & 1) || !wait1(&p_ready[g & 1], (g >> 1) & 1)) {
+          const uint32_t slot = g % C::SLOTS;
+          if (!wait1(&v_full[slot], (g / C::SLOTS) & 1) || !wait1(&p_ready[g & 1], (g >> 1) & 1)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t v_desc = umma_desc_sw128(smem_u32(smem + slot * C::TILE), C::k8 ? C::TILE : C::TILE / 2, 1024);
+          const uint64_t v_desc = umma_desc_sw128(smem_u32(sV + slot * C::TILE), C::k8 ? C::TILE : C::TILE / 2, 1024);
           const uint64_t p_desc = umma_desc_sw128(smem_u32(sP + (g & 1) * C::PB), 0, 1024);
           const uint32_t d = tmem_base + C::OCOL;
           const bool add = t > seg.lo;     // the first tile of an item overwrites
@@ -396,10 +434,14 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
               mma_f16_ss(d, v_desc + k * (2048 >> 4), p_desc + (k >> 2) * (C::PR * 128 / 16) + (k & 3) * 2, id_o, add || k > 0);
           }
           tc_commit(&o_done[g & 1]);
-          tc_commit(&empty[slot]);
+          tc_commit(&v_empty[slot]);
+          if (more && !early && !scores(g + 1, first, ahead_item)) {
+            ok = false;
+            break;
+          }
         }
         Segment to;
-        left = next_segment<RP>(c, da.team, seg, to);
+        left = next_segment<RP>(c, table, gridDim.x, seg, to);
         seg = to;
       }
     }
@@ -483,7 +525,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
     load_q(seg);
     store_q(0);
     softmax_sync();
-    PartRecord rec{-1, 1};
+    PartRecord rec{-1, 0, 0, 0};
     uint32_t g = 0;            // tiles so far
     // A wait that gave up does not end the loops: the barriers below need every warp.
     bool ok = true;
@@ -493,8 +535,8 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
       for (int i = 0; i < RP; ++i) pre[i] = sDown[(item & 1) * 16 + i] * (ksc * a.scale_log2);
       const float v_scale = vsc;
       Segment next;
-      const bool more = next_segment<RP>(c, da.team, seg, next);
-      if (more) load_q(next);
+      const bool more = next_segment<RP>(c, table, gridDim.x, seg, next);
+      if (more) load_q(next);   // on its way during this item's first tile
       const int k_len = seg.s.k_len, shift = seg.shift;
       const RowMask first = row_mask(c, k_len, shift), last = row_mask(c, k_len, (seg.rows - 1) / group + shift);
       float m_ref[RP], l_run[RP];
@@ -537,15 +579,18 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             }
           }
           // a V row that no query row sees must not reach the product
-          const uint32_t n_v = 2 * g + 1, v_slot = n_v % C::SLOTS;
-          ok = ok && wwait(&full[v_slot], (n_v / C::SLOTS) & 1);
-          if (ok && (col >= last.hi || (col < first.lo && col >= c.sinks))) {
-            uint8_t* v = smem + v_slot * C::TILE + tid * 128;
+          const uint32_t v_slot = g % C::SLOTS;
+          ok = ok && wwait(&v_full[v_slot], (g / C::SLOTS) & 1);
+          if (ok) {
+            // this warp's 32 rows, four at a time, eight lanes a row
 #pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
-            if constexpr (!C::k8) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + C::TILE / 2 + i * 16) = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 8; ++i) {
+              const int row = warp * 32 + i * 4 + (lane >> 3), key = j0 + row;
+              if (key >= last.hi || (key < first.lo && key >= c.sinks)) {
+                uint8_t* v = sV + v_slot * C::TILE + row * 128 + (lane & 7) * 16;
+                *reinterpret_cast<uint4*>(v) = make_uint4(0, 0, 0, 0);
+                if constexpr (!C::k8) *reinterpret_cast<uint4*>(v + C::TILE / 2) = make_uint4(0, 0, 0, 0);
+              }
             }
           }
         }
@@ -645,15 +690,12 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
       tmem_ld_wait();
       tc_fence_before();   // the next item's first product overwrites O after its P, which this thread has yet to store
       const bool whole = seg.lo == 0 && seg.hi == seg.n;
-      const int part = 2 * blockIdx.x + (seg.lo == 0 ? 1 : 0);
-      if (!whole) {
-        if (seg.lo == 0)
-          rec.tail_item = seg.b * a.Hk + seg.hk;
-        else
-          rec.head_ends = seg.hi == seg.n;
-      }
+      const int part = 2 * cta + (seg.lo == 0 ? 1 : 0);
+      if (!whole && seg.lo == 0)   // the last of the run: each later team takes `run` tiles of the rest
+        rec = PartRecord{seg.b * a.Hk + seg.hk, 1 + (seg.n - seg.hi + run - 1) / run, seg.s.q_begin, seg.rows};
       if (ok) {
         int tok = 0, in = 0;
+        float my_l = 0.f, my_m = 0.f;       // of row tid
 #pragma unroll
         for (int r = 0; r < RP; ++r) {
           if (r < seg.rows) {
@@ -669,12 +711,9 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
               reinterpret_cast<T*>(a.out)[qtok * a.o_rs + (int64_t)h * a.o_hs + tid] = Cvt<T>::from_f32(v);
             else
               da.part_o[((int64_t)part * RP + r) * HD + tid] = v;
-            if (tid == 0) {
-              const float lse2 = l == 0.f ? -INFINITY : m_ref[r] + log2f(l);
-              if (!whole)
-                da.part_lse[part * RP + r] = lse2;
-              else if (a.lse)
-                a.lse[(int64_t)h * a.total_q + qtok] = l == 0.f ? INFINITY : lse2 * 0.6931471805599453f;
+            if (tid == r) {
+              my_l = l;
+              my_m = m_ref[r];
             }
           }
           if (++in == group) {
@@ -682,11 +721,19 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             ++tok;
           }
         }
+        if (tid < seg.rows && (!whole || a.lse)) {
+          const float lse2 = my_l == 0.f ? -INFINITY : my_m + log2f(my_l);
+          if (!whole)
+            da.part_lse[part * RP + tid] = lse2;
+          else
+            a.lse[(int64_t)(seg.hk * group + tid % group) * a.total_q + seg.s.q_begin + tid / group] =
+                my_l == 0.f ? INFINITY : lse2 * 0.6931471805599453f;
+        }
       }
       if (!more) break;
       seg = next;
     }
-    if (tid == 0) da.record[blockIdx.x] = rec;
+    if (tid == 0) da.record[cta] = rec;
   }
 
   // ================================ teardown ======================================
@@ -702,49 +749,54 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   }
 }
 
-// Joins the parts of the items that runs cut.  Block (i, r) does row r of the item whose start, but not end, CTA i holds: its
-// tail part, then the head parts of the same member of the teams after it, up to the one the item ends in.  Four groups of 128 threads take
-// every fourth part; their sums are added in a fixed order.
+// Joins the parts of the items that runs cut.  Block i does the item whose start, but not end, CTA i holds: its tail part, then
+// the head parts of the same member of the teams after it.  A group of 128 threads takes a row at a time; items in many parts
+// (few, long sequences) have their parts dealt out over the groups instead, whose sums are added in a fixed order.
+constexpr int kJoinGroups = 4;
 template <typename T, int RP>
-__global__ void __launch_bounds__(512) attn_cache_join_kernel(DecodeArgs da, int ctas) {
+__global__ void __launch_bounds__(kJoinGroups * 128) attn_cache_join_kernel(DecodeArgs da, int ctas) {
   const AttnArgs& a = da.c.a;
-  __shared__ float s_acc[3][HD], s_w[4], s_max[16];
-  const int i = blockIdx.x, r = blockIdx.y;
+  __shared__ float s_acc[kJoinGroups][HD], s_w[kJoinGroups];
+  asm volatile("griddepcontrol.wait;" ::: "memory");              // launched early: the parts are complete after this
+  const int i = blockIdx.x;
+  const PartRecord rec = da.record[i];
   if (*reinterpret_cast<volatile int*>(a.status) != 0) return;   // the parts and the records may be missing
-  const int item = da.record[i].tail_item;
-  if (item < 0) return;
-  const int b = item / a.Hk, hk = item - b * a.Hk;
-  const SeqInfo s = seq_info(a, b);
-  if (r >= min(s.q_len * a.group, RP)) return;
+  if (rec.item < 0) return;
+  const int hk = rec.item % a.Hk;
+  const int n = min(rec.parts, 1 + (ctas - 1 - i) / da.team);
   const int grp = threadIdx.x >> 7, d = threadIdx.x & 127;
-  int n = 2;                              // parts
-  while (i + n * da.team < ctas && !da.record[i + (n - 1) * da.team].head_ends) ++n;
-  auto slot = [&](int k) { return (int64_t)(k == 0 ? 2 * i + 1 : 2 * (i + k * da.team)) * RP + r; };
-  float m = -INFINITY;
-  for (int k = threadIdx.x; k < n; k += 512) m = fmaxf(m, da.part_lse[slot(k)]);
-  m = warp_max(m);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
-  __syncthreads();
+  const bool deal = n > 8;
+  for (int r = deal ? 0 : grp; r < rec.rows; r += deal ? 1 : kJoinGroups) {
+    auto slot = [&](int k) { return (int64_t)(k == 0 ? 2 * i + 1 : 2 * (i + k * da.team)) * RP + r; };
+    float m = -INFINITY;
+    for (int k = 0; k < n; ++k) m = fmaxf(m, da.part_lse[slot(k)]);
+    const float ms = m == -INFINITY ? 0.f : m;
+    float acc = 0.f, wsum = 0.f;
+#pragma unroll 4
+    for (int k = deal ? grp : 0; k < n; k += deal ? kJoinGroups : 1) {
+      const float w = exp2f(da.part_lse[slot(k)] - ms), o = da.part_o[slot(k) * HD + d];
+      wsum += w;
+      if (w != 0.f) acc += w * o;   // NaN goes on
+    }
+    if (deal) {
+      __syncthreads();
+      s_acc[grp][d] = acc;
+      if (d == 0) s_w[grp] = wsum;
+      __syncthreads();
+      acc = wsum = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) m = fmaxf(m, s_max[k]);
-  const float ms = m == -INFINITY ? 0.f : m;
-  float acc = 0.f, wsum = 0.f;
-  for (int k = grp; k < n; k += 4) {
-    const float w = exp2f(da.part_lse[slot(k)] - ms);
-    wsum += w;
-    if (w != 0.f) acc += w * da.part_o[slot(k) * HD + d];   // NaN goes on
+      for (int k = 0; k < kJoinGroups; ++k) {
+        acc += s_acc[k][d];
+        wsum += s_w[k];
+      }
+      if (grp != 0) continue;
+    }
+    const int64_t qtok = rec.q_begin + r / a.group;
+    const int h = hk * a.group + r % a.group;
+    reinterpret_cast<T*>(a.out)[qtok * a.o_rs + (int64_t)h * a.o_hs + d] = Cvt<T>::from_f32(wsum == 0.f ? 0.f : acc / wsum);
+    if (a.lse && d == 0)
+      a.lse[(int64_t)h * a.total_q + qtok] = wsum == 0.f ? INFINITY : (m + log2f(wsum)) * 0.6931471805599453f;
   }
-  if (grp > 0) s_acc[grp - 1][d] = acc;
-  if (d == 0) s_w[grp] = wsum;
-  __syncthreads();
-  if (grp > 0) return;
-  acc = ((acc + s_acc[0][d]) + (s_acc[1][d] + s_acc[2][d]));
-  wsum = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]);
-  const int64_t qtok = s.q_begin + r / a.group;
-  const int h = hk * a.group + r % a.group;
-  reinterpret_cast<T*>(a.out)[qtok * a.o_rs + (int64_t)h * a.o_hs + d] = Cvt<T>::from_f32(wsum == 0.f ? 0.f : acc / wsum);
-  if (a.lse && d == 0)
-    a.lse[(int64_t)h * a.total_q + qtok] = wsum == 0.f ? INFINITY : (m + log2f(wsum)) * 0.6931471805599453f;
 }
 
 template <typename T, int KIND, int RP>
@@ -775,16 +827,28 @@ int launch(DecodeArgs& da, cudaStream_t st) {
                                     C::SMEM));
     attr_dev = dev;
   }
-  const int ctas = C::CTAS * num_sms();
   da.team = 1;
   for (int t = 2; t <= 16; ++t)
     if (a.Hk % t == 0) da.team = t;
+  da.rounds = a.Hk / da.team;
+  const int teams = C::CTAS * num_sms() / da.team, ctas = teams * da.team;
   da.part_o = a.ws_o;
   da.part_lse = a.ws_o + (int64_t)2 * ctas * RP * HD;
   da.record = reinterpret_cast<PartRecord*>(da.part_lse + 2 * ctas * RP);
-  attn_cache_decode_tcgen05_kernel<T, KIND, RP><<<ctas, NUM_THREADS, C::SMEM, st>>>(maps[0], maps[1], da);
+  attn_cache_decode_tcgen05_kernel<T, KIND, RP><<<dim3(da.team, teams), NUM_THREADS, C::SMEM, st>>>(maps[0], maps[1], da);
   FG_CHECK_LAUNCH("attn_cache_decode_tcgen05_kernel");
-  attn_cache_join_kernel<T, RP><<<dim3(ctas, a.max_q * a.group), 512, 0, st>>>(da, ctas);
+  // The joining kernel is launched while this one still runs (programmatic dependent launch) and waits for its end on the
+  // device: the launch's latency is out of the way.
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kJoinGroups * 128);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  FG_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_cache_join_kernel<T, RP>, da, ctas));
   FG_CHECK_LAUNCH("attn_cache_join_kernel");
   return FG_OK;
 }
