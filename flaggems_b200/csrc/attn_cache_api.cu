@@ -65,6 +65,13 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
     plan.bytes = attn_cache_decode_sm100_bytes(b.max_seqlen_q * group, sms);
     return plan;
   }
+  if (b.max_seqlen_q * group > 16 && tma && b.head_dim == 128 && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 &&
+      b.q_head_stride > 0 && b.q_row_stride > 0 && workspace) {
+    plan.path = kPathChunk;            // cuts the keys itself, on the device
+    plan.splits = plan.tiles_per_split = 1;
+    plan.bytes = attn_cache_chunk_bytes(b.max_seqlen_q, group, b.batch, b.num_heads_k, b.max_seqlen_k / 128 + 1, sms);
+    if (plan.bytes > 0) return plan;
+  }
   if (b.max_seqlen_q * group <= 16 && tma) {
     // Enough CTAs to balance contexts of very different length over all SMs (two resident each), but no range shorter
     // than 256 keys.
@@ -76,15 +83,6 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
     plan.tiles_per_split = (int)(chunk / bn);
     plan.splits = (int)((keys + chunk - 1) / chunk);
     if (plan.splits < 1) plan.splits = 1;
-  } else if (b.head_dim == 128 && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 && tma && b.q_head_stride > 0 &&
-             b.q_row_stride > 0) {
-    plan.path = kPathChunk;
-    const int64_t tokens = 128 / group;                        // of a Q tile; two tiles a CTA when there are more
-    const int64_t per_cta = b.max_seqlen_q > tokens ? 2 * tokens : tokens;
-    const int64_t mb = (b.max_seqlen_q + per_cta - 1) / per_cta;
-    const int64_t tiles = (most_keys(p, per_cta) + 127) / 128;
-    split_plan(mb * b.num_heads_k * b.batch, tiles, (int64_t)sms * 2, 8, &plan);
-    if (mb * b.num_heads_k * b.batch >= sms) plan.splits = 1;
   } else {
     plan.path = kPathGeneric;
     const int64_t mb = (b.max_seqlen_q * group + 63) / 64;

@@ -1,8 +1,11 @@
 // Attention of a chunk of new tokens over an 8-bit or windowed cache, head dim 128, on the tcgen05 tensor cores.
 //
-// CTA = one or two 128-row Q tiles of one (sequence, KV head) and a range of its K/V tiles of 128 keys.  A row is a
-// (token, head of the group) pair, so a chunk of a few tokens fills the tiles as well as a long one, and all query heads
-// of the group share every K/V tile.  A tile holds floor(128 / group) tokens.
+// An item is one or two 128-row Q tiles of one (sequence, KV head).  A row is a (token, head of the group) pair, so a chunk of a
+// few tokens fills the tiles as well as a long one, and all query heads of the group share every K/V tile.  A tile holds
+// floor(128 / group) tokens.  The kernel is persistent, one CTA an SM: the K/V tiles (128 keys) of all items, laid end to end,
+// are cut into equal runs, one per CTA, so that few long items and many short ones fill the SMs alike (in whole items, 336
+// CTAs on 148 SMs would take three rounds for 2.27).  The parts of an item that runs cut are joined by a second kernel, in
+// order.  Nothing synchronises the CTA between items: the roles follow the barrier phases with running counters.
 //
 //   warps 0-7    softmax, one warpgroup per Q tile, one thread per row (TMEM lane = row): scores of 64 keys from TMEM to
 //                registers, mask, running maximum (raised only when it grows by more than 8 in log2 units), exponentials,
@@ -10,9 +13,11 @@
 //   warp 8       TMA producer: Q once, then K and V tiles, walking the tile runs (first tokens, then the window)
 //   warps 9, 10  score-issuing thread of each Q tile: S = Q K^T, 64 keys a step
 //   warp 11      O += P V of both tiles
-//   warps 12-15  8-bit caches: widen each K/V tile from the 16 KB landing slots to the fp16 tiles that the tensor cores
-//                read (128-byte swizzled, K-major), zeroing V rows that no row of the CTA sees; for bf16 queries they first
-//                bring Q to fp16, each row by a power of two
+//   warps 12-15  8-bit caches: widen the K/V tiles from six 16 KB landing slots to fp16 units of 64 keys (two of K, two of V;
+//                128-byte swizzled rows) for the tensor cores, zeroing V rows that no row of the item sees.  The depth is in
+//                the landing slots because that is where the latency is: with one slot for K and one for V (and units of 128
+//                keys) a tile took a copy's latency and a conversion in turn, 831 us for two chunks of 2048 tokens.  (bf16 queries are brought
+//                to fp16, each row by a power of two, by the softmax warps before an item's first step.)
 // TMEM columns: tile t has its scores at t*128 (64 columns), two probability buffers at t*128+64 and +96, its output at
 // 256+t*128.  Every wait is an mbarrier wait with a limit.
 #include "attn_cache_common.cuh"
@@ -29,17 +34,88 @@ constexpr int TMA_WARP = 8, MMA_WARP0 = 9, CONV_WARP0 = 12;
 constexpr int TMEM_COLS = 512;
 constexpr float kRescaleThreshold = 8.0f;    // log2 units
 
+constexpr int kMinRun = 4;                   // fewest K/V tiles that a run is worth starting a CTA for
+constexpr int kInfo = 32;                    // sequences of a run whose lengths are kept in shared memory
+
 constexpr int threads_of(int kind) { return kind == kCache16 ? 12 * 32 : 16 * 32; }
-constexpr int smem_of(int kind) { return 6 * TILE_BYTES + (kind == kCache16 ? 0 : 2 * RAW_BYTES) + 1024 + 256 + 2 * BM * 4; }
+constexpr int RAW_SLOTS = 6;                 // 8-bit tiles on their way or being widened
+// Keys of a 16-bit stage (two of K, two of V): 64 where 8-bit tiles are widened into them, else a whole tile as it arrives.
+constexpr int unit_of(int kind) { return kind == kCache16 ? BN : STEP; }
+constexpr int smem_of(int kind) {
+  return 2 * TILE_BYTES + 4 * unit_of(kind) * 256 + (kind == kCache16 ? 0 : RAW_SLOTS * RAW_BYTES) + 1024 + 512 + kInfo * 16;
+}
+
+// What a CTA leaves for the joining kernel: the KV head of the item whose start it holds but not its end (or -1), in how many
+// parts the item is, its first query row and its tokens.
+struct PartRecord {
+  int hk, parts, q_row, tokens;
+};
 
 struct ChunkArgs {
   CacheAttnArgs c;
-  int tiles;            // Q tiles per CTA (1 or 2)
+  int tiles;            // Q tiles of an item (1 or 2)
   int tokens;           // tokens of a Q tile
   int page_rows;        // keys per TMA box
   int pages_per_tile;
-  int num_mb;           // Q tile pairs of the longest chunk
+  int num_mb;           // items of the longest chunk, for each KV head
+  float* part_o;        // [2 * CTAs][tiles * 128][128]: head part, tail part of each CTA
+  float* part_lse;      // [2 * CTAs][tiles * 128]
+  PartRecord* record;   // [CTAs]
 };
+
+// One item's part of a CTA's run.
+struct Segment {
+  int b, m, hk, lo, hi, n;      // K/V tiles [lo, hi) of the n of (sequence b, Q tiles m, KV head hk)
+  int left;                     // tiles of the run from lo on
+  int m0, nt, shift, steps;     // first token; Q tiles that hold one; position of token 0; steps of 64 keys
+  SeqInfo s;
+  TileSpan span;
+  RowMask first, last;          // what the first and the last token see
+};
+__device__ __forceinline__ int item_tiles(const ChunkArgs& pa, const SeqInfo& s, int m, TileSpan& span) {
+  const int m0 = m * pa.tiles * pa.tokens;
+  if (m0 >= s.q_len) return 0;
+  const int shift = s.k_len - s.q_len;
+  span = tile_span<BN>(pa.c, s.k_len, m0 + shift, min(s.q_len, m0 + pa.tiles * pa.tokens) - 1 + shift);
+  return max(span.n, 1);        // nothing visible: one tile, all of it masked, gives the zeros
+}
+// Lengths of the sequences [b0, b0 + n) as the CTA found them at its start; the others come from global memory.
+struct InfoTable {
+  const SeqInfo* info;
+  int b0, n;
+};
+__device__ __forceinline__ void set_part(Segment& g, int lo) {
+  g.lo = lo;
+  g.hi = min(g.n, lo + g.left);
+  // the second half of the last tile is left out when nothing of it is visible
+  g.steps = 2 * (g.hi - g.lo) - (g.hi == g.n && g.span.tile(g.n - 1) * BN + STEP >= g.last.hi ? 1 : 0);
+}
+__device__ __forceinline__ void fill_segment(const ChunkArgs& pa, const InfoTable& table, Segment& g) {
+  g.s = (unsigned)(g.b - table.b0) < (unsigned)table.n ? table.info[g.b - table.b0] : seq_info(pa.c.a, g.b);
+  g.n = item_tiles(pa, g.s, g.m, g.span);
+  g.m0 = g.m * pa.tiles * pa.tokens;
+  g.nt = g.m0 + pa.tokens < g.s.q_len ? pa.tiles : 1;
+  g.shift = g.s.k_len - g.s.q_len;
+  g.first = row_mask(pa.c, g.s.k_len, g.m0 + g.shift);
+  g.last = row_mask(pa.c, g.s.k_len, min(g.s.q_len, g.m0 + pa.tiles * pa.tokens) - 1 + g.shift);
+}
+// The part after `g`, in place; false when the run ends with g.
+__device__ __forceinline__ bool next_segment(const ChunkArgs& pa, const InfoTable& table, Segment& g) {
+  g.left -= g.hi - g.lo;
+  if (g.left <= 0) return false;
+  if (++g.hk == pa.c.a.Hk) {
+    g.hk = 0;
+    do {
+      if (++g.m == pa.num_mb) {
+        g.m = 0;
+        if (++g.b >= pa.c.a.batch) return false;
+      }
+      fill_segment(pa, table, g);
+    } while (g.n == 0);
+  }
+  set_part(g, 0);
+  return true;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -76,46 +152,24 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   constexpr bool kBf16 = std::is_same<M, __nv_bfloat16>::value;
   constexpr bool kConvQ = !std::is_same<T, M>::value;
   constexpr bool kWiden = KIND != kCache16;
+  constexpr int THREADS = threads_of(KIND);
+  constexpr int UNIT_HALF = unit_of(KIND) * 128;   // bytes of one 64-column half of a stage
+  constexpr int UNIT = 2 * UNIT_HALF;
   const CacheAttnArgs& c = pa.c;
   const AttnArgs& a = c.a;
   const int NT = pa.tiles;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  // heaviest (latest) query blocks of all sequences and heads first
-  int idx = blockIdx.x;
-  const int split = idx % a.num_splits;
-  idx /= a.num_splits;
-  const int hk = idx % a.Hk;
-  idx /= a.Hk;
-  const int b = idx % a.batch;
-  const int m0 = (pa.num_mb - 1 - idx / a.batch) * NT * pa.tokens;   // first token
-  const SeqInfo s = seq_info(a, b);
-  if (m0 >= s.q_len) return;
-  __shared__ int s_drain;
-  if (threadIdx.x == 0) s_drain = *reinterpret_cast<volatile int*>(a.status);
-  __syncthreads();
-  if (s_drain != 0) return;   // a wait gave up on this device: finish the launch quickly
-
-  const int shift = s.k_len - s.q_len;
-  const int m_last = min(s.q_len, m0 + NT * pa.tokens) - 1;          // last token
-  const TileSpan span = tile_span<BN>(c, s.k_len, m0 + shift, m_last + shift);
-  const int i_begin = split * c.tiles_per_split;
-  const int n_tiles = max(0, (a.num_splits > 1 ? min(span.n, i_begin + c.tiles_per_split) : span.n) - i_begin);
-  const RowMask cta_first = row_mask(c, s.k_len, m0 + shift), cta_last = row_mask(c, s.k_len, m_last + shift);
-  // steps of 64 keys; the second half of the last tile is left out when it is not visible
-  const int n_steps = n_tiles == 0 ? 0
-                                   : 2 * n_tiles - (span.tile(i_begin + n_tiles - 1) * BN + STEP >= cta_last.hi ? 1 : 0);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                       // [2 tiles][2 halves][128 x 64]
   uint8_t* sK = smem + 2 * TILE_BYTES;      // [2 stages]
-  uint8_t* sV = smem + 4 * TILE_BYTES;      // [2 stages]
-  uint8_t* sR = smem + 6 * TILE_BYTES;      // [2 slots] 8-bit tiles as they arrive: K, V, K, V, ...
-  uint8_t* rest = sR + (kWiden ? 2 * RAW_BYTES : 0);
+  uint8_t* sV = sK + 2 * UNIT;              // [2 stages]
+  uint8_t* sR = sV + 2 * UNIT;              // [RAW_SLOTS] 8-bit tiles as they arrive: K, V, K, V, ...
+  uint8_t* rest = sR + (kWiden ? RAW_SLOTS * RAW_BYTES : 0);
   uint64_t* bars = reinterpret_cast<uint64_t*>(rest);
-  uint64_t* q_full = bars;            // Q tiles have landed
-  uint64_t* q_ready = bars + 1;       // ... and hold M
+  uint64_t* q_full = bars;            // Q tiles of an item have landed
+  uint64_t* q_empty = bars + 1;       // every score of an item has been computed: Q may be overwritten
   uint64_t* k_full = bars + 2;        // [2]
   uint64_t* k_empty = bars + 4;       // [2]
   uint64_t* v_full = bars + 6;        // [2]
@@ -124,16 +178,26 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   uint64_t* s_free = bars + 12;       // [2 tiles] ... and have been read into registers
   uint64_t* p_ready = bars + 14;      // [2 tiles][2 probability buffers]
   uint64_t* o_done = bars + 18;       // [2 tiles][2]: P V of even / odd steps
-  uint64_t* r_full = bars + 22;       // [2 slots]
-  uint64_t* r_empty = bars + 24;      // [2 slots]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  uint64_t* q_ready = bars + 22;      // [2 tiles] the tile's Q holds M
+  uint64_t* o_free = bars + 24;       // [2 tiles] the output of the previous item has been read out
+  uint64_t* r_full = bars + 26;       // [RAW_SLOTS]
+  uint64_t* r_empty = r_full + RAW_SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + RAW_SLOTS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* sDown = reinterpret_cast<float*>(rest + 256);   // [2 tiles][128]
+  SeqInfo* sInfo = reinterpret_cast<SeqInfo*>(rest + 512);   // [kInfo]
 
-  if (threadIdx.x == 0) {
+  __shared__ int s_drain, s_sum[THREADS / 32], s_off, s_pair;
+  // ---- this CTA's run: tiles [begin, begin + run) of all items' tiles; a pair is (sequence, Q tiles), the items of a pair are
+  // its KV heads
+  const int pairs = a.batch * pa.num_mb;
+  TileSpan span;
+  int mine = 0;
+  if (tid < pairs) mine = item_tiles(pa, seq_info(a, tid / pa.num_mb), tid % pa.num_mb, span) * a.Hk;
+  if (tid == 0) {
+    s_drain = *reinterpret_cast<volatile int*>(a.status);
     *abort_flag = 0;
     mbar_init(q_full, 1);
-    mbar_init(q_ready, 4);            // one arrival per widening warp
+    mbar_init(q_empty, NT);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], kWiden ? 4 : 1);
       mbar_init(&k_empty[i], NT);
@@ -141,6 +205,10 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4);       // one arrival per softmax warp of the tile
+      mbar_init(&q_ready[i], 4);
+      mbar_init(&o_free[i], 4);
+    }
+    for (int i = 0; i < RAW_SLOTS; ++i) {
       mbar_init(&r_full[i], 1);
       mbar_init(&r_empty[i], 4);
     }
@@ -151,6 +219,50 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
   }
+  int total = mine;
+  for (int p = tid + THREADS; p < pairs; p += THREADS)
+    total += item_tiles(pa, seq_info(a, p / pa.num_mb), p % pa.num_mb, span) * a.Hk;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) s_sum[warp] = total;
+  __syncthreads();
+  if (s_drain != 0) return;   // a wait gave up on this device: finish the launch quickly
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) total += s_sum[i];
+  const int run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kMinRun);
+  const int64_t begin = (int64_t)run * blockIdx.x;
+  if (begin >= total) {
+    if (tid == 0) pa.record[blockIdx.x] = PartRecord{-1, 0, 0, 0};
+    return;
+  }
+  int before = 0;
+  for (int p0 = 0;; p0 += THREADS) {
+    if (p0 > 0) {
+      const int p = p0 + tid;
+      mine = p < pairs ? item_tiles(pa, seq_info(a, p / pa.num_mb), p % pa.num_mb, span) * a.Hk : 0;
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    int base = before;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) {
+      if (i < warp) base += s_sum[i];
+      before += s_sum[i];
+    }
+    if (mine > 0 && base + incl - mine <= begin && begin < base + incl) {
+      s_pair = p0 + tid;
+      s_off = (int)begin - (base + incl - mine);
+    }
+    if (before > begin) break;
+  }
   if (warp == MMA_WARP0) {
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
@@ -159,10 +271,22 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // lane 0 polls for its warp, so that a wait that gave up takes the whole warp the same way
+  Segment seg;
+  seg.b = s_pair / pa.num_mb;
+  seg.m = s_pair - seg.b * pa.num_mb;
+  const InfoTable table{sInfo, seg.b, min(kInfo, a.batch - seg.b)};
+  if (tid < table.n) sInfo[tid] = seq_info(a, seg.b + tid);
+  __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;");   // the joining kernel may be set up: it waits for this one's end
+  seg.left = min(total - (int)begin, run);
+  fill_segment(pa, table, seg);
+  seg.hk = s_off / seg.n;
+  set_part(seg, s_off - seg.hk * seg.n);
+
   auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
     return mbar_wait(bar, parity, abort_flag, a.status, kStatusAttnTimeout);
   };
+  // lane 0 polls for its warp, so that a wait that gave up takes the whole warp the same way
   auto wwait = [&](uint64_t* bar, uint32_t parity) -> bool {
     int r = 1;
     if (lane == 0) r = wait1(bar, parity) ? 1 : 0;
@@ -171,69 +295,72 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     return r != 0;
   };
 
-  if (n_steps > 0 && warp == TMA_WARP) {
+  if (warp == TMA_WARP) {
     // ================================ TMA producer ================================
-    if (lane == 0) {
-      mbar_expect_tx(q_full, NT * 2 * pa.tokens * a.group * 128);
-      for (int t = 0; t < NT; ++t)
-        for (int hf = 0; hf < 2; ++hf)
-          tma_load_3d(sQ + t * TILE_BYTES + hf * HALF_BYTES, &tmap_q, q_full, hf * 64, hk * a.group,
-                      s.q_begin + m0 + t * pa.tokens);
-    }
-    __syncwarp();
-    const int32_t* bt_row = a.paged ? a.block_table + (int64_t)b * a.bt_stride : nullptr;
-    const int last_page = a.paged ? max(0, (s.k_len - 1) / a.block_size) : 0;
+    // Lane i holds the place of the i-th page of a tile, or -1 where no row of the item sees any of its keys: such a page is
+    // not fetched (its scores are masked and its V rows zeroed).
     auto lookup = [&](int j, int& page, int& row) {
+      const int tok = seg.span.tile(j) * BN + lane * pa.page_rows;
+      page = -1;
+      row = seg.s.k_begin + tok;
+      if (lane >= pa.pages_per_tile || tok >= seg.last.hi || (tok + pa.page_rows <= seg.first.lo && tok >= c.sinks)) return;
       page = 0;
-      row = 0;
-      if (j >= n_tiles) return;
-      const int tok = span.tile(i_begin + j) * BN + lane * pa.page_rows;
-      if (!a.paged) {
-        row = s.k_begin + tok;
-      } else if (lane < pa.pages_per_tile) {
+      if (a.paged) {
         const int pg = tok / a.block_size;
         row = tok - pg * a.block_size;
-        page = cache_page(c, bt_row, min(pg, last_page));  // past the sequence: any valid page (those keys are masked)
+        page = cache_page(c, a.block_table + (int64_t)seg.b * a.bt_stride, pg);
       }
     };
-    int page, row;
-    lookup(0, page, row);
+    uint32_t item = 0, kv = 0;     // items and K/V tiles so far
     bool ok = true;
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      int npage, nrow;
-      lookup(j + 1, npage, nrow);
-      for (int which = 0; which < 2; ++which) {
-        const CUtensorMap* tm = which ? &tmap_v : &tmap_k;
-        if constexpr (kWiden) {
-          const uint32_t n = 2 * j + which;
-          const int slot = n & 1;
-          if (!wwait(&r_empty[slot], ((n >> 1) & 1) ^ 1)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) mbar_expect_tx(&r_full[slot], RAW_BYTES);
-          __syncwarp();
-          if (lane < pa.pages_per_tile)
-            tma_load_4d(sR + slot * RAW_BYTES + lane * pa.page_rows * 128, tm, &r_full[slot], 0, hk, row, page);
-        } else {
-          const int stg = j & 1;
-          uint64_t* full = which ? &v_full[stg] : &k_full[stg];
-          if (!wwait(which ? &v_empty[stg] : &k_empty[stg], ((j >> 1) & 1) ^ 1)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) mbar_expect_tx(full, TILE_BYTES);
-          __syncwarp();
-          if (lane < pa.pages_per_tile) {
-            uint8_t* dst = (which ? sV : sK) + stg * TILE_BYTES + lane * pa.page_rows * 128;
-            for (int hf = 0; hf < 2; ++hf) tma_load_4d(dst + hf * HALF_BYTES, tm, full, hf * 64, hk, row, page);
+    do {
+      int page, row;
+      lookup(seg.lo, page, row);
+      if (item > 0 && !wwait(q_empty, (item - 1) & 1)) break;
+      if (lane == 0) {
+        mbar_expect_tx(q_full, seg.nt * 2 * pa.tokens * a.group * 128);
+        for (int t = 0; t < seg.nt; ++t)
+          for (int hf = 0; hf < 2; ++hf)
+            tma_load_3d(sQ + t * TILE_BYTES + hf * HALF_BYTES, &tmap_q, q_full, hf * 64, seg.hk * a.group,
+                        seg.s.q_begin + seg.m0 + t * pa.tokens);
+      }
+      __syncwarp();
+      ++item;
+      for (int j = seg.lo; j < seg.hi && ok; ++j, ++kv) {
+        int npage = -1, nrow = 0;
+        if (j + 1 < seg.hi) lookup(j + 1, npage, nrow);   // in flight while this tile is issued
+        const int pages = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        for (int which = 0; which < 2; ++which) {
+          const CUtensorMap* tm = which ? &tmap_v : &tmap_k;
+          if constexpr (kWiden) {
+            const uint32_t n = 2 * kv + which, slot = n % RAW_SLOTS;
+            if (!wwait(&r_empty[slot], ((n / RAW_SLOTS) & 1) ^ 1)) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) mbar_expect_tx(&r_full[slot], pages * pa.page_rows * 128);
+            __syncwarp();
+            if (page >= 0) tma_load_4d(sR + slot * RAW_BYTES + lane * pa.page_rows * 128, tm, &r_full[slot], 0, seg.hk, row, page);
+          } else {
+            const int stg = kv & 1;
+            uint64_t* full = which ? &v_full[stg] : &k_full[stg];
+            if (!wwait(which ? &v_empty[stg] : &k_empty[stg], ((kv >> 1) & 1) ^ 1)) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) mbar_expect_tx(full, pages * pa.page_rows * 256);
+            __syncwarp();
+            if (page >= 0) {
+              uint8_t* dst = (which ? sV : sK) + stg * TILE_BYTES + lane * pa.page_rows * 128;
+              for (int hf = 0; hf < 2; ++hf) tma_load_4d(dst + hf * HALF_BYTES, tm, full, hf * 64, seg.hk, row, page);
+            }
           }
         }
+        page = npage;
+        row = nrow;
       }
-      page = npage;
-      row = nrow;
-    }
-  } else if (n_steps > 0 && warp >= MMA_WARP0 && warp < MMA_WARP0 + NT) {
+    } while (ok && next_segment(pa, table, seg));
+  } else if (warp >= MMA_WARP0 && warp < MMA_WARP0 + NT) {
     // ================================ scores of one tile ==========================
     const int t = warp - MMA_WARP0;
     if (lane == 0) {
@@ -242,304 +369,364 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       const uint32_t q_lo = (uint32_t)umma_desc_sw128(smem_u32(sQ + t * TILE_BYTES), 0, 1024);
       const uint32_t k_lo0 = (uint32_t)umma_desc_sw128(smem_u32(sK), 0, 1024);
       const uint32_t s_tmem = tmem_base + t * 128;
-      bool ok = wait1(kConvQ ? q_ready : q_full, 0);
-      for (int i = 0; i < n_steps && ok; ++i) {
-        const int j = i >> 1, stg = j & 1;
-        if (!(i & 1) && !wait1(&k_full[stg], (j >> 1) & 1)) break;
-        // the previous step's scores must have been read out
-        if (i > 0 && !wait1(&s_free[t], (i - 1) & 1)) break;
-        // the softmax warps will store P(i) over the buffer that the P V of step i - 2 reads
-        if (i >= 2 && !wait1(&o_done[t * 2 + (i & 1)], ((i - 2) >> 1) & 1)) break;
-        tc_fence_after();
-        const uint32_t k_lo = k_lo0 + stg * (TILE_BYTES >> 4) + (i & 1) * (STEP * 128 >> 4);
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = ((k >> 2) * HALF_BYTES + (k & 3) * 32) >> 4;
-          mma_f16_ss_lohi(s_tmem, q_lo + off, k_lo + off, desc_hi, idesc, k != 0 ? 1u : 0u);
+      uint32_t item = 0, used = 0, unit0 = 0, g = 0;   // items, items of this tile, stages filled and this tile's steps so far
+      bool ok = true;
+      do {
+        const bool on = t < seg.nt;
+        if (on) {
+          if (!(kConvQ ? wait1(&q_ready[t], used & 1) : wait1(q_full, item & 1))) break;
+          ++used;
         }
-        tc_commit(&s_full[t]);
-        if ((i & 1) || i == n_steps - 1) tc_commit(&k_empty[stg]);
-      }
+        ++item;
+        for (int i = 0; i < seg.steps && ok; ++i) {
+          const uint32_t unit = unit0 + (uint32_t)(kWiden ? i : i >> 1), stg = unit & 1;
+          if ((kWiden || !(i & 1)) && !wait1(&k_full[stg], (unit >> 1) & 1)) {
+            ok = false;
+            break;
+          }
+          if (on) {
+            // the previous step's scores must have been read out; and the softmax warps will store P over the buffer that the
+            // P V two steps back reads (steps 0 and 1: the softmax warps waited for the previous item's last P V)
+            if ((g > 0 && !wait1(&s_free[t], (g - 1) & 1)) || (i >= 2 && !wait1(&o_done[t * 2 + (g & 1)], ((g - 2) >> 1) & 1))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t k_lo = k_lo0 + stg * (UNIT >> 4) + (kWiden ? 0 : (i & 1) * (STEP * 128 >> 4));
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+              mma_f16_ss_lohi(s_tmem, q_lo + (((k >> 2) * HALF_BYTES + (k & 3) * 32) >> 4),
+                              k_lo + (((k >> 2) * UNIT_HALF + (k & 3) * 32) >> 4), desc_hi, idesc, k != 0 ? 1u : 0u);
+            tc_commit(&s_full[t]);
+            ++g;
+          }
+          if (kWiden || (i & 1) || i == seg.steps - 1) tc_commit(&k_empty[stg]);
+          if (i == seg.steps - 1) tc_commit(q_empty);
+        }
+        unit0 += (uint32_t)(kWiden ? seg.steps : seg.hi - seg.lo);
+      } while (ok && next_segment(pa, table, seg));
     }
-  } else if (n_steps > 0 && warp == MMA_WARP0 + 2) {
+  } else if (warp == MMA_WARP0 + 2) {
     // ================================ O += P V of both tiles =======================
     if (lane == 0) {
       const uint32_t idesc = umma_idesc_f16(kBf16, false, true, BM, HD);   // V is MN-major
       const uint32_t desc_hi = (uint32_t)(umma_desc_sw128(0, 0, 1024) >> 32);
-      const uint32_t v_lo0 = (uint32_t)umma_desc_sw128(smem_u32(sV), HALF_BYTES, 1024);
+      const uint32_t v_lo0 = (uint32_t)umma_desc_sw128(smem_u32(sV), UNIT_HALF, 1024);
+      uint32_t used[2] = {0, 0}, unit0 = 0, g[2] = {0, 0};
       bool ok = true;
-      for (int i = 0; i < n_steps && ok; ++i) {
-        const int j = i >> 1, stg = j & 1;
-        if (!(i & 1) && !wait1(&v_full[stg], (j >> 1) & 1)) break;
-        const uint32_t v_lo = v_lo0 + stg * (TILE_BYTES >> 4) + (i & 1) * (4 * 2048 >> 4);
-        for (int t = 0; t < NT && ok; ++t) {
-          if (!wait1(&p_ready[t * 2 + (i & 1)], (i >> 1) & 1)) {
+      do {
+        for (int i = 0; i < seg.steps && ok; ++i) {
+          const uint32_t unit = unit0 + (uint32_t)(kWiden ? i : i >> 1), stg = unit & 1;
+          if ((kWiden || !(i & 1)) && !wait1(&v_full[stg], (unit >> 1) & 1)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint32_t p_tmem = tmem_base + t * 128 + STEP + (i & 1) * 32;
-          const uint32_t o_tmem = tmem_base + 256 + t * 128;
+          const uint32_t v_lo = v_lo0 + stg * (UNIT >> 4) + (kWiden ? 0 : (i & 1) * (4 * 2048 >> 4));
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_f16_ts_lohi(o_tmem, p_tmem + k * 8, v_lo + k * (2048 >> 4), desc_hi, idesc, (i > 0 || k > 0) ? 1u : 0u);
-          tc_commit(&o_done[t * 2 + (i & 1)]);
+          for (int t = 0; t < 2; ++t) {
+            if (t >= seg.nt || !ok) continue;
+            const uint32_t par = g[t] & 1;
+            // the first product of an item overwrites O: the previous item's must have been read out
+            if (!wait1(&p_ready[t * 2 + par], (g[t] >> 1) & 1) || (i == 0 && used[t] > 0 && !wait1(&o_free[t], (used[t] - 1) & 1))) {
+              ok = false;
+              continue;
+            }
+            tc_fence_after();
+            const uint32_t p_tmem = tmem_base + t * 128 + STEP + par * 32;
+            const uint32_t o_tmem = tmem_base + 256 + t * 128;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_f16_ts_lohi(o_tmem, p_tmem + k * 8, v_lo + k * (2048 >> 4), desc_hi, idesc, (i > 0 || k > 0) ? 1u : 0u);
+            tc_commit(&o_done[t * 2 + par]);
+            ++g[t];
+          }
+          if (ok && (kWiden || (i & 1) || i == seg.steps - 1)) tc_commit(&v_empty[stg]);
         }
-        if (ok && ((i & 1) || i == n_steps - 1)) tc_commit(&v_empty[stg]);
-      }
+        unit0 += (uint32_t)(kWiden ? seg.steps : seg.hi - seg.lo);
+        ++used[0];
+        used[1] += seg.nt > 1;
+      } while (ok && next_segment(pa, table, seg));
     }
-  } else if (kWiden && n_steps > 0 && warp >= CONV_WARP0) {
+  } else if (kWiden && warp >= CONV_WARP0) {
     // ================================ widening =====================================
     if constexpr (kWiden) {
       const int w = warp - CONV_WARP0;
-      bool ok = true;
-      if constexpr (kConvQ) {
-        ok = wwait(q_full, 0);
-        if (ok) {
-          const int r = w * 32 + lane;   // a thread per row
-          for (int t = 0; t < NT; ++t) {
-            uint8_t* q = sQ + t * TILE_BYTES + r * 128;
-            float top = 0.f;
-#pragma unroll 4
-            for (int ch = 0; ch < 16; ++ch) {
-              float f[8];
-              Vec16<T>::unpack(*reinterpret_cast<const uint4*>(q + (ch >> 3) * HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4)), f);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
-            }
-            float up, down;
-            row_power(top, up, down);
-#pragma unroll 4
-            for (int ch = 0; ch < 16; ++ch) {
-              uint4* at = reinterpret_cast<uint4*>(q + (ch >> 3) * HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4));
-              float f[8];
-              Vec16<T>::unpack(*at, f);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) f[e] *= up;
-              *at = Vec16<__half>::pack(f);
-            }
-            sDown[t * BM + r] = down;
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(q_ready);
-        }
-      }
       // lane = (row of four, 16-byte piece): eight lanes read one row's 128 bytes and write one row's 128 bytes of
       // either half at a time (pieces 4-7 store their second eight values first), without bank conflicts
       const int ch = lane & 7, sub = lane >> 3;
-      for (int n = 0; n < 2 * n_tiles && ok; ++n) {
-        const int j = n >> 1, stg = j & 1, slot = n & 1;
-        const bool is_v = n & 1;
-        if (!wwait(&r_full[slot], j & 1) || !wwait(is_v ? &v_empty[stg] : &k_empty[stg], ((j >> 1) & 1) ^ 1)) break;
-        const uint8_t* src = sR + slot * RAW_BYTES;
-        uint8_t* dst = (is_v ? sV : sK) + stg * TILE_BYTES + (ch >> 2) * HALF_BYTES;
-        const int j0 = span.tile(i_begin + j) * BN;
-        const bool zero = is_v && (j0 + BN > cta_last.hi || (j0 < cta_first.lo && j0 + BN > c.sinks));
+      uint32_t n = 0, unit0 = 0;     // 8-bit tiles and units so far
+      bool ok = true;
+      do {
+        for (int j = seg.lo; j < seg.hi && ok; ++j) {
+          const int j0 = seg.span.tile(j) * BN;
+          for (int which = 0; which < 2 && ok; ++which, ++n) {
+            const uint32_t slot = n % RAW_SLOTS;
+            uint64_t* full = which ? v_full : k_full;
+            uint64_t* empty = which ? v_empty : k_empty;
+            if (!wwait(&r_full[slot], (n / RAW_SLOTS) & 1)) {
+              ok = false;
+              break;
+            }
+            const bool zero = which && (j0 + BN > seg.last.hi || (j0 < seg.first.lo && j0 + BN > c.sinks));
+            for (int h = 0; h < 2; ++h) {
+              const int i = 2 * (j - seg.lo) + h;
+              if (i >= seg.steps) break;             // the half of the last tile that nobody sees
+              const uint32_t unit = unit0 + (uint32_t)i, stg = unit & 1;
+              if (!wwait(&empty[stg], ((unit >> 1) & 1) ^ 1)) {
+                ok = false;
+                break;
+              }
+              const uint8_t* src = sR + slot * RAW_BYTES + h * (STEP * 128);
+              uint8_t* dst = (which ? sV : sK) + stg * UNIT + (ch >> 2) * UNIT_HALF;
+              uint4 raw[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int r = w * 32 + k * 4 + sub;
-          uint4 raw = *reinterpret_cast<const uint4*>(src + r * 128 + ((ch ^ (r & 7)) << 4));
-          if (zero) {   // V rows that no row of the CTA sees must not reach the products
-            const int col = j0 + r;
-            if (col >= cta_last.hi || (col < cta_first.lo && col >= c.sinks)) raw = make_uint4(0, 0, 0, 0);
+              for (int k = 0; k < 4; ++k) {
+                const int r = w * 16 + k * 4 + sub;
+                raw[k] = *reinterpret_cast<const uint4*>(src + r * 128 + ((ch ^ (r & 7)) << 4));
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int r = w * 16 + k * 4 + sub;
+                if (zero) {   // V rows that no row of the item sees must not reach the products
+                  const int col = j0 + h * STEP + r;
+                  if (col >= seg.last.hi || (col < seg.first.lo && col >= c.sinks)) raw[k] = make_uint4(0, 0, 0, 0);
+                }
+                uint4 lo, hi;
+                fp8x4_to_f16x4<KIND>(raw[k].x, lo.x, lo.y);
+                fp8x4_to_f16x4<KIND>(raw[k].y, lo.z, lo.w);
+                fp8x4_to_f16x4<KIND>(raw[k].z, hi.x, hi.y);
+                fp8x4_to_f16x4<KIND>(raw[k].w, hi.z, hi.w);
+                const bool swap = ch & 4;
+                const int c0 = (ch & 3) * 2 + (swap ? 1 : 0);
+                uint8_t* row = dst + r * 128;
+                *reinterpret_cast<uint4*>(row + ((c0 ^ (r & 7)) << 4)) = swap ? hi : lo;
+                *reinterpret_cast<uint4*>(row + (((c0 ^ 1) ^ (r & 7)) << 4)) = swap ? lo : hi;
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&full[stg]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&r_empty[slot]);
           }
-          uint4 lo, hi;
-          fp8x4_to_f16x4<KIND>(raw.x, lo.x, lo.y);
-          fp8x4_to_f16x4<KIND>(raw.y, lo.z, lo.w);
-          fp8x4_to_f16x4<KIND>(raw.z, hi.x, hi.y);
-          fp8x4_to_f16x4<KIND>(raw.w, hi.z, hi.w);
-          const bool swap = ch & 4;
-          const int c0 = (ch & 3) * 2 + (swap ? 1 : 0);
-          uint8_t* row = dst + r * 128;
-          *reinterpret_cast<uint4*>(row + ((c0 ^ (r & 7)) << 4)) = swap ? hi : lo;
-          *reinterpret_cast<uint4*>(row + (((c0 ^ 1) ^ (r & 7)) << 4)) = swap ? lo : hi;
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(is_v ? &v_full[stg] : &k_full[stg]);
-          mbar_arrive(&r_empty[slot]);
-        }
-      }
+        unit0 += (uint32_t)seg.steps;
+      } while (ok && next_segment(pa, table, seg));
     }
   } else if (warp < 4 * NT) {
     // ================================ softmax / epilogue ===========================
     const int t = warp >> 2;
     const int r = (warp & 3) * 32 + lane;     // row inside the tile == TMEM lane
+    const int in_tok = r / a.group, in_head = r - in_tok * a.group;
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_addr + t * 128;
     const uint32_t o_addr = tmem_base + lane_addr + 256 + t * 128;
-    const int tile_first = m0 + t * pa.tokens;
-    const int tok = tile_first + r / a.group, h = hk * a.group + r % a.group;
-    const bool valid = r < pa.tokens * a.group && tok < s.q_len;
-    const int64_t qtok = s.q_begin + tok;
-    const RowMask mask = row_mask(c, s.k_len, tok + shift);
-    // what the first and the last row of the tile see: steps between need no mask
-    const RowMask first = row_mask(c, s.k_len, tile_first + shift);
-    const RowMask last = row_mask(c, s.k_len, min(tile_first + pa.tokens, s.q_len) - 1 + shift);
-    float m_used = -INFINITY, l_run = 0.f;
-    float scale = a.scale_log2 * cache_scale(c.k_scale, c.ks_batch, c.ks_head, b, hk);
+    PartRecord rec{-1, 0, 0, 0};
+    uint32_t item = 0, kv = 0, g = 0;         // items, K/V tiles and this tile's steps so far
     bool ok = true;
-    if constexpr (kConvQ) {
-      if (n_steps > 0) {
-        ok = wwait(q_ready, 0);
-        scale *= sDown[t * BM + r];
-      }
-    }
-    const bool odd_scale = !(scale > 0.f);    // a K scale that is zero, negative or NaN: scale the scores first
-
-    for (int i = 0; i < n_steps && ok; ++i) {
-      const uint32_t p_addr = s_addr + STEP + (i & 1) * 32;
-      if (!wwait(&s_full[t], i & 1)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      float sv[64];
-      tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
-      tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[t]);   // the next step's scores may be computed into the same columns
-      float sc = scale;
-      if (odd_scale) {
-#pragma unroll
-        for (int e = 0; e < 64; ++e) sv[e] *= scale;
-        sc = 1.f;
-      }
-      const int col0 = span.tile(i_begin + (i >> 1)) * BN + (i & 1) * STEP;
-      if (col0 + STEP > first.hi || (col0 < last.lo && col0 + STEP > c.sinks)) {
-#pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (mask.dead(col0 + e)) sv[e] = -INFINITY;
-      }
-      float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
-#pragma unroll
-      for (int e = 4; e < 64; e += 8) {
-        m4[0] = max3(m4[0], sv[e], sv[e + 1]);
-        m4[1] = max3(m4[1], sv[e + 2], sv[e + 3]);
-        if (e + 4 < 64) {
-          m4[2] = max3(m4[2], sv[e + 4], sv[e + 5]);
-          m4[3] = max3(m4[3], sv[e + 6], sv[e + 7]);
+    do {
+      if (t >= seg.nt) {                      // no token in this tile
+        if constexpr (kConvQ) {               // but no phase of q_full is left out: its parity could not tell them apart
+          if (!wwait(q_full, item & 1)) break;
         }
+        ++item;
+        kv += (uint32_t)(seg.hi - seg.lo);
+        continue;
       }
-      const float m_tile = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * sc;   // sc > 0; -inf stays -inf
-      const bool raise = m_tile > m_used + kRescaleThreshold || (m_used == -INFINITY && m_tile > -INFINITY);
-      if (i > 0 && __any_sync(0xffffffffu, raise)) {
-        // every P V issued so far must have landed before O is touched
-        if (!wwait(&o_done[t * 2 + ((i - 1) & 1)], ((i - 1) >> 1) & 1)) {
+      const int tile_first = seg.m0 + t * pa.tokens;
+      const int tok = tile_first + in_tok, h = seg.hk * a.group + in_head;
+      const bool valid = in_tok < pa.tokens && tok < seg.s.q_len;
+      const int k_len = seg.s.k_len;
+      const RowMask mask = row_mask(c, k_len, tok + seg.shift);
+      // what the first and the last row of the tile see: steps between need no mask
+      const RowMask first = row_mask(c, k_len, tile_first + seg.shift);
+      const RowMask last = row_mask(c, k_len, min(tile_first + pa.tokens, seg.s.q_len) - 1 + seg.shift);
+      float m_used = -INFINITY, l_run = 0.f;
+      float scale = a.scale_log2 * cache_scale(c.k_scale, c.ks_batch, c.ks_head, seg.b, seg.hk);
+      const float v_scale = cache_scale(c.v_scale, c.vs_batch, c.vs_head, seg.b, seg.hk);
+      if constexpr (kConvQ) {
+        // my row of Q, from bf16 to fp16 with its power of two
+        if (!wwait(q_full, item & 1)) break;
+        uint8_t* q = sQ + t * TILE_BYTES + r * 128;
+        float top = 0.f;
+#pragma unroll 4
+        for (int ch = 0; ch < 16; ++ch) {
+          float f[8];
+          Vec16<T>::unpack(*reinterpret_cast<const uint4*>(q + (ch >> 3) * HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4)), f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+        }
+        float up, down;
+        row_power(top, up, down);
+#pragma unroll 4
+        for (int ch = 0; ch < 16; ++ch) {
+          uint4* at = reinterpret_cast<uint4*>(q + (ch >> 3) * HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4));
+          float f[8];
+          Vec16<T>::unpack(*at, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] *= up;
+          *at = Vec16<__half>::pack(f);
+        }
+        scale *= down;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_ready[t]);
+      }
+      ++item;
+      const bool odd_scale = !(scale > 0.f);  // a K scale that is zero, negative or NaN: scale the scores first
+
+      for (int i = 0; i < seg.steps; ++i, ++g) {
+        const uint32_t p_addr = s_addr + STEP + (g & 1) * 32;
+        if (!wwait(&s_full[t], g & 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const float f = raise ? ex2(m_used - m_tile) : 1.0f;
-#pragma unroll 1
-        for (int q = 0; q < 8; ++q) {
-          uint32_t o[16];
-          tmem_ld16(o_addr + q * 16, o);
-          tmem_ld_wait();
+        float sv[64];
+        tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
+        tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);   // the next step's scores may be computed into the same columns
+        float sc = scale;
+        if (odd_scale) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st16(o_addr + q * 16, o);
+          for (int e = 0; e < 64; ++e) sv[e] *= scale;
+          sc = 1.f;
         }
-        l_run *= f;
-      }
-      if (raise) m_used = m_tile;
-      const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
-      if constexpr (!kWiden) {
-        // V rows of this step that no row of the CTA sees must not reach the products: zeroed in place, by each tile's
-        // warps for themselves (the other tile writes the same zeros)
-        if (col0 + STEP > cta_last.hi || (col0 < cta_first.lo && col0 + STEP > c.sinks)) {
-          const int j = i >> 1, stg = j & 1;
-          if (!wwait(&v_full[stg], (j >> 1) & 1)) {
+        const int col0 = seg.span.tile(seg.lo + (i >> 1)) * BN + (i & 1) * STEP;
+        if (col0 + STEP > first.hi || (col0 < last.lo && col0 + STEP > c.sinks)) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (mask.dead(col0 + e)) sv[e] = -INFINITY;
+        }
+        float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
+#pragma unroll
+        for (int e = 4; e < 64; e += 8) {
+          m4[0] = max3(m4[0], sv[e], sv[e + 1]);
+          m4[1] = max3(m4[1], sv[e + 2], sv[e + 3]);
+          if (e + 4 < 64) {
+            m4[2] = max3(m4[2], sv[e + 4], sv[e + 5]);
+            m4[3] = max3(m4[3], sv[e + 6], sv[e + 7]);
+          }
+        }
+        const float m_tile = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * sc;   // sc > 0; -inf stays -inf
+        const bool raise = m_tile > m_used + kRescaleThreshold || (m_used == -INFINITY && m_tile > -INFINITY);
+        if (i > 0 && __any_sync(0xffffffffu, raise)) {
+          // every P V issued so far must have landed before O is touched
+          if (!wwait(&o_done[t * 2 + ((g - 1) & 1)], ((g - 1) >> 1) & 1)) {
             ok = false;
             break;
           }
-          uint8_t* vt = sV + stg * TILE_BYTES + (i & 1) * STEP * 128;
-          for (int at = r; at < STEP * 16; at += 128) {
-            const int row = at / 16, ch = at % 16, col = col0 + row;
-            if (col >= cta_last.hi || (col < cta_first.lo && col >= c.sinks))
-              *reinterpret_cast<uint4*>(vt + (ch >> 3) * HALF_BYTES + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
-      }
-      float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-      {
-        const uint64_t sc2 = pack2f(sc, sc), ng2 = pack2f(neg_m, neg_m);
-#pragma unroll
-        for (int e = 0; e < 64; e += 2) fma2(sv[e], sv[e + 1], sc2, ng2);
-      }
-#pragma unroll
-      for (int e = 0; e < 64; ++e) sv[e] = ex2(sv[e]);
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = sv[q * 32 + 2 * e], p1 = sv[q * 32 + 2 * e + 1];
-          add2(sum4[(e & 1) * 2], sum4[(e & 1) * 2 + 1], p0, p1);
-          pk[e] = Pair<M>::pack(p0, p1);
-        }
-        tmem_st16(p_addr + q * 16, pk);
-      }
-      l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[t * 2 + (i & 1)]);
-    }
-
-    // ---- epilogue: normalise my row of O and write it out
-    if (ok && n_steps > 0) {
-      ok = wwait(&o_done[t * 2 + ((n_steps - 1) & 1)], ((n_steps - 1) >> 1) & 1);
-      tc_fence_after();
-    }
-    if (ok) {
-      // a NaN sum stays one: only a row that saw nothing is set to zero
-      const float inv = l_run == 0.f ? 0.f : cache_scale(c.v_scale, c.vs_batch, c.vs_head, b, hk) / l_run;
-      const bool parts = a.num_splits > 1;
-      char* orow = parts ? reinterpret_cast<char*>(a.ws_o + (((int64_t)split * a.total_q + qtok) * a.H + h) * HD)
-                         : reinterpret_cast<char*>(a.out) + (qtok * a.o_rs + (int64_t)h * a.o_hs) * 2;
-      // an empty split's partial output is never read (its weight is zero)
-      if (n_steps > 0 || !parts) {
+          tc_fence_after();
+          const float f = raise ? ex2(m_used - m_tile) : 1.0f;
 #pragma unroll 1
-        for (int q = 0; q < 8; ++q) {
-          uint32_t o[16];
-          if (n_steps > 0) {
+          for (int q = 0; q < 8; ++q) {
+            uint32_t o[16];
             tmem_ld16(o_addr + q * 16, o);
             tmem_ld_wait();
-          } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = 0u;
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(o_addr + q * 16, o);
           }
-          float f[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv;
-          if (valid && parts) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<float4*>(orow + q * 64 + e * 16) = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-          } else if (valid) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              *reinterpret_cast<uint4*>(orow + q * 32 + e * 16) =
-                  make_uint4(Pair<T>::pack(f[8 * e], f[8 * e + 1]), Pair<T>::pack(f[8 * e + 2], f[8 * e + 3]),
-                             Pair<T>::pack(f[8 * e + 4], f[8 * e + 5]), Pair<T>::pack(f[8 * e + 6], f[8 * e + 7]));
-          }
-          __syncwarp();
+          l_run *= f;
         }
+        if (raise) m_used = m_tile;
+        const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+        if constexpr (!kWiden) {
+          // V rows of this step that no row of the item sees must not reach the products: zeroed in place, by each tile's
+          // warps for themselves (the other tile writes the same zeros)
+          if (col0 + STEP > seg.last.hi || (col0 < seg.first.lo && col0 + STEP > c.sinks)) {
+            const uint32_t tile = kv + (uint32_t)(i >> 1), stg = tile & 1;
+            if (!wwait(&v_full[stg], (tile >> 1) & 1)) {
+              ok = false;
+              break;
+            }
+            uint8_t* vt = sV + stg * UNIT + (i & 1) * STEP * 128;
+            for (int at = r; at < STEP * 16; at += 128) {
+              const int row = at / 16, ch = at % 16, col = col0 + row;
+              if (col >= seg.last.hi || (col < seg.first.lo && col >= c.sinks))
+                *reinterpret_cast<uint4*>(vt + (ch >> 3) * HALF_BYTES + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+        }
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+        {
+          const uint64_t sc2 = pack2f(sc, sc), ng2 = pack2f(neg_m, neg_m);
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) fma2(sv[e], sv[e + 1], sc2, ng2);
+        }
+#pragma unroll
+        for (int e = 0; e < 64; ++e) sv[e] = ex2(sv[e]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = sv[q * 32 + 2 * e], p1 = sv[q * 32 + 2 * e + 1];
+            add2(sum4[(e & 1) * 2], sum4[(e & 1) * 2 + 1], p0, p1);
+            pk[e] = Pair<M>::pack(p0, p1);
+          }
+          tmem_st16(p_addr + q * 16, pk);
+        }
+        l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[t * 2 + (g & 1)]);
       }
-      if (valid) {
+      if (!ok) break;
+      kv += (uint32_t)(seg.hi - seg.lo);
+
+      // ---- epilogue: normalise my row of O and write it out
+      if (!wwait(&o_done[t * 2 + ((g - 1) & 1)], ((g - 1) >> 1) & 1)) break;
+      tc_fence_after();
+      // a NaN sum stays one: only a row that saw nothing is set to zero
+      const float inv = l_run == 0.f ? 0.f : v_scale / l_run;
+      const bool whole = seg.lo == 0 && seg.hi == seg.n;
+      const int64_t qtok = seg.s.q_begin + tok;
+      const int64_t part = ((int64_t)2 * blockIdx.x + (seg.lo == 0 ? 1 : 0)) * (NT * BM) + t * BM + r;
+      if (!whole && seg.lo == 0)   // the last of the run: each later CTA takes `run` tiles of the rest
+        rec = PartRecord{seg.hk, 1 + (seg.n - seg.hi + run - 1) / run, seg.s.q_begin + seg.m0, seg.s.q_len - seg.m0};
+      char* orow = whole ? reinterpret_cast<char*>(a.out) + (qtok * a.o_rs + (int64_t)h * a.o_hs) * 2
+                         : reinterpret_cast<char*>(pa.part_o + part * HD);
+#pragma unroll 1
+      for (int q = 0; q < 8; ++q) {
+        uint32_t o[16];
+        tmem_ld16(o_addr + q * 16, o);
+        tmem_ld_wait();
+        if (q == 7) {   // my row is in registers: the next item's first product may overwrite it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_free[t]);
+        }
+        float f[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv;
+        if (valid && !whole) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<float4*>(orow + q * 64 + e * 16) = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+        } else if (valid) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<uint4*>(orow + q * 32 + e * 16) =
+                make_uint4(Pair<T>::pack(f[8 * e], f[8 * e + 1]), Pair<T>::pack(f[8 * e + 2], f[8 * e + 3]),
+                           Pair<T>::pack(f[8 * e + 4], f[8 * e + 5]), Pair<T>::pack(f[8 * e + 6], f[8 * e + 7]));
+        }
+        __syncwarp();
+      }
+      if (valid && (!whole || a.lse)) {
         const float lse2 = l_run == 0.f ? -INFINITY : m_used + log2f(l_run);
-        if (parts)
-          a.ws_lse[((int64_t)split * a.H + h) * a.total_q + qtok] = lse2;
-        else if (a.lse)
+        if (!whole)
+          pa.part_lse[part] = lse2;
+        else
           a.lse[(int64_t)h * a.total_q + qtok] = l_run == 0.f ? INFINITY : lse2 * 0.6931471805599453f;
       }
-    }
+    } while (next_segment(pa, table, seg));
+    if (tid == 0) pa.record[blockIdx.x] = rec;
   }
 
   // ================================ teardown ======================================
@@ -553,6 +740,60 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     tc_fence_after();
     tmem_dealloc(tmem_base, TMEM_COLS);
   }
+}
+
+// Joins the parts of the items that runs cut: warp w of block (i, y) does row 8 y + w of the item whose start, but not end, CTA i
+// holds: its tail part, then the head parts of the CTAs after it, in order.
+constexpr int kJoinWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_cache_join_rows_kernel(ChunkArgs pa, int ctas) {
+  const AttnArgs& a = pa.c.a;
+  asm volatile("griddepcontrol.wait;" ::: "memory");              // launched early: the parts are complete after this
+  const int i = blockIdx.x, lane = threadIdx.x & 31;
+  const PartRecord rec = pa.record[i];
+  if (*reinterpret_cast<volatile int*>(a.status) != 0) return;   // the parts and the records may be missing
+  if (rec.hk < 0) return;
+  const int rows = pa.tiles * BM;
+  const int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
+  const int in_tile = row % BM, in_tok = in_tile / a.group;
+  const int tok = row / BM * pa.tokens + in_tok;
+  if (in_tok >= pa.tokens || tok >= rec.tokens) return;
+  const int n = min(rec.parts, ctas - i);
+  auto slot = [&](int k) { return (int64_t)(k == 0 ? 2 * i + 1 : 2 * (i + k)) * rows + row; };
+  float m = -INFINITY;
+  for (int k = lane; k < n; k += 32) m = fmaxf(m, pa.part_lse[slot(k)]);
+  m = warp_max(m);
+  const float ms = m == -INFINITY ? 0.f : m;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float wsum = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < n; ++k) {
+    const float w = exp2f(pa.part_lse[slot(k)] - ms);
+    const float4 o = *reinterpret_cast<const float4*>(pa.part_o + slot(k) * HD + lane * 4);
+    wsum += w;
+    if (w != 0.f) {   // NaN goes on
+      acc.x += w * o.x;
+      acc.y += w * o.y;
+      acc.z += w * o.z;
+      acc.w += w * o.w;
+    }
+  }
+  const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
+  const int64_t qtok = rec.q_row + tok;
+  const int h = rec.hk * a.group + in_tile - in_tok * a.group;
+  uint2 w2;
+  w2.x = Pair<T>::pack(acc.x * inv, acc.y * inv);
+  w2.y = Pair<T>::pack(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + qtok * a.o_rs + (int64_t)h * a.o_hs + lane * 4) = w2;
+  if (a.lse && lane == 0)
+    a.lse[(int64_t)h * a.total_q + qtok] = wsum == 0.f ? INFINITY : (m + log2f(wsum)) * 0.6931471805599453f;
+}
+
+// Q tiles of an item, tokens of a tile and items (for each KV head) of the longest chunk.
+void chunk_shape(int64_t max_q, int64_t group, int* tiles, int* tokens, int64_t* num_mb) {
+  *tokens = (int)(BM / group);
+  *tiles = max_q > *tokens ? 2 : 1;
+  *num_mb = (max_q + *tiles * *tokens - 1) / (*tiles * *tokens);
 }
 
 template <typename T, int KIND>
@@ -588,10 +829,24 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
     FG_CUDA_OK(cudaFuncSetAttribute(attn_cache_chunk_kernel<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_dev = dev;
   }
-  const int64_t ctas = (int64_t)pa.num_mb * a.batch * a.Hk * a.num_splits;
-  if (ctas > 2147483647LL) return fail(FG_ERR_TOO_LARGE, "flash_attn_cache: too many query blocks");
-  attn_cache_chunk_kernel<T, KIND><<<(unsigned)ctas, threads_of(KIND), smem, st>>>(tq, maps[0], maps[1], pa);
+  const int ctas = num_sms();
+  pa.part_o = a.ws_o;
+  pa.part_lse = pa.part_o + (int64_t)2 * ctas * pa.tiles * BM * HD;
+  pa.record = reinterpret_cast<PartRecord*>(pa.part_lse + (int64_t)2 * ctas * pa.tiles * BM);
+  attn_cache_chunk_kernel<T, KIND><<<ctas, threads_of(KIND), smem, st>>>(tq, maps[0], maps[1], pa);
   FG_CHECK_LAUNCH("attn_cache_chunk_kernel");
+  // Launched while the kernel above still runs (programmatic dependent launch); it waits for its end on the device.
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, (unsigned)(pa.tiles * BM / kJoinWarps));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  FG_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_cache_join_rows_kernel<T>, pa, ctas));
+  FG_CHECK_LAUNCH("attn_cache_join_rows_kernel");
   return FG_OK;
 }
 
@@ -604,13 +859,22 @@ int launch_kind(ChunkArgs& pa, int kind, cudaStream_t st) {
 
 }  // namespace
 
+// Bytes of workspace: a head and a tail part, and a record, for each CTA.  0: more tiles than the kernel counts in 32 bits.
+int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t tiles_k, int sms) {
+  int tiles, tokens;
+  int64_t num_mb;
+  chunk_shape(max_q, group, &tiles, &tokens, &num_mb);
+  if (batch * num_mb > 2147483647LL / 2 || batch * num_mb * heads_k > 2147483647LL / tiles_k) return 0;
+  return (int64_t)sms * (2 * tiles * BM * (HD + 1) * 4 + (int64_t)sizeof(PartRecord));
+}
+
 int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st) {
   ChunkArgs pa;
   pa.c = c;
   if (!c.a.status) return fail(FG_ERR_CUDA, "flash_attn_cache: device status word unavailable");
-  pa.tokens = BM / c.a.group;
-  pa.tiles = c.a.max_q > pa.tokens ? 2 : 1;
-  pa.num_mb = (c.a.max_q + pa.tiles * pa.tokens - 1) / (pa.tiles * pa.tokens);
+  int64_t num_mb;
+  chunk_shape(c.a.max_q, c.a.group, &pa.tiles, &pa.tokens, &num_mb);
+  pa.num_mb = (int)num_mb;
   return dtype == FG_BF16 ? launch_kind<__nv_bfloat16>(pa, kind, st) : launch_kind<__half>(pa, kind, st);
 }
 

@@ -448,8 +448,8 @@ typedef struct {
 } fg_attn_cache_params;
 FG_API int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream);
 FG_API int64_t fg_flash_attn_cache_workspace_bytes(const fg_attn_cache_params* p);
-/* Which kernel family fg_flash_attn_cache picks: 0 general (mma.sync), 1 tcgen05 (head dim 128); for at most
- * 16 query rows per sequence and KV head 2 TMA-fed (mma.sync), 3 tcgen05 (head dim 128, with a workspace).  Pure host
+/* Which kernel family fg_flash_attn_cache picks: 0 general (mma.sync), 1 tcgen05; for at most 16 query rows per
+ * sequence and KV head 2 TMA-fed (mma.sync), 3 tcgen05.  The tcgen05 kernels take head dim 128 and need a workspace.  Pure host
  * logic. */
 FG_API int fg_flash_attn_cache_path(const fg_attn_cache_params* p);
 

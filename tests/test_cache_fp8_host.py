@@ -83,9 +83,11 @@ def test_small_workspace_is_refused():
 def test_workspace_goes_by_what_is_visible():
     """A window bounds the keys that are split, however long the context."""
     need = lambda **kw: _lib.load().fg_flash_attn_cache_workspace_bytes(ctypes.byref(params(**kw)))
-    for size in (dict(head_dim=64), dict(head_dim=256, max_seqlen_q=30, total_q=100), dict(max_seqlen_q=30, total_q=100)):
+    for size in (dict(head_dim=64), dict(head_dim=256, max_seqlen_q=30, total_q=100)):
         long, windowed = need(max_seqlen_k=10 ** 6, **size), need(max_seqlen_k=10 ** 6, window_left=2047, sink_tokens=4, **size)
         assert 0 < windowed < long and windowed == need(max_seqlen_k=10 ** 5, window_left=2047, sink_tokens=4, **size)
+    chunk = dict(max_seqlen_q=30, total_q=100)
+    assert need(max_seqlen_k=10 ** 6, **chunk) == need(max_seqlen_k=10, **chunk) > need() > 0
     assert need(max_seqlen_k=10 ** 6) == need(max_seqlen_k=10)        # head parts and tail parts of a fixed number of CTAs
 
 
