@@ -69,7 +69,7 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
       b.q_head_stride > 0 && b.q_row_stride > 0 && workspace) {
     plan.path = kPathChunk;            // cuts the keys itself, on the device
     plan.splits = plan.tiles_per_split = 1;
-    plan.bytes = attn_cache_chunk_bytes(b.max_seqlen_q, group, b.batch, b.num_heads_k, b.max_seqlen_k / 128 + 1, sms);
+    plan.bytes = attn_cache_chunk_bytes(b.max_seqlen_q, group, b.batch, b.num_heads_k, b.max_seqlen_k / 64 + 1, sms);
     if (plan.bytes > 0) return plan;
   }
   if (b.max_seqlen_q * group <= 16 && tma) {

@@ -2,7 +2,7 @@
 //
 // An item is one or two 128-row Q tiles of one (sequence, KV head).  A row is a (token, head of the group) pair, so a chunk of a
 // few tokens fills the tiles as well as a long one, and all query heads of the group share every K/V tile.  A tile holds
-// floor(128 / group) tokens.  The kernel is persistent, one CTA an SM: the K/V tiles (128 keys) of all items, laid end to end,
+// floor(128 / group) tokens.  The kernel is persistent, one CTA an SM: the K/V tiles (64 keys) of all items, laid end to end,
 // are cut into equal runs, one per CTA, so that few long items and many short ones fill the SMs alike (in whole items, 336
 // CTAs on 148 SMs would take three rounds for 2.27).  The parts of an item that runs cut are joined by a second kernel, in
 // order.  Nothing synchronises the CTA between items: the roles follow the barrier phases with running counters.
@@ -10,14 +10,18 @@
 //   warps 0-7    softmax, one warpgroup per Q tile, one thread per row (TMEM lane = row): scores of 64 keys from TMEM to
 //                registers, mask, running maximum (raised only when it grows by more than 8 in log2 units), exponentials,
 //                probabilities back to TMEM as 16 bit; at the end they normalise and write the output rows
-//   warp 8       TMA producer: Q once, then K and V tiles, walking the tile runs (first tokens, then the window)
-//   warps 9, 10  score-issuing thread of each Q tile: S = Q K^T, 64 keys a step
+//   16-bit caches:
+//   warps 8, 9   TMA producers of K (and Q) and of V, walking the tile runs (first tokens, then the window).  A page of 16 keys is
+//                two boxes, and a warp issues one in about 95 clocks: one warp for both would need 1900 clocks a tile
+//   warp 10      scores of both Q tiles: S = Q K^T, 64 keys a step
+//   8-bit caches:
+//   warp 8       TMA producer of Q; warps 9, 10 the scores of one Q tile each
+//   warps 12-15  load K and V rows (one tile ahead, in registers), widen them to fp16 and store them as the 128-byte
+//                swizzled tiles that the tensor cores read; rows that no row of the item sees are neither read nor kept.
+//                (Landing the 8-bit tiles in shared memory by TMA first costs two more waits and a read for each: two chunks
+//                of 2048 tokens took 789 us.)  bf16 queries are brought to fp16, each row by a power of two, by the softmax
+//                warps before an item's first step.
 //   warp 11      O += P V of both tiles
-//   warps 12-15  8-bit caches: widen the K/V tiles from six 16 KB landing slots to fp16 units of 64 keys (two of K, two of V;
-//                128-byte swizzled rows) for the tensor cores, zeroing V rows that no row of the item sees.  The depth is in
-//                the landing slots because that is where the latency is: with one slot for K and one for V (and units of 128
-//                keys) a tile took a copy's latency and a conversion in turn, 831 us for two chunks of 2048 tokens.  (bf16 queries are brought
-//                to fp16, each row by a power of two, by the softmax warps before an item's first step.)
 // TMEM columns: tile t has its scores at t*128 (64 columns), two probability buffers at t*128+64 and +96, its output at
 // 256+t*128.  Every wait is an mbarrier wait with a limit.
 #include "attn_cache_common.cuh"
@@ -26,24 +30,21 @@
 namespace fg {
 namespace {
 
-constexpr int BM = 128, BN = 128, HD = 128, STEP = 64;
+constexpr int BM = 128, BN = 64, HD = 128;
 constexpr int HALF_BYTES = 128 * 64 * 2;     // one [128 x 64] swizzled 16-bit sub-tile
 constexpr int TILE_BYTES = 2 * HALF_BYTES;   // 32 KB
-constexpr int RAW_BYTES = BN * HD;           // one 8-bit K or V tile, 16 KB
-constexpr int TMA_WARP = 8, MMA_WARP0 = 9, CONV_WARP0 = 12;
+constexpr int UNIT_HALF = BN * 128;          // one [64 keys x 64 columns] swizzled half of a 16-bit K or V tile
+constexpr int UNIT = 2 * UNIT_HALF;          // 16 KB
+constexpr int TMA_WARP = 8, MMA_WARP0 = 9, PV_WARP = 11, CONV_WARP0 = 12;
+constexpr int STAGES = 4;                    // 16-bit tiles of K, and of V
 constexpr int TMEM_COLS = 512;
 constexpr float kRescaleThreshold = 8.0f;    // log2 units
 
-constexpr int kMinRun = 4;                   // fewest K/V tiles that a run is worth starting a CTA for
+constexpr int kMinRun = 8;                   // fewest K/V tiles that a run is worth starting a CTA for
 constexpr int kInfo = 32;                    // sequences of a run whose lengths are kept in shared memory
 
 constexpr int threads_of(int kind) { return kind == kCache16 ? 12 * 32 : 16 * 32; }
-constexpr int RAW_SLOTS = 6;                 // 8-bit tiles on their way or being widened
-// Keys of a 16-bit stage (two of K, two of V): 64 where 8-bit tiles are widened into them, else a whole tile as it arrives.
-constexpr int unit_of(int kind) { return kind == kCache16 ? BN : STEP; }
-constexpr int smem_of(int kind) {
-  return 2 * TILE_BYTES + 4 * unit_of(kind) * 256 + (kind == kCache16 ? 0 : RAW_SLOTS * RAW_BYTES) + 1024 + 512 + kInfo * 16;
-}
+constexpr int SMEM_BYTES = 2 * TILE_BYTES + 2 * STAGES * UNIT + 1024 + 512 + kInfo * 16;
 
 // What a CTA leaves for the joining kernel: the KV head of the item whose start it holds but not its end (or -1), in how many
 // parts the item is, its first query row and its tokens.
@@ -67,7 +68,7 @@ struct ChunkArgs {
 struct Segment {
   int b, m, hk, lo, hi, n;      // K/V tiles [lo, hi) of the n of (sequence b, Q tiles m, KV head hk)
   int left;                     // tiles of the run from lo on
-  int m0, nt, shift, steps;     // first token; Q tiles that hold one; position of token 0; steps of 64 keys
+  int m0, nt, shift;            // first token; Q tiles that hold one; position of token 0
   SeqInfo s;
   TileSpan span;
   RowMask first, last;          // what the first and the last token see
@@ -87,8 +88,6 @@ struct InfoTable {
 __device__ __forceinline__ void set_part(Segment& g, int lo) {
   g.lo = lo;
   g.hi = min(g.n, lo + g.left);
-  // the second half of the last tile is left out when nothing of it is visible
-  g.steps = 2 * (g.hi - g.lo) - (g.hi == g.n && g.span.tile(g.n - 1) * BN + STEP >= g.last.hi ? 1 : 0);
 }
 __device__ __forceinline__ void fill_segment(const ChunkArgs& pa, const InfoTable& table, Segment& g) {
   g.s = (unsigned)(g.b - table.b0) < (unsigned)table.n ? table.info[g.b - table.b0] : seq_info(pa.c.a, g.b);
@@ -153,8 +152,6 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   constexpr bool kConvQ = !std::is_same<T, M>::value;
   constexpr bool kWiden = KIND != kCache16;
   constexpr int THREADS = threads_of(KIND);
-  constexpr int UNIT_HALF = unit_of(KIND) * 128;   // bytes of one 64-column half of a stage
-  constexpr int UNIT = 2 * UNIT_HALF;
   const CacheAttnArgs& c = pa.c;
   const AttnArgs& a = c.a;
   const int NT = pa.tiles;
@@ -163,26 +160,23 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                       // [2 tiles][2 halves][128 x 64]
-  uint8_t* sK = smem + 2 * TILE_BYTES;      // [2 stages]
-  uint8_t* sV = sK + 2 * UNIT;              // [2 stages]
-  uint8_t* sR = sV + 2 * UNIT;              // [RAW_SLOTS] 8-bit tiles as they arrive: K, V, K, V, ...
-  uint8_t* rest = sR + (kWiden ? RAW_SLOTS * RAW_BYTES : 0);
+  uint8_t* sK = smem + 2 * TILE_BYTES;      // [STAGES]
+  uint8_t* sV = sK + STAGES * UNIT;         // [STAGES]
+  uint8_t* rest = sV + STAGES * UNIT;
   uint64_t* bars = reinterpret_cast<uint64_t*>(rest);
   uint64_t* q_full = bars;            // Q tiles of an item have landed
   uint64_t* q_empty = bars + 1;       // every score of an item has been computed: Q may be overwritten
-  uint64_t* k_full = bars + 2;        // [2]
-  uint64_t* k_empty = bars + 4;       // [2]
-  uint64_t* v_full = bars + 6;        // [2]
-  uint64_t* v_empty = bars + 8;       // [2]
-  uint64_t* s_full = bars + 10;       // [2 tiles] scores of a step have landed in the tile's score buffer
-  uint64_t* s_free = bars + 12;       // [2 tiles] ... and have been read into registers
-  uint64_t* p_ready = bars + 14;      // [2 tiles][2 probability buffers]
-  uint64_t* o_done = bars + 18;       // [2 tiles][2]: P V of even / odd steps
-  uint64_t* q_ready = bars + 22;      // [2 tiles] the tile's Q holds M
-  uint64_t* o_free = bars + 24;       // [2 tiles] the output of the previous item has been read out
-  uint64_t* r_full = bars + 26;       // [RAW_SLOTS]
-  uint64_t* r_empty = r_full + RAW_SLOTS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + RAW_SLOTS);
+  uint64_t* k_full = bars + 2;        // [STAGES]
+  uint64_t* k_empty = bars + 6;
+  uint64_t* v_full = bars + 10;
+  uint64_t* v_empty = bars + 14;
+  uint64_t* s_full = bars + 18;       // [2 tiles] scores of a step have landed in the tile's score buffer
+  uint64_t* s_free = bars + 20;       // [2 tiles] ... and have been read into registers
+  uint64_t* p_ready = bars + 22;      // [2 tiles][2 probability buffers]
+  uint64_t* o_done = bars + 26;       // [2 tiles][2]: P V of even / odd steps
+  uint64_t* q_ready = bars + 30;      // [2 tiles] the tile's Q holds M
+  uint64_t* o_free = bars + 32;       // [2 tiles] the output of the previous item has been read out
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   SeqInfo* sInfo = reinterpret_cast<SeqInfo*>(rest + 512);   // [kInfo]
 
@@ -197,20 +191,18 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     s_drain = *reinterpret_cast<volatile int*>(a.status);
     *abort_flag = 0;
     mbar_init(q_full, 1);
-    mbar_init(q_empty, NT);
-    for (int i = 0; i < 2; ++i) {
+    mbar_init(q_empty, kWiden ? NT : 1);   // one arrival per score-issuing thread
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(&k_full[i], kWiden ? 4 : 1);
-      mbar_init(&k_empty[i], NT);
+      mbar_init(&k_empty[i], kWiden ? NT : 1);
       mbar_init(&v_full[i], kWiden ? 4 : 1);
       mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4);       // one arrival per softmax warp of the tile
       mbar_init(&q_ready[i], 4);
       mbar_init(&o_free[i], 4);
-    }
-    for (int i = 0; i < RAW_SLOTS; ++i) {
-      mbar_init(&r_full[i], 1);
-      mbar_init(&r_empty[i], 4);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&p_ready[i], 4);
     for (int i = 0; i < 4; ++i) mbar_init(&o_done[i], 1);
@@ -295,8 +287,9 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     return r != 0;
   };
 
-  if (warp == TMA_WARP) {
-    // ================================ TMA producer ================================
+  if (warp == TMA_WARP || (!kWiden && warp == TMA_WARP + 1)) {
+    // ================================ TMA producers of K and Q, and of V ===========
+    const bool is_v = warp != TMA_WARP;
     // Lane i holds the place of the i-th page of a tile, or -1 where no row of the item sees any of its keys: such a page is
     // not fetched (its scores are masked and its V rows zeroed).
     auto lookup = [&](int j, int& page, int& row) {
@@ -311,138 +304,130 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         page = cache_page(c, a.block_table + (int64_t)seg.b * a.bt_stride, pg);
       }
     };
+    const CUtensorMap* tm = is_v ? &tmap_v : &tmap_k;
+    uint8_t* ring = is_v ? sV : sK;
+    uint64_t* full = is_v ? v_full : k_full;
+    uint64_t* empty = is_v ? v_empty : k_empty;
     uint32_t item = 0, kv = 0;     // items and K/V tiles so far
     bool ok = true;
     do {
-      int page, row;
-      lookup(seg.lo, page, row);
-      if (item > 0 && !wwait(q_empty, (item - 1) & 1)) break;
-      if (lane == 0) {
-        mbar_expect_tx(q_full, seg.nt * 2 * pa.tokens * a.group * 128);
-        for (int t = 0; t < seg.nt; ++t)
-          for (int hf = 0; hf < 2; ++hf)
-            tma_load_3d(sQ + t * TILE_BYTES + hf * HALF_BYTES, &tmap_q, q_full, hf * 64, seg.hk * a.group,
-                        seg.s.q_begin + seg.m0 + t * pa.tokens);
-      }
-      __syncwarp();
-      ++item;
-      for (int j = seg.lo; j < seg.hi && ok; ++j, ++kv) {
-        int npage = -1, nrow = 0;
-        if (j + 1 < seg.hi) lookup(j + 1, npage, nrow);   // in flight while this tile is issued
-        const int pages = __popc(__ballot_sync(0xffffffffu, page >= 0));
-        for (int which = 0; which < 2; ++which) {
-          const CUtensorMap* tm = which ? &tmap_v : &tmap_k;
-          if constexpr (kWiden) {
-            const uint32_t n = 2 * kv + which, slot = n % RAW_SLOTS;
-            if (!wwait(&r_empty[slot], ((n / RAW_SLOTS) & 1) ^ 1)) {
-              ok = false;
-              break;
-            }
-            if (lane == 0) mbar_expect_tx(&r_full[slot], pages * pa.page_rows * 128);
-            __syncwarp();
-            if (page >= 0) tma_load_4d(sR + slot * RAW_BYTES + lane * pa.page_rows * 128, tm, &r_full[slot], 0, seg.hk, row, page);
-          } else {
-            const int stg = kv & 1;
-            uint64_t* full = which ? &v_full[stg] : &k_full[stg];
-            if (!wwait(which ? &v_empty[stg] : &k_empty[stg], ((kv >> 1) & 1) ^ 1)) {
-              ok = false;
-              break;
-            }
-            if (lane == 0) mbar_expect_tx(full, pages * pa.page_rows * 256);
-            __syncwarp();
-            if (page >= 0) {
-              uint8_t* dst = (which ? sV : sK) + stg * TILE_BYTES + lane * pa.page_rows * 128;
-              for (int hf = 0; hf < 2; ++hf) tma_load_4d(dst + hf * HALF_BYTES, tm, full, hf * 64, seg.hk, row, page);
-            }
-          }
+      int page = -1, row = 0;
+      if constexpr (!kWiden) lookup(seg.lo, page, row);
+      if (!is_v) {
+        if (item > 0 && !wwait(q_empty, (item - 1) & 1)) break;
+        if (lane == 0) {
+          mbar_expect_tx(q_full, seg.nt * 2 * pa.tokens * a.group * 128);
+          for (int t = 0; t < seg.nt; ++t)
+            for (int hf = 0; hf < 2; ++hf)
+              tma_load_3d(sQ + t * TILE_BYTES + hf * HALF_BYTES, &tmap_q, q_full, hf * 64, seg.hk * a.group,
+                          seg.s.q_begin + seg.m0 + t * pa.tokens);
         }
-        page = npage;
-        row = nrow;
-      }
-    } while (ok && next_segment(pa, table, seg));
-  } else if (warp >= MMA_WARP0 && warp < MMA_WARP0 + NT) {
-    // ================================ scores of one tile ==========================
-    const int t = warp - MMA_WARP0;
-    if (lane == 0) {
-      const uint32_t idesc = umma_idesc_f16(kBf16, false, false, BM, STEP);
-      const uint32_t desc_hi = (uint32_t)(umma_desc_sw128(0, 0, 1024) >> 32);
-      const uint32_t q_lo = (uint32_t)umma_desc_sw128(smem_u32(sQ + t * TILE_BYTES), 0, 1024);
-      const uint32_t k_lo0 = (uint32_t)umma_desc_sw128(smem_u32(sK), 0, 1024);
-      const uint32_t s_tmem = tmem_base + t * 128;
-      uint32_t item = 0, used = 0, unit0 = 0, g = 0;   // items, items of this tile, stages filled and this tile's steps so far
-      bool ok = true;
-      do {
-        const bool on = t < seg.nt;
-        if (on) {
-          if (!(kConvQ ? wait1(&q_ready[t], used & 1) : wait1(q_full, item & 1))) break;
-          ++used;
-        }
+        __syncwarp();
         ++item;
-        for (int i = 0; i < seg.steps && ok; ++i) {
-          const uint32_t unit = unit0 + (uint32_t)(kWiden ? i : i >> 1), stg = unit & 1;
-          if ((kWiden || !(i & 1)) && !wait1(&k_full[stg], (unit >> 1) & 1)) {
+      }
+      if constexpr (!kWiden) {
+        for (int j = seg.lo; j < seg.hi; ++j, ++kv) {
+          int npage = -1, nrow = 0;
+          if (j + 1 < seg.hi) lookup(j + 1, npage, nrow);   // in flight while this tile is issued
+          const int pages = __popc(__ballot_sync(0xffffffffu, page >= 0));
+          const uint32_t stg = kv % STAGES;
+          if (!wwait(&empty[stg], ((kv / STAGES) & 1) ^ 1)) {
             ok = false;
             break;
           }
-          if (on) {
+          if (lane == 0) mbar_expect_tx(&full[stg], pages * pa.page_rows * 256);
+          __syncwarp();
+          if (page >= 0) {
+            uint8_t* dst = ring + stg * UNIT + lane * pa.page_rows * 128;
+            for (int hf = 0; hf < 2; ++hf) tma_load_4d(dst + hf * UNIT_HALF, tm, &full[stg], hf * 64, seg.hk, row, page);
+          }
+          page = npage;
+          row = nrow;
+        }
+      }
+    } while (ok && next_segment(pa, table, seg));
+  } else if (kWiden ? warp >= MMA_WARP0 && warp < MMA_WARP0 + NT : warp == MMA_WARP0 + 1) {
+    // ================================ scores =======================================
+    if (lane == 0) {
+      constexpr int TILES = kWiden ? 1 : 2;              // Q tiles of this thread
+      const int t0 = kWiden ? warp - MMA_WARP0 : 0;
+      const uint32_t idesc = umma_idesc_f16(kBf16, false, false, BM, BN);
+      const uint32_t desc_hi = (uint32_t)(umma_desc_sw128(0, 0, 1024) >> 32);
+      const uint32_t k_lo0 = (uint32_t)umma_desc_sw128(smem_u32(sK), 0, 1024);
+      uint32_t item = 0, kv = 0, g[TILES] = {};   // items, K/V tiles, and steps of each Q tile so far
+      bool ok = true;
+      do {
+        ok = wait1(kConvQ ? &q_ready[t0] : q_full, item & 1);
+        ++item;
+        for (int i = seg.lo; i < seg.hi && ok; ++i, ++kv) {
+          const uint32_t stg = kv % STAGES;
+          if (!wait1(&k_full[stg], (kv / STAGES) & 1)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int x = 0; x < TILES; ++x) {
+            const int t = t0 + x;
+            if (t >= seg.nt || !ok) continue;
             // the previous step's scores must have been read out; and the softmax warps will store P over the buffer that the
             // P V two steps back reads (steps 0 and 1: the softmax warps waited for the previous item's last P V)
-            if ((g > 0 && !wait1(&s_free[t], (g - 1) & 1)) || (i >= 2 && !wait1(&o_done[t * 2 + (g & 1)], ((g - 2) >> 1) & 1))) {
+            if ((g[x] > 0 && !wait1(&s_free[t], (g[x] - 1) & 1)) ||
+                (i >= seg.lo + 2 && !wait1(&o_done[t * 2 + (g[x] & 1)], ((g[x] - 2) >> 1) & 1))) {
               ok = false;
-              break;
+              continue;
             }
             tc_fence_after();
-            const uint32_t k_lo = k_lo0 + stg * (UNIT >> 4) + (kWiden ? 0 : (i & 1) * (STEP * 128 >> 4));
+            const uint32_t q_lo = (uint32_t)umma_desc_sw128(smem_u32(sQ + t * TILE_BYTES), 0, 1024);
+            const uint32_t k_lo = k_lo0 + stg * (UNIT >> 4);
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k)
-              mma_f16_ss_lohi(s_tmem, q_lo + (((k >> 2) * HALF_BYTES + (k & 3) * 32) >> 4),
+              mma_f16_ss_lohi(tmem_base + t * 128, q_lo + (((k >> 2) * HALF_BYTES + (k & 3) * 32) >> 4),
                               k_lo + (((k >> 2) * UNIT_HALF + (k & 3) * 32) >> 4), desc_hi, idesc, k != 0 ? 1u : 0u);
             tc_commit(&s_full[t]);
-            ++g;
+            ++g[x];
           }
-          if (kWiden || (i & 1) || i == seg.steps - 1) tc_commit(&k_empty[stg]);
-          if (i == seg.steps - 1) tc_commit(q_empty);
+          if (!ok) break;
+          tc_commit(&k_empty[stg]);
+          if (i == seg.hi - 1) tc_commit(q_empty);
         }
-        unit0 += (uint32_t)(kWiden ? seg.steps : seg.hi - seg.lo);
       } while (ok && next_segment(pa, table, seg));
     }
-  } else if (warp == MMA_WARP0 + 2) {
+  } else if (warp == PV_WARP) {
     // ================================ O += P V of both tiles =======================
     if (lane == 0) {
       const uint32_t idesc = umma_idesc_f16(kBf16, false, true, BM, HD);   // V is MN-major
       const uint32_t desc_hi = (uint32_t)(umma_desc_sw128(0, 0, 1024) >> 32);
       const uint32_t v_lo0 = (uint32_t)umma_desc_sw128(smem_u32(sV), UNIT_HALF, 1024);
-      uint32_t used[2] = {0, 0}, unit0 = 0, g[2] = {0, 0};
+      uint32_t used[2] = {0, 0}, kv = 0, g[2] = {0, 0};
       bool ok = true;
       do {
-        for (int i = 0; i < seg.steps && ok; ++i) {
-          const uint32_t unit = unit0 + (uint32_t)(kWiden ? i : i >> 1), stg = unit & 1;
-          if ((kWiden || !(i & 1)) && !wait1(&v_full[stg], (unit >> 1) & 1)) {
+        for (int i = seg.lo; i < seg.hi && ok; ++i, ++kv) {
+          const uint32_t stg = kv % STAGES;
+          if (!wait1(&v_full[stg], (kv / STAGES) & 1)) {
             ok = false;
             break;
           }
-          const uint32_t v_lo = v_lo0 + stg * (UNIT >> 4) + (kWiden ? 0 : (i & 1) * (4 * 2048 >> 4));
+          const uint32_t v_lo = v_lo0 + stg * (UNIT >> 4);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (t >= seg.nt || !ok) continue;
             const uint32_t par = g[t] & 1;
             // the first product of an item overwrites O: the previous item's must have been read out
-            if (!wait1(&p_ready[t * 2 + par], (g[t] >> 1) & 1) || (i == 0 && used[t] > 0 && !wait1(&o_free[t], (used[t] - 1) & 1))) {
+            if (!wait1(&p_ready[t * 2 + par], (g[t] >> 1) & 1) || (i == seg.lo && used[t] > 0 && !wait1(&o_free[t], (used[t] - 1) & 1))) {
               ok = false;
               continue;
             }
             tc_fence_after();
-            const uint32_t p_tmem = tmem_base + t * 128 + STEP + par * 32;
+            const uint32_t p_tmem = tmem_base + t * 128 + BN + par * 32;
             const uint32_t o_tmem = tmem_base + 256 + t * 128;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mma_f16_ts_lohi(o_tmem, p_tmem + k * 8, v_lo + k * (2048 >> 4), desc_hi, idesc, (i > 0 || k > 0) ? 1u : 0u);
+              mma_f16_ts_lohi(o_tmem, p_tmem + k * 8, v_lo + k * (2048 >> 4), desc_hi, idesc, (i > seg.lo || k > 0) ? 1u : 0u);
             tc_commit(&o_done[t * 2 + par]);
             ++g[t];
           }
-          if (ok && (kWiden || (i & 1) || i == seg.steps - 1)) tc_commit(&v_empty[stg]);
+          if (ok) tc_commit(&v_empty[stg]);
         }
-        unit0 += (uint32_t)(kWiden ? seg.steps : seg.hi - seg.lo);
         ++used[0];
         used[1] += seg.nt > 1;
       } while (ok && next_segment(pa, table, seg));
@@ -454,64 +439,75 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       // lane = (row of four, 16-byte piece): eight lanes read one row's 128 bytes and write one row's 128 bytes of
       // either half at a time (pieces 4-7 store their second eight values first), without bank conflicts
       const int ch = lane & 7, sub = lane >> 3;
-      uint32_t n = 0, unit0 = 0;     // 8-bit tiles and units so far
+      const uint8_t* base[2] = {reinterpret_cast<const uint8_t*>(a.k) + ch * 16, reinterpret_cast<const uint8_t*>(a.v) + ch * 16};
+      const int page_shift = a.paged ? 31 - __clz(a.block_size) : 0;   // a power of two of at least 8
+      uint4 next[2][4];              // K and V rows w * 16 + k * 4 + sub of the next tile
+      auto load = [&](int j) {
+        const int row0 = seg.span.tile(j) * BN + w * 16;
+        int page[2] = {0, 0};        // of the rows' first and second eight
+        if (a.paged) {
+          const int32_t* bt_row = a.block_table + (int64_t)seg.b * a.bt_stride;
+          page[0] = cache_page(c, bt_row, row0 >> page_shift);
+          page[1] = cache_page(c, bt_row, (row0 + 8) >> page_shift);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int col = row0 + k * 4 + sub;
+          const bool seen = col < seg.last.hi && (col >= seg.first.lo || col < c.sinks);
+          const int64_t in = a.paged ? col & (a.block_size - 1) : seg.s.k_begin + col;
+#pragma unroll
+          for (int which = 0; which < 2; ++which)
+            next[which][k] = seen ? ldg16_stream(base[which] + page[k >> 1] * (which ? a.v_bs : a.k_bs) +
+                                                 in * (which ? a.v_rs : a.k_rs) + seg.hk * (which ? a.v_hs : a.k_hs))
+                                  : make_uint4(0, 0, 0, 0);
+        }
+      };
+      uint32_t kv = 0;     // K/V tiles so far
       bool ok = true;
+      load(seg.lo);
       do {
-        for (int j = seg.lo; j < seg.hi && ok; ++j) {
-          const int j0 = seg.span.tile(j) * BN;
-          for (int which = 0; which < 2 && ok; ++which, ++n) {
-            const uint32_t slot = n % RAW_SLOTS;
-            uint64_t* full = which ? v_full : k_full;
-            uint64_t* empty = which ? v_empty : k_empty;
-            if (!wwait(&r_full[slot], (n / RAW_SLOTS) & 1)) {
+        Segment cur = seg;
+        for (int j = cur.lo; j < cur.hi && ok; ++j, ++kv) {
+          uint4 raw[2][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            raw[0][k] = next[0][k];
+            raw[1][k] = next[1][k];
+          }
+          if (j + 1 < cur.hi)
+            load(j + 1);
+          else if (next_segment(pa, table, seg))
+            load(seg.lo);
+          else
+            ok = false;              // the last tile of the run
+          const uint32_t stg = kv % STAGES;
+#pragma unroll
+          for (int which = 0; which < 2; ++which) {
+            if (!wwait(which ? &v_empty[stg] : &k_empty[stg], ((kv / STAGES) & 1) ^ 1)) {
               ok = false;
               break;
             }
-            const bool zero = which && (j0 + BN > seg.last.hi || (j0 < seg.first.lo && j0 + BN > c.sinks));
-            for (int h = 0; h < 2; ++h) {
-              const int i = 2 * (j - seg.lo) + h;
-              if (i >= seg.steps) break;             // the half of the last tile that nobody sees
-              const uint32_t unit = unit0 + (uint32_t)i, stg = unit & 1;
-              if (!wwait(&empty[stg], ((unit >> 1) & 1) ^ 1)) {
-                ok = false;
-                break;
-              }
-              const uint8_t* src = sR + slot * RAW_BYTES + h * (STEP * 128);
-              uint8_t* dst = (which ? sV : sK) + stg * UNIT + (ch >> 2) * UNIT_HALF;
-              uint4 raw[4];
+            uint8_t* dst = (which ? sV : sK) + stg * UNIT + (ch >> 2) * UNIT_HALF;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int r = w * 16 + k * 4 + sub;
-                raw[k] = *reinterpret_cast<const uint4*>(src + r * 128 + ((ch ^ (r & 7)) << 4));
-              }
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int r = w * 16 + k * 4 + sub;
-                if (zero) {   // V rows that no row of the item sees must not reach the products
-                  const int col = j0 + h * STEP + r;
-                  if (col >= seg.last.hi || (col < seg.first.lo && col >= c.sinks)) raw[k] = make_uint4(0, 0, 0, 0);
-                }
-                uint4 lo, hi;
-                fp8x4_to_f16x4<KIND>(raw[k].x, lo.x, lo.y);
-                fp8x4_to_f16x4<KIND>(raw[k].y, lo.z, lo.w);
-                fp8x4_to_f16x4<KIND>(raw[k].z, hi.x, hi.y);
-                fp8x4_to_f16x4<KIND>(raw[k].w, hi.z, hi.w);
-                const bool swap = ch & 4;
-                const int c0 = (ch & 3) * 2 + (swap ? 1 : 0);
-                uint8_t* row = dst + r * 128;
-                *reinterpret_cast<uint4*>(row + ((c0 ^ (r & 7)) << 4)) = swap ? hi : lo;
-                *reinterpret_cast<uint4*>(row + (((c0 ^ 1) ^ (r & 7)) << 4)) = swap ? lo : hi;
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&full[stg]);
+            for (int k = 0; k < 4; ++k) {
+              const int r = w * 16 + k * 4 + sub;
+              uint4 lo, hi;
+              fp8x4_to_f16x4<KIND>(raw[which][k].x, lo.x, lo.y);
+              fp8x4_to_f16x4<KIND>(raw[which][k].y, lo.z, lo.w);
+              fp8x4_to_f16x4<KIND>(raw[which][k].z, hi.x, hi.y);
+              fp8x4_to_f16x4<KIND>(raw[which][k].w, hi.z, hi.w);
+              const bool swap = ch & 4;
+              const int c0 = (ch & 3) * 2 + (swap ? 1 : 0);
+              uint8_t* row = dst + r * 128;
+              *reinterpret_cast<uint4*>(row + ((c0 ^ (r & 7)) << 4)) = swap ? hi : lo;
+              *reinterpret_cast<uint4*>(row + (((c0 ^ 1) ^ (r & 7)) << 4)) = swap ? lo : hi;
             }
+            fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&r_empty[slot]);
+            if (lane == 0) mbar_arrive(which ? &v_full[stg] : &k_full[stg]);
           }
         }
-        unit0 += (uint32_t)seg.steps;
-      } while (ok && next_segment(pa, table, seg));
+      } while (ok);
     }
   } else if (warp < 4 * NT) {
     // ================================ softmax / epilogue ===========================
@@ -526,8 +522,11 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     bool ok = true;
     do {
       if (t >= seg.nt) {                      // no token in this tile
-        if constexpr (kConvQ) {               // but no phase of q_full is left out: its parity could not tell them apart
+        if constexpr (kConvQ) {
+          // But every item's q_full is waited for, and q_ready holds its Q until then: a barrier may not run two phases ahead
+          // of one that waits for it, since a parity cannot tell them apart.
           if (!wwait(q_full, item & 1)) break;
+          if (lane == 0) mbar_arrive(&q_ready[t]);
         }
         ++item;
         kv += (uint32_t)(seg.hi - seg.lo);
@@ -575,8 +574,8 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       ++item;
       const bool odd_scale = !(scale > 0.f);  // a K scale that is zero, negative or NaN: scale the scores first
 
-      for (int i = 0; i < seg.steps; ++i, ++g) {
-        const uint32_t p_addr = s_addr + STEP + (g & 1) * 32;
+      for (int i = seg.lo; i < seg.hi; ++i, ++g, ++kv) {
+        const uint32_t p_addr = s_addr + BN + (g & 1) * 32;
         if (!wwait(&s_full[t], g & 1)) {
           ok = false;
           break;
@@ -595,11 +594,15 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           for (int e = 0; e < 64; ++e) sv[e] *= scale;
           sc = 1.f;
         }
-        const int col0 = seg.span.tile(seg.lo + (i >> 1)) * BN + (i & 1) * STEP;
-        if (col0 + STEP > first.hi || (col0 < last.lo && col0 + STEP > c.sinks)) {
+        const int col0 = seg.span.tile(i) * BN;
+        if (col0 + BN > first.hi || (col0 < last.lo && col0 + BN > c.sinks)) {
+          // a bit for each key of the tile: below hi, and not below lo or below the first tokens' end
+          auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+          const int hi = mask.hi - col0, lo = mask.lo - col0, sk = c.sinks - col0;
+          const uint32_t seen[2] = {below(hi) & (~below(lo) | below(sk)), below(hi - 32) & (~below(lo - 32) | below(sk - 32))};
 #pragma unroll
           for (int e = 0; e < 64; ++e)
-            if (mask.dead(col0 + e)) sv[e] = -INFINITY;
+            if (!((seen[e >> 5] >> (e & 31)) & 1u)) sv[e] = -INFINITY;
         }
         float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
 #pragma unroll
@@ -613,7 +616,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         }
         const float m_tile = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * sc;   // sc > 0; -inf stays -inf
         const bool raise = m_tile > m_used + kRescaleThreshold || (m_used == -INFINITY && m_tile > -INFINITY);
-        if (i > 0 && __any_sync(0xffffffffu, raise)) {
+        if (i > seg.lo && __any_sync(0xffffffffu, raise)) {
           // every P V issued so far must have landed before O is touched
           if (!wwait(&o_done[t * 2 + ((g - 1) & 1)], ((g - 1) >> 1) & 1)) {
             ok = false;
@@ -637,17 +640,17 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         if constexpr (!kWiden) {
           // V rows of this step that no row of the item sees must not reach the products: zeroed in place, by each tile's
           // warps for themselves (the other tile writes the same zeros)
-          if (col0 + STEP > seg.last.hi || (col0 < seg.first.lo && col0 + STEP > c.sinks)) {
-            const uint32_t tile = kv + (uint32_t)(i >> 1), stg = tile & 1;
-            if (!wwait(&v_full[stg], (tile >> 1) & 1)) {
+          if (col0 + BN > seg.last.hi || (col0 < seg.first.lo && col0 + BN > c.sinks)) {
+            const uint32_t stg = kv % STAGES;
+            if (!wwait(&v_full[stg], (kv / STAGES) & 1)) {
               ok = false;
               break;
             }
-            uint8_t* vt = sV + stg * UNIT + (i & 1) * STEP * 128;
-            for (int at = r; at < STEP * 16; at += 128) {
+            uint8_t* vt = sV + stg * UNIT;
+            for (int at = r; at < BN * 16; at += 128) {
               const int row = at / 16, ch = at % 16, col = col0 + row;
               if (col >= seg.last.hi || (col < seg.first.lo && col >= c.sinks))
-                *reinterpret_cast<uint4*>(vt + (ch >> 3) * HALF_BYTES + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(vt + (ch >> 3) * UNIT_HALF + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
           }
@@ -678,7 +681,6 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         if (lane == 0) mbar_arrive(&p_ready[t * 2 + (g & 1)]);
       }
       if (!ok) break;
-      kv += (uint32_t)(seg.hi - seg.lo);
 
       // ---- epilogue: normalise my row of O and write it out
       if (!wwait(&o_done[t * 2 + ((g - 1) & 1)], ((g - 1) >> 1) & 1)) break;
@@ -687,11 +689,11 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       const float inv = l_run == 0.f ? 0.f : v_scale / l_run;
       const bool whole = seg.lo == 0 && seg.hi == seg.n;
       const int64_t qtok = seg.s.q_begin + tok;
-      const int64_t part = ((int64_t)2 * blockIdx.x + (seg.lo == 0 ? 1 : 0)) * (NT * BM) + t * BM + r;
+      const int64_t part = ((int64_t)2 * blockIdx.x + (seg.lo == 0 ? 1 : 0)) * NT + t;   // 128 rows
       if (!whole && seg.lo == 0)   // the last of the run: each later CTA takes `run` tiles of the rest
         rec = PartRecord{seg.hk, 1 + (seg.n - seg.hi + run - 1) / run, seg.s.q_begin + seg.m0, seg.s.q_len - seg.m0};
-      char* orow = whole ? reinterpret_cast<char*>(a.out) + (qtok * a.o_rs + (int64_t)h * a.o_hs) * 2
-                         : reinterpret_cast<char*>(pa.part_o + part * HD);
+      T* orow = reinterpret_cast<T*>(a.out) + qtok * a.o_rs + (int64_t)h * a.o_hs;
+      float4* prow = reinterpret_cast<float4*>(pa.part_o + part * BM * HD) + r;   // 16-byte piece p of row r at p * 128 + r
 #pragma unroll 1
       for (int q = 0; q < 8; ++q) {
         uint32_t o[16];
@@ -705,23 +707,23 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         float f[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv;
-        if (valid && !whole) {
+        if (!whole) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<float4*>(orow + q * 64 + e * 16) = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+            prow[(q * 4 + e) * BM] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
         } else if (valid) {
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<uint4*>(orow + q * 32 + e * 16) =
+            *reinterpret_cast<uint4*>(orow + q * 16 + e * 8) =
                 make_uint4(Pair<T>::pack(f[8 * e], f[8 * e + 1]), Pair<T>::pack(f[8 * e + 2], f[8 * e + 3]),
                            Pair<T>::pack(f[8 * e + 4], f[8 * e + 5]), Pair<T>::pack(f[8 * e + 6], f[8 * e + 7]));
         }
         __syncwarp();
       }
-      if (valid && (!whole || a.lse)) {
+      if (!whole || (valid && a.lse)) {
         const float lse2 = l_run == 0.f ? -INFINITY : m_used + log2f(l_run);
         if (!whole)
-          pa.part_lse[part] = lse2;
+          pa.part_lse[part * BM + r] = lse2;
         else
           a.lse[(int64_t)h * a.total_q + qtok] = l_run == 0.f ? INFINITY : lse2 * 0.6931471805599453f;
       }
@@ -742,50 +744,51 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   }
 }
 
-// Joins the parts of the items that runs cut: warp w of block (i, y) does row 8 y + w of the item whose start, but not end, CTA i
-// holds: its tail part, then the head parts of the CTAs after it, in order.
-constexpr int kJoinWarps = 8;
+// Joins the parts of the items that runs cut.  Block (i, t, y) does dims [32 y, 32 y + 32) of Q tile t of the item whose start, but
+// not end, CTA i holds, a row a thread: its tail part, then the head parts of the CTAs after it, in order.
 template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) attn_cache_join_rows_kernel(ChunkArgs pa, int ctas) {
+__global__ void __launch_bounds__(BM) attn_cache_join_rows_kernel(ChunkArgs pa, int ctas) {
   const AttnArgs& a = pa.c.a;
   asm volatile("griddepcontrol.wait;" ::: "memory");              // launched early: the parts are complete after this
-  const int i = blockIdx.x, lane = threadIdx.x & 31;
+  const int i = blockIdx.x, t = blockIdx.y, r = threadIdx.x;
   const PartRecord rec = pa.record[i];
   if (*reinterpret_cast<volatile int*>(a.status) != 0) return;   // the parts and the records may be missing
-  if (rec.hk < 0) return;
-  const int rows = pa.tiles * BM;
-  const int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
-  const int in_tile = row % BM, in_tok = in_tile / a.group;
-  const int tok = row / BM * pa.tokens + in_tok;
-  if (in_tok >= pa.tokens || tok >= rec.tokens) return;
+  const int in_tok = r / a.group, tok = t * pa.tokens + in_tok;
+  if (rec.hk < 0 || in_tok >= pa.tokens || tok >= rec.tokens) return;
   const int n = min(rec.parts, ctas - i);
-  auto slot = [&](int k) { return (int64_t)(k == 0 ? 2 * i + 1 : 2 * (i + k)) * rows + row; };
+  auto slot = [&](int k) { return (int64_t)(k == 0 ? 2 * i + 1 : 2 * (i + k)) * pa.tiles + t; };
   float m = -INFINITY;
-  for (int k = lane; k < n; k += 32) m = fmaxf(m, pa.part_lse[slot(k)]);
-  m = warp_max(m);
+  for (int k = 0; k < n; ++k) m = fmaxf(m, pa.part_lse[slot(k) * BM + r]);
   const float ms = m == -INFINITY ? 0.f : m;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float wsum = 0.f;
-#pragma unroll 4
+  float acc[32], wsum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) acc[e] = 0.f;
   for (int k = 0; k < n; ++k) {
-    const float w = exp2f(pa.part_lse[slot(k)] - ms);
-    const float4 o = *reinterpret_cast<const float4*>(pa.part_o + slot(k) * HD + lane * 4);
+    const float w = exp2f(pa.part_lse[slot(k) * BM + r] - ms);
+    const float4* o = reinterpret_cast<const float4*>(pa.part_o + slot(k) * BM * HD) + blockIdx.z * 8 * BM + r;
     wsum += w;
-    if (w != 0.f) {   // NaN goes on
-      acc.x += w * o.x;
-      acc.y += w * o.y;
-      acc.z += w * o.z;
-      acc.w += w * o.w;
+    if (w == 0.f) continue;   // NaN goes on
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float4 v = o[e * BM];
+      acc[4 * e] += w * v.x;
+      acc[4 * e + 1] += w * v.y;
+      acc[4 * e + 2] += w * v.z;
+      acc[4 * e + 3] += w * v.w;
     }
   }
   const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
   const int64_t qtok = rec.q_row + tok;
-  const int h = rec.hk * a.group + in_tile - in_tok * a.group;
-  uint2 w2;
-  w2.x = Pair<T>::pack(acc.x * inv, acc.y * inv);
-  w2.y = Pair<T>::pack(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + qtok * a.o_rs + (int64_t)h * a.o_hs + lane * 4) = w2;
-  if (a.lse && lane == 0)
+  const int h = rec.hk * a.group + r - in_tok * a.group;
+  T* out = reinterpret_cast<T*>(a.out) + qtok * a.o_rs + (int64_t)h * a.o_hs + blockIdx.z * 32;
+#pragma unroll
+  for (int e = 0; e < 32; e += 8) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = acc[e + k] * inv;
+    stg16(out + e, Vec16<T>::pack(f));
+  }
+  if (a.lse && blockIdx.z == 0)
     a.lse[(int64_t)h * a.total_q + qtok] = wsum == 0.f ? INFINITY : (m + log2f(wsum)) * 0.6931471805599453f;
 }
 
@@ -821,7 +824,7 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
                            : encode_tmap_8bit(&maps[i], i ? a.v : a.k, 4, dims, strides, box);
     if (rc != FG_OK) return rc;
   }
-  constexpr int smem = smem_of(KIND);
+  constexpr int smem = SMEM_BYTES;
   static thread_local int attr_dev = -1;
   int dev = 0;
   FG_CUDA_OK(cudaGetDevice(&dev));
@@ -840,8 +843,8 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, (unsigned)(pa.tiles * BM / kJoinWarps));
-  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.gridDim = dim3((unsigned)ctas, (unsigned)pa.tiles, HD / 32);
+  cfg.blockDim = dim3(BM);
   cfg.stream = st;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
