@@ -15,6 +15,7 @@ struct Plan {
   int path;
   int splits, tiles_per_split;
   int64_t bytes;       // of workspace
+  int64_t dense;       // rows of each sequence in a 16-bit copy of an 8-bit store, or 0
 };
 
 // Keys that one sequence can have visible to one row tile: everything, or window and first tokens.
@@ -56,6 +57,7 @@ bool tma_ready(const fg_attn_cache_params* p) {
 Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
   const fg_attn_params& b = p->base;
   Plan plan;
+  plan.dense = 0;
   const int64_t group = b.num_heads / b.num_heads_k;
   const bool tma = tma_ready(p);
   if (b.max_seqlen_q * group <= 16 && tma && b.head_dim == 128 && b.softcap == 0.0 && workspace &&
@@ -69,8 +71,15 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
       b.q_head_stride > 0 && b.q_row_stride > 0 && workspace) {
     plan.path = kPathChunk;            // cuts the keys itself, on the device
     plan.splits = plan.tiles_per_split = 1;
-    plan.bytes = attn_cache_chunk_bytes(b.max_seqlen_q, group, b.batch, b.num_heads_k, b.max_seqlen_k / 64 + 1, sms);
+    // An 8-bit store is widened once, ahead of the attention, when at least four items (of 256 query rows) read each key and
+    // the copy takes at most 1 GiB.
+    const int64_t rows = (b.max_seqlen_k + 63) / 64 * 64;
+    if (is_fp8(p->cache_dtype) && b.max_seqlen_q * group >= 1024 && rows > 0 &&
+        b.batch * rows <= (1ll << 30) / (4 * 128 * b.num_heads_k))
+      plan.dense = rows;
+    plan.bytes = attn_cache_chunk_bytes(b.max_seqlen_q, group, b.batch, b.num_heads_k, b.max_seqlen_k, plan.dense, sms);
     if (plan.bytes > 0) return plan;
+    plan.dense = 0;
   }
   if (b.max_seqlen_q * group <= 16 && tma) {
     // Enough CTAs to balance contexts of very different length over all SMs (two resident each), but no range shorter
@@ -209,6 +218,7 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   }
   a.num_splits = plan.splits;
   c.tiles_per_split = plan.tiles_per_split;
+  c.dense = plan.dense;
   const int kind = p->cache_dtype == FG_E4M3 ? kCacheE4M3 : p->cache_dtype == FG_E5M2 ? kCacheE5M2 : kCache16;
   cudaStream_t st = (cudaStream_t)stream;
   FG_REQUIRE((b.max_seqlen_q * a.group + 63) / 64 * plan.splits <= 2147483647LL, "flash_attn_cache: too many row tiles");

@@ -19,9 +19,13 @@
 //   warps 12-15  load K and V rows (one tile ahead, in registers), widen them to fp16 and store them as the 128-byte
 //                swizzled tiles that the tensor cores read; rows that no row of the item sees are neither read nor kept.
 //                (Landing the 8-bit tiles in shared memory by TMA first costs two more waits and a read for each: two chunks
-//                of 2048 tokens took 789 us.)  bf16 queries are brought to fp16, each row by a power of two, by the softmax
-//                warps before an item's first step.
+//                of 2048 tokens took 789 us, 663 us so.)
 //   warp 11      O += P V of both tiles
+// Widening inside the kernel makes a step half as long again, and every item widens the keys it reads anew.  Where the chunk is
+// long (several items read each key) and the store's 16-bit copy is not too large, a kernel before this one widens the visible
+// rows once into the workspace, and this one reads them as a 16-bit store (attn_cache_api.cu has the rule).
+// Over 8-bit caches bf16 queries are brought to fp16, each row by a power of two, by the softmax warps before an item's first
+// step.
 // TMEM columns: tile t has its scores at t*128 (64 columns), two probability buffers at t*128+64 and +96, its output at
 // 256+t*128.  Every wait is an mbarrier wait with a limit.
 #include "attn_cache_common.cuh"
@@ -90,7 +94,7 @@ __device__ __forceinline__ void set_part(Segment& g, int lo) {
   g.hi = min(g.n, lo + g.left);
 }
 __device__ __forceinline__ void fill_segment(const ChunkArgs& pa, const InfoTable& table, Segment& g) {
-  g.s = (unsigned)(g.b - table.b0) < (unsigned)table.n ? table.info[g.b - table.b0] : seq_info(pa.c.a, g.b);
+  g.s = (unsigned)(g.b - table.b0) < (unsigned)table.n ? table.info[g.b - table.b0] : cache_seq_info(pa.c, g.b);
   g.n = item_tiles(pa, g.s, g.m, g.span);
   g.m0 = g.m * pa.tiles * pa.tokens;
   g.nt = g.m0 + pa.tokens < g.s.q_len ? pa.tiles : 1;
@@ -142,12 +146,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-template <typename T, int KIND>
+// T: type of q and out; KIND: what K and V are read as; M: type of the products
+template <typename T, int KIND, typename M>
 __global__ void __launch_bounds__(threads_of(KIND), 1)
 attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                         const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ ChunkArgs pa) {
   using namespace sm100;
-  using M = typename std::conditional<KIND == kCache16, T, __half>::type;   // type of the products
   constexpr bool kBf16 = std::is_same<M, __nv_bfloat16>::value;
   constexpr bool kConvQ = !std::is_same<T, M>::value;
   constexpr bool kWiden = KIND != kCache16;
@@ -186,7 +190,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   const int pairs = a.batch * pa.num_mb;
   TileSpan span;
   int mine = 0;
-  if (tid < pairs) mine = item_tiles(pa, seq_info(a, tid / pa.num_mb), tid % pa.num_mb, span) * a.Hk;
+  if (tid < pairs) mine = item_tiles(pa, cache_seq_info(c, tid / pa.num_mb), tid % pa.num_mb, span) * a.Hk;
   if (tid == 0) {
     s_drain = *reinterpret_cast<volatile int*>(a.status);
     *abort_flag = 0;
@@ -213,7 +217,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   }
   int total = mine;
   for (int p = tid + THREADS; p < pairs; p += THREADS)
-    total += item_tiles(pa, seq_info(a, p / pa.num_mb), p % pa.num_mb, span) * a.Hk;
+    total += item_tiles(pa, cache_seq_info(c, p / pa.num_mb), p % pa.num_mb, span) * a.Hk;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) s_sum[warp] = total;
@@ -232,7 +236,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   for (int p0 = 0;; p0 += THREADS) {
     if (p0 > 0) {
       const int p = p0 + tid;
-      mine = p < pairs ? item_tiles(pa, seq_info(a, p / pa.num_mb), p % pa.num_mb, span) * a.Hk : 0;
+      mine = p < pairs ? item_tiles(pa, cache_seq_info(c, p / pa.num_mb), p % pa.num_mb, span) * a.Hk : 0;
     }
     int incl = mine;
 #pragma unroll
@@ -267,7 +271,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   seg.b = s_pair / pa.num_mb;
   seg.m = s_pair - seg.b * pa.num_mb;
   const InfoTable table{sInfo, seg.b, min(kInfo, a.batch - seg.b)};
-  if (tid < table.n) sInfo[tid] = seq_info(a, seg.b + tid);
+  if (tid < table.n) sInfo[tid] = cache_seq_info(c, seg.b + tid);
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;");   // the joining kernel may be set up: it waits for this one's end
   seg.left = min(total - (int)begin, run);
@@ -298,7 +302,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       row = seg.s.k_begin + tok;
       if (lane >= pa.pages_per_tile || tok >= seg.last.hi || (tok + pa.page_rows <= seg.first.lo && tok >= c.sinks)) return;
       page = 0;
-      if (a.paged) {
+      if (c.pages()) {
         const int pg = tok / a.block_size;
         row = tok - pg * a.block_size;
         page = cache_page(c, a.block_table + (int64_t)seg.b * a.bt_stride, pg);
@@ -357,7 +361,8 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       uint32_t item = 0, kv = 0, g[TILES] = {};   // items, K/V tiles, and steps of each Q tile so far
       bool ok = true;
       do {
-        ok = wait1(kConvQ ? &q_ready[t0] : q_full, item & 1);
+        // (of every Q tile of this thread, whether it holds a token or not)
+        ok = wait1(kConvQ ? &q_ready[t0] : q_full, item & 1) && (!kConvQ || t0 + TILES > NT || TILES == 1 || wait1(&q_ready[1], item & 1));
         ++item;
         for (int i = seg.lo; i < seg.hi && ok; ++i, ++kv) {
           const uint32_t stg = kv % STAGES;
@@ -799,11 +804,12 @@ void chunk_shape(int64_t max_q, int64_t group, int* tiles, int* tokens, int64_t*
   *num_mb = (max_q + *tiles * *tokens - 1) / (*tiles * *tokens);
 }
 
-template <typename T, int KIND>
+template <typename T, int KIND, typename M>
 int launch(ChunkArgs& pa, cudaStream_t st) {
   const AttnArgs& a = pa.c.a;
   constexpr int ES = KIND == kCache16 ? 2 : 1;
-  pa.page_rows = a.paged && a.block_size < BN ? a.block_size : BN;
+  const bool pages = pa.c.pages();
+  pa.page_rows = pages && a.block_size < BN ? a.block_size : BN;
   pa.pages_per_tile = BN / pa.page_rows;
   CUtensorMap tq, maps[2];
   {
@@ -816,9 +822,9 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
   for (int i = 0; i < 2; ++i) {
     const uint64_t hs = (uint64_t)(i ? a.v_hs : a.k_hs) * ES, rs = (uint64_t)(i ? a.v_rs : a.k_rs) * ES;
     const uint64_t bs = (uint64_t)(i ? a.v_bs : a.k_bs) * ES;
-    const uint64_t rows = a.paged ? (uint64_t)a.block_size : (uint64_t)(a.total_k > 0 ? a.total_k : 1);
-    const uint64_t dims[4] = {(uint64_t)HD, (uint64_t)a.Hk, rows, a.paged ? (uint64_t)a.num_blocks : 1};
-    const uint64_t strides[3] = {hs, rs, a.paged ? bs : rs * rows};
+    const uint64_t rows = pages ? (uint64_t)a.block_size : (uint64_t)(a.total_k > 0 ? a.total_k : 1);
+    const uint64_t dims[4] = {(uint64_t)HD, (uint64_t)a.Hk, rows, pages ? (uint64_t)a.num_blocks : 1};
+    const uint64_t strides[3] = {hs, rs, pages ? bs : rs * rows};
     const uint32_t box[4] = {(uint32_t)(128 / ES), 1, (uint32_t)pa.page_rows, 1};
     const int rc = ES == 2 ? encode_tmap_16bit(&maps[i], i ? a.v : a.k, 4, dims, strides, box)
                            : encode_tmap_8bit(&maps[i], i ? a.v : a.k, 4, dims, strides, box);
@@ -829,14 +835,14 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
   int dev = 0;
   FG_CUDA_OK(cudaGetDevice(&dev));
   if (attr_dev != dev) {
-    FG_CUDA_OK(cudaFuncSetAttribute(attn_cache_chunk_kernel<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    FG_CUDA_OK(cudaFuncSetAttribute(attn_cache_chunk_kernel<T, KIND, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_dev = dev;
   }
   const int ctas = num_sms();
   pa.part_o = a.ws_o;
   pa.part_lse = pa.part_o + (int64_t)2 * ctas * pa.tiles * BM * HD;
   pa.record = reinterpret_cast<PartRecord*>(pa.part_lse + (int64_t)2 * ctas * pa.tiles * BM);
-  attn_cache_chunk_kernel<T, KIND><<<ctas, threads_of(KIND), smem, st>>>(tq, maps[0], maps[1], pa);
+  attn_cache_chunk_kernel<T, KIND, M><<<ctas, threads_of(KIND), smem, st>>>(tq, maps[0], maps[1], pa);
   FG_CHECK_LAUNCH("attn_cache_chunk_kernel");
   // Launched while the kernel above still runs (programmatic dependent launch); it waits for its end on the device.
   cudaLaunchAttribute early;
@@ -853,22 +859,97 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
   return FG_OK;
 }
 
+// Widens the rows of an 8-bit store that some query sees: token j of sequence b to row b * dense + j of fp16 [rows, Hk, 128] K and V.
+// A block does 16 tokens; a thread 16 values at a time, four of them in flight.
+constexpr int kWidenRows = 16;
+template <int KIND>
+__global__ void __launch_bounds__(256) attn_cache_widen_kernel(CacheAttnArgs c, __half* k16, __half* v16, int64_t dense) {
+  const AttnArgs& a = c.a;
+  __shared__ int64_t s_row[2][kWidenRows];       // of K and V: elements from the store's base, or -1
+  const int b = blockIdx.y, tok0 = blockIdx.x * kWidenRows;
+  const SeqInfo s = seq_info(a, b);
+  const RowMask first = row_mask(c, s.k_len, s.k_len - s.q_len), last = row_mask(c, s.k_len, s.k_len - 1);
+  if (s.q_len < 1 || tok0 >= last.hi || (tok0 + kWidenRows <= first.lo && tok0 >= c.sinks)) return;
+  if (threadIdx.x < kWidenRows) {
+    const int tok = tok0 + threadIdx.x;
+    const bool seen = tok < last.hi && tok < dense && (tok >= first.lo || tok < c.sinks);
+    const int32_t* bt_row = a.paged ? a.block_table + (int64_t)b * a.bt_stride : nullptr;
+    s_row[0][threadIdx.x] = seen ? cache_row(c, bt_row, s.k_begin, tok, a.k_rs, a.k_bs) : -1;
+    s_row[1][threadIdx.x] = seen ? cache_row(c, bt_row, s.k_begin, tok, a.v_rs, a.v_bs) : -1;
+  }
+  __syncthreads();
+  const int per_row = a.Hk * (HD / 16), total = 2 * kWidenRows * per_row;
+  for (int base = threadIdx.x; base < total; base += 4 * 256) {
+    uint4 raw[4];
+    __half* dst[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + u * 256;
+      dst[u] = nullptr;
+      if (i >= total) continue;
+      const int ch = i & 7, hk = (i >> 3) % a.Hk, row = i / per_row;
+      const bool is_v = row >= kWidenRows;
+      const int r = is_v ? row - kWidenRows : row;
+      const int64_t at = s_row[is_v][r];
+      if (at < 0) continue;
+      raw[u] = ldg16_stream(reinterpret_cast<const uint8_t*>(is_v ? a.v : a.k) + at + (int64_t)hk * (is_v ? a.v_hs : a.k_hs) + ch * 16);
+      dst[u] = (is_v ? v16 : k16) + (((int64_t)b * dense + tok0 + r) * a.Hk + hk) * HD + ch * 16;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (dst[u] == nullptr) continue;
+      uint4 lo, hi;
+      fp8x4_to_f16x4<KIND>(raw[u].x, lo.x, lo.y);
+      fp8x4_to_f16x4<KIND>(raw[u].y, lo.z, lo.w);
+      fp8x4_to_f16x4<KIND>(raw[u].z, hi.x, hi.y);
+      fp8x4_to_f16x4<KIND>(raw[u].w, hi.z, hi.w);
+      stg16(dst[u], lo);
+      stg16(dst[u] + 8, hi);
+    }
+  }
+}
+
+// Bytes of the parts and records that come first in the workspace.
+int64_t part_bytes(int tiles, int sms) {
+  return ((int64_t)sms * (2 * tiles * BM * (HD + 1) * 4 + (int64_t)sizeof(PartRecord)) + 1023) / 1024 * 1024;
+}
+
 template <typename T>
 int launch_kind(ChunkArgs& pa, int kind, cudaStream_t st) {
-  if (kind == kCacheE4M3) return launch<T, kCacheE4M3>(pa, st);
-  if (kind == kCacheE5M2) return launch<T, kCacheE5M2>(pa, st);
-  return launch<T, kCache16>(pa, st);
+  CacheAttnArgs& c = pa.c;
+  if (kind == kCache16) return launch<T, kCache16, T>(pa, st);
+  if (c.dense > 0) {   // rows of a sequence in the 16-bit copy
+    AttnArgs& a = c.a;
+    const int64_t rows = a.batch * c.dense;
+    __half* k16 = reinterpret_cast<__half*>(reinterpret_cast<char*>(a.ws_o) + part_bytes(pa.tiles, num_sms()));
+    __half* v16 = k16 + rows * a.Hk * HD;
+    const dim3 grid((unsigned)((c.dense + kWidenRows - 1) / kWidenRows), (unsigned)a.batch);
+    if (kind == kCacheE4M3)
+      attn_cache_widen_kernel<kCacheE4M3><<<grid, 256, 0, st>>>(c, k16, v16, c.dense);
+    else
+      attn_cache_widen_kernel<kCacheE5M2><<<grid, 256, 0, st>>>(c, k16, v16, c.dense);
+    FG_CHECK_LAUNCH("attn_cache_widen_kernel");
+    a.k = k16;
+    a.v = v16;
+    a.total_k = rows;
+    a.k_hs = a.v_hs = HD;
+    a.k_rs = a.v_rs = (int64_t)a.Hk * HD;
+    return launch<T, kCache16, __half>(pa, st);
+  }
+  if (kind == kCacheE4M3) return launch<T, kCacheE4M3, __half>(pa, st);
+  return launch<T, kCacheE5M2, __half>(pa, st);
 }
 
 }  // namespace
 
-// Bytes of workspace: a head and a tail part, and a record, for each CTA.  0: more tiles than the kernel counts in 32 bits.
-int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t tiles_k, int sms) {
+// Bytes of workspace: a head and a tail part, and a record, for each CTA; with `dense` rows for each sequence also their 16-bit copy.
+// 0: more tiles than the kernel counts in 32 bits.
+int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t max_k, int64_t dense, int sms) {
   int tiles, tokens;
   int64_t num_mb;
   chunk_shape(max_q, group, &tiles, &tokens, &num_mb);
-  if (batch * num_mb > 2147483647LL / 2 || batch * num_mb * heads_k > 2147483647LL / tiles_k) return 0;
-  return (int64_t)sms * (2 * tiles * BM * (HD + 1) * 4 + (int64_t)sizeof(PartRecord));
+  if (batch * num_mb > 2147483647LL / 2 || batch * num_mb * heads_k > 2147483647LL / (max_k / BN + 1)) return 0;
+  return part_bytes(tiles, sms) + 2 * batch * dense * heads_k * HD * 2;
 }
 
 int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st) {

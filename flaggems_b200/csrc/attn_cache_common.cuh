@@ -27,7 +27,14 @@ struct CacheAttnArgs {
   int sinks;
   int table_cols;                          // entries of a block table row
   int tiles_per_split;                     // K/V tiles of one split
+  int64_t dense;                           // chunk kernel: rows of each sequence in a 16-bit copy that k and v point at; 0: none
+  __host__ __device__ bool pages() const { return a.paged && dense == 0; }
 };
+__device__ __forceinline__ SeqInfo cache_seq_info(const CacheAttnArgs& c, int b) {
+  SeqInfo s = seq_info(c.a, b);
+  if (c.dense > 0) s.k_begin = (int)(b * c.dense);
+  return s;
+}
 
 __device__ __forceinline__ float cache_scale(const float* s, int64_t batch_stride, int64_t head_stride, int b, int hk) {
   return s ? s[b * batch_stride + hk * head_stride] : 1.f;
@@ -103,7 +110,7 @@ int attn_cache_generic(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t
 int attn_cache_decode(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
 int64_t attn_cache_decode_sm100_bytes(int64_t rows, int sms);
 int attn_cache_decode_sm100(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
-int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t tiles_k, int sms);
+int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t max_k, int64_t dense, int sms);
 int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
 int attn_cache_combine(const CacheAttnArgs& c, int dtype, cudaStream_t st);
 
