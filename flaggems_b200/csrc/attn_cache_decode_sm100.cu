@@ -179,7 +179,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   uint8_t* sV = sK + C::SLOTS * C::TILE;                             // [VS]
   uint8_t* sQ = sV + C::SLOTS * C::TILE;                             // [2 buffers]: items alternate
   uint8_t* sP = sQ + 2 * C::QB;                                   // [2 buffers]: tiles alternate
-  uint8_t* rest = sP + 2 * C::PB;                                 // 1024 bytes
+  uint8_t* rest = sP + 2 * C::PB;                                 // 384 bytes of barriers, 640 of scratch
   uint64_t* k_full = reinterpret_cast<uint64_t*>(rest);           // [KS]
   uint64_t* k_empty = k_full + C::SLOTS;
   uint64_t* v_full = k_empty + C::SLOTS;    // [VS]
@@ -191,7 +191,8 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   uint64_t* q_ready = o_done + 2;        // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* sMax = reinterpret_cast<float*>(rest + 256);             // [4 warps][16]
+  static_assert((4 * C::SLOTS + 10) * 8 + 8 <= 384, "the barriers end before the scratch");
+  float* sMax = reinterpret_cast<float*>(rest + 384);             // [4 warps][16]
   float* sSum = sMax + 64;                                        // [4 warps][16]
   float* sDown = sSum + 64;                                       // [2 buffers][16]
   SeqInfo* sInfo = reinterpret_cast<SeqInfo*>(rest + 1024);       // [kInfo]

@@ -358,6 +358,15 @@ def test_fp8_decode(fg, dtype, cache, dim, heads, hk):
     check(fg, [1] * 6, [1, 17, 64, 463, 1328, 129], heads, hk, dim, 16, dtype, cache, scale_shape="heads")
 
 
+@pytest.mark.parametrize("cache", [E4M3, torch.bfloat16])
+@pytest.mark.parametrize("heads, hk, tokens", [(7, 1, 1), (16, 1, 1), (4, 1, 4), (4, 4, 1), (4, 1, 40)])
+def test_many_long_sequences(fg, cache, heads, hk, tokens):
+    """Runs of tiles that are cut in the middle of sequences, with waits long enough to look at the abort flag."""
+    lens = [2000 + (i * 997) % 3000 for i in range(48)]
+    window = (-1, -1) if cache in TOP else (4500, 0)
+    check(fg, [tokens] * 48, lens, heads, hk, 128, 16, torch.bfloat16, cache, window=window, sinks=4, scale_shape="heads")
+
+
 @pytest.mark.parametrize("dtype, cache", [(torch.bfloat16, E4M3), (torch.float16, E5M2)])
 @pytest.mark.parametrize("dim", [64, 128, 256, 72])
 @pytest.mark.parametrize("heads, hk", HEADS)
