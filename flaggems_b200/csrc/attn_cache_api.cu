@@ -158,7 +158,7 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
     FG_REQUIRE(p->block_table_cols > 0 && p->block_table_cols <= 2147483647LL, "flash_attn_cache: block_table has no columns");
   } else {
     FG_REQUIRE(b.cu_seqlens_k != nullptr, "cu_seqlens_k or seqused_k must be provided");
-    FG_REQUIRE(b.total_k >= 0, "flash_attn_cache: negative total_k");
+    FG_REQUIRE(b.total_k >= 0 && b.total_k <= 2147483647LL, "flash_attn_cache: bad total_k");
   }
   FG_REQUIRE(aligned16(b.q) && aligned16(b.k) && aligned16(b.v) && aligned16(b.out),
              "flash_attn_cache: tensors must be 16-byte aligned");

@@ -809,6 +809,7 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
   const AttnArgs& a = pa.c.a;
   constexpr int ES = KIND == kCache16 ? 2 : 1;
   const bool pages = pa.c.pages();
+  const int64_t stored = pa.c.dense > 0 ? a.batch * pa.c.dense : a.total_k;   // rows of a store without pages
   pa.page_rows = pages && a.block_size < BN ? a.block_size : BN;
   pa.pages_per_tile = BN / pa.page_rows;
   CUtensorMap tq, maps[2];
@@ -822,7 +823,7 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
   for (int i = 0; i < 2; ++i) {
     const uint64_t hs = (uint64_t)(i ? a.v_hs : a.k_hs) * ES, rs = (uint64_t)(i ? a.v_rs : a.k_rs) * ES;
     const uint64_t bs = (uint64_t)(i ? a.v_bs : a.k_bs) * ES;
-    const uint64_t rows = pages ? (uint64_t)a.block_size : (uint64_t)(a.total_k > 0 ? a.total_k : 1);
+    const uint64_t rows = pages ? (uint64_t)a.block_size : (uint64_t)(stored > 0 ? stored : 1);
     const uint64_t dims[4] = {(uint64_t)HD, (uint64_t)a.Hk, rows, pages ? (uint64_t)a.num_blocks : 1};
     const uint64_t strides[3] = {hs, rs, pages ? bs : rs * rows};
     const uint32_t box[4] = {(uint32_t)(128 / ES), 1, (uint32_t)pa.page_rows, 1};
@@ -867,7 +868,7 @@ __global__ void __launch_bounds__(256) attn_cache_widen_kernel(CacheAttnArgs c, 
   const AttnArgs& a = c.a;
   __shared__ int64_t s_row[2][kWidenRows];       // of K and V: elements from the store's base, or -1
   const int b = blockIdx.y, tok0 = blockIdx.x * kWidenRows;
-  const SeqInfo s = seq_info(a, b);
+  const SeqInfo s = stored_seq_info(c, b);
   const RowMask first = row_mask(c, s.k_len, s.k_len - s.q_len), last = row_mask(c, s.k_len, s.k_len - 1);
   if (s.q_len < 1 || tok0 >= last.hi || (tok0 + kWidenRows <= first.lo && tok0 >= c.sinks)) return;
   if (threadIdx.x < kWidenRows) {
@@ -931,7 +932,6 @@ int launch_kind(ChunkArgs& pa, int kind, cudaStream_t st) {
     FG_CHECK_LAUNCH("attn_cache_widen_kernel");
     a.k = k16;
     a.v = v16;
-    a.total_k = rows;
     a.k_hs = a.v_hs = HD;
     a.k_rs = a.v_rs = (int64_t)a.Hk * HD;
     return launch<T, kCache16, __half>(pa, st);

@@ -30,8 +30,22 @@ struct CacheAttnArgs {
   int64_t dense;                           // chunk kernel: rows of each sequence in a 16-bit copy that k and v point at; 0: none
   __host__ __device__ bool pages() const { return a.paged && dense == 0; }
 };
-__device__ __forceinline__ SeqInfo cache_seq_info(const CacheAttnArgs& c, int b) {
+// Lengths that contradict the sizes of the call (rows behind q or K/V, more keys than max_seqlen_k, by which the work was counted on
+// the host) are cut, so that they cannot fault.
+__device__ __forceinline__ SeqInfo stored_seq_info(const CacheAttnArgs& c, int b) {
   SeqInfo s = seq_info(c.a, b);
+  s.q_begin = max(0, min(s.q_begin, (int)c.a.total_q));
+  s.q_len = min(s.q_len, (int)c.a.total_q - s.q_begin);
+  s.k_len = min(s.k_len, c.a.max_k);
+  if (!c.a.paged) {
+    s.k_begin = max(0, min(s.k_begin, (int)c.a.total_k));
+    s.k_len = min(s.k_len, (int)c.a.total_k - s.k_begin);
+  }
+  return s;
+}
+// As the attention kernels see it: k_begin in the 16-bit copy when there is one.
+__device__ __forceinline__ SeqInfo cache_seq_info(const CacheAttnArgs& c, int b) {
+  SeqInfo s = stored_seq_info(c, b);
   if (c.dense > 0) s.k_begin = (int)(b * c.dense);
   return s;
 }

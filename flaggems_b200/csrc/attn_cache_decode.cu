@@ -69,7 +69,7 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + STAGES);
 
   const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
-  const SeqInfo s = seq_info(a, b);
+  const SeqInfo s = cache_seq_info(c, b);
   const int group = a.group;
   const int rows = min(s.q_len * group, 16);
   if (rows < 1) return;

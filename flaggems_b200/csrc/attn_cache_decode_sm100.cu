@@ -112,7 +112,7 @@ struct InfoTable {
 };
 template <int RP>
 __device__ __forceinline__ void fill_segment(const CacheAttnArgs& c, const InfoTable& table, Segment& g, int lo) {
-  g.s = (unsigned)(g.b - table.b0) < (unsigned)table.n ? table.info[g.b - table.b0] : seq_info(c.a, g.b);
+  g.s = (unsigned)(g.b - table.b0) < (unsigned)table.n ? table.info[g.b - table.b0] : cache_seq_info(c, g.b);
   g.n = item_tiles<RP>(c, g.s, g.span);
   g.rows = min(g.s.q_len * c.a.group, RP);
   g.shift = g.s.k_len - g.s.q_len;
@@ -203,7 +203,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   const int rounds = da.rounds, cta = blockIdx.y * gridDim.x + blockIdx.x;   // block (member, team)
   TileSpan span;
   SeqInfo mine_info{0, 0, 0, 0};          // of sequence tid, for batches of at most a thread each
-  if (tid < a.batch) mine_info = seq_info(a, tid);
+  if (tid < a.batch) mine_info = cache_seq_info(c, tid);
   if (tid == 0) {
     s_drain = *reinterpret_cast<volatile int*>(a.status);
     for (int i = 0; i < C::SLOTS; ++i) {
@@ -229,7 +229,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   int mine = tid < a.batch ? item_tiles<RP>(c, mine_info, span) * rounds : 0;
   int total = mine;
   for (int b = tid + NUM_THREADS; b < a.batch; b += NUM_THREADS)
-    total += item_tiles<RP>(c, seq_info(a, b), span) * rounds;
+    total += item_tiles<RP>(c, cache_seq_info(c, b), span) * rounds;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) s_sum[warp] = total;
@@ -250,7 +250,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
     if (b0 > 0) {
       mine = 0;
       if (b0 + tid < a.batch) {
-        mine_info = seq_info(a, b0 + tid);
+        mine_info = cache_seq_info(c, b0 + tid);
         mine = item_tiles<RP>(c, mine_info, span) * rounds;
       }
     }

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(NTHREADS) attn_cache_generic_kernel(CacheAttnA
   const int m_block = num_mb - 1 - blockIdx.x / a.num_splits;  // long (late) causal rows first
   const int split = blockIdx.x % a.num_splits;
   const int hk = blockIdx.y, b = blockIdx.z;
-  const SeqInfo s = seq_info(a, b);
+  const SeqInfo s = cache_seq_info(c, b);
   const int rows = s.q_len * a.group;
   const int r0 = m_block * BM;
   if (r0 >= rows) return;

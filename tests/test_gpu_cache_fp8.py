@@ -546,6 +546,106 @@ def test_two_captured_graphs_and_another_stream(fg):
             assert torch.equal(s["rows"][i][s["cu_k"][1:].long() - 1], want)
 
 
+def test_large_groups_many_sequences_and_nothing_cached(fg):
+    # more heads of a group than a tile of the general kernel has rows, and than one of the tensor-core kernel has
+    check(fg, [3, 1, 40], [90, 5, 300], 72, 1, 128, 16, torch.bfloat16, E4M3)
+    check(fg, [2, 1], [90, 5], 160, 1, 128, 16, torch.bfloat16, E4M3)
+    check(fg, [3, 1], [90, 5], 80, 1, 64, 16, torch.float16, E4M3)
+    # more sequences than a block has threads
+    lens = [1 + (i * 37) % 150 for i in range(600)]
+    check(fg, [1] * 600, lens, 4, 2, 128, 16, torch.bfloat16, E4M3)
+    check(fg, [i % 3 + (i == 7) * 30 for i in range(600)], lens, 4, 2, 128, 16, torch.bfloat16, torch.bfloat16, window=(60, 0), sinks=4)
+    # nothing cached at all
+    for cache, dim in ((E4M3, 128), (torch.bfloat16, 128), (E4M3, 64)):
+        for q_lens in ([1, 1], [30, 200]):
+            check(fg, q_lens, [0, 0], 4, 2, dim, 16, torch.bfloat16, cache, window=(9, 0), sinks=2)
+
+
+@pytest.mark.parametrize("window", [(-1, -1), (200, 0)])
+@pytest.mark.parametrize("contiguous", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_long_chunks_over_an_8_bit_store(fg, dtype, contiguous, window):
+    """Chunks that are long enough for the store to be widened ahead of the attention."""
+    check(fg, [600, 1, 0, 130], [900, 700, 33, 130], 8, 4, 128, 16, dtype, E4M3, window=window, sinks=3, contiguous=contiguous,
+          scale_shape="one" if contiguous else "batch")
+
+
+@pytest.mark.parametrize("cache", [E4M3, torch.bfloat16])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [40, 3, 130]])
+def test_without_a_workspace(fg, monkeypatch, cache, q_lens):
+    monkeypatch.setattr(_lib.load(), "fg_flash_attn_cache_workspace_bytes", lambda params: 0)
+    for dim in (128, 64):
+        check(fg, q_lens, [3000, 77, 515], 8, 2, dim, 16, torch.bfloat16, cache, window=(2500, 0), sinks=4)
+
+
+@pytest.mark.parametrize("paged_store", [True, False])
+@pytest.mark.parametrize("dim", [128, 64])
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_lengths_that_contradict_the_call_are_cut(fg, q_len, dim, paged_store):
+    """More keys than max_seqlen_k, and rows behind q or K/V: the results are those of the lengths cut to what there is."""
+    g = gen(11)
+    heads, hk = 8, 2
+    q = randn(g, 2 * q_len, heads, dim).to(torch.bfloat16)
+    cu = torch.tensor([0, q_len, 2 * q_len], dtype=torch.int32, device=DEV)
+    kc, vc, table, _ = paged(g, [200, 150], 16, hk, dim, E4M3, torch.ones(1, device=DEV), torch.ones(1, device=DEV))
+    flat = [torch.randint(0, 100, (350, hk, dim), generator=g, device=DEV, dtype=torch.uint8).view(E4M3) for _ in range(2)]
+
+    def run(cu_q, lens, max_k):
+        lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        out = torch.full_like(q, 7.0)
+        if paged_store:
+            return fg.flash_attn_varlen_func(q, kc, vc, q_len, cu_q, max_k, seqused_k=lens, causal=True, block_table=table, out=out)
+        cu_k = torch.cat([lens.new_zeros(1), lens.cumsum(0, dtype=torch.int32)])
+        return fg.flash_attn_varlen_func(q, *flat, q_len, cu_q, max_k, cu_seqlens_k=cu_k, causal=True, out=out)
+
+    assert torch.equal(run(cu, [200, 10 ** 8], 200)[:q_len], run(cu, [200, 150], 200)[:q_len])
+    far = torch.tensor([0, q_len, 10 ** 9], dtype=torch.int32, device=DEV)
+    assert torch.equal(run(far, [200, 150], 200)[:q_len], run(cu, [200, 150], 200)[:q_len])
+    run(torch.tensor([0, 10 ** 8, 2 * 10 ** 8], dtype=torch.int32, device=DEV), [2 * 10 ** 9, 50], 200)
+    run(torch.tensor([-5, 10, 3], dtype=torch.int32, device=DEV), [-4, 50], 200)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("form", ["short", "long", "windowed"])
+def test_chunks_in_two_captured_graphs(fg, form):
+    g = gen(12)
+    page, hk, heads, dim = 16, 2, 8, 128
+    cache = torch.bfloat16 if form == "windowed" else E4M3
+    q_lens, lens = ([400, 3], [1500, 900]) if form == "long" else ([30, 3], [1500, 900])
+    scale = torch.tensor([0.012], device=DEV)
+    kw = dict(window_size=(300, 0), sink_tokens=4) if form == "windowed" else dict(k_descale=scale, v_descale=scale)
+    eight = None if form == "windowed" else scale
+    runs = []
+    for _ in range(2):
+        kc, vc, table, _ = paged(g, lens, page, hk, dim, cache, eight, eight)
+        runs.append((randn(g, sum(q_lens), heads, dim).to(torch.bfloat16), kc, vc, max(q_lens),
+                     torch.tensor([0] + q_lens, device=DEV).cumsum(0, dtype=torch.int32), max(lens), table,
+                     torch.tensor(lens, dtype=torch.int32, device=DEV)))
+
+    def step(r):
+        return fg.flash_attn_varlen_func(*r[:6], seqused_k=r[7], causal=True, block_table=r[6], **kw)
+
+    eager = [step(r).clone() for r in runs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for r in runs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(r))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for o in outs:
+            o.fill_(7.0)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o, e in zip(outs, eager):
+            assert torch.equal(o, e)
+
+
 def test_attention_refusals(fg):
     kc = torch.zeros((4, 16, 2, 64), dtype=E4M3, device=DEV)
     q = torch.zeros((2, 4, 64), dtype=torch.bfloat16, device=DEV)
