@@ -34,13 +34,10 @@
 namespace fg {
 namespace {
 
-constexpr int BM = 128, BN = 64, HD = 128;
-constexpr int HALF_BYTES = 128 * 64 * 2;     // one [128 x 64] swizzled 16-bit sub-tile
-constexpr int TILE_BYTES = 2 * HALF_BYTES;   // 32 KB
-constexpr int UNIT_HALF = BN * 128;          // one [64 keys x 64 columns] swizzled half of a 16-bit K or V tile
-constexpr int UNIT = 2 * UNIT_HALF;          // 16 KB
+constexpr int BM = 128, BN = 64;
+constexpr int HALF_BYTES = 128 * 64 * 2;     // one [128 x 64] swizzled 16-bit piece of a Q tile
+constexpr int UNIT_HALF = BN * 128;          // one [64 keys x 64 columns] swizzled piece of a 16-bit K or V tile
 constexpr int TMA_WARP = 8, MMA_WARP0 = 9, PV_WARP = 11, CONV_WARP0 = 12;
-constexpr int STAGES = 4;                    // 16-bit tiles of K, and of V
 constexpr int TMEM_COLS = 512;
 constexpr float kRescaleThreshold = 8.0f;    // log2 units
 
@@ -48,7 +45,17 @@ constexpr int kMinRun = 8;                   // fewest K/V tiles that a run is w
 constexpr int kInfo = 32;                    // sequences of a run whose lengths are kept in shared memory
 
 constexpr int threads_of(int kind) { return kind == kCache16 ? 12 * 32 : 16 * 32; }
-constexpr int SMEM_BYTES = 2 * TILE_BYTES + 2 * STAGES * UNIT + 1024 + 512 + kInfo * 16;
+
+// By head dim.  At 256 a Q tile takes 64 KB of shared memory and its output half of the tensor memory: one tile, two stages.
+template <int HD>
+struct Shape {
+  static constexpr int PIECES = HD / 64;                   // 64-column pieces of a row
+  static constexpr int TILES = HD > 128 ? 1 : 2;           // Q tiles of an item, at most
+  static constexpr int TILE_BYTES = PIECES * HALF_BYTES;   // a Q tile
+  static constexpr int UNIT = PIECES * UNIT_HALF;          // a 16-bit K or V tile
+  static constexpr int STAGES = HD > 128 ? 2 : 4;          // tiles of K, and of V
+  static constexpr int SMEM = TILES * TILE_BYTES + 2 * STAGES * UNIT + 1024 + 512 + kInfo * 16;
+};
 
 // What a CTA leaves for the joining kernel: the KV head of the item whose start it holds but not its end (or -1), in how many
 // parts the item is, its first query row and its tokens.
@@ -73,6 +80,7 @@ struct Segment {
   int b, m, hk, lo, hi, n;      // K/V tiles [lo, hi) of the n of (sequence b, Q tiles m, KV head hk)
   int left;                     // tiles of the run from lo on
   int m0, nt, shift;            // first token; Q tiles that hold one; position of token 0
+  int gap;                      // 16-bit copy of an 8-bit store: rows between first tokens and window that it leaves out
   SeqInfo s;
   TileSpan span;
   RowMask first, last;          // what the first and the last token see
@@ -83,6 +91,15 @@ __device__ __forceinline__ int item_tiles(const ChunkArgs& pa, const SeqInfo& s,
   const int shift = s.k_len - s.q_len;
   span = tile_span<BN>(pa.c, s.k_len, m0 + shift, min(s.q_len, m0 + pa.tiles * pa.tokens) - 1 + shift);
   return max(span.n, 1);        // nothing visible: one tile, all of it masked, gives the zeros
+}
+// The 16-bit copy of an 8-bit store holds the tiles that some query of the sequence sees, without a gap between the first tokens
+// and the window: tokens from `win` on come `gap` rows earlier.
+struct CopySpan {
+  int win, gap;
+};
+__device__ __forceinline__ CopySpan copy_span(const CacheAttnArgs& c, const SeqInfo& s) {
+  const TileSpan t = tile_span<BN>(c, s.k_len, s.k_len - s.q_len, s.k_len - 1);
+  return CopySpan{t.win * BN, (t.win - t.sink) * BN};
 }
 // Lengths of the sequences [b0, b0 + n) as the CTA found them at its start; the others come from global memory.
 struct InfoTable {
@@ -101,6 +118,7 @@ __device__ __forceinline__ void fill_segment(const ChunkArgs& pa, const InfoTabl
   g.shift = g.s.k_len - g.s.q_len;
   g.first = row_mask(pa.c, g.s.k_len, g.m0 + g.shift);
   g.last = row_mask(pa.c, g.s.k_len, min(g.s.q_len, g.m0 + pa.tiles * pa.tokens) - 1 + g.shift);
+  g.gap = pa.c.dense > 0 ? copy_span(pa.c, g.s).gap : 0;
 }
 // The part after `g`, in place; false when the run ends with g.
 __device__ __forceinline__ bool next_segment(const ChunkArgs& pa, const InfoTable& table, Segment& g) {
@@ -146,8 +164,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// T: type of q and out; KIND: what K and V are read as; M: type of the products
-template <typename T, int KIND, typename M>
+// T: type of q and out; KIND: what K and V are read as; M: type of the products; HD: head dim
+template <typename T, int KIND, typename M, int HD>
 __global__ void __launch_bounds__(threads_of(KIND), 1)
 attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                         const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ ChunkArgs pa) {
@@ -156,6 +174,9 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   constexpr bool kConvQ = !std::is_same<T, M>::value;
   constexpr bool kWiden = KIND != kCache16;
   constexpr int THREADS = threads_of(KIND);
+  using G = Shape<HD>;
+  constexpr int PIECES = G::PIECES, TILE_BYTES = G::TILE_BYTES, UNIT = G::UNIT, STAGES = G::STAGES;
+  static_assert(!kWiden || HD == 128, "the widening warps take rows of 128");
   const CacheAttnArgs& c = pa.c;
   const AttnArgs& a = c.a;
   const int NT = pa.tiles;
@@ -163,8 +184,8 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                       // [2 tiles][2 halves][128 x 64]
-  uint8_t* sK = smem + 2 * TILE_BYTES;      // [STAGES]
+  uint8_t* sQ = smem;                       // [tiles][pieces][128 x 64]
+  uint8_t* sK = smem + G::TILES * TILE_BYTES;   // [STAGES]
   uint8_t* sV = sK + STAGES * UNIT;         // [STAGES]
   uint8_t* rest = sV + STAGES * UNIT;
   uint64_t* bars = reinterpret_cast<uint64_t*>(rest);
@@ -299,7 +320,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     auto lookup = [&](int j, int& page, int& row) {
       const int tok = seg.span.tile(j) * BN + lane * pa.page_rows;
       page = -1;
-      row = seg.s.k_begin + tok;
+      row = seg.s.k_begin + tok - (j < seg.span.sink ? 0 : seg.gap);
       if (lane >= pa.pages_per_tile || tok >= seg.last.hi || (tok + pa.page_rows <= seg.first.lo && tok >= c.sinks)) return;
       page = 0;
       if (c.pages()) {
@@ -320,9 +341,9 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       if (!is_v) {
         if (item > 0 && !wwait(q_empty, (item - 1) & 1)) break;
         if (lane == 0) {
-          mbar_expect_tx(q_full, seg.nt * 2 * pa.tokens * a.group * 128);
+          mbar_expect_tx(q_full, seg.nt * PIECES * pa.tokens * a.group * 128);
           for (int t = 0; t < seg.nt; ++t)
-            for (int hf = 0; hf < 2; ++hf)
+            for (int hf = 0; hf < PIECES; ++hf)
               tma_load_3d(sQ + t * TILE_BYTES + hf * HALF_BYTES, &tmap_q, q_full, hf * 64, seg.hk * a.group,
                           seg.s.q_begin + seg.m0 + t * pa.tokens);
         }
@@ -339,11 +360,11 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             ok = false;
             break;
           }
-          if (lane == 0) mbar_expect_tx(&full[stg], pages * pa.page_rows * 256);
+          if (lane == 0) mbar_expect_tx(&full[stg], pages * pa.page_rows * (HD * 2));
           __syncwarp();
           if (page >= 0) {
             uint8_t* dst = ring + stg * UNIT + lane * pa.page_rows * 128;
-            for (int hf = 0; hf < 2; ++hf) tma_load_4d(dst + hf * UNIT_HALF, tm, &full[stg], hf * 64, seg.hk, row, page);
+            for (int hf = 0; hf < PIECES; ++hf) tma_load_4d(dst + hf * UNIT_HALF, tm, &full[stg], hf * 64, seg.hk, row, page);
           }
           page = npage;
           row = nrow;
@@ -554,7 +575,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         uint8_t* q = sQ + t * TILE_BYTES + r * 128;
         float top = 0.f;
 #pragma unroll 4
-        for (int ch = 0; ch < 16; ++ch) {
+        for (int ch = 0; ch < HD / 8; ++ch) {
           float f[8];
           Vec16<T>::unpack(*reinterpret_cast<const uint4*>(q + (ch >> 3) * HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4)), f);
 #pragma unroll
@@ -563,7 +584,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         float up, down;
         row_power(top, up, down);
 #pragma unroll 4
-        for (int ch = 0; ch < 16; ++ch) {
+        for (int ch = 0; ch < HD / 8; ++ch) {
           uint4* at = reinterpret_cast<uint4*>(q + (ch >> 3) * HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4));
           float f[8];
           Vec16<T>::unpack(*at, f);
@@ -630,7 +651,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           tc_fence_after();
           const float f = raise ? ex2(m_used - m_tile) : 1.0f;
 #pragma unroll 1
-          for (int q = 0; q < 8; ++q) {
+          for (int q = 0; q < HD / 16; ++q) {
             uint32_t o[16];
             tmem_ld16(o_addr + q * 16, o);
             tmem_ld_wait();
@@ -652,8 +673,8 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
               break;
             }
             uint8_t* vt = sV + stg * UNIT;
-            for (int at = r; at < BN * 16; at += 128) {
-              const int row = at / 16, ch = at % 16, col = col0 + row;
+            for (int at = r; at < BN * (HD / 8); at += 128) {
+              const int row = at / (HD / 8), ch = at % (HD / 8), col = col0 + row;
               if (col >= seg.last.hi || (col < seg.first.lo && col >= c.sinks))
                 *reinterpret_cast<uint4*>(vt + (ch >> 3) * UNIT_HALF + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
@@ -700,11 +721,11 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       T* orow = reinterpret_cast<T*>(a.out) + qtok * a.o_rs + (int64_t)h * a.o_hs;
       float4* prow = reinterpret_cast<float4*>(pa.part_o + part * BM * HD) + r;   // 16-byte piece p of row r at p * 128 + r
 #pragma unroll 1
-      for (int q = 0; q < 8; ++q) {
+      for (int q = 0; q < HD / 16; ++q) {
         uint32_t o[16];
         tmem_ld16(o_addr + q * 16, o);
         tmem_ld_wait();
-        if (q == 7) {   // my row is in registers: the next item's first product may overwrite it
+        if (q == HD / 16 - 1) {   // my row is in registers: the next item's first product may overwrite it
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&o_free[t]);
@@ -751,7 +772,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
 
 // Joins the parts of the items that runs cut.  Block (i, t, y) does dims [32 y, 32 y + 32) of Q tile t of the item whose start, but
 // not end, CTA i holds, a row a thread: its tail part, then the head parts of the CTAs after it, in order.
-template <typename T>
+template <typename T, int HD>
 __global__ void __launch_bounds__(BM) attn_cache_join_rows_kernel(ChunkArgs pa, int ctas) {
   const AttnArgs& a = pa.c.a;
   asm volatile("griddepcontrol.wait;" ::: "memory");              // launched early: the parts are complete after this
@@ -798,13 +819,13 @@ __global__ void __launch_bounds__(BM) attn_cache_join_rows_kernel(ChunkArgs pa, 
 }
 
 // Q tiles of an item, tokens of a tile and items (for each KV head) of the longest chunk.
-void chunk_shape(int64_t max_q, int64_t group, int* tiles, int* tokens, int64_t* num_mb) {
+void chunk_shape(int64_t max_q, int64_t group, int64_t head_dim, int* tiles, int* tokens, int64_t* num_mb) {
   *tokens = (int)(BM / group);
-  *tiles = max_q > *tokens ? 2 : 1;
+  *tiles = max_q > *tokens && head_dim <= 128 ? 2 : 1;
   *num_mb = (max_q + *tiles * *tokens - 1) / (*tiles * *tokens);
 }
 
-template <typename T, int KIND, typename M>
+template <typename T, int KIND, typename M, int HD>
 int launch(ChunkArgs& pa, cudaStream_t st) {
   const AttnArgs& a = pa.c.a;
   constexpr int ES = KIND == kCache16 ? 2 : 1;
@@ -831,19 +852,19 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
                            : encode_tmap_8bit(&maps[i], i ? a.v : a.k, 4, dims, strides, box);
     if (rc != FG_OK) return rc;
   }
-  constexpr int smem = SMEM_BYTES;
+  constexpr int smem = Shape<HD>::SMEM;
   static thread_local int attr_dev = -1;
   int dev = 0;
   FG_CUDA_OK(cudaGetDevice(&dev));
   if (attr_dev != dev) {
-    FG_CUDA_OK(cudaFuncSetAttribute(attn_cache_chunk_kernel<T, KIND, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    FG_CUDA_OK(cudaFuncSetAttribute(attn_cache_chunk_kernel<T, KIND, M, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_dev = dev;
   }
   const int ctas = num_sms();
   pa.part_o = a.ws_o;
   pa.part_lse = pa.part_o + (int64_t)2 * ctas * pa.tiles * BM * HD;
   pa.record = reinterpret_cast<PartRecord*>(pa.part_lse + (int64_t)2 * ctas * pa.tiles * BM);
-  attn_cache_chunk_kernel<T, KIND, M><<<ctas, threads_of(KIND), smem, st>>>(tq, maps[0], maps[1], pa);
+  attn_cache_chunk_kernel<T, KIND, M, HD><<<ctas, threads_of(KIND), smem, st>>>(tq, maps[0], maps[1], pa);
   FG_CHECK_LAUNCH("attn_cache_chunk_kernel");
   // Launched while the kernel above still runs (programmatic dependent launch); it waits for its end on the device.
   cudaLaunchAttribute early;
@@ -855,31 +876,35 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  FG_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_cache_join_rows_kernel<T>, pa, ctas));
+  FG_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_cache_join_rows_kernel<T, HD>, pa, ctas));
   FG_CHECK_LAUNCH("attn_cache_join_rows_kernel");
   return FG_OK;
 }
 
-// Widens the rows of an 8-bit store that some query sees: token j of sequence b to row b * dense + j of fp16 [rows, Hk, 128] K and V.
+// Widens the rows of an 8-bit store that some query sees: the tokens of sequence b, in the order of copy_span, to the rows from
+// b * dense on of fp16 [rows, Hk, D] K and V.
 // A block does 16 tokens; a thread 16 values at a time, four of them in flight.
 constexpr int kWidenRows = 16;
 template <int KIND>
 __global__ void __launch_bounds__(256) attn_cache_widen_kernel(CacheAttnArgs c, __half* k16, __half* v16, int64_t dense) {
   const AttnArgs& a = c.a;
   __shared__ int64_t s_row[2][kWidenRows];       // of K and V: elements from the store's base, or -1
-  const int b = blockIdx.y, tok0 = blockIdx.x * kWidenRows;
-  const SeqInfo s = stored_seq_info(c, b);
+  const SeqInfo s = stored_seq_info(c, blockIdx.y);
+  if (s.q_len < 1) return;
+  const CopySpan copy = copy_span(c, s);
+  const int b = blockIdx.y, row0 = blockIdx.x * kWidenRows, tok0 = row0 + (row0 + copy.gap < copy.win ? 0 : copy.gap);
   const RowMask first = row_mask(c, s.k_len, s.k_len - s.q_len), last = row_mask(c, s.k_len, s.k_len - 1);
-  if (s.q_len < 1 || tok0 >= last.hi || (tok0 + kWidenRows <= first.lo && tok0 >= c.sinks)) return;
+  if (tok0 >= last.hi || (tok0 + kWidenRows <= first.lo && tok0 >= c.sinks)) return;
   if (threadIdx.x < kWidenRows) {
     const int tok = tok0 + threadIdx.x;
-    const bool seen = tok < last.hi && tok < dense && (tok >= first.lo || tok < c.sinks);
+    const bool seen = tok < last.hi && (tok >= first.lo || tok < c.sinks);
     const int32_t* bt_row = a.paged ? a.block_table + (int64_t)b * a.bt_stride : nullptr;
     s_row[0][threadIdx.x] = seen ? cache_row(c, bt_row, s.k_begin, tok, a.k_rs, a.k_bs) : -1;
     s_row[1][threadIdx.x] = seen ? cache_row(c, bt_row, s.k_begin, tok, a.v_rs, a.v_bs) : -1;
   }
   __syncthreads();
-  const int per_row = a.Hk * (HD / 16), total = 2 * kWidenRows * per_row;
+  const int pieces = a.D >> 4, shift = 31 - __clz(pieces);   // a power of two
+  const int per_row = a.Hk * pieces, total = 2 * kWidenRows * per_row;
   for (int base = threadIdx.x; base < total; base += 4 * 256) {
     uint4 raw[4];
     __half* dst[4];
@@ -888,13 +913,13 @@ __global__ void __launch_bounds__(256) attn_cache_widen_kernel(CacheAttnArgs c, 
       const int i = base + u * 256;
       dst[u] = nullptr;
       if (i >= total) continue;
-      const int ch = i & 7, hk = (i >> 3) % a.Hk, row = i / per_row;
+      const int ch = i & (pieces - 1), hk = (i >> shift) % a.Hk, row = i / per_row;
       const bool is_v = row >= kWidenRows;
       const int r = is_v ? row - kWidenRows : row;
       const int64_t at = s_row[is_v][r];
       if (at < 0) continue;
       raw[u] = ldg16_stream(reinterpret_cast<const uint8_t*>(is_v ? a.v : a.k) + at + (int64_t)hk * (is_v ? a.v_hs : a.k_hs) + ch * 16);
-      dst[u] = (is_v ? v16 : k16) + (((int64_t)b * dense + tok0 + r) * a.Hk + hk) * HD + ch * 16;
+      dst[u] = (is_v ? v16 : k16) + (((int64_t)b * dense + row0 + r) * a.Hk + hk) * a.D + ch * 16;
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -911,19 +936,26 @@ __global__ void __launch_bounds__(256) attn_cache_widen_kernel(CacheAttnArgs c, 
 }
 
 // Bytes of the parts and records that come first in the workspace.
-int64_t part_bytes(int tiles, int sms) {
-  return ((int64_t)sms * (2 * tiles * BM * (HD + 1) * 4 + (int64_t)sizeof(PartRecord)) + 1023) / 1024 * 1024;
+int64_t part_bytes(int tiles, int64_t head_dim, int sms) {
+  return ((int64_t)sms * (2 * tiles * BM * (head_dim + 1) * 4 + (int64_t)sizeof(PartRecord)) + 1023) / 1024 * 1024;
+}
+
+template <typename T, typename M>
+int launch_16(ChunkArgs& pa, cudaStream_t st) {
+  if (pa.c.a.D == 64) return launch<T, kCache16, M, 64>(pa, st);
+  if (pa.c.a.D == 256) return launch<T, kCache16, M, 256>(pa, st);
+  return launch<T, kCache16, M, 128>(pa, st);
 }
 
 template <typename T>
 int launch_kind(ChunkArgs& pa, int kind, cudaStream_t st) {
   CacheAttnArgs& c = pa.c;
-  if (kind == kCache16) return launch<T, kCache16, T>(pa, st);
+  if (kind == kCache16) return launch_16<T, T>(pa, st);
   if (c.dense > 0) {   // rows of a sequence in the 16-bit copy
     AttnArgs& a = c.a;
     const int64_t rows = a.batch * c.dense;
-    __half* k16 = reinterpret_cast<__half*>(reinterpret_cast<char*>(a.ws_o) + part_bytes(pa.tiles, num_sms()));
-    __half* v16 = k16 + rows * a.Hk * HD;
+    __half* k16 = reinterpret_cast<__half*>(reinterpret_cast<char*>(a.ws_o) + part_bytes(pa.tiles, a.D, num_sms()));
+    __half* v16 = k16 + rows * a.Hk * a.D;
     const dim3 grid((unsigned)((c.dense + kWidenRows - 1) / kWidenRows), (unsigned)a.batch);
     if (kind == kCacheE4M3)
       attn_cache_widen_kernel<kCacheE4M3><<<grid, 256, 0, st>>>(c, k16, v16, c.dense);
@@ -932,24 +964,25 @@ int launch_kind(ChunkArgs& pa, int kind, cudaStream_t st) {
     FG_CHECK_LAUNCH("attn_cache_widen_kernel");
     a.k = k16;
     a.v = v16;
-    a.k_hs = a.v_hs = HD;
-    a.k_rs = a.v_rs = (int64_t)a.Hk * HD;
-    return launch<T, kCache16, __half>(pa, st);
+    a.k_hs = a.v_hs = a.D;
+    a.k_rs = a.v_rs = (int64_t)a.Hk * a.D;
+    return launch_16<T, __half>(pa, st);
   }
-  if (kind == kCacheE4M3) return launch<T, kCacheE4M3, __half>(pa, st);
-  return launch<T, kCacheE5M2, __half>(pa, st);
+  if (kind == kCacheE4M3) return launch<T, kCacheE4M3, __half, 128>(pa, st);
+  return launch<T, kCacheE5M2, __half, 128>(pa, st);
 }
 
 }  // namespace
 
 // Bytes of workspace: a head and a tail part, and a record, for each CTA; with `dense` rows for each sequence also their 16-bit copy.
 // 0: more tiles than the kernel counts in 32 bits.
-int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t max_k, int64_t dense, int sms) {
+int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t head_dim, int64_t max_k,
+                               int64_t dense, int sms) {
   int tiles, tokens;
   int64_t num_mb;
-  chunk_shape(max_q, group, &tiles, &tokens, &num_mb);
+  chunk_shape(max_q, group, head_dim, &tiles, &tokens, &num_mb);
   if (batch * num_mb > 2147483647LL / 2 || batch * num_mb * heads_k > 2147483647LL / (max_k / BN + 1)) return 0;
-  return part_bytes(tiles, sms) + 2 * batch * dense * heads_k * HD * 2;
+  return part_bytes(tiles, head_dim, sms) + 2 * batch * dense * heads_k * head_dim * 2;
 }
 
 int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st) {
@@ -957,7 +990,7 @@ int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t s
   pa.c = c;
   if (!c.a.status) return fail(FG_ERR_CUDA, "flash_attn_cache: device status word unavailable");
   int64_t num_mb;
-  chunk_shape(c.a.max_q, c.a.group, &pa.tiles, &pa.tokens, &num_mb);
+  chunk_shape(c.a.max_q, c.a.group, c.a.D, &pa.tiles, &pa.tokens, &num_mb);
   pa.num_mb = (int)num_mb;
   return dtype == FG_BF16 ? launch_kind<__nv_bfloat16>(pa, kind, st) : launch_kind<__half>(pa, kind, st);
 }

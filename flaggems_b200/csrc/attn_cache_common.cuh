@@ -124,7 +124,8 @@ int attn_cache_generic(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t
 int attn_cache_decode(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
 int64_t attn_cache_decode_sm100_bytes(int64_t rows, int sms);
 int attn_cache_decode_sm100(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
-int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t max_k, int64_t dense, int sms);
+int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t head_dim, int64_t max_k,
+                               int64_t dense, int sms);
 int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
 int attn_cache_combine(const CacheAttnArgs& c, int dtype, cudaStream_t st);
 
