@@ -94,6 +94,7 @@ class AttnCacheParams(C.Structure):
 CACHE_WRITE = struct.Struct("=7Q12q2i")
 CACHE_GATHER = struct.Struct("=9Q15q2i")
 ATTN_CACHE = struct.Struct("=11Q29q2d4i2Q6q2i")
+WORKSPACE = struct.Struct("=Qq")   # its pointer and bytes, at byte 80 of ATTN_CACHE
 
 
 class GemmPlan(C.Structure):
@@ -227,7 +228,7 @@ def stream_ptr(device: torch.device) -> int:
 
 _HERE = contextlib.nullcontext()
 # the stream handle without a torch.cuda.Stream object around it
-_raw_stream = torch._C._cuda_getCurrentRawStream
+raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def on_device(device: torch.device):
@@ -239,10 +240,10 @@ def call(device: torch.device, fn, *args) -> None:
     """``fn(*args, stream)`` on the current stream of ``device``, with that device current."""
     index = device.index
     if torch.cuda.current_device() == index:
-        rc = fn(*args, _raw_stream(index))
+        rc = fn(*args, raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(*args, raw_stream(index))
     if rc < 0:
         check(rc)
 

@@ -60,6 +60,10 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
   plan.dense = 0;
   const int64_t group = b.num_heads / b.num_heads_k;
   const bool tma = tma_ready(p);
+  // At head dim 64 an 8-bit store's copy has to pay for itself: 1056 tiles of the general kernel (two chunks of up to 300 tokens)
+  // take 21 us there and 29 us with the copy, 15872 (eight of up to 64 tokens over 4000) 152 and 60 us.
+  const bool few = b.head_dim == 64 && is_fp8(p->cache_dtype) &&
+                   b.batch * b.num_heads_k * ((b.max_seqlen_q * group + 63) / 64) * ((most_keys(p, b.max_seqlen_q) + 63) / 64) < 1536;
   if (b.max_seqlen_q * group <= 16 && tma && b.head_dim == 128 && b.softcap == 0.0 && workspace &&
       b.batch * b.num_heads_k * (b.max_seqlen_k / 128 + 1) <= 2147483647LL) {
     plan.path = kPathDecodeSm100;      // cuts the keys itself, on the device
@@ -67,7 +71,7 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
     plan.bytes = attn_cache_decode_sm100_bytes(b.max_seqlen_q * group, sms);
     return plan;
   }
-  if (b.max_seqlen_q * group > 16 && tma && (b.head_dim == 64 || b.head_dim == 128 || b.head_dim == 256) && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 &&
+  if (b.max_seqlen_q * group > 16 && tma && !few && (b.head_dim == 64 || b.head_dim == 128 || b.head_dim == 256) && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 &&
       b.q_head_stride > 0 && b.q_row_stride > 0 && workspace) {
     plan.path = kPathChunk;            // cuts the keys itself, on the device
     plan.splits = plan.tiles_per_split = 1;

@@ -83,6 +83,7 @@ struct DecodeArgs {
   float* part_o;        // [2 * CTAs][RP][128]: head part, tail part of each CTA
   float* part_lse;      // [2 * CTAs][RP]
   PartRecord* record;   // [CTAs]
+  int min_run;          // fewest tiles of a run
   int team, rounds;     // CTAs of a team, a divisor of the KV heads; KV heads of each member
 };
 
@@ -238,7 +239,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   total = 0;
 #pragma unroll
   for (int i = 0; i < NUM_THREADS / 32; ++i) total += s_sum[i];
-  const int run = max((total + (int)gridDim.y - 1) / (int)gridDim.y, kMinRun);
+  const int run = max((total + (int)gridDim.y - 1) / (int)gridDim.y, da.min_run);
   const int64_t begin = (int64_t)run * blockIdx.y;
   if (begin >= total) {
     if (tid == 0) da.record[cta] = PartRecord{-1, 0, 0, 0};
@@ -832,6 +833,7 @@ int launch(DecodeArgs& da, cudaStream_t st) {
   for (int t = 2; t <= 16; ++t)
     if (a.Hk % t == 0) da.team = t;
   da.rounds = a.Hk / da.team;
+  da.min_run = max(1, min(kMinRun, (a.max_k + BN - 1) / BN));   // short items need not share a CTA
   const int teams = C::CTAS * num_sms() / da.team, ctas = teams * da.team;
   da.part_o = a.ws_o;
   da.part_lse = a.ws_o + (int64_t)2 * ctas * RP * HD;

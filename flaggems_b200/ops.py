@@ -464,8 +464,10 @@ def _flash_attn_cache(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seql
     dev = _lib.require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, seqused_k, block_table, alibi_slopes, out)
     if alibi_slopes is not None:
         raise RuntimeError("flash_attn_varlen_func: ALiBi is not supported with 8-bit K/V or sink_tokens")
-    if q.stride(-1) != 1:
+    qst = q.stride()
+    if qst[-1] != 1:
         q = q.contiguous()
+        qst = q.stride()
     max_seqlen_q, max_seqlen_k = int(max_seqlen_q), int(max_seqlen_k)
     dtype, cache_dtype, shape = q.dtype, k.dtype, k.shape
     fp8 = _lib.FP8_CODE.get(cache_dtype)
@@ -488,13 +490,15 @@ def _flash_attn_cache(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seql
         used = seqused_k.data_ptr()
     if out is None:
         out = torch.empty_like(q)
+        ost = out.stride()
     else:
-        assert out.stride(-1) == 1 and out.dtype == dtype and out.shape == q.shape
+        ost = out.stride()
+        assert out.dtype == dtype and out.shape == q.shape and ost[-1] == 1
     lse = torch.empty((num_heads, total_q), dtype=torch.float32, device=dev) if return_softmax_lse else None
     if paged:
-        assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
-        assert block_table.shape[0] == batch
-        table, table_stride, table_cols = block_table.data_ptr(), block_table.stride(0), block_table.shape[1]
+        tsh, tst = block_table.shape, block_table.stride()
+        assert block_table.dtype == torch.int32 and len(tsh) == 2 and tsh[0] == batch and tst[1] == 1
+        table, table_stride, table_cols = block_table.data_ptr(), tst[0], tsh[1]
         num_blocks, block_size = shape[0], shape[1]
         block_stride, row_stride, head_stride, _ = kst
     else:
@@ -506,24 +510,24 @@ def _flash_attn_cache(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seql
     if fp8 is not None:
         ks, ksb, ksh = _descale("k_descale", k_descale, batch, num_heads_k, dev)
         vs, vsb, vsh = _descale("v_descale", v_descale, batch, num_heads_k, dev)
-    qst, ost = q.stride(), out.stride()
-    # before and behind the workspace, in the order of AttnCacheParams
-    head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-            cu_seqlens_q.data_ptr(), cu_k, used, table, 0)
-    tail = (qst[0], qst[1], row_stride, head_stride, block_stride, row_stride, head_stride, block_stride, ost[0], ost[1],
-            table_stride, 0, total_q, batch, num_heads, num_heads_k, head_size, max_seqlen_q, max_seqlen_k, block_size,
-            num_blocks, window[0], window[1], total_k, 0, 0, 0, 0, softmax_scale, softcap, 1 if causal else 0, code, 0, 0,
-            ks, vs, ksb, ksh, vsb, vsh, sink_tokens, table_cols, code if fp8 is None else fp8, 0)
+    # in the order of AttnCacheParams; the workspace is filled in behind the ten pointers
+    params = _lib.ATTN_CACHE.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        cu_seqlens_q.data_ptr(), cu_k, used, table, 0, 0, 0,
+        qst[0], qst[1], row_stride, head_stride, block_stride, row_stride, head_stride, block_stride, ost[0], ost[1],
+        table_stride, 0, total_q, batch, num_heads, num_heads_k, head_size, max_seqlen_q, max_seqlen_k, block_size,
+        num_blocks, window[0], window[1], total_k, 0, 0, 0, 0, softmax_scale, softcap, 1 if causal else 0, code, 0, 0,
+        ks, vs, ksb, ksh, vsb, vsh, sink_tokens, table_cols, code if fp8 is None else fp8, 0)
     lib = _lib.load()
-    pack = _lib.ATTN_CACHE.pack
     with _lib.on_device(dev):
-        params = pack(*head, 0, 0, *tail)
         nbytes = lib.fg_flash_attn_cache_workspace_bytes(params)
         if nbytes > 0:
             # a buffer of the call's own: the allocator keeps it from other streams, and a captured graph keeps its own
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            params = pack(*head, ws.data_ptr(), nbytes, *tail)
-        _lib.call(dev, lib.fg_flash_attn_cache, params)
+            params = params[:80] + _lib.WORKSPACE.pack(ws.data_ptr(), nbytes) + params[96:]
+        rc = lib.fg_flash_attn_cache(params, _lib.raw_stream(dev.index))
+    if rc < 0:
+        _lib.check(rc)
     return (out, lse) if return_softmax_lse else out
 
 

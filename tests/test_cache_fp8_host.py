@@ -105,7 +105,8 @@ def test_path_by_sizes():
     assert path() == 3 and path(max_seqlen_q=4, total_q=16) == 3      # 4 tokens of a group of 4: 16 rows
     assert path(max_seqlen_q=5, total_q=20) == 1 and path(max_seqlen_q=3000, total_q=9000) == 1
     assert path(head_dim=64) == 2 and path(softcap=5.0) == 2 and path(head_dim=72, max_seqlen_q=5, total_q=20) == 0
-    assert path(head_dim=64, max_seqlen_q=5, total_q=20) == path(head_dim=256, max_seqlen_q=5, total_q=20) == 1
+    assert path(head_dim=64, max_seqlen_q=1000, total_q=4000) == path(head_dim=256, max_seqlen_q=5, total_q=20) == 1
+    assert path(head_dim=64, max_seqlen_q=5, total_q=20, max_seqlen_k=600) == 0       # too few tiles for a widened copy
     assert path(block_size=24) == 0 and path(block_size=4) == 0 and path(k_row_stride=264) == 0   # pages or strides TMA cannot take
     assert path(cache_dtype=_lib.FG_BF16, k_row_stride=264, sink_tokens=1, window_left=7) == 3    # 528 bytes are fine
     assert path(num_heads=400, num_heads_k=2) == 0                    # a group of 200
