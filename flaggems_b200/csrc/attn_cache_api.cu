@@ -15,8 +15,14 @@ struct Plan {
   int path;
   int splits, tiles_per_split;
   int64_t bytes;       // of workspace
+  int whole;           // tensor-core kernels: no item is cut
   int64_t dense;       // rows of each sequence in a 16-bit copy of an 8-bit store, or 0
 };
+
+// Most tiles of 128 keys of an item for which the tensor-core kernels cut no item: one launch less, and no workspace.  Cut and whole:
+// 16 decodes of up to 1000 keys 20.1 and 15.8 us, of up to 2000 21.9 and 22.9 us (2 of them 17.6 and 22.5 us); 16 chunks of up
+// to 200 tokens over up to 500 keys 81.7 and 61.9 us, 8 of up to 60 over up to 1000 31.7 and 32.4 us.
+constexpr int64_t kWholeDecode = 8, kWholeChunk = 4;
 
 // Keys that one sequence can have visible to one row tile: everything, or window and first tokens.
 int64_t most_keys(const fg_attn_cache_params* p, int64_t tokens) {
@@ -58,23 +64,27 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
   const fg_attn_params& b = p->base;
   Plan plan;
   plan.dense = 0;
+  plan.whole = 0;
   const int64_t group = b.num_heads / b.num_heads_k;
   const bool tma = tma_ready(p);
   // At head dim 64 an 8-bit store's copy has to pay for itself: 1056 tiles of the general kernel (two chunks of up to 300 tokens)
   // take 21 us there and 29 us with the copy, 15872 (eight of up to 64 tokens over 4000) 152 and 60 us.
   const bool few = b.head_dim == 64 && is_fp8(p->cache_dtype) &&
                    b.batch * b.num_heads_k * ((b.max_seqlen_q * group + 63) / 64) * ((most_keys(p, b.max_seqlen_q) + 63) / 64) < 1536;
-  if (b.max_seqlen_q * group <= 16 && tma && b.head_dim == 128 && b.softcap == 0.0 && workspace &&
+  const int64_t key_tiles = (most_keys(p, b.max_seqlen_q) + 127) / 128;
+  if (b.max_seqlen_q * group <= 16 && tma && b.head_dim == 128 && b.softcap == 0.0 && (workspace || key_tiles <= kWholeDecode) &&
       b.batch * b.num_heads_k * (b.max_seqlen_k / 128 + 1) <= 2147483647LL) {
     plan.path = kPathDecodeSm100;      // cuts the keys itself, on the device
     plan.splits = plan.tiles_per_split = 1;
-    plan.bytes = attn_cache_decode_sm100_bytes(b.max_seqlen_q * group, sms);
+    plan.whole = key_tiles <= kWholeDecode;
+    plan.bytes = plan.whole ? 0 : attn_cache_decode_sm100_bytes(b.max_seqlen_q * group, sms);
     return plan;
   }
   if (b.max_seqlen_q * group > 16 && tma && !few && (b.head_dim == 64 || b.head_dim == 128 || b.head_dim == 256) && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 &&
-      b.q_head_stride > 0 && b.q_row_stride > 0 && workspace) {
+      b.q_head_stride > 0 && b.q_row_stride > 0) {
     plan.path = kPathChunk;            // cuts the keys itself, on the device
     plan.splits = plan.tiles_per_split = 1;
+    plan.whole = key_tiles <= kWholeChunk;
     // An 8-bit store is widened once, ahead of the attention, when at least four items (of 256 query rows) read each key and
     // the copy takes at most 1 GiB.  The kernel's own widening is for head dim 128: at the others shorter chunks are too.
     int64_t rows = (b.max_seqlen_k + 63) / 64 * 64;
@@ -87,9 +97,10 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
         b.batch * rows <= (1ll << 30) / (4 * b.head_dim * b.num_heads_k))
       plan.dense = rows;
     plan.bytes =
-        attn_cache_chunk_bytes(b.max_seqlen_q, group, b.batch, b.num_heads_k, b.head_dim, b.max_seqlen_k, plan.dense, sms);
-    if (plan.bytes > 0 && (!is_fp8(p->cache_dtype) || b.head_dim == 128 || plan.dense > 0)) return plan;
-    plan.dense = 0;
+        attn_cache_chunk_bytes(b.max_seqlen_q, group, b.batch, b.num_heads_k, b.head_dim, b.max_seqlen_k, plan.dense, plan.whole, sms);
+    if (plan.bytes >= 0 && (workspace || plan.bytes == 0) && (!is_fp8(p->cache_dtype) || b.head_dim == 128 || plan.dense > 0))
+      return plan;
+    plan.dense = plan.whole = 0;
   }
   if (b.max_seqlen_q * group <= 16 && tma) {
     // Enough CTAs to balance contexts of very different length over all SMs (two resident each), but no range shorter
@@ -229,6 +240,7 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   a.num_splits = plan.splits;
   c.tiles_per_split = plan.tiles_per_split;
   c.dense = plan.dense;
+  c.whole = plan.whole;
   const int kind = p->cache_dtype == FG_E4M3 ? kCacheE4M3 : p->cache_dtype == FG_E5M2 ? kCacheE5M2 : kCache16;
   cudaStream_t st = (cudaStream_t)stream;
   FG_REQUIRE((b.max_seqlen_q * a.group + 63) / 64 * plan.splits <= 2147483647LL, "flash_attn_cache: too many row tiles");

@@ -109,9 +109,9 @@ struct InfoTable {
   const SeqInfo* info;
   int b0, n;
 };
-__device__ __forceinline__ void set_part(Segment& g, int lo) {
+__device__ __forceinline__ void set_part(const ChunkArgs& pa, Segment& g, int lo) {
   g.lo = lo;
-  g.hi = min(g.n, lo + g.left);
+  g.hi = pa.c.whole ? g.n : min(g.n, lo + g.left);
 }
 __device__ __forceinline__ void fill_segment(const ChunkArgs& pa, const InfoTable& table, Segment& g) {
   g.s = (unsigned)(g.b - table.b0) < (unsigned)table.n ? table.info[g.b - table.b0] : cache_seq_info(pa.c, g.b);
@@ -125,7 +125,7 @@ __device__ __forceinline__ void fill_segment(const ChunkArgs& pa, const InfoTabl
 }
 // The part after `g`, in place; false when the run ends with g.
 __device__ __forceinline__ bool next_segment(const ChunkArgs& pa, const InfoTable& table, Segment& g) {
-  g.left -= g.hi - g.lo;
+  g.left -= item_weight(pa.c, g.hi - g.lo);
   if (g.left <= 0) return false;
   if (++g.hk == pa.c.a.Hk) {
     g.hk = 0;
@@ -137,7 +137,7 @@ __device__ __forceinline__ bool next_segment(const ChunkArgs& pa, const InfoTabl
       fill_segment(pa, table, g);
     } while (g.n == 0);
   }
-  set_part(g, 0);
+  set_part(pa, g, 0);
   return true;
 }
 
@@ -214,7 +214,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   const int pairs = a.batch * pa.num_mb;
   TileSpan span;
   int mine = 0;
-  if (tid < pairs) mine = item_tiles(pa, cache_seq_info(c, tid / pa.num_mb), tid % pa.num_mb, span) * a.Hk;
+  if (tid < pairs) mine = item_weight(c, item_tiles(pa, cache_seq_info(c, tid / pa.num_mb), tid % pa.num_mb, span)) * a.Hk;
   if (tid == 0) {
     s_drain = *reinterpret_cast<volatile int*>(a.status);
     *abort_flag = 0;
@@ -241,7 +241,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   }
   int total = mine;
   for (int p = tid + THREADS; p < pairs; p += THREADS)
-    total += item_tiles(pa, cache_seq_info(c, p / pa.num_mb), p % pa.num_mb, span) * a.Hk;
+    total += item_weight(c, item_tiles(pa, cache_seq_info(c, p / pa.num_mb), p % pa.num_mb, span)) * a.Hk;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) s_sum[warp] = total;
@@ -253,14 +253,14 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   const int run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, pa.min_run);
   const int64_t begin = (int64_t)run * blockIdx.x;
   if (begin >= total) {
-    if (tid == 0) pa.record[blockIdx.x] = PartRecord{-1, 0, 0, 0};
+    if (tid == 0 && !c.whole) pa.record[blockIdx.x] = PartRecord{-1, 0, 0, 0};
     return;
   }
   int before = 0;
   for (int p0 = 0;; p0 += THREADS) {
     if (p0 > 0) {
       const int p = p0 + tid;
-      mine = p < pairs ? item_tiles(pa, cache_seq_info(c, p / pa.num_mb), p % pa.num_mb, span) * a.Hk : 0;
+      mine = p < pairs ? item_weight(c, item_tiles(pa, cache_seq_info(c, p / pa.num_mb), p % pa.num_mb, span)) * a.Hk : 0;
     }
     int incl = mine;
 #pragma unroll
@@ -300,8 +300,9 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   asm volatile("griddepcontrol.launch_dependents;");   // the joining kernel may be set up: it waits for this one's end
   seg.left = min(total - (int)begin, run);
   fill_segment(pa, table, seg);
-  seg.hk = s_off / seg.n;
-  set_part(seg, s_off - seg.hk * seg.n);
+  const int weight = item_weight(c, seg.n);
+  seg.hk = s_off / weight;
+  set_part(pa, seg, s_off - seg.hk * weight);
 
   auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
     return mbar_wait(bar, parity, abort_flag, a.status, kStatusAttnTimeout);
@@ -757,7 +758,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           a.lse[(int64_t)h * a.total_q + qtok] = l_run == 0.f ? INFINITY : lse2 * 0.6931471805599453f;
       }
     } while (next_segment(pa, table, seg));
-    if (tid == 0) pa.record[blockIdx.x] = rec;
+    if (tid == 0 && !c.whole) pa.record[blockIdx.x] = rec;
   }
 
   // ================================ teardown ======================================
@@ -869,6 +870,7 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
   pa.record = reinterpret_cast<PartRecord*>(pa.part_lse + (int64_t)2 * ctas * pa.tiles * BM);
   attn_cache_chunk_kernel<T, KIND, M, HD><<<ctas, threads_of(KIND), smem, st>>>(tq, maps[0], maps[1], pa);
   FG_CHECK_LAUNCH("attn_cache_chunk_kernel");
+  if (pa.c.whole) return FG_OK;
   // Launched while the kernel above still runs (programmatic dependent launch); it waits for its end on the device.
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -957,7 +959,7 @@ int launch_kind(ChunkArgs& pa, int kind, cudaStream_t st) {
   if (c.dense > 0) {   // rows of a sequence in the 16-bit copy
     AttnArgs& a = c.a;
     const int64_t rows = a.batch * c.dense;
-    __half* k16 = reinterpret_cast<__half*>(reinterpret_cast<char*>(a.ws_o) + part_bytes(pa.tiles, a.D, num_sms()));
+    __half* k16 = reinterpret_cast<__half*>(reinterpret_cast<char*>(a.ws_o) + (c.whole ? 0 : part_bytes(pa.tiles, a.D, num_sms())));
     __half* v16 = k16 + rows * a.Hk * a.D;
     const dim3 grid((unsigned)((c.dense + kWidenRows - 1) / kWidenRows), (unsigned)a.batch);
     if (kind == kCacheE4M3)
@@ -978,14 +980,14 @@ int launch_kind(ChunkArgs& pa, int kind, cudaStream_t st) {
 }  // namespace
 
 // Bytes of workspace: a head and a tail part, and a record, for each CTA; with `dense` rows for each sequence also their 16-bit copy.
-// 0: more tiles than the kernel counts in 32 bits.
+// -1: more tiles than the kernel counts in 32 bits.
 int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t head_dim, int64_t max_k,
-                               int64_t dense, int sms) {
+                               int64_t dense, bool whole, int sms) {
   int tiles, tokens;
   int64_t num_mb;
   chunk_shape(max_q, group, head_dim, &tiles, &tokens, &num_mb);
-  if (batch * num_mb > 2147483647LL / 2 || batch * num_mb * heads_k > 2147483647LL / (max_k / BN + 1)) return 0;
-  return part_bytes(tiles, head_dim, sms) + 2 * batch * dense * heads_k * head_dim * 2;
+  if (batch * num_mb > 2147483647LL / 2 || batch * num_mb * heads_k > 2147483647LL / (max_k / BN + 1)) return -1;
+  return (whole ? 0 : part_bytes(tiles, head_dim, sms)) + 2 * batch * dense * heads_k * head_dim * 2;
 }
 
 int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st) {
@@ -995,7 +997,7 @@ int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t s
   int64_t num_mb;
   chunk_shape(c.a.max_q, c.a.group, c.a.D, &pa.tiles, &pa.tokens, &num_mb);
   pa.num_mb = (int)num_mb;
-  pa.min_run = max(1, min(kMinRun, (c.a.max_k + BN - 1) / BN));   // short items need not share a CTA
+  pa.min_run = max(1, min(kMinRun, c.whole ? 1 : (c.a.max_k + BN - 1) / BN));   // short items need not share a CTA
   return dtype == FG_BF16 ? launch_kind<__nv_bfloat16>(pa, kind, st) : launch_kind<__half>(pa, kind, st);
 }
 

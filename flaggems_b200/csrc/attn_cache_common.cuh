@@ -28,6 +28,7 @@ struct CacheAttnArgs {
   int table_cols;                          // entries of a block table row
   int tiles_per_split;                     // K/V tiles of one split
   int64_t dense;                           // chunk kernel: rows of each sequence in a 16-bit copy that k and v point at; 0: none
+  int whole;                               // tensor-core kernels: runs are cut between items only, and nothing is joined
   __host__ __device__ bool pages() const { return a.paged && dense == 0; }
 };
 // Lengths that contradict the sizes of the call (rows behind q or K/V, more keys than max_seqlen_k, by which the work was counted on
@@ -107,6 +108,9 @@ __device__ __forceinline__ RowMask row_mask(const CacheAttnArgs& c, int k_len, i
   return m;
 }
 
+// What an item of n K/V tiles counts where the tiles of all items are cut into runs.
+__device__ __forceinline__ int item_weight(const CacheAttnArgs& c, int n) { return c.whole ? min(n, 1) : n; }
+
 // Power of two (as a float) that takes a row whose largest magnitude is `top` to [2^14, 2^15), and its inverse.
 __device__ __forceinline__ void row_power(float top, float& up, float& down) {
   const int e = (int)((__float_as_uint(top) >> 23) & 0xff);   // biased exponent; 0 for zero and subnormals
@@ -125,7 +129,7 @@ int attn_cache_decode(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t 
 int64_t attn_cache_decode_sm100_bytes(int64_t rows, int sms);
 int attn_cache_decode_sm100(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
 int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t head_dim, int64_t max_k,
-                               int64_t dense, int sms);
+                               int64_t dense, bool whole, int sms);
 int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
 int attn_cache_combine(const CacheAttnArgs& c, int dtype, cudaStream_t st);
 

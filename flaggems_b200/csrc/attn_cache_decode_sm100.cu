@@ -118,19 +118,19 @@ __device__ __forceinline__ void fill_segment(const CacheAttnArgs& c, const InfoT
   g.rows = min(g.s.q_len * c.a.group, RP);
   g.shift = g.s.k_len - g.s.q_len;
   g.lo = lo;
-  g.hi = min(g.n, lo + g.left);
+  g.hi = c.whole ? g.n : min(g.n, lo + g.left);
 }
 // The part after `g`; false when the run ends with g.
 template <int RP>
 __device__ __forceinline__ bool next_segment(const CacheAttnArgs& c, const InfoTable& table, int team, const Segment& g,
                                              Segment& to) {
   to = g;
-  to.left = g.left - (g.hi - g.lo);
+  to.left = g.left - item_weight(c, g.hi - g.lo);
   if (to.left <= 0) return false;
   to.hk += team;
   if (to.hk < c.a.Hk) {
     to.lo = 0;
-    to.hi = min(to.n, to.left);
+    to.hi = c.whole ? to.n : min(to.n, to.left);
     return true;
   }
   to.hk -= c.a.Hk;
@@ -227,10 +227,10 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
   }
-  int mine = tid < a.batch ? item_tiles<RP>(c, mine_info, span) * rounds : 0;
+  int mine = tid < a.batch ? item_weight(c, item_tiles<RP>(c, mine_info, span)) * rounds : 0;
   int total = mine;
   for (int b = tid + NUM_THREADS; b < a.batch; b += NUM_THREADS)
-    total += item_tiles<RP>(c, cache_seq_info(c, b), span) * rounds;
+    total += item_weight(c, item_tiles<RP>(c, cache_seq_info(c, b), span)) * rounds;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) s_sum[warp] = total;
@@ -242,7 +242,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   const int run = max((total + (int)gridDim.y - 1) / (int)gridDim.y, da.min_run);
   const int64_t begin = (int64_t)run * blockIdx.y;
   if (begin >= total) {
-    if (tid == 0) da.record[cta] = PartRecord{-1, 0, 0, 0};
+    if (tid == 0 && !c.whole) da.record[cta] = PartRecord{-1, 0, 0, 0};
     return;
   }
   // the sequence that holds tile `begin`
@@ -252,7 +252,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
       mine = 0;
       if (b0 + tid < a.batch) {
         mine_info = cache_seq_info(c, b0 + tid);
-        mine = item_tiles<RP>(c, mine_info, span) * rounds;
+        mine = item_weight(c, item_tiles<RP>(c, mine_info, span)) * rounds;
       }
     }
     int incl = mine;
@@ -292,10 +292,11 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   seg.b = s_b;
   seg.left = min(total - (int)begin, run);
   fill_segment<RP>(c, table, seg, 0);
-  const int round = rounds > 1 ? s_off / seg.n : 0;
+  const int weight = item_weight(c, seg.n);
+  const int round = rounds > 1 ? s_off / weight : 0;
   seg.hk = round * gridDim.x + blockIdx.x;
-  seg.lo = s_off - round * seg.n;
-  seg.hi = min(seg.n, seg.lo + seg.left);
+  seg.lo = s_off - round * weight;
+  seg.hi = c.whole ? seg.n : min(seg.n, seg.lo + seg.left);
   auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
     return mbar_wait(bar, parity, abort_flag, a.status, kStatusAttnTimeout);
   };
@@ -735,7 +736,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
       if (!more) break;
       seg = next;
     }
-    if (tid == 0) da.record[cta] = rec;
+    if (tid == 0 && !c.whole) da.record[cta] = rec;
   }
 
   // ================================ teardown ======================================
@@ -833,13 +834,14 @@ int launch(DecodeArgs& da, cudaStream_t st) {
   for (int t = 2; t <= 16; ++t)
     if (a.Hk % t == 0) da.team = t;
   da.rounds = a.Hk / da.team;
-  da.min_run = max(1, min(kMinRun, (a.max_k + BN - 1) / BN));   // short items need not share a CTA
+  da.min_run = max(1, min(kMinRun, da.c.whole ? 1 : (a.max_k + BN - 1) / BN));   // short items need not share a CTA
   const int teams = C::CTAS * num_sms() / da.team, ctas = teams * da.team;
   da.part_o = a.ws_o;
   da.part_lse = a.ws_o + (int64_t)2 * ctas * RP * HD;
   da.record = reinterpret_cast<PartRecord*>(da.part_lse + 2 * ctas * RP);
   attn_cache_decode_tcgen05_kernel<T, KIND, RP><<<dim3(da.team, teams), NUM_THREADS, C::SMEM, st>>>(maps[0], maps[1], da);
   FG_CHECK_LAUNCH("attn_cache_decode_tcgen05_kernel");
+  if (da.c.whole) return FG_OK;
   // The joining kernel is launched while this one still runs (programmatic dependent launch) and waits for its end on the
   // device: the launch's latency is out of the way.
   cudaLaunchAttribute early;

@@ -87,13 +87,14 @@ def test_workspace_goes_by_what_is_visible():
         long, windowed = need(max_seqlen_k=10 ** 6, **size), need(max_seqlen_k=10 ** 6, window_left=2047, sink_tokens=4, **size)
         assert 0 < windowed < long and windowed == need(max_seqlen_k=10 ** 5, window_left=2047, sink_tokens=4, **size)
     chunk = dict(max_seqlen_q=30, total_q=100)
-    assert need(max_seqlen_k=10 ** 6, **chunk) == need(max_seqlen_k=10, **chunk) > need() > 0
+    assert need(max_seqlen_k=10 ** 6, **chunk) == need(max_seqlen_k=10 ** 4, **chunk) > need(max_seqlen_k=10 ** 4) > 0
+    assert need(max_seqlen_k=100, **chunk) == need(max_seqlen_k=100) == 0      # short contexts are not cut
     # a long chunk: the 16-bit copy of an 8-bit store comes on top, until it would be larger than 1 GiB
     long = dict(max_seqlen_q=256, total_q=1000)
     copy = need(max_seqlen_k=6400, **long) - need(max_seqlen_k=6400, cache_dtype=_lib.FG_BF16, **long)
     assert copy == 2 * 4 * 6400 * 2 * 128 * 2
     assert need(max_seqlen_k=10 ** 6, **long) == need(max_seqlen_k=10 ** 6, cache_dtype=_lib.FG_BF16, **long)
-    assert need(max_seqlen_k=10 ** 6) == need(max_seqlen_k=10)        # head parts and tail parts of a fixed number of CTAs
+    assert need(max_seqlen_k=10 ** 6) == need(max_seqlen_k=10 ** 4)        # head parts and tail parts of a fixed number of CTAs
     # chunks whose 8-bit store is widened ahead of the attention: the copy holds what is visible
     for size in (dict(head_dim=256, max_seqlen_q=30, total_q=100), dict(max_seqlen_q=600, total_q=1000)):
         long, windowed = need(max_seqlen_k=10 ** 5, **size), need(max_seqlen_k=10 ** 5, window_left=2047, sink_tokens=4, **size)
