@@ -24,6 +24,15 @@ struct Plan {
 // to 200 tokens over up to 500 keys 81.7 and 61.9 us, 8 of up to 60 over up to 1000 31.7 and 32.4 us.
 constexpr int64_t kWholeDecode = 8, kWholeChunk = 4;
 
+// Fewest tiles of 128 keys, of all sequences and KV heads, for which the decode form on tcgen05 is worth its longer way through a
+// tile, which grows with the query rows; below, the mma.sync form splits the keys over more and smaller CTAs.  On mma.sync and on
+// tcgen05, 8-bit: 4 rows of 128: 256 tiles 12.3 and 15.6 us, 704 19.7 and 17.2; 8 rows: 704 21.7 and 21.5, 2048 33.8 and 30.5;
+// 16 rows: 2048 39.7 and 44.4, 8192 140 and 91; 4 rows of 256: 256 16.4 and 18.2, 704 33.8 and 21.3; 16: 48.7 and 43.6.
+int64_t least_decode(int64_t rows, int64_t head_dim) {
+  if (head_dim == 256) return 400;
+  return rows <= 4 ? 600 : rows <= 8 ? 1800 : 4000;
+}
+
 // Keys that one sequence can have visible to one row tile: everything, or window and first tokens.
 int64_t most_keys(const fg_attn_cache_params* p, int64_t tokens) {
   const fg_attn_params& b = p->base;
@@ -72,12 +81,14 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
   const bool few = b.head_dim == 64 && is_fp8(p->cache_dtype) &&
                    b.batch * b.num_heads_k * ((b.max_seqlen_q * group + 63) / 64) * ((most_keys(p, b.max_seqlen_q) + 63) / 64) < 1536;
   const int64_t key_tiles = (most_keys(p, b.max_seqlen_q) + 127) / 128;
-  if (b.max_seqlen_q * group <= 16 && tma && b.head_dim == 128 && b.softcap == 0.0 && (workspace || key_tiles <= kWholeDecode) &&
+  const bool decode_dim = (b.head_dim == 64 || b.head_dim == 128 || (b.head_dim == 256 && is_fp8(p->cache_dtype))) &&
+                          b.batch * b.num_heads_k * key_tiles >= least_decode(b.max_seqlen_q * group, b.head_dim);
+  if (b.max_seqlen_q * group <= 16 && tma && decode_dim && b.softcap == 0.0 && (workspace || key_tiles <= kWholeDecode) &&
       b.batch * b.num_heads_k * (b.max_seqlen_k / 128 + 1) <= 2147483647LL) {
     plan.path = kPathDecodeSm100;      // cuts the keys itself, on the device
     plan.splits = plan.tiles_per_split = 1;
     plan.whole = key_tiles <= kWholeDecode;
-    plan.bytes = plan.whole ? 0 : attn_cache_decode_sm100_bytes(b.max_seqlen_q * group, sms);
+    plan.bytes = plan.whole ? 0 : attn_cache_decode_sm100_bytes(b.max_seqlen_q * group, b.head_dim, sms);
     return plan;
   }
   if (b.max_seqlen_q * group > 16 && tma && !few && (b.head_dim == 64 || b.head_dim == 128 || b.head_dim == 256) && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 &&

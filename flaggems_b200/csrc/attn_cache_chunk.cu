@@ -716,7 +716,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       if (!wwait(&o_done[t * 2 + ((g - 1) & 1)], ((g - 1) >> 1) & 1)) break;
       tc_fence_after();
       // a NaN sum stays one: only a row that saw nothing is set to zero
-      const float inv = l_run == 0.f ? 0.f : v_scale / l_run;
+      const float inv = v_scale / l_run;
       const bool whole = seg.lo == 0 && seg.hi == seg.n;
       const int64_t qtok = seg.s.q_begin + tok;
       const int64_t part = ((int64_t)2 * blockIdx.x + (seg.lo == 0 ? 1 : 0)) * NT + t;   // 128 rows
@@ -736,7 +736,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         }
         float f[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv;
+        for (int e = 0; e < 16; ++e) f[e] = l_run == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
         if (!whole) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -788,16 +788,17 @@ __global__ void __launch_bounds__(BM) attn_cache_join_rows_kernel(ChunkArgs pa, 
   const int n = min(rec.parts, ctas - i);
   auto slot = [&](int k) { return (int64_t)(k == 0 ? 2 * i + 1 : 2 * (i + k)) * pa.tiles + t; };
   float m = -INFINITY;
+#pragma unroll 16
   for (int k = 0; k < n; ++k) m = fmaxf(m, pa.part_lse[slot(k) * BM + r]);
   const float ms = m == -INFINITY ? 0.f : m;
   float acc[32], wsum = 0.f;
 #pragma unroll
   for (int e = 0; e < 32; ++e) acc[e] = 0.f;
+#pragma unroll 4   // an item may be in many parts: their loads are in flight together
   for (int k = 0; k < n; ++k) {
     const float w = exp2f(pa.part_lse[slot(k) * BM + r] - ms);
     const float4* o = reinterpret_cast<const float4*>(pa.part_o + slot(k) * BM * HD) + blockIdx.z * 8 * BM + r;
     wsum += w;
-    if (w == 0.f) continue;   // NaN goes on
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float4 v = o[e * BM];
@@ -997,7 +998,10 @@ int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t s
   int64_t num_mb;
   chunk_shape(c.a.max_q, c.a.group, c.a.D, &pa.tiles, &pa.tokens, &num_mb);
   pa.num_mb = (int)num_mb;
-  pa.min_run = max(1, min(kMinRun, c.whole ? 1 : (c.a.max_k + BN - 1) / BN));   // short items need not share a CTA
+  // Short items need not share a CTA.  An item of n tiles in n / run parts takes about 1 us a tile and 0.5 us a part to join: run is
+  // at least the root of n / 2 (20 tokens over 16000 keys: 55 us in runs of 4 tiles, 38 in runs of 11).
+  const int longest = (c.a.max_k + BN - 1) / BN;
+  pa.min_run = c.whole ? 1 : max(max(1, min(kMinRun, longest)), (int)sqrtf(0.5f * longest));
   return dtype == FG_BF16 ? launch_kind<__nv_bfloat16>(pa, kind, st) : launch_kind<__half>(pa, kind, st);
 }
 

@@ -126,7 +126,7 @@ __device__ __forceinline__ void row_power(float top, float& up, float& down) {
 // Kernel families of fg_flash_attn_cache.
 int attn_cache_generic(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
 int attn_cache_decode(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
-int64_t attn_cache_decode_sm100_bytes(int64_t rows, int sms);
+int64_t attn_cache_decode_sm100_bytes(int64_t rows, int64_t head_dim, int sms);
 int attn_cache_decode_sm100(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st);
 int64_t attn_cache_chunk_bytes(int64_t max_q, int64_t group, int64_t batch, int64_t heads_k, int64_t head_dim, int64_t max_k,
                                int64_t dense, bool whole, int sms);

@@ -39,7 +39,7 @@
 namespace fg {
 namespace {
 
-constexpr int BN = 128, HD = 128, NUM_THREADS = 224;
+constexpr int BN = 128, NUM_THREADS = 224;
 constexpr int TMA_WARP = 4, MMA_WARP = 6;
 constexpr float kRaise = 4.0f;               // log2 units
 constexpr float kPScale = 2048.0f;           // of P before it is split (8-bit caches)
@@ -48,8 +48,8 @@ constexpr int kInfo = 32;                    // sequences of a run whose lengths
 
 constexpr int up(int n, int to) { return (n + to - 1) / to * to; }
 
-// T: query type; KIND: cache; RP: query rows, rounded up to 4, 8 or 16
-template <typename T, int KIND, int RP>
+// T: query type; KIND: cache; RP: query rows, rounded up to 4, 8 or 16; HD: head dim
+template <typename T, int KIND, int RP, int HD>
 struct Cfg {
   static constexpr bool k8 = KIND != kCache16;
   static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -59,16 +59,28 @@ struct Cfg {
   // Rows of Q and P that shared memory holds: whole 8-row swizzle groups.  Where the product has 8 columns more, it reads
   // whatever follows there; nothing uses those columns.
   static constexpr int QR = up(RP * PQ, 8), PR = up(RP * PP, 8);
-  static constexpr int TILE = BN * HD * (k8 ? 1 : 2);         // bytes of a K or V tile
-  // One CTA an SM, or two where 128 registers a thread are enough; 192 KB of tiles on their way in either form.
-  static constexpr int CTAS = k8 && RP == 4 ? 2 : 1;
-  static constexpr int SLOTS = k8 ? 6 / CTAS : 3;             // tiles of each ring
-  static constexpr int QB = QR * HD * (k8 ? 1 : 2);           // bytes of one Q buffer
+  static constexpr int ES = k8 ? 1 : 2;                       // bytes of a cached value, and of a piece of Q or P
+  static constexpr int ROW = HD * ES;                         // bytes of a cached row: 64, 128 or 256
+  static constexpr int ATOM = ROW < 128 ? ROW : 128;          // ... in one swizzled column block (TMA box)
+  static constexpr int BLOCKS = ROW / ATOM;
+  static constexpr int BLOCK = BN * ATOM;                     // bytes of a tile's column block
+  static constexpr int TILE = BN * ROW;                       // bytes of a K or V tile
+  static constexpr int OM = HD > 128 ? 2 : 1;                 // products P V of 128 dims; at 64 the upper half repeats the lower
+  // One CTA an SM, or two where 128 registers a thread are enough.
+  static constexpr int CTAS = k8 && RP == 4 && HD <= 128 ? 2 : 1;
+  static constexpr int QW = ROW > 128 ? 2 : 1;                // 128-byte column blocks of a Q buffer
+  static constexpr int QB = QR * QW * 128;                    // bytes of one Q buffer
   static constexpr int PB = PR * BN * (k8 ? 1 : 2);           // bytes of one P buffer
+  static constexpr int REST = 2 * QB + 2 * PB + 1024 + 1024 + kInfo * 16;
+  // tiles of each ring: what shared memory holds (192 KB of tiles on their way where they divide it), and the barriers' space
+  static constexpr int FIT = ((CTAS == 2 ? 115712 : 232448) - REST) / (2 * TILE);
+  static constexpr int SLOTS = FIT < 9 ? FIT : 9;
   static constexpr int SCOL = NS <= 32 ? 32 : 64;             // TMEM columns of one score buffer
   static constexpr int OCOL = 2 * SCOL;
-  static constexpr int TCOLS = OCOL + NP <= 128 ? 128 : 256;
-  static constexpr int SMEM = 2 * SLOTS * TILE + 2 * QB + 2 * PB + 1024 + 1024 + kInfo * 16;
+  static constexpr int TCOLS = OCOL + OM * NP <= 128 ? 128 : 256;
+  static_assert(OCOL + OM * NP <= 256, "tensor memory");
+  static constexpr int QV = HD * RP / 128 < 4 ? 4 : HD * RP / 128;   // values of a Q row that a thread splits
+  static constexpr int SMEM = 2 * SLOTS * TILE + REST;
 };
 
 // What a CTA leaves for the joining kernel: the item whose start it holds but not its end (or -1), in how many parts the item
@@ -163,12 +175,12 @@ __device__ __forceinline__ uint16_t f16x2_to_e5m2x2(uint32_t h) {
   return r;
 }
 
-template <typename T, int KIND, int RP>
-__global__ void __launch_bounds__(NUM_THREADS, Cfg<T, KIND, RP>::CTAS)
+template <typename T, int KIND, int RP, int HD>
+__global__ void __launch_bounds__(NUM_THREADS, Cfg<T, KIND, RP, HD>::CTAS)
 attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                                  const __grid_constant__ DecodeArgs da) {
   using namespace sm100;
-  using C = Cfg<T, KIND, RP>;
+  using C = Cfg<T, KIND, RP, HD>;
   const CacheAttnArgs& c = da.c;
   const AttnArgs& a = c.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -353,9 +365,10 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
         if (lane == 0) mbar_expect_tx(&full[slot], pages * da.page_rows * (C::TILE / BN));
         __syncwarp();
         if (page >= 0) {
-          uint8_t* dst = ring + slot * C::TILE + lane * da.page_rows * 128;
-          tma_load_4d(dst, tm, &full[slot], 0, seg.hk, row, page);
-          if constexpr (!C::k8) tma_load_4d(dst + C::TILE / 2, tm, &full[slot], 64, seg.hk, row, page);
+          uint8_t* dst = ring + slot * C::TILE + lane * da.page_rows * C::ATOM;
+#pragma unroll
+          for (int i = 0; i < C::BLOCKS; ++i)
+            tma_load_4d(dst + i * C::BLOCK, tm, &full[slot], i * (C::ATOM / C::ES), seg.hk, row, page);
         }
         page = npage;
         row = nrow;
@@ -368,8 +381,12 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
     if (lane == 0) {
       const uint32_t id_s = C::k8 ? umma_idesc_f8(KIND == kCacheE5M2, false, false, false, BN, C::NS)
                                   : umma_idesc_f16(C::kBf16, false, false, BN, C::NS);
-      const uint32_t id_o = C::k8 ? umma_idesc_f8(KIND == kCacheE5M2, true, true, false, HD, C::NP)
-                                  : umma_idesc_f16(C::kBf16, true, false, HD, C::NP);
+      const uint32_t id_o = C::k8 ? umma_idesc_f8(KIND == kCacheE5M2, true, true, false, 128, C::NP)
+                                  : umma_idesc_f16(C::kBf16, true, false, 128, C::NP);
+      // A product takes 32 bytes of K's and Q's rows at a time, four to a 128-byte column block.
+      auto kv_desc = [](uint32_t at, uint32_t lbo) {
+        return C::ATOM == 64 ? umma_desc_sw64(at, lbo, 512) : umma_desc_sw128(at, lbo, 1024);
+      };
       // scores of tile g of the run (tiles count on through all items); `item`: the how-manieth
       auto scores_ready = [&](uint32_t g, bool first, uint32_t item) -> bool {   // without waiting
         return (!first || mbar_test(&q_ready[item & 1], (item >> 1) & 1)) && mbar_test(&k_full[g % C::SLOTS], (g / C::SLOTS) & 1) &&
@@ -381,17 +398,17 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
         if (!wait1(&k_full[slot], (g / C::SLOTS) & 1)) return false;
         if (g >= 2 && !wait1(&s_free[g & 1], ((g - 2) >> 1) & 1)) return false;   // scores two tiles back are read
         tc_fence_after();
-        const uint64_t k_desc = umma_desc_sw128(smem_u32(sK + slot * C::TILE), 0, 1024);
+        const uint64_t k_desc = kv_desc(smem_u32(sK + slot * C::TILE), 0);
         const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ + (item & 1) * C::QB), 0, 1024);
         const uint32_t d = tmem_base + (g & 1) * C::SCOL;
-        if constexpr (C::k8) {
 #pragma unroll
-          for (int k = 0; k < HD / 32; ++k) mma_f8_ss(d, k_desc + k * 2, q_desc + k * 2, id_s, k != 0);
-        } else {
-#pragma unroll
-          for (int k = 0; k < HD / 16; ++k)
-            mma_f16_ss(d, k_desc + (k >> 2) * (C::TILE / 2 / 16) + (k & 3) * 2, q_desc + (k >> 2) * (C::QR * 128 / 16) + (k & 3) * 2,
-                       id_s, k != 0);
+        for (int k = 0; k < C::ROW / 32; ++k) {
+          const uint64_t kd = k_desc + (k >> 2) * (C::BLOCK / 16) + (k & 3) * 2;
+          const uint64_t qd = q_desc + (k >> 2) * (C::QR * 128 / 16) + (k & 3) * 2;
+          if constexpr (C::k8)
+            mma_f8_ss(d, kd, qd, id_s, k != 0);
+          else
+            mma_f16_ss(d, kd, qd, id_s, k != 0);
         }
         tc_commit(&s_full[g & 1]);
         tc_commit(&k_empty[slot]);
@@ -424,17 +441,22 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             break;
           }
           tc_fence_after();
-          const uint64_t v_desc = umma_desc_sw128(smem_u32(sV + slot * C::TILE), C::k8 ? C::TILE : C::TILE / 2, 1024);
+          // 128 dims are one column block of 8-bit rows or two of 16-bit ones; 64 dims are read twice
+          const uint64_t v_desc = kv_desc(smem_u32(sV + slot * C::TILE), HD == 64 ? 0 : C::BLOCK);
           const uint64_t p_desc = umma_desc_sw128(smem_u32(sP + (g & 1) * C::PB), 0, 1024);
-          const uint32_t d = tmem_base + C::OCOL;
           const bool add = t > seg.lo;     // the first tile of an item overwrites
-          if constexpr (C::k8) {
 #pragma unroll
-            for (int k = 0; k < BN / 32; ++k) mma_f8_ss(d, v_desc + k * (4096 >> 4), p_desc + k * 2, id_o, add || k > 0);
-          } else {
+          for (int m = 0; m < C::OM; ++m) {
+            const uint32_t d = tmem_base + C::OCOL + m * C::NP;
+            if constexpr (C::k8) {
 #pragma unroll
-            for (int k = 0; k < BN / 16; ++k)
-              mma_f16_ss(d, v_desc + k * (2048 >> 4), p_desc + (k >> 2) * (C::PR * 128 / 16) + (k & 3) * 2, id_o, add || k > 0);
+              for (int k = 0; k < BN / 32; ++k)
+                mma_f8_ss(d, v_desc + m * (C::BLOCK >> 4) + k * (32 * C::ATOM >> 4), p_desc + k * 2, id_o, add || k > 0);
+            } else {
+#pragma unroll
+              for (int k = 0; k < BN / 16; ++k)
+                mma_f16_ss(d, v_desc + k * (2048 >> 4), p_desc + (k >> 2) * (C::PR * 128 / 16) + (k & 3) * 2, id_o, add || k > 0);
+            }
           }
           tc_commit(&o_done[g & 1]);
           tc_commit(&v_empty[slot]);
@@ -451,10 +473,10 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
   } else {
     // ================================ softmax / output =============================
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
-    // ---- an item's Q: 128 / RP threads a row, RP values each, loaded ahead and then split into pieces
-    constexpr int TPR = 128 / RP;
-    const int q_row = tid / TPR, d0 = (tid % TPR) * RP;
-    uint32_t qw[RP / 2];
+    // ---- an item's Q: QV values of a row a thread, loaded ahead and then split into pieces
+    constexpr int TPR = HD / C::QV;
+    const int q_row = tid / TPR, d0 = (tid % TPR) * C::QV;    // rows from RP on: nothing to do
+    uint32_t qw[C::QV / 2];
     float ksc = 1.f, vsc = 1.f;
     auto load_q = [&](const Segment& g) {
       const bool live = q_row < g.rows;
@@ -462,7 +484,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
       const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(g.s.q_begin + tok) * a.q_rs +
                    (int64_t)(g.hk * group + (live ? q_row - tok * group : 0)) * a.q_hs + d0;
 #pragma unroll
-      for (int i = 0; i < RP / 4; ++i) {
+      for (int i = 0; i < C::QV / 4; ++i) {
         const uint2 u = live ? *reinterpret_cast<const uint2*>(q + i * 4) : make_uint2(0, 0);
         qw[2 * i] = u.x;
         qw[2 * i + 1] = u.y;
@@ -474,10 +496,10 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
       uint8_t* buf = sQ + (item & 1) * C::QB;
       float down = 1.f;
       if constexpr (C::k8) {
-        float x[RP], top = 0.f;
+        float x[C::QV], top = 0.f;
         bool bad = false;
 #pragma unroll
-        for (int i = 0; i < RP / 2; ++i) {
+        for (int i = 0; i < C::QV / 2; ++i) {
           const float2 f = Pair<T>::unpack(qw[i]);
           x[2 * i] = f.x;
           x[2 * i + 1] = f.y;
@@ -494,13 +516,13 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
         up *= 0.0078125f;          // [2^14, 2^15) -> [2^7, 2^8)
         down = bad ? NAN : down * 128.f;   // infinities and NaN have no pieces: the whole row is NaN
 #pragma unroll
-        for (int i = 0; i < RP; ++i) x[i] *= up;
+        for (int i = 0; i < C::QV; ++i) x[i] *= up;
 #pragma unroll
         for (int p = 0; p < C::PQ; ++p) {
           const int n = p * RP + q_row;
-          uint8_t* dst = buf + n * 128 + (((d0 >> 4) ^ (n & 7)) << 4) + (d0 & 15);
 #pragma unroll
-          for (int i = 0; i < RP / 4; ++i) {
+          for (int i = 0; i < C::QV / 4; ++i) {
+            const int d = d0 + i * 4;
             const uint16_t e0 = f32x2_to_fp8x2<kCacheE4M3>(x[4 * i], x[4 * i + 1]);
             const uint16_t e1 = f32x2_to_fp8x2<kCacheE4M3>(x[4 * i + 2], x[4 * i + 3]);
             const float2 f0 = Pair<__half>::unpack(fp8x2_to_f16x2<kCacheE4M3>(e0));
@@ -509,18 +531,21 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             x[4 * i + 1] -= f0.y;
             x[4 * i + 2] -= f1.x;
             x[4 * i + 3] -= f1.y;
-            *reinterpret_cast<uint32_t*>(dst + i * 4) = e0 | ((uint32_t)e1 << 16);
+            if (q_row < RP)
+              *reinterpret_cast<uint32_t*>(buf + (d >> 7) * (C::QR * 128) + n * 128 + ((((d & 127) >> 4) ^ (n & 7)) << 4) + (d & 15)) =
+                  e0 | ((uint32_t)e1 << 16);
           }
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < RP / 4; ++i) {
+        for (int i = 0; i < C::QV / 4; ++i) {
           const int d = d0 + i * 4;
-          *reinterpret_cast<uint2*>(buf + (d >> 6) * (C::QR * 128) + q_row * 128 + ((((d & 63) >> 3) ^ (q_row & 7)) << 4) +
+          if (q_row < RP)
+            *reinterpret_cast<uint2*>(buf + (d >> 6) * (C::QR * 128) + q_row * 128 + ((((d & 63) >> 3) ^ (q_row & 7)) << 4) +
                                     (d & 7) * 2) = make_uint2(qw[2 * i], qw[2 * i + 1]);
         }
       }
-      if (tid % TPR == 0) sDown[(item & 1) * 16 + q_row] = down;
+      if (tid % TPR == 0 && q_row < RP) sDown[(item & 1) * 16 + q_row] = down;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_ready[item & 1]);
@@ -585,14 +610,15 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
           const uint32_t v_slot = g % C::SLOTS;
           ok = ok && wwait(&v_full[v_slot], (g / C::SLOTS) & 1);
           if (ok) {
-            // this warp's 32 rows, four at a time, eight lanes a row
+            // this warp's 32 rows, a group of lanes a row and column block
+            constexpr int LPR = C::ATOM / 16;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = warp * 32 + i * 4 + (lane >> 3), key = j0 + row;
+            for (int i = 0; i < LPR; ++i) {
+              const int row = warp * 32 + i * (32 / LPR) + lane / LPR, key = j0 + row;
               if (key >= last.hi || (key < first.lo && key >= c.sinks)) {
-                uint8_t* v = sV + v_slot * C::TILE + row * 128 + (lane & 7) * 16;
-                *reinterpret_cast<uint4*>(v) = make_uint4(0, 0, 0, 0);
-                if constexpr (!C::k8) *reinterpret_cast<uint4*>(v + C::TILE / 2) = make_uint4(0, 0, 0, 0);
+                uint8_t* v = sV + v_slot * C::TILE + row * C::ATOM + (lane % LPR) * 16;
+#pragma unroll
+                for (int blk = 0; blk < C::BLOCKS; ++blk) *reinterpret_cast<uint4*>(v + blk * C::BLOCK) = make_uint4(0, 0, 0, 0);
               }
             }
           }
@@ -620,13 +646,13 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             ok = ok && wwait(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);   // every product so far has landed
             tc_fence_after();
 #pragma unroll
-            for (int q = 0; q < C::NP / 16; ++q) {
+            for (int q = 0; q < C::OM * C::NP / 16; ++q) {
               uint32_t o[16];
               tmem_ld16(tmem_base + lane_addr + C::OCOL + q * 16, o);
               tmem_ld_wait();
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                if (q * 16 + e < C::PP * RP) o[e] = __float_as_uint(__uint_as_float(o[e]) * f[(q * 16 + e) % RP]);
+                if ((q * 16 + e) % C::NP < C::PP * RP) o[e] = __float_as_uint(__uint_as_float(o[e]) * f[(q * 16 + e) % C::NP % RP]);
               tmem_st16(tmem_base + lane_addr + C::OCOL + q * 16, o);
             }
             tmem_st_wait();
@@ -686,9 +712,9 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
       softmax_sync();
       ok = ok && wwait(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
       tc_fence_after();
-      uint32_t o[C::NP];
+      uint32_t o[C::OM * C::NP];
 #pragma unroll
-      for (int q = 0; q < C::NP / 16; ++q)
+      for (int q = 0; q < C::OM * C::NP / 16; ++q)
         tmem_ld16(tmem_base + lane_addr + C::OCOL + q * 16, *reinterpret_cast<uint32_t(*)[16]>(&o[q * 16]));
       tmem_ld_wait();
       tc_fence_before();   // the next item's first product overwrites O after its P, which this thread has yet to store
@@ -702,18 +728,23 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
 #pragma unroll
         for (int r = 0; r < RP; ++r) {
           if (r < seg.rows) {
-            float v = __uint_as_float(o[r]);
-#pragma unroll
-            for (int p = 1; p < C::PP; ++p) v += __uint_as_float(o[p * RP + r]);
             const float l = (sSum[r] + sSum[16 + r]) + (sSum[32 + r] + sSum[48 + r]);
-            // a NaN sum stays one: only a row that saw nothing is set to zero
-            v = l == 0.f ? 0.f : v * (C::k8 ? 1.f / kPScale : 1.f) * (v_scale / l);
             const int64_t qtok = seg.s.q_begin + tok;
             const int h = seg.hk * group + in;
-            if (whole)
-              reinterpret_cast<T*>(a.out)[qtok * a.o_rs + (int64_t)h * a.o_hs + tid] = Cvt<T>::from_f32(v);
-            else
-              da.part_o[((int64_t)part * RP + r) * HD + tid] = v;
+#pragma unroll
+            for (int m = 0; m < C::OM; ++m) {
+              float v = __uint_as_float(o[m * C::NP + r]);
+#pragma unroll
+              for (int p = 1; p < C::PP; ++p) v += __uint_as_float(o[m * C::NP + p * RP + r]);
+              // a NaN sum stays one: only a row that saw nothing is set to zero
+              v = l == 0.f ? 0.f : v * (C::k8 ? 1.f / kPScale : 1.f) * (v_scale / l);
+              const int d = m * 128 + tid;
+              if (HD == 64 && tid >= 64) continue;
+              if (whole)
+                reinterpret_cast<T*>(a.out)[qtok * a.o_rs + (int64_t)h * a.o_hs + d] = Cvt<T>::from_f32(v);
+              else
+                da.part_o[((int64_t)part * RP + r) * HD + d] = v;
+            }
             if (tid == r) {
               my_l = l;
               my_m = m_ref[r];
@@ -753,12 +784,13 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
 }
 
 // Joins the parts of the items that runs cut.  Block i does the item whose start, but not end, CTA i holds: its tail part, then
-// the head parts of the same member of the teams after it.  A group of 128 threads takes a row at a time; items in many parts
+// the head parts of the same member of the teams after it.  A group of HD threads takes a row at a time; items in many parts
 // (few, long sequences) have their parts dealt out over the groups instead, whose sums are added in a fixed order.
-constexpr int kJoinGroups = 4;
-template <typename T, int RP>
-__global__ void __launch_bounds__(kJoinGroups * 128) attn_cache_join_kernel(DecodeArgs da, int ctas) {
+constexpr int kJoinThreads = 512;
+template <typename T, int RP, int HD>
+__global__ void __launch_bounds__(kJoinThreads) attn_cache_join_kernel(DecodeArgs da, int ctas) {
   const AttnArgs& a = da.c.a;
+  constexpr int kJoinGroups = kJoinThreads / HD;
   __shared__ float s_acc[kJoinGroups][HD], s_w[kJoinGroups];
   asm volatile("griddepcontrol.wait;" ::: "memory");              // launched early: the parts are complete after this
   const int i = blockIdx.x;
@@ -767,11 +799,12 @@ __global__ void __launch_bounds__(kJoinGroups * 128) attn_cache_join_kernel(Deco
   if (rec.item < 0) return;
   const int hk = rec.item % a.Hk;
   const int n = min(rec.parts, 1 + (ctas - 1 - i) / da.team);
-  const int grp = threadIdx.x >> 7, d = threadIdx.x & 127;
+  const int grp = threadIdx.x / HD, d = threadIdx.x % HD;
   const bool deal = n > 8;
   for (int r = deal ? 0 : grp; r < rec.rows; r += deal ? 1 : kJoinGroups) {
     auto slot = [&](int k) { return (int64_t)(k == 0 ? 2 * i + 1 : 2 * (i + k * da.team)) * RP + r; };
     float m = -INFINITY;
+#pragma unroll 8
     for (int k = 0; k < n; ++k) m = fmaxf(m, da.part_lse[slot(k)]);
     const float ms = m == -INFINITY ? 0.f : m;
     float acc = 0.f, wsum = 0.f;
@@ -802,12 +835,12 @@ __global__ void __launch_bounds__(kJoinGroups * 128) attn_cache_join_kernel(Deco
   }
 }
 
-template <typename T, int KIND, int RP>
+template <typename T, int KIND, int RP, int HD>
 int launch(DecodeArgs& da, cudaStream_t st) {
-  using C = Cfg<T, KIND, RP>;
+  using C = Cfg<T, KIND, RP, HD>;
   static_assert(C::SMEM <= 232448 && C::CTAS * (C::SMEM + 1024) <= 233472, "CTAs an SM");
   const AttnArgs& a = da.c.a;
-  constexpr int ES = C::k8 ? 1 : 2;
+  constexpr int ES = C::ES;
   da.page_rows = a.paged && a.block_size < BN ? a.block_size : BN;
   da.pages_per_tile = BN / da.page_rows;
   CUtensorMap maps[2];
@@ -817,7 +850,7 @@ int launch(DecodeArgs& da, cudaStream_t st) {
     const uint64_t rows = a.paged ? (uint64_t)a.block_size : (uint64_t)(a.total_k > 0 ? a.total_k : 1);
     const uint64_t dims[4] = {(uint64_t)HD, (uint64_t)a.Hk, rows, a.paged ? (uint64_t)a.num_blocks : 1};
     const uint64_t strides[3] = {hs, rs, a.paged ? bs : rs * rows};
-    const uint32_t box[4] = {(uint32_t)(128 / ES), 1, (uint32_t)da.page_rows, 1};
+    const uint32_t box[4] = {(uint32_t)(C::ATOM / ES), 1, (uint32_t)da.page_rows, 1};
     const int rc = ES == 2 ? encode_tmap_16bit(&maps[i], i ? a.v : a.k, 4, dims, strides, box)
                            : encode_tmap_8bit(&maps[i], i ? a.v : a.k, 4, dims, strides, box);
     if (rc != FG_OK) return rc;
@@ -826,7 +859,7 @@ int launch(DecodeArgs& da, cudaStream_t st) {
   int dev = 0;
   FG_CUDA_OK(cudaGetDevice(&dev));
   if (attr_dev != dev) {
-    FG_CUDA_OK(cudaFuncSetAttribute(attn_cache_decode_tcgen05_kernel<T, KIND, RP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    FG_CUDA_OK(cudaFuncSetAttribute(attn_cache_decode_tcgen05_kernel<T, KIND, RP, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     C::SMEM));
     attr_dev = dev;
   }
@@ -839,7 +872,7 @@ int launch(DecodeArgs& da, cudaStream_t st) {
   da.part_o = a.ws_o;
   da.part_lse = a.ws_o + (int64_t)2 * ctas * RP * HD;
   da.record = reinterpret_cast<PartRecord*>(da.part_lse + 2 * ctas * RP);
-  attn_cache_decode_tcgen05_kernel<T, KIND, RP><<<dim3(da.team, teams), NUM_THREADS, C::SMEM, st>>>(maps[0], maps[1], da);
+  attn_cache_decode_tcgen05_kernel<T, KIND, RP, HD><<<dim3(da.team, teams), NUM_THREADS, C::SMEM, st>>>(maps[0], maps[1], da);
   FG_CHECK_LAUNCH("attn_cache_decode_tcgen05_kernel");
   if (da.c.whole) return FG_OK;
   // The joining kernel is launched while this one still runs (programmatic dependent launch) and waits for its end on the
@@ -849,36 +882,44 @@ int launch(DecodeArgs& da, cudaStream_t st) {
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kJoinGroups * 128);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  FG_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_cache_join_kernel<T, RP>, da, ctas));
+  FG_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_cache_join_kernel<T, RP, HD>, da, ctas));
   FG_CHECK_LAUNCH("attn_cache_join_kernel");
   return FG_OK;
 }
 
-template <typename T, int KIND>
+template <typename T, int KIND, int HD>
 int launch_rows(DecodeArgs& da, cudaStream_t st) {
   const int rows = da.c.a.max_q * da.c.a.group;
-  if (rows <= 4) return launch<T, KIND, 4>(da, st);
-  if (rows <= 8) return launch<T, KIND, 8>(da, st);
-  return launch<T, KIND, 16>(da, st);
+  if (rows <= 4) return launch<T, KIND, 4, HD>(da, st);
+  if (rows <= 8) return launch<T, KIND, 8, HD>(da, st);
+  return launch<T, KIND, 16, HD>(da, st);
+}
+
+template <typename T, int KIND>
+int launch_dim(DecodeArgs& da, cudaStream_t st) {
+  if (da.c.a.D == 64) return launch_rows<T, KIND, 64>(da, st);
+  if constexpr (KIND != kCache16)
+    if (da.c.a.D == 256) return launch_rows<T, KIND, 256>(da, st);
+  return launch_rows<T, KIND, 128>(da, st);
 }
 
 template <typename T>
 int launch_kind(DecodeArgs& da, int kind, cudaStream_t st) {
-  if (kind == kCacheE4M3) return launch_rows<T, kCacheE4M3>(da, st);
-  if (kind == kCacheE5M2) return launch_rows<T, kCacheE5M2>(da, st);
-  return launch_rows<T, kCache16>(da, st);
+  if (kind == kCacheE4M3) return launch_dim<T, kCacheE4M3>(da, st);
+  if (kind == kCacheE5M2) return launch_dim<T, kCacheE5M2>(da, st);
+  return launch_dim<T, kCache16>(da, st);
 }
 
 }  // namespace
 
 // Bytes of workspace for `rows` query rows of a sequence and KV head: a head and a tail part, and a record, for each CTA.
-int64_t attn_cache_decode_sm100_bytes(int64_t rows, int sms) {
+int64_t attn_cache_decode_sm100_bytes(int64_t rows, int64_t head_dim, int sms) {
   const int64_t rp = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
-  return 2 * (int64_t)sms * (2 * rp * (HD + 1) * 4 + (int64_t)sizeof(PartRecord));
+  return 2 * (int64_t)sms * (2 * rp * (head_dim + 1) * 4 + (int64_t)sizeof(PartRecord));
 }
 
 int attn_cache_decode_sm100(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t st) {

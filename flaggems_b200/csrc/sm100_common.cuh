@@ -276,6 +276,10 @@ __host__ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr,
   d |= (uint64_t)2 << 61;
   return d;
 }
+// The same for rows of 64 bytes (layout type 4 = SWIZZLE_64B); 8-row groups are 512 bytes.
+__host__ __device__ __forceinline__ uint64_t umma_desc_sw64(uint32_t smem_addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+  return (umma_desc_sw128(smem_addr, lbo_bytes, sbo_bytes) & ~(7ull << 61)) | (uint64_t)4 << 61;
+}
 // Instruction descriptor for kind::f16 with fp32 accumulation.
 //   bits [4,6) D format (1 = f32); [7,10) A format, [10,13) B format (0 = f16, 1 = bf16);
 //   bit 15 A major, bit 16 B major (0 = K-major, 1 = MN-major);

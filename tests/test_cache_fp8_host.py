@@ -69,9 +69,9 @@ def test_nothing_to_do_is_no_call():
 
 def test_small_workspace_is_refused():
     lib = _lib.load()
-    p = params(max_seqlen_k=60000, batch=1, total_q=1, head_dim=64)
+    p = params(max_seqlen_k=60000, batch=1, total_q=1, head_dim=80)
     need = lib.fg_flash_attn_cache_workspace_bytes(ctypes.byref(p))
-    assert need > 0 and need % (8 * 65 * 4) == 0
+    assert need > 0 and need % (8 * 81 * 4) == 0
     p.base.workspace, p.base.workspace_bytes = 0x10000, need - 4
     with pytest.raises(RuntimeError, match="workspace of"):
         _lib.check(lib.fg_flash_attn_cache(ctypes.byref(p), None))
@@ -83,7 +83,7 @@ def test_small_workspace_is_refused():
 def test_workspace_goes_by_what_is_visible():
     """A window bounds the keys that are split, however long the context."""
     need = lambda **kw: _lib.load().fg_flash_attn_cache_workspace_bytes(ctypes.byref(params(**kw)))
-    for size in (dict(head_dim=64), dict(head_dim=248, max_seqlen_q=30, total_q=100)):
+    for size in (dict(head_dim=80), dict(head_dim=248, max_seqlen_q=30, total_q=100)):
         long, windowed = need(max_seqlen_k=10 ** 6, **size), need(max_seqlen_k=10 ** 6, window_left=2047, sink_tokens=4, **size)
         assert 0 < windowed < long and windowed == need(max_seqlen_k=10 ** 5, window_left=2047, sink_tokens=4, **size)
     chunk = dict(max_seqlen_q=30, total_q=100)
@@ -102,14 +102,16 @@ def test_workspace_goes_by_what_is_visible():
 
 
 def test_path_by_sizes():
-    path = lambda **kw: _lib.load().fg_flash_attn_cache_path(ctypes.byref(params(**kw)))
+    path = lambda **kw: _lib.load().fg_flash_attn_cache_path(ctypes.byref(params(**{"max_seqlen_k": 10 ** 5, **kw})))
+    assert path(max_seqlen_k=1000) == 2      # too few tiles of keys
     assert path() == 3 and path(max_seqlen_q=4, total_q=16) == 3      # 4 tokens of a group of 4: 16 rows
     assert path(max_seqlen_q=5, total_q=20) == 1 and path(max_seqlen_q=3000, total_q=9000) == 1
-    assert path(head_dim=64) == 2 and path(softcap=5.0) == 2 and path(head_dim=72, max_seqlen_q=5, total_q=20) == 0
+    assert path(head_dim=64) == path(head_dim=256) == 3 and path(head_dim=80) == path(head_dim=256, cache_dtype=_lib.FG_BF16) == 2
+    assert path(softcap=5.0) == 2 and path(head_dim=72, max_seqlen_q=5, total_q=20) == 0
     assert path(head_dim=64, max_seqlen_q=1000, total_q=4000) == path(head_dim=256, max_seqlen_q=5, total_q=20) == 1
     assert path(head_dim=64, max_seqlen_q=5, total_q=20, max_seqlen_k=600) == 0       # too few tiles for a widened copy
     assert path(block_size=24) == 0 and path(block_size=4) == 0 and path(k_row_stride=264) == 0   # pages or strides TMA cannot take
-    assert path(cache_dtype=_lib.FG_BF16, k_row_stride=264, sink_tokens=1, window_left=7) == 3    # 528 bytes are fine
+    assert path(cache_dtype=_lib.FG_BF16, k_row_stride=264, sink_tokens=1, window_left=70000) == 3    # 528 bytes are fine
     assert path(num_heads=400, num_heads_k=2) == 0                    # a group of 200
 
 

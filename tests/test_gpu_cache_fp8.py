@@ -296,7 +296,9 @@ def attention(q_lens, k_lens, q, rows, ks, vs, scale, causal, window, sinks, sof
 
 
 def check(fg, q_lens, k_lens, heads, hk, dim, page, dtype, cache, causal=True, window=(-1, -1), sinks=0, softcap=0.0,
-          scale_shape="one", seed=0, behind=3, contiguous=False, spread=1.0):
+          scale_shape="one", seed=0, behind=3, contiguous=False, spread=1.0, bound=0):
+    """`bound`: max_seqlen_k that the call is given, where it is not the longest sequence."""
+    bound = bound or max(k_lens)
     g = gen(seed + sum(k_lens) + dim)
     eight = cache in TOP
     batch = len(k_lens)
@@ -327,7 +329,7 @@ def check(fg, q_lens, k_lens, heads, hk, dim, page, dtype, cache, causal=True, w
         descale = dict(k_descale=wide(ks), v_descale=wide(vs))
     out = torch.full((total + behind, heads, dim), 7.0, dtype=dtype, device=DEV)
     got, lse = fg.flash_attn_varlen_func(
-        q, kc, vc, max(q_lens), cu, max(k_lens), softmax_scale=dim ** -0.5, causal=causal, window_size=window,
+        q, kc, vc, max(q_lens), cu, bound, softmax_scale=dim ** -0.5, causal=causal, window_size=window,
         softcap=softcap, sink_tokens=sinks, out=out, return_softmax_lse=True, **where, **descale)
     assert got is out and (out[total:] == 7.0).all()
     one = torch.ones(1, device=DEV)
@@ -342,7 +344,7 @@ def check(fg, q_lens, k_lens, heads, hk, dim, page, dtype, cache, causal=True, w
     assert (lse[empty] == math.inf).all()
     assert ((lse[~empty] - wlse[~empty]).abs() <= lse_tol[~empty]).all()
     again = fg.flash_attn_varlen_func(
-        q, kc, vc, max(q_lens), cu, max(k_lens), softmax_scale=dim ** -0.5, causal=causal, window_size=window,
+        q, kc, vc, max(q_lens), cu, bound, softmax_scale=dim ** -0.5, causal=causal, window_size=window,
         softcap=softcap, sink_tokens=sinks, out=torch.full_like(out, 7.0), **where, **descale)
     assert torch.equal(again, out)          # the same inputs, the same bits
 
@@ -544,6 +546,26 @@ def test_two_captured_graphs_and_another_stream(fg):
         for i, which in enumerate((0, 1)):
             want = (quantise(s["new"][:, which], scale, E4M3).float() * scale).to(torch.bfloat16)
             assert torch.equal(s["rows"][i][s["cu_k"][1:].long() - 1], want)
+
+
+@pytest.mark.parametrize("dtype, cache", [(torch.bfloat16, E4M3), (torch.float16, E4M3), (torch.bfloat16, E5M2), (torch.float16, E5M2)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads, hk, tokens", [(4, 4, 1), (8, 2, 1), (7, 1, 1), (4, 1, 4), (48, 3, 1)])
+def test_fp8_decode_with_a_large_bound(fg, dtype, cache, dim, heads, hk, tokens):
+    """Enough keys, by max_seqlen_k, for the kernels that walk long contexts."""
+    check(fg, [tokens] * 6, [tokens, 17, 64, 463, 1328, 129], heads, hk, dim, 16, dtype, cache, scale_shape="batch", bound=200000)
+    check(fg, [tokens, 0, tokens, 1], [3, 50, 0, 700], heads, hk, dim, 64, dtype, cache, causal=False, window=(-1, 3), bound=400000)
+
+
+@pytest.mark.parametrize("cache", [torch.bfloat16, torch.float16, E4M3])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window, sinks", [((100, 0), 130), ((31, 0), 4), ((0, 0), 1)])
+@pytest.mark.parametrize("heads, hk, batch", [(16, 4, 64), (56, 8, 64), (48, 3, 270)])
+def test_windowed_decode_of_many_sequences(fg, cache, dim, window, sinks, heads, hk, batch):
+    if (dim, cache) in ((256, torch.bfloat16), (256, torch.float16)) or (batch == 270 and (window[0] != 100 or dim == 64)):
+        pytest.skip("not this kernel")
+    dtype = torch.bfloat16 if cache == E4M3 else cache
+    check(fg, [1] * batch, [1 + (i * 61) % 900 for i in range(batch)], heads, hk, dim, 16, dtype, cache, window=window, sinks=sinks)
 
 
 def test_large_groups_many_sequences_and_nothing_cached(fg):
