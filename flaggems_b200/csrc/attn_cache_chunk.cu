@@ -1,10 +1,10 @@
-// Attention of a chunk of new tokens over an 8-bit or windowed cache, head dim 128, on the tcgen05 tensor cores.
+// Attention of a chunk of new tokens over an 8-bit or windowed cache, head dim 64, 128 or 256, on the tcgen05 tensor cores.
 //
 // An item is one or two 128-row Q tiles of one (sequence, KV head).  A row is a (token, head of the group) pair, so a chunk of a
 // few tokens fills the tiles as well as a long one, and all query heads of the group share every K/V tile.  A tile holds
-// floor(128 / group) tokens.  The kernel is persistent, one CTA an SM: the K/V tiles (64 keys) of all items, laid end to end,
+// floor(128 / group) tokens (at head dim 256 an item is one tile).  The kernel is persistent, one CTA an SM: the K/V tiles (64 keys) of all items, laid end to end,
 // are cut into equal runs, one per CTA, so that few long items and many short ones fill the SMs alike (in whole items, 336
-// CTAs on 148 SMs would take three rounds for 2.27).  The parts of an item that runs cut are joined by a second kernel, in
+// CTAs on 148 SMs would take three rounds for 2.27).  Short items are not cut (attn_cache_api.cu has the rule).  The parts of an item that runs cut are joined by a second kernel, in
 // order.  Nothing synchronises the CTA between items: the roles follow the barrier phases with running counters.
 //
 //   warps 0-7    softmax, one warpgroup per Q tile, one thread per row (TMEM lane = row): scores of 64 keys from TMEM to
@@ -14,7 +14,7 @@
 //   warps 8, 9   TMA producers of K (and Q) and of V, walking the tile runs (first tokens, then the window).  A page of 16 keys is
 //                two boxes, and a warp issues one in about 95 clocks: one warp for both would need 1900 clocks a tile
 //   warp 10      scores of both Q tiles: S = Q K^T, 64 keys a step
-//   8-bit caches:
+//   8-bit caches (head dim 128):
 //   warp 8       TMA producer of Q; warps 9, 10 the scores of one Q tile each
 //   warps 12-15  load K and V rows (one tile ahead, in registers), widen them to fp16 and store them as the 128-byte
 //                swizzled tiles that the tensor cores read; rows that no row of the item sees are neither read nor kept.
@@ -23,7 +23,13 @@
 //   warp 11      O += P V of both tiles
 // Widening inside the kernel makes a step half as long again, and every item widens the keys it reads anew.  Where the chunk is
 // long (several items read each key) and the store's 16-bit copy is not too large, a kernel before this one widens the visible
-// rows once into the workspace, and this one reads them as a 16-bit store (attn_cache_api.cu has the rule).
+// rows once into the workspace, and this one reads them as a 16-bit store (attn_cache_api.cu has the rule; two chunks of 2048
+// tokens 505 us, the copy included).  At head dims 64 and 256 that is the only form.
+// What bounds it: with two Q tiles of head dim 128 a step of 64 keys is 2 x 2 products of 128 x 64 x 128, 1024 clocks of the tensor
+// cores at 4096 multiply-adds a clock, and 16384 exponentials, 1024 clocks of the special function units at 16 a clock.  Long
+// chunks reach half of a large library product's rate, since each of the two waits for the other at times; short ones are bound
+// by the start and the joining of the items.
+// Two 2048-token prompts at head dim 256 621 us, at 64 234 us (mma.sync: 1654 and 343).
 // Over 8-bit caches bf16 queries are brought to fp16, each row by a power of two, by the softmax warps before an item's first
 // step.
 // TMEM columns: tile t has its scores at t*128 (64 columns), two probability buffers at t*128+64 and +96, its output at

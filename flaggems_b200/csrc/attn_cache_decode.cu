@@ -1,5 +1,8 @@
 // Attention of a few query rows (at most 16 (token, head of the group) pairs of a sequence) over an 8-bit or windowed
-// cache: single-token decode, and a few tokens at a time.  Memory bound: every cached byte is read once.
+// cache: single-token decode, and a few tokens at a time.  Every cached byte is read once.  For few keys in all, where many small
+// CTAs hide the way through a tile better than the tcgen05 form's runs, and for what that form does not take (soft-capping, 16-bit
+// head dim 256, other head dims); attn_cache_api.cu has the rule and both sides' times.  Long contexts it moves at about
+// 2.5 TB/s (8-bit head dim 128), bound by the widening.
 //
 // CTA = (range of K/V tiles, KV head, sequence), 5 warps:
 //   warp 0     producer: walks the tile runs (first tokens, then the window), looks the pages of each tile up and

@@ -423,7 +423,8 @@ FG_API int fg_gather_cache_flash(const fg_cache_gather_params* p, void* stream);
  * `sink_tokens` keys visible.  No counterpart in the reference.
  *
  * `base` as for fg_flash_attn_varlen, without ALiBi and batch strides; q and out are of base.dtype, K/V of cache_dtype
- * (base.dtype, FG_E4M3 or FG_E5M2; strides in elements of the cache, multiples of 8).  Key j is visible to the query
+ * (base.dtype, FG_E4M3 or FG_E5M2; strides in elements of the cache, multiples of 8).  max_seqlen_k must not be below any
+ * sequence's length: longer ones are cut to it, and rows behind q or a contiguous K/V are not touched.  Key j is visible to the query
  * at position p of its sequence (p = i + k_len - q_len) iff j < k_len, j <= p + window_right (causal: j <= p), and
  * j >= p - window_left or j < sink_tokens.  Rows with no visible key produce 0 and an LSE of +inf; rows of q outside
  * [cu_seqlens_q[0], cu_seqlens_q[batch]) leave out and lse as they were.  K/V that no query of a 64-key tile's
@@ -449,8 +450,8 @@ typedef struct {
 FG_API int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream);
 FG_API int64_t fg_flash_attn_cache_workspace_bytes(const fg_attn_cache_params* p);
 /* Which kernel family fg_flash_attn_cache picks: 0 general (mma.sync), 1 tcgen05; for at most 16 query rows per
- * sequence and KV head 2 TMA-fed (mma.sync), 3 tcgen05.  The tcgen05 kernels take head dim 128 and need a workspace.  Pure host
- * logic. */
+ * sequence and KV head 2 TMA-fed (mma.sync), 3 tcgen05.  The tcgen05 kernels take head dims 64, 128 and 256 and, beyond short
+ * contexts, need a workspace.  Pure host logic. */
 FG_API int fg_flash_attn_cache_path(const fg_attn_cache_params* p);
 
 /* ------------------------------------------------------------------------
