@@ -421,7 +421,8 @@ def test_query_magnitudes(fg, spread):
         check(fg, q_lens, [200, 90], 8, 2, 128, 16, torch.bfloat16, E4M3, spread=spread)
 
 
-def test_long_context_offsets(fg):
+@pytest.mark.parametrize("bound", [190, 10 ** 6])
+def test_long_context_offsets(fg, bound):
     """A cache of more than 2^32 bytes: the last pages are used."""
     page, hk, dim = 64, 8, 128
     blocks = (2 ** 32 + 2 ** 28) // (page * hk * dim)
@@ -446,14 +447,15 @@ def test_long_context_offsets(fg):
         q = randn(g, sum(q_lens), 32, dim).to(torch.bfloat16)
         cu = torch.tensor([0] + q_lens, device=DEV).cumsum(0, dtype=torch.int32)
         out = fg.flash_attn_varlen_func(
-            q, kc, vc, max(q_lens), cu, 190, seqused_k=torch.tensor(lens, dtype=torch.int32, device=DEV), causal=True,
+            q, kc, vc, max(q_lens), cu, bound, seqused_k=torch.tensor(lens, dtype=torch.int32, device=DEV), causal=True,
             block_table=table, k_descale=scale, v_descale=scale)
         want, _, tol, _ = attention(q_lens, lens, q, rows, [scale] * 2, [scale] * 2, dim ** -0.5, True, (-1, -1), 0, 0.0,
                                     torch.bfloat16, E4M3)
         assert ((out.double() - want).abs() <= tol).all()
 
 
-def test_nan_that_a_query_sees_reaches_its_row(fg):
+@pytest.mark.parametrize("bound", [100, 10 ** 6])
+def test_nan_that_a_query_sees_reaches_its_row(fg, bound):
     page, hk, dim = 16, 2, 128
     g = gen(4)
     one = torch.ones(1, device=DEV)
@@ -463,7 +465,7 @@ def test_nan_that_a_query_sees_reaches_its_row(fg):
         cu = torch.tensor([0] + q_lens, device=DEV).cumsum(0, dtype=torch.int32)
         q = randn(g, sum(q_lens), 4, dim).to(torch.bfloat16)
         out, lse = fg.flash_attn_varlen_func(
-            q, kc, vc, max(q_lens), cu, 100, seqused_k=torch.tensor([100, 60], dtype=torch.int32, device=DEV), causal=True,
+            q, kc, vc, max(q_lens), cu, bound, seqused_k=torch.tensor([100, 60], dtype=torch.int32, device=DEV), causal=True,
             block_table=table, return_softmax_lse=True)
         n = q_lens[0]
         assert out[:n, :2].isnan().all() and out[:n, 2:].isfinite().all() and out[n:].isfinite().all()
@@ -494,7 +496,8 @@ def test_strided_tensors_and_out_views(fg):
         assert (hold[:, 0] == 7.0).all() and (hold[:, -1] == 7.0).all()
 
 
-def test_two_captured_graphs_and_another_stream(fg):
+@pytest.mark.parametrize("bound", [2000, 10 ** 6])
+def test_two_captured_graphs_and_another_stream(fg, bound):
     """Write, attend and read back captured in two graphs, replayed at the same time on two streams."""
     g = gen(7)
     page, hk, heads, dim, batch = 16, 8, 32, 128, 6
@@ -515,7 +518,7 @@ def test_two_captured_graphs_and_another_stream(fg):
     def step(s):
         fg.reshape_and_cache_flash(s["new"][:, 0], s["new"][:, 1], s["kc"], s["vc"], s["slots"], "fp8", scale, scale)
         fg.gather_cache_flash(s["kc"], s["vc"], *s["rows"], s["table"], s["cu_k"], "fp8", scale, scale)
-        return fg.flash_attn_varlen_func(s["q"], s["kc"], s["vc"], 1, s["cu"], 2000, seqused_k=s["lens"], causal=True,
+        return fg.flash_attn_varlen_func(s["q"], s["kc"], s["vc"], 1, s["cu"], bound, seqused_k=s["lens"], causal=True,
                                          block_table=s["table"], k_descale=scale, v_descale=scale)
 
     eager = [step(s).clone() for s in runs]
@@ -555,6 +558,23 @@ def test_fp8_decode_with_a_large_bound(fg, dtype, cache, dim, heads, hk, tokens)
     """Enough keys, by max_seqlen_k, for the kernels that walk long contexts."""
     check(fg, [tokens] * 6, [tokens, 17, 64, 463, 1328, 129], heads, hk, dim, 16, dtype, cache, scale_shape="batch", bound=200000)
     check(fg, [tokens, 0, tokens, 1], [3, 50, 0, 700], heads, hk, dim, 64, dtype, cache, causal=False, window=(-1, 3), bound=400000)
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_decode_with_a_large_bound_by_page_size(fg, page, dim):
+    check(fg, [1, 1, 1], [300, 77, 515], 8, 2, dim, page, torch.bfloat16, E4M3, bound=10 ** 6)
+    check(fg, [1, 1, 0], [300, 77, 515], 16, 1, dim, page, torch.float16, E5M2, bound=10 ** 6, contiguous=True)
+    check(fg, [2, 1], [300, 1], 8, 2, dim, page, torch.bfloat16, E4M3, bound=10 ** 6, spread=1e-30)
+
+
+@pytest.mark.parametrize("dtype, cache", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), (torch.bfloat16, E4M3),
+                                          (torch.float16, E5M2)])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("window, sinks", [((100, 0), 130), ((1000, 0), 4), ((30, 0), 1)])
+def test_windowed_chunks_at_other_head_dims(fg, dtype, cache, dim, window, sinks):
+    check(fg, [200, 70, 1, 300], [200, 500, 900, 1500], 16, 4, dim, 16, dtype, cache, window=window, sinks=sinks)
+    check(fg, [20, 7, 9], [2000, 500, 9], 4, 4, dim, 64, dtype, cache, window=window, sinks=sinks)
 
 
 @pytest.mark.parametrize("cache", [torch.bfloat16, torch.float16, E4M3])
