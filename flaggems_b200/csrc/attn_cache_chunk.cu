@@ -78,7 +78,6 @@ struct ChunkArgs {
   int page_rows;        // keys per TMA box
   int pages_per_tile;
   int num_mb;           // items of the longest chunk, for each KV head
-  int min_run;          // fewest K/V tiles of a run
   float* part_o;        // [2 * CTAs][tiles * 128][128]: head part, tail part of each CTA
   float* part_lse;      // [2 * CTAs][tiles * 128]
   PartRecord* record;   // [CTAs]
@@ -214,13 +213,16 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   SeqInfo* sInfo = reinterpret_cast<SeqInfo*>(rest + 512);   // [kInfo]
 
-  __shared__ int s_drain, s_sum[THREADS / 32], s_off, s_pair;
+  __shared__ int s_drain, s_sum[THREADS / 32], s_top[THREADS / 32], s_off, s_pair;
   // ---- this CTA's run: tiles [begin, begin + run) of all items' tiles; a pair is (sequence, Q tiles), the items of a pair are
   // its KV heads
   const int pairs = a.batch * pa.num_mb;
   TileSpan span;
-  int mine = 0;
-  if (tid < pairs) mine = item_weight(c, item_tiles(pa, cache_seq_info(c, tid / pa.num_mb), tid % pa.num_mb, span)) * a.Hk;
+  int mine = 0, longest = 0;
+  if (tid < pairs) {
+    longest = item_tiles(pa, cache_seq_info(c, tid / pa.num_mb), tid % pa.num_mb, span);
+    mine = item_weight(c, longest) * a.Hk;
+  }
   if (tid == 0) {
     s_drain = *reinterpret_cast<volatile int*>(a.status);
     *abort_flag = 0;
@@ -246,17 +248,30 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     prefetch_tmap(&tmap_v);
   }
   int total = mine;
-  for (int p = tid + THREADS; p < pairs; p += THREADS)
-    total += item_weight(c, item_tiles(pa, cache_seq_info(c, p / pa.num_mb), p % pa.num_mb, span)) * a.Hk;
+  for (int p = tid + THREADS; p < pairs; p += THREADS) {
+    const int n = item_tiles(pa, cache_seq_info(c, p / pa.num_mb), p % pa.num_mb, span);
+    longest = max(longest, n);
+    total += item_weight(c, n) * a.Hk;
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) s_sum[warp] = total;
+  if (lane == 0) {
+    s_sum[warp] = total;
+    s_top[warp] = longest;
+  }
   __syncthreads();
   if (s_drain != 0) return;   // a wait gave up on this device: finish the launch quickly
   total = 0;
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) total += s_sum[i];
-  const int run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, pa.min_run);
+  for (int i = 0; i < THREADS / 32; ++i) {
+    total += s_sum[i];
+    longest = max(longest, s_top[i]);
+  }
+  // Short items need not share a CTA.  An item of n tiles in n / run parts takes about 1 us a tile and 0.5 us a part to join: run is
+  // at least the root of n / 2 (20 tokens over 16000 keys: 55 us in runs of 4 tiles, 38 in runs of 11).
+  const int min_run = c.whole ? 1 : max(min(kMinRun, longest), (int)sqrtf(0.5f * longest));
+  const int run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, max(min_run, 1));
   const int64_t begin = (int64_t)run * blockIdx.x;
   if (begin >= total) {
     if (tid == 0 && !c.whole) pa.record[blockIdx.x] = PartRecord{-1, 0, 0, 0};
@@ -1004,10 +1019,6 @@ int attn_cache_chunk(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t s
   int64_t num_mb;
   chunk_shape(c.a.max_q, c.a.group, c.a.D, &pa.tiles, &pa.tokens, &num_mb);
   pa.num_mb = (int)num_mb;
-  // Short items need not share a CTA.  An item of n tiles in n / run parts takes about 1 us a tile and 0.5 us a part to join: run is
-  // at least the root of n / 2 (20 tokens over 16000 keys: 55 us in runs of 4 tiles, 38 in runs of 11).
-  const int longest = (c.a.max_k + BN - 1) / BN;
-  pa.min_run = c.whole ? 1 : max(max(1, min(kMinRun, longest)), (int)sqrtf(0.5f * longest));
   return dtype == FG_BF16 ? launch_kind<__nv_bfloat16>(pa, kind, st) : launch_kind<__half>(pa, kind, st);
 }
 
