@@ -11,11 +11,15 @@
 // on rows that are not there.
 //
 // 8-bit caches: Q and P are split into 8-bit pieces, each with columns of its own, and the columns are added up in fp32.
-//   Q   a row is multiplied by a power of two that takes its largest value to [2^7, 2^8) and parted into e4m3 pieces, each
-//       the rounding of what the previous left: 2 pieces hold the 8 bits of a bf16 significand, 3 the 11 bits of fp16,
-//       down to 2^-18 of the row's largest value (an e4m3 subnormal step)
-//   P   2^11 p (p <= 2^4, see below), rounded to fp16, in four e5m2 pieces of three bits, which hold all of it down to
-//       2^-28; e5m2 for its range: long contexts have many small probabilities
+// A piece is the rounding of what the ones before it left, times a power of two that brings it back to the top of the type's
+// range: a common scale would cut all pieces at the same subnormal step.
+//   Q   a row is multiplied by a power of two that takes its largest value to [2^7, 2^8) and parted into three e4m3 pieces, 2^5
+//       apart: exact for bf16 and fp16 values down to 2^-17 of the row's largest one, and within 2^-27 of it below (a
+//       subnormal step of the last piece).  Rows whose largest channel meets small keys need that range; two pieces would do
+//       for the 8 bits of bf16 near the top, but end at 2^-22.  The third costs nothing at 4 rows (its columns are there
+//       anyway) and most at 16 rows of 256 dims, 172 -> 180 us for 64 sequences.
+//   P   2^11 p (p <= 2^4, see below), rounded to fp16 (2^-12 of itself, or 2^-36), in four e5m2 pieces of three bits, 2^3
+//       apart, which hold every fp16 value exactly; e5m2 for its range: long contexts have many small probabilities
 // 16-bit caches: Q as it is; P in one fp16 piece, or two bf16 pieces (2^-17).
 //
 // The running maximum is shared by the CTA and raised only when a score exceeds it by more than 4 (log2 units); the warps
@@ -48,6 +52,8 @@ constexpr int BN = 128, NUM_THREADS = 224;
 constexpr int TMA_WARP = 4, MMA_WARP = 6;
 constexpr float kRaise = 4.0f;               // log2 units
 constexpr float kPScale = 2048.0f;           // of P before it is split (8-bit caches)
+constexpr float kQStep = 32.f;               // a residual of Q is at most half an e4m3 step of four bits: 2^3 below 2^8
+constexpr float kPStep = 8.f;                // of P at most half an e5m2 step of three bits: 2^11 below 2^15
 
 constexpr int kInfo = 32;                    // sequences of a run whose lengths are kept in shared memory
 
@@ -58,7 +64,7 @@ template <typename T, int KIND, int RP, int HD>
 struct Cfg {
   static constexpr bool k8 = KIND != kCache16;
   static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  static constexpr int PQ = !k8 ? 1 : (kBf16 ? 2 : 3);        // pieces of Q
+  static constexpr int PQ = k8 ? 3 : 1;                       // pieces of Q
   static constexpr int PP = k8 ? 4 : (kBf16 ? 2 : 1);         // pieces of P
   static constexpr int NS = up(RP * PQ, 16), NP = up(RP * PP, 16);   // columns of the two products
   // Rows of Q and P that shared memory holds: whole 8-row swizzle groups.  Where the product has 8 columns more, it reads
@@ -532,10 +538,10 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             const uint16_t e1 = f32x2_to_fp8x2<kCacheE4M3>(x[4 * i + 2], x[4 * i + 3]);
             const float2 f0 = Pair<__half>::unpack(fp8x2_to_f16x2<kCacheE4M3>(e0));
             const float2 f1 = Pair<__half>::unpack(fp8x2_to_f16x2<kCacheE4M3>(e1));
-            x[4 * i] -= f0.x;
-            x[4 * i + 1] -= f0.y;
-            x[4 * i + 2] -= f1.x;
-            x[4 * i + 3] -= f1.y;
+            x[4 * i] = (x[4 * i] - f0.x) * kQStep;
+            x[4 * i + 1] = (x[4 * i + 1] - f0.y) * kQStep;
+            x[4 * i + 2] = (x[4 * i + 2] - f1.x) * kQStep;
+            x[4 * i + 3] = (x[4 * i + 3] - f1.y) * kQStep;
             if (q_row < RP)
               *reinterpret_cast<uint32_t*>(buf + (d >> 7) * (C::QR * 128) + n * 128 + ((((d & 127) >> 4) ^ (n & 7)) << 4) + (d & 15)) =
                   e0 | ((uint32_t)e1 << 16);
@@ -593,9 +599,9 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
           if (lane == 0) mbar_arrive(&s_free[g & 1]);
 #pragma unroll
           for (int r = 0; r < RP; ++r) {
-            float v = __uint_as_float(col[r]);
+            float v = __uint_as_float(col[(C::PQ - 1) * RP + r]);   // the smallest piece first
 #pragma unroll
-            for (int p = 1; p < C::PQ; ++p) v += __uint_as_float(col[p * RP + r]);
+            for (int p = C::PQ - 2; p >= 0; --p) v = fmaf(v, 1.f / kQStep, __uint_as_float(col[p * RP + r]));
             x[r] = v * pre[r];
           }
         }
@@ -680,7 +686,8 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
               const uint16_t e = f16x2_to_e5m2x2(h);
               const uint32_t back = fp8x2_to_f16x2<kCacheE5M2>(e);
               const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&back));
-              h = *reinterpret_cast<const uint32_t*>(&d);
+              const __half2 rest = __hmul2(d, __float2half2_rn(kPStep));
+              h = *reinterpret_cast<const uint32_t*>(&rest);
               const int n = p * RP + r;
               buf[n * 128 + ((ch ^ (n & 7)) << 4) + at] = (uint8_t)(e & 0xff);
               buf[(n + 1) * 128 + ((ch ^ ((n + 1) & 7)) << 4) + at] = (uint8_t)(e >> 8);
@@ -738,9 +745,9 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             const int h = seg.hk * group + in;
 #pragma unroll
             for (int m = 0; m < C::OM; ++m) {
-              float v = __uint_as_float(o[m * C::NP + r]);
+              float v = __uint_as_float(o[m * C::NP + (C::PP - 1) * RP + r]);
 #pragma unroll
-              for (int p = 1; p < C::PP; ++p) v += __uint_as_float(o[m * C::NP + p * RP + r]);
+              for (int p = C::PP - 2; p >= 0; --p) v = fmaf(v, C::k8 ? 1.f / kPStep : 1.f, __uint_as_float(o[m * C::NP + p * RP + r]));
               // a NaN sum stays one: only a row that saw nothing is set to zero
               v = l == 0.f ? 0.f : v * (C::k8 ? 1.f / kPScale : 1.f) * (v_scale / l);
               const int d = m * 128 + tid;
