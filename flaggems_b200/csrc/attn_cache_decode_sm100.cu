@@ -14,7 +14,7 @@
 // A piece is the rounding of what the ones before it left, times a power of two that brings it back to the top of the type's
 // range: a common scale would cut all pieces at the same subnormal step.
 //   Q   a row is multiplied by a power of two that takes its largest value to [2^7, 2^8) and parted into three e4m3 pieces, 2^5
-//       apart: exact for bf16 and fp16 values down to 2^-17 of the row's largest one, and within 2^-27 of it below (a
+//       apart: exact for bf16 and fp16 values down to 2^-16 of the row's largest one, and within 2^-27 of it below (a
 //       subnormal step of the last piece).  Rows whose largest channel meets small keys need that range; two pieces would do
 //       for the 8 bits of bf16 near the top, but end at 2^-22.  The third costs nothing at 4 rows (its columns are there
 //       anyway) and most at 16 rows of 256 dims, 172 -> 180 us for 64 sequences.
@@ -66,6 +66,7 @@ struct Cfg {
   static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   static constexpr int PQ = k8 ? 3 : 1;                       // pieces of Q
   static constexpr int PP = k8 ? 4 : (kBf16 ? 2 : 1);         // pieces of P
+  static constexpr bool kPieces = PP > 1 && KIND != kCacheE4M3;   // V may hold infinities, and meets several pieces (e4m3 has none)
   static constexpr int NS = up(RP * PQ, 16), NP = up(RP * PP, 16);   // columns of the two products
   // Rows of Q and P that shared memory holds: whole 8-row swizzle groups.  Where the product has 8 columns more, it reads
   // whatever follows there; nothing uses those columns.
@@ -184,6 +185,77 @@ __device__ __forceinline__ uint16_t f16x2_to_e5m2x2(uint32_t h) {
   uint16_t r;
   asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(h));
   return r;
+}
+
+// ---- Infinities.  Piece by piece a product with an infinity may be a NaN where the whole is none (a later piece can be zero or
+// of the other sign).  A NaN is looked into where it shows up, outside the loops' registers; finite values never come here.
+
+// Which query rows see +inf, -inf or NaN among the V values of dim d at the keys of segment g: bits r, 16 + r, 32 + r.
+template <typename T, int KIND>
+__device__ __noinline__ uint64_t odd_values(const CacheAttnArgs& c, const Segment& g, int d) {
+  using E = typename std::conditional<KIND == kCache16, T, uint8_t>::type;
+  const int group = c.a.group;
+  const E* v = reinterpret_cast<const E*>(c.a.v) + (int64_t)g.hk * c.a.v_hs + d;
+  const int32_t* bt_row = c.a.paged ? c.a.block_table + (int64_t)g.b * c.a.bt_stride : nullptr;
+  uint64_t bits = 0;
+  for (int t = g.lo; t < g.hi; ++t) {
+    const int j0 = g.span.tile(t) * BN, end = min(j0 + BN, g.s.k_len);
+    for (int j = j0; j < end; j += 8) {          // rows of one page
+      const int64_t row = cache_row(c, bt_row, g.s.k_begin, j, c.a.v_rs, c.a.v_bs);
+      E raw[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) raw[i] = j + i < end ? v[row + i * c.a.v_rs] : E{};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float x;
+        if constexpr (KIND == kCache16)
+          x = Cvt<T>::to_f32(raw[i]);
+        else
+          x = Pair<__half>::unpack(fp8x2_to_f16x2<KIND>(raw[i])).x;
+        if (j + i >= end || fabsf(x) < INFINITY) continue;
+        for (int r = 0; r < g.rows; ++r)
+          if (!row_mask(c, g.s.k_len, r / group + g.shift).dead(j + i)) bits |= 1ull << (r + (x != x ? 32 : x > 0.f ? 0 : 16));
+      }
+    }
+    const uint64_t nan = bits >> 32 | (bits & bits >> 16);
+    if ((nan & 0xffff) == (1ull << g.rows) - 1) break;      // every row has its NaN
+  }
+  return bits;
+}
+
+// Puts the infinities where bits of `odd` (16 m + r) say that dim m * 128 + threadIdx.x of row r came out as a NaN.
+template <typename T, int KIND, int RP, int HD>
+__device__ __noinline__ void write_infinities(const DecodeArgs& da, const Segment& g, int part, uint32_t odd, float v_scale) {
+  const AttnArgs& a = da.c.a;
+  for (int m = 0; m < 2; ++m) {
+    if ((odd >> (16 * m) & 0xffff) == 0) continue;
+    const int d = m * 128 + threadIdx.x;
+    const uint64_t seen = odd_values<T, KIND>(da.c, g, d);
+    for (int r = 0; r < g.rows; ++r) {
+      const bool up = seen >> r & 1, down = seen >> (16 + r) & 1, nan = seen >> (32 + r) & 1;
+      if (!(odd >> (16 * m + r) & 1) || nan || up == down) continue;
+      const float v = (up ? INFINITY : -INFINITY) * v_scale;
+      const int tok = r / a.group;
+      if (part < 0)
+        reinterpret_cast<T*>(a.out)[(int64_t)(g.s.q_begin + tok) * a.o_rs + (int64_t)(g.hk * a.group + r - tok * a.group) * a.o_hs + d] =
+            Cvt<T>::from_f32(v);
+      else
+        da.part_o[((int64_t)part * RP + r) * HD + d] = v;
+    }
+  }
+}
+
+// The score of row r (times log2 e) at key `key`, in fp32.
+template <typename T, int KIND, int HD>
+__device__ __noinline__ float whole_score(const CacheAttnArgs& c, const Segment& g, int r, int key) {
+  const AttnArgs& a = c.a;
+  const int tok = r / a.group;
+  const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(g.s.q_begin + tok) * a.q_rs + (int64_t)(g.hk * a.group + r - tok * a.group) * a.q_hs;
+  const int32_t* bt_row = a.paged ? a.block_table + (int64_t)g.b * a.bt_stride : nullptr;
+  const uint8_t* k = reinterpret_cast<const uint8_t*>(a.k) + cache_row(c, bt_row, g.s.k_begin, key, a.k_rs, a.k_bs) + (int64_t)g.hk * a.k_hs;
+  float sum = 0.f;
+  for (int d = 0; d < HD; ++d) sum = fmaf(Cvt<T>::to_f32(q[d]), Pair<__half>::unpack(fp8x2_to_f16x2<KIND>(k[d])).x, sum);
+  return sum * (cache_scale(c.k_scale, c.ks_batch, c.ks_head, g.b, g.hk) * a.scale_log2);
 }
 
 template <typename T, int KIND, int RP, int HD>
@@ -636,8 +708,17 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
         }
         bool raise = false;
 #pragma unroll
-        for (int r = 0; r < RP; ++r) raise = raise || x[r] > m_ref[r] + kRaise;
+        for (int r = 0; r < RP; ++r)   // where keys may be infinite, a NaN too
+          raise = raise || (KIND == kCacheE5M2 ? !(x[r] <= m_ref[r] + kRaise) : x[r] > m_ref[r] + kRaise);
         if (softmax_any(raise)) {
+          if constexpr (KIND == kCacheE5M2) {
+#pragma unroll
+            for (int r = 0; r < RP; ++r)   // rows of Q that hold a NaN or an infinity keep theirs
+              if (r < seg.rows && x[r] != x[r] && pre[r] == pre[r]) {
+                const Segment copy = seg;
+                x[r] = whole_score<T, KIND, HD>(c, copy, r, j0 + tid);
+              }
+          }
           // exact maxima of the tile, shared by the four warps
 #pragma unroll
           for (int r = 0; r < RP; ++r) {
@@ -737,6 +818,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
       if (ok) {
         int tok = 0, in = 0;
         float my_l = 0.f, my_m = 0.f;       // of row tid
+        uint32_t odd = 0;                   // bit 16 m + r: dim m * 128 + tid of row r is a NaN, and its scores are not
 #pragma unroll
         for (int r = 0; r < RP; ++r) {
           if (r < seg.rows) {
@@ -752,6 +834,7 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
               v = l == 0.f ? 0.f : v * (C::k8 ? 1.f / kPScale : 1.f) * (v_scale / l);
               const int d = m * 128 + tid;
               if (HD == 64 && tid >= 64) continue;
+              if (C::kPieces && v != v && l == l) odd |= 1u << (16 * m + r);
               if (whole)
                 reinterpret_cast<T*>(a.out)[qtok * a.o_rs + (int64_t)h * a.o_hs + d] = Cvt<T>::from_f32(v);
               else
@@ -766,6 +849,10 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             in = 0;
             ++tok;
           }
+        }
+        if (C::kPieces && odd != 0) {
+          const Segment copy = seg;         // keeps seg itself in registers
+          write_infinities<T, KIND, RP, HD>(da, copy, whole ? -1 : part, odd, v_scale);
         }
         if (tid < seg.rows && (!whole || a.lse)) {
           const float lse2 = my_l == 0.f ? -INFINITY : my_m + log2f(my_l);

@@ -429,7 +429,8 @@ FG_API int fg_gather_cache_flash(const fg_cache_gather_params* p, void* stream);
  * j >= p - window_left or j < sink_tokens.  Rows with no visible key produce 0 and an LSE of +inf; rows of q outside
  * [cu_seqlens_q[0], cu_seqlens_q[batch]) leave out and lse as they were.  K/V that no query of a 64-key tile's
  * readers sees take no part, whatever they hold (freed pages under a window); a NaN or infinity in a V row that
- * some query of a tile sees can reach the others of that tile.
+ * some query of a tile sees can reach the others of that tile.  Infinities that a query sees count: among its V values they are
+ * its output (NaN when both signs meet), a score of -inf takes its key out, +inf leaves no number.
  * k_scale / v_scale: what a cached value is multiplied by, batch and head strides in elements (0 = shared), NULL = 1;
  * they must be NULL for a 16-bit cache.
  * workspace: at least fg_flash_attn_cache_workspace_bytes(p) bytes of 16-byte aligned device memory that no other call in

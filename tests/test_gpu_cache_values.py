@@ -101,3 +101,81 @@ def test_outlying_channels_give_the_same_in_every_form(fg):
     few, many = (call(fg, [1, 1, 1], bound, q, rows, E4M3, scale=scale)[1] for bound in (0, 10 ** 6))
     # 2^-27 of 4096 in 128 channels, with keys of 4.5 standard deviations at most; beside it the sums' own roundings
     assert ((few - many).abs() <= 128 * 2.0 ** -15 * 4.5 * 128 ** -0.5 + 1e-4).all()
+
+
+@pytest.mark.parametrize("q_lens, bound", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 256, 72])
+@pytest.mark.parametrize("dtype, cache", [(BF16, E5M2), (FP16, E5M2), (BF16, BF16), (FP16, FP16)])
+def test_infinite_values_that_every_query_sees(fg, dtype, cache, dim, q_lens, bound):
+    """An infinity among the V values of a channel is that channel's output, two of opposite signs or a NaN are a NaN, and the
+    other channels are what they are."""
+    g = gen(dim)
+    window, sinks = ((-1, -1), 0) if cache in TOP else ((10 ** 5, 0), 4)
+    if bound == 0 and cache not in TOP:
+        window = (600, 0)         # shorter than the longest sequence, longer than every chunk
+    scale = torch.tensor([0.01 if cache in TOP else 1.0], device=DEV)
+    rows = random_rows(g, 2, dim, cache, scale)
+    clean = [[t.clone() for t in pair] for pair in rows]
+    for b, (_, v) in enumerate(rows):     # keys 0 to 3 and the first new token's own are seen by every query
+        last = LENS[b] - q_lens[b]
+        poke(v, (1, 0, 5), math.inf)
+        poke(v, (last, 0, 9), -math.inf)
+        poke(v, (2, 1, 11), math.inf)
+        poke(v, (3, 1, 11), math.inf)
+        poke(v, (2, 1, 20), math.inf)
+        poke(v, (last, 1, 20), -math.inf)
+        poke(v, (0, 1, 21), math.nan)
+    q = randn(g, sum(q_lens), 8, dim).to(dtype)
+    out, lse = call(fg, q_lens, bound, q, rows, cache, window=window, sinks=sinks, scale=scale if cache in TOP else None)
+    want, wlse, tol, lse_tol = attention(q_lens, LENS, q, clean, [scale] * 3, [scale] * 3, dim ** -0.5, True, window, sinks, 0.0,
+                                         dtype, cache)
+    odd = torch.zeros((8, dim), dtype=torch.float64, device=DEV)
+    odd[:4, 5], odd[:4, 9], odd[4:, 11] = math.inf, -math.inf, math.inf
+    odd[4:, 20:22] = math.nan
+    want = want + odd
+    ok = odd == 0
+    assert torch.equal(out[:, ~ok].nan_to_num(7.0), want[:, ~ok].to(dtype).nan_to_num(7.0))
+    assert ((out[:, ok].double() - want[:, ok]).abs() <= tol[:, ok]).all()
+    assert ((lse.double() - wlse).abs() <= lse_tol).all()
+
+
+@pytest.mark.parametrize("q_lens, bound", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_infinite_keys(fg, dtype, dim, q_lens, bound):
+    """A score of -inf takes its key out; +inf, or both in one product, leave no number."""
+    g = gen(dim + 1)
+    scale = torch.tensor([0.01], device=DEV)
+    rows = random_rows(g, 2, dim, E5M2, scale)
+    q = randn(g, sum(q_lens), 8, dim)
+    q[:, :, 5] = q[:, :, 5].abs() + 0.1
+    q[:, :, 6] = -q[:, :, 6].abs() - 0.1
+    q = q.to(dtype)
+    clean = [[t.clone() for t in pair] for pair in rows]
+    for b, (k, v) in enumerate(rows):
+        for j, channel, value in ((2, 5, -math.inf), (30, 6, math.inf), (LENS[b] - q_lens[b], 5, -math.inf)):
+            poke(k, (j, 0, channel), value)
+            # in the definition: a key so small that its probability is below any rounding
+            poke(clean[b][0], (j, 0, channel), -57344.0 if channel == 5 else 57344.0)
+        poke(k, (1, 1, 6), -math.inf)
+    out, lse = call(fg, q_lens, bound, q, rows, E5M2, scale=scale)
+    ends = torch.tensor(q_lens).cumsum(0).tolist()
+    at = 0
+    for b, end in enumerate(ends):
+        # keys far below, with their part of the sum's rounding error left out of the bound
+        k, v = clean[b][0].double() * 0.01, clean[b][1].double() * 0.01
+        k, v = k[:, 0], v[:, 0]
+        p = torch.arange(end - at, device=DEV).view(-1, 1) + LENS[b] - (end - at)
+        for h in range(4):
+            qq = q[at:end, h].double()
+            a = (qq @ k.T * dim ** -0.5).masked_fill(torch.arange(LENS[b], device=DEV) > p, -math.inf)
+            keep = k.abs().amax(-1) < 500
+            a[:, ~keep] = -math.inf
+            w = torch.softmax(a, -1)
+            size = w @ v.abs()
+            ds = (dim + 8) * 2.0 ** -22 * dim ** -0.5 * (qq.abs() @ k[keep].abs().T).amax(-1, keepdim=True)
+            tol = U[dtype] * (w @ v).abs() + (2.0 ** -11 + 2 * ds + 2.0 ** -16) * size + LENS[b] * 2.0 ** -25 * v.abs().max()
+            assert ((out[at:end, h].double() - w @ v).abs() <= tol).all()
+            assert ((lse[h, at:end].double() - torch.logsumexp(a, -1)).abs() <= 2 * ds[:, 0] + 2.0 ** -12).all()
+        at = end
+    assert out[:, 4:].isnan().all() and lse[4:].isnan().all()
