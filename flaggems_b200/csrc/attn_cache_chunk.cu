@@ -32,6 +32,8 @@
 // Two 2048-token prompts at head dim 256 621 us, at 64 234 us (mma.sync: 1654 and 343).
 // Over 8-bit caches bf16 queries are brought to fp16, each row by a power of two, by the softmax warps before an item's first
 // step.
+// P is rounded once: to fp16 (2^-12 of itself, or 2^-32 of its row's largest), and over a bf16 cache to bf16 (2^-9): a second piece, which
+// the decode kernel has, would double the products P V, and those bound the step.
 // TMEM columns: tile t has its scores at t*128 (64 columns), two probability buffers at t*128+64 and +96, its output at
 // 256+t*128.  Every wait is an mbarrier wait with a limit.
 #include "attn_cache_common.cuh"
@@ -182,6 +184,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   constexpr bool kConvQ = !std::is_same<T, M>::value;
   constexpr bool kWiden = KIND != kCache16;
   constexpr int THREADS = threads_of(KIND);
+  constexpr float kShift = p_shift<M>(kRescaleThreshold);
   using G = Shape<HD>;
   constexpr int PIECES = G::PIECES, TILE_BYTES = G::TILE_BYTES, UNIT = G::UNIT, STAGES = G::STAGES;
   static_assert(!kWiden || HD == 128, "the widening warps take rows of 128");
@@ -687,7 +690,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           l_run *= f;
         }
         if (raise) m_used = m_tile;
-        const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+        const float neg_m = m_used == -INFINITY ? 0.f : kShift - m_used;
         if constexpr (!kWiden) {
           // V rows of this step that no row of the item sees must not reach the products: zeroed in place, by each tile's
           // warps for themselves (the other tile writes the same zeros)
@@ -772,7 +775,7 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         __syncwarp();
       }
       if (!whole || (valid && a.lse)) {
-        const float lse2 = l_run == 0.f ? -INFINITY : m_used + log2f(l_run);
+        const float lse2 = l_run == 0.f ? -INFINITY : m_used - kShift + log2f(l_run);
         if (!whole)
           pa.part_lse[part * BM + r] = lse2;
         else

@@ -8,12 +8,16 @@
 // The 8-bit types are subsets of fp16 and the products run in fp16 with fp32 accumulators: exact for K and V, and for
 // fp16 queries.  A bf16 query row is multiplied by a power of two that brings its largest value to [2^14, 2^15): its
 // 8-bit significands stay exact down to 2^-31 of the row's largest, and the power is taken out of the scores in fp32.
-// Probabilities are rounded to fp16 (2^-12), four times finer than bf16 would be; their sum is taken before that.
+// Probabilities are rounded to fp16 (2^-12 of themselves; four times finer than bf16, 2^-9, which a bf16 cache takes), and their
+// sum is taken before that.  fp16 ends at 2^-25: they are multiplied by a power of two that takes the largest to 2^15, which the
+// division by the sum takes out, so that many small ones beside a first token that draws all attention are not lost.
 //
 // `group` query heads share a KV head.  The rows of a tile are (token, head of the group) pairs, head fastest, so that
 // every K/V byte is fetched once for all of them.
 #pragma once
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "attn_common.cuh"
 #include "fp8.cuh"
@@ -121,6 +125,12 @@ __device__ __forceinline__ void row_power(float top, float& up, float& down) {
   const int k = min(14 - (max(e, 1) - 127), 112);
   up = __int_as_float((127 + k) << 23);
   down = __int_as_float((127 - k) << 23);
+}
+
+// log2 of what probabilities of at most 2^most are multiplied by before they are rounded to M.
+template <typename M>
+__host__ __device__ constexpr float p_shift(float most) {
+  return std::is_same<M, __half>::value ? 15.f - most : 0.f;
 }
 
 // Kernel families of fg_flash_attn_cache.

@@ -63,6 +63,7 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   using L = Tile<KIND, DP>;
   using M = typename std::conditional<KIND == kCache16, T, __half>::type;   // type of the products
   constexpr int BN = L::BN, KPW = L::KPW, STAGES = L::STAGES;
+  constexpr float kShift = p_shift<M>(0.f);
   const CacheAttnArgs& c = da.c;
   const AttnArgs& a = c.a;
   extern __shared__ uint8_t smem_raw[];
@@ -301,11 +302,12 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
       }
-      float corr[2], msafe[2];
+      float corr[2], mp[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        msafe[r] = mx[r] == -INFINITY ? 0.f : mx[r];
-        corr[r] = ex2(m_run[r] - msafe[r]);
+        const float msafe = mx[r] == -INFINITY ? 0.f : mx[r];
+        corr[r] = ex2(m_run[r] - msafe);
+        mp[r] = msafe - kShift;
         m_run[r] = mx[r];
         l_run[r] *= corr[r];
       }
@@ -321,8 +323,8 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       uint32_t pf[KPW / 16][4];
 #pragma unroll
       for (int nt = 0; nt < KPW / 8; ++nt) {
-        const float p0 = ex2(sacc[nt][0] - msafe[0]), p1 = ex2(sacc[nt][1] - msafe[0]);
-        const float p2 = ex2(sacc[nt][2] - msafe[1]), p3 = ex2(sacc[nt][3] - msafe[1]);
+        const float p0 = ex2(sacc[nt][0] - mp[0]), p1 = ex2(sacc[nt][1] - mp[0]);
+        const float p2 = ex2(sacc[nt][2] - mp[1]), p3 = ex2(sacc[nt][3] - mp[1]);
         l_run[0] += p0 + p1;
         l_run[1] += p2 + p3;
         pf[nt >> 1][(nt & 1) * 2 + 0] = pack_pair<M>(p0, p1);
@@ -422,7 +424,7 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
                 pack_pair<T>(x * inv, y * inv);
         }
         if (d == 0) {
-          const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+          const float lse2 = l == 0.f ? -INFINITY : m - kShift + log2f(l);
           if (a.num_splits > 1)
             a.ws_lse[((int64_t)split * a.H + h) * a.total_q + qtok] = lse2;
           else if (a.lse)

@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(NTHREADS) attn_cache_generic_kernel(CacheAttnA
   float l_run[2] = {0.f, 0.f};
   const int row_in_tile = warp * 16 + (lane >> 2);  // + 8 for the second row
   const float ksc = cache_scale(c.k_scale, c.ks_batch, c.ks_head, b, hk);
+  constexpr float kShift = p_shift<M>(0.f);
   float pre[2];                                      // takes the accumulator to the scores
   RowMask mask[2];
   __syncthreads();                                   // sDown
@@ -236,11 +237,12 @@ __global__ void __launch_bounds__(NTHREADS) attn_cache_generic_kernel(CacheAttnA
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
     }
-    float corr[2], msafe[2];
+    float corr[2], mp[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      msafe[r] = mx[r] == -INFINITY ? 0.f : mx[r];
-      corr[r] = exp2f(m_run[r] - msafe[r]);  // m_run == -inf -> 0
+      const float msafe = mx[r] == -INFINITY ? 0.f : mx[r];
+      corr[r] = exp2f(m_run[r] - msafe);  // m_run == -inf -> 0
+      mp[r] = msafe - kShift;
       m_run[r] = mx[r];
       l_run[r] *= corr[r];
     }
@@ -254,8 +256,8 @@ __global__ void __launch_bounds__(NTHREADS) attn_cache_generic_kernel(CacheAttnA
     uint32_t pf[BN / 16][4];  // P as A fragments (k = kv index)
 #pragma unroll
     for (int nt = 0; nt < BN / 8; ++nt) {
-      const float p0 = exp2f(sacc[nt][0] - msafe[0]), p1 = exp2f(sacc[nt][1] - msafe[0]);
-      const float p2 = exp2f(sacc[nt][2] - msafe[1]), p3 = exp2f(sacc[nt][3] - msafe[1]);
+      const float p0 = exp2f(sacc[nt][0] - mp[0]), p1 = exp2f(sacc[nt][1] - mp[0]);
+      const float p2 = exp2f(sacc[nt][2] - mp[1]), p3 = exp2f(sacc[nt][3] - mp[1]);
       l_run[0] += p0 + p1;
       l_run[1] += p2 + p3;
       pf[nt >> 1][(nt & 1) * 2 + 0] = pack_pair<M>(p0, p1);
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(NTHREADS) attn_cache_generic_kernel(CacheAttnA
     const float inv = l_run[r] == 0.f ? 0.f : vsc / l_run[r];
     const int tok = row / a.group, h = hk * a.group + row - tok * a.group;
     const int64_t qtok = s.q_begin + tok;
-    const float lse2 = l_run[r] == 0.f ? -INFINITY : m_run[r] + log2f(l_run[r]);
+    const float lse2 = l_run[r] == 0.f ? -INFINITY : m_run[r] - kShift + log2f(l_run[r]);
     if (a.num_splits > 1) {
       float* out = a.ws_o + (((int64_t)split * a.total_q + qtok) * a.H + h) * a.D;
 #pragma unroll

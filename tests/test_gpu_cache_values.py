@@ -179,3 +179,42 @@ def test_infinite_keys(fg, dtype, dim, q_lens, bound):
             assert ((lse[h, at:end].double() - torch.logsumexp(a, -1)).abs() <= 2 * ds[:, 0] + 2.0 ** -12).all()
         at = end
     assert out[:, 4:].isnan().all() and lse[4:].isnan().all()
+
+
+@pytest.mark.parametrize("q_lens, bound", FORMS)
+@pytest.mark.parametrize("gap", [16.0, 18.0])
+@pytest.mark.parametrize("dim", [64, 128, 256, 72])
+@pytest.mark.parametrize("dtype, cache", [(BF16, E4M3), (FP16, E5M2), (FP16, FP16)])
+def test_small_probabilities_beside_a_first_token(fg, dtype, cache, dim, gap, q_lens, bound):
+    """The first token draws nearly all attention and its value is zero, as trained models have it: the output is the sum of many
+    probabilities of about e^-gap.  A probability may be off by 2^-11 of itself or 2^-32 of the row's largest."""
+    g = gen(int(gap) + dim)
+    eight = cache in TOP
+    window, sinks = ((-1, -1), 0) if eight else ((600, 0), 4)
+    scale = torch.tensor([2.0 ** -6 if eight else 1.0], device=DEV)
+    rows = random_rows(g, 2, dim, cache, scale)
+    u = torch.zeros(dim, device=DEV)
+    u[:8] = 1.0                        # the first token's direction: eight channels that the other keys leave alone
+    for k, v in rows:
+        poke(k, (slice(1, None), slice(None), slice(0, 8)), 0.0)
+        poke(k, 0, 0.0)
+        poke(v, 0, 0.0)
+        k0 = 4.0 / scale.item()
+        poke(k, (0, slice(None), slice(0, 8)), k0)
+    q = 0.5 * randn(g, sum(q_lens), 8, dim)
+    q[:, :, :8] = gap * dim ** 0.5 / (8 * 4.0)
+    q = q.to(dtype)
+    out, lse = call(fg, q_lens, bound, q, rows, cache, window=window, sinks=sinks, scale=scale if eight else None)
+    want, wlse, tol, lse_tol = attention(q_lens, LENS, q, rows, [scale] * 3, [scale] * 3, dim ** -0.5, True, window, sinks, 0.0,
+                                         dtype, cache)
+    # The outputs are about 2^-18.  fp16 values below 2^-14 are multiples of 2^-24: rounding one to them moves it by up to 2^-25,
+    # whatever its size, which the share of the value in the bound does not hold.
+    tol += 2.0 ** -25 if dtype == FP16 else 0.0
+    at = 0
+    for b, n in enumerate(q_lens):     # the bound of test_gpu_cache_fp8 takes 2^-25 a key; here it is 2^-32
+        top = (rows[b][1].double() * scale.double()).abs().max()
+        tol[at:at + n] -= LENS[b] * (2.0 ** -25 - 2.0 ** -32) * top
+        at += n
+    worst = ((out.double() - want).abs() / tol).max().item()
+    assert worst <= 1.0, f"error {worst:.3g} of the bound"
+    assert ((lse.double() - wlse).abs() <= lse_tol).all()
