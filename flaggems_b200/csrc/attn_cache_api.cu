@@ -33,6 +33,12 @@ int64_t least_decode(int64_t rows, int64_t head_dim) {
   return rows <= 4 ? 600 : rows <= 8 ? 1800 : 4000;
 }
 
+// Most bytes of partial results of the mma.sync decode form, whose splits go by max_seqlen_k: a captured step's bound may be far
+// above its contexts, and ranges that no sequence reaches cost an empty CTA and a place in the workspace each.  256 decodes of up to
+// 8192 keys (soft-capped, 32 heads over 8) under a bound of 131072 in ranges of 1024 keys, 541 MB, and 16384 keys, 34 MB: 1732 and
+// 894 us; under a bound of 10^6 7209 and 898 us.
+constexpr int64_t kMostSplitBytes = 64ll << 20;
+
 // Keys that one sequence can have visible to one row tile: everything, or window and first tokens.
 int64_t most_keys(const fg_attn_cache_params* p, int64_t tokens) {
   const fg_attn_params& b = p->base;
@@ -121,6 +127,8 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
     const int64_t keys = most_keys(p, b.max_seqlen_q), ctas = b.num_heads_k * b.batch;
     int64_t chunk = 1024;
     while (chunk > 256 && ctas * ((keys + chunk - 1) / chunk) < (int64_t)sms * 2 * 8) chunk >>= 1;
+    const int64_t split_bytes = (b.total_q > 0 ? b.total_q : 1) * b.num_heads * (b.head_dim + 1) * 4;
+    while (chunk < keys && (keys + chunk - 1) / chunk > kMostSplitBytes / split_bytes) chunk <<= 1;
     plan.tiles_per_split = (int)(chunk / bn);
     plan.splits = (int)((keys + chunk - 1) / chunk);
     if (plan.splits < 1) plan.splits = 1;

@@ -101,6 +101,21 @@ def test_workspace_goes_by_what_is_visible():
         assert 0 < windowed < long // 5 and windowed == need(max_seqlen_k=10 ** 6, window_left=2047, sink_tokens=4, **size)
 
 
+def test_workspace_of_the_split_decode_form_is_bounded():
+    """Soft-capping and odd head dims split by max_seqlen_k: large batches with a bound far above their contexts stay small."""
+    need = lambda **kw: _lib.load().fg_flash_attn_cache_workspace_bytes(ctypes.byref(params(**kw)))
+    path = lambda **kw: _lib.load().fg_flash_attn_cache_path(ctypes.byref(params(**kw)))
+    for batch in (1, 4, 64, 256, 4096):
+        for heads, heads_k in ((8, 2), (32, 8), (128, 8)):
+            for form in (dict(softcap=50.0), dict(head_dim=96), dict(head_dim=256, cache_dtype=_lib.FG_BF16, window_left=10 ** 5)):
+                for bound in (1000, 131072, 10 ** 6, 10 ** 7):
+                    size = dict(batch=batch, total_q=batch, num_heads=heads, num_heads_k=heads_k, max_seqlen_k=bound, **form)
+                    assert path(**size) == 2 and need(**size) <= 64 * 2 ** 20
+                    small = dict(size, max_seqlen_k=min(bound, 8000))
+                    assert need(**size) > 0 or need(**small) == 0 or batch * heads >= 4096   # few rows are split all the same
+    assert need(total_q=0, softcap=50.0, max_seqlen_k=10 ** 6) == 0
+
+
 def test_path_by_sizes():
     path = lambda **kw: _lib.load().fg_flash_attn_cache_path(ctypes.byref(params(**{"max_seqlen_k": 10 ** 5, **kw})))
     assert path(max_seqlen_k=1000) == 2      # too few tiles of keys

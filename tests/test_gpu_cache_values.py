@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_cache_fp8 import DEV, E4M3, E5M2, TOP, U, attention, gen, quantise, randn
+from test_gpu_cache_fp8 import DEV, E4M3, E5M2, TOP, U, attention, check, gen, quantise, randn
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -218,3 +218,11 @@ def test_small_probabilities_beside_a_first_token(fg, dtype, cache, dim, gap, q_
     worst = ((out.double() - want).abs() / tol).max().item()
     assert worst <= 1.0, f"error {worst:.3g} of the bound"
     assert ((lse.double() - wlse).abs() <= lse_tol).all()
+
+
+@pytest.mark.parametrize("kw", [dict(dim=128, softcap=30.0), dict(dim=96), dict(dim=256, cache=BF16, window=(10 ** 5, 0), sinks=4)])
+def test_long_ranges_of_a_large_bound(fg, kw):
+    """So many rows that the ranges of the keys grow with the bound: sequences shorter than one, longer, and as long as several."""
+    kw = {"cache": E4M3, **kw}
+    lens = [1 + (i * 977) % 3000 for i in range(44)] + [40000, 16384, 16385, 0]
+    check(fg, [1] * 48, lens, 32, 8, page=16, dtype=BF16, bound=10 ** 6, **kw)
