@@ -85,7 +85,7 @@ class AttnCacheParams(C.Structure):
         + [(n, C.c_int64) for n in (
             "k_scale_batch_stride", "k_scale_head_stride", "v_scale_batch_stride", "v_scale_head_stride",
             "sink_tokens", "block_table_cols")]
-        + [(n, C.c_int32) for n in ("cache_dtype", "reserved")]
+        + [(n, C.c_int32) for n in ("cache_dtype", "flags")]
     )
 
 
@@ -95,6 +95,7 @@ CACHE_WRITE = struct.Struct("=7Q12q2i")
 CACHE_GATHER = struct.Struct("=9Q15q2i")
 ATTN_CACHE = struct.Struct("=11Q29q2d4i2Q6q2i")
 WORKSPACE = struct.Struct("=Qq")   # its pointer and bytes, at byte 80 of ATTN_CACHE
+CACHE_NO_COPY = struct.pack("=i", 1)   # the flags, at the end of ATTN_CACHE
 
 
 class GemmPlan(C.Structure):

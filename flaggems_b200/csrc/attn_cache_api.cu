@@ -110,7 +110,7 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
       const int64_t seen = (p->sink_tokens + 63) / 64 * 64 + (b.window_left + right + b.max_seqlen_q + 2 * 63) / 64 * 64;
       if (seen < rows) rows = seen;
     }
-    if (is_fp8(p->cache_dtype) && (b.max_seqlen_q * group >= 1024 || b.head_dim != 128) && rows > 0 &&
+    if (!(p->flags & FG_CACHE_NO_COPY) && is_fp8(p->cache_dtype) && (b.max_seqlen_q * group >= 1024 || b.head_dim != 128) && rows > 0 &&
         b.batch * rows <= (1ll << 30) / (4 * b.head_dim * b.num_heads_k))
       plan.dense = rows;
     plan.bytes =
@@ -174,6 +174,7 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
              "flash_attn_cache: the cache must hold the type of the queries or an 8-bit type");
   FG_REQUIRE(is_fp8(p->cache_dtype) || (p->k_scale == nullptr && p->v_scale == nullptr),
              "flash_attn_cache: scales belong to an 8-bit cache");
+  FG_REQUIRE((p->flags & ~FG_CACHE_NO_COPY) == 0, "flash_attn_cache: unknown flags %d", p->flags);
   FG_REQUIRE(b.batch >= 0 && b.total_q >= 0, "flash_attn_cache: negative size");
   FG_REQUIRE(b.num_heads > 0 && b.num_heads_k > 0, "flash_attn_cache: head counts must be positive");
   FG_REQUIRE(b.num_heads % b.num_heads_k == 0, "Number of heads in key/value must divide number of heads in query");

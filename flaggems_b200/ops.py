@@ -325,7 +325,10 @@ def flash_attn_varlen_func(
     ``(batch, nheads_k)``, None is 1.  They are ignored for 16-bit K/V, as in the reference.
     With a left window, the first ``sink_tokens`` keys of each sequence stay visible beside
     it (the causal mask still holds).  Neither goes with ALiBi.  Rows of ``q`` outside the
-    sequences leave ``out`` as it was in these forms.
+    sequences leave ``out`` as it was in these forms; ``max_seqlen_k`` may be larger than the
+    longest sequence but not smaller (longer ones are cut to it), and ``q`` stays 16-bit
+    (``q_descale`` is accepted and ignored).  Their workspace, up to about 1 GiB for long chunks
+    over 8-bit K/V, is allocated for the call; without memory for it the call runs slower.
     """
     logger.debug("GEMS FLASH_ATTN_VARLEN_FUNC")
     assert cu_seqlens_k is not None or seqused_k is not None, "cu_seqlens_k or seqused_k must be provided"
@@ -457,6 +460,22 @@ def _descale(what, scale, batch, heads, dev):
                        f"({batch}, {heads}), got {tuple(scale.shape)}")
 
 
+def _cache_workspace(lib, params, nbytes, dev):
+    """``(buffer, parameter block that names it)``.  The buffer is the call's own: the allocator keeps it from other streams, and a
+    captured graph keeps its own.  Where memory is short the call goes on with less: without the 16-bit copy that a long chunk
+    makes of an 8-bit store, then without a workspace."""
+    block, need, last = params, nbytes, 0
+    while need > 0 and need != last:
+        try:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            return ws, block[:80] + _lib.WORKSPACE.pack(ws.data_ptr(), need) + block[96:]
+        except torch.OutOfMemoryError:
+            logger.warning("flash_attn_varlen_func: no memory for a workspace of %d bytes, going on with less", need)
+        block, last = params[:-4] + _lib.CACHE_NO_COPY, need
+        need = lib.fg_flash_attn_cache_workspace_bytes(block)
+    return None, block
+
+
 def _flash_attn_cache(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seqlens_k, seqused_k, softmax_scale, causal,
                       window, softcap, alibi_slopes, block_table, return_softmax_lse, out, k_descale, v_descale,
                       sink_tokens):
@@ -522,9 +541,7 @@ def _flash_attn_cache(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seql
     with _lib.on_device(dev):
         nbytes = lib.fg_flash_attn_cache_workspace_bytes(params)
         if nbytes > 0:
-            # a buffer of the call's own: the allocator keeps it from other streams, and a captured graph keeps its own
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            params = params[:80] + _lib.WORKSPACE.pack(ws.data_ptr(), nbytes) + params[96:]
+            ws, params = _cache_workspace(lib, params, nbytes, dev)
         rc = lib.fg_flash_attn_cache(params, _lib.raw_stream(dev.index))
     if rc < 0:
         _lib.check(rc)

@@ -437,6 +437,10 @@ FG_API int fg_gather_cache_flash(const fg_cache_gather_params* p, void* stream);
  * flight uses, or NULL to forbid splitting the keys over CTAs.  Two captured graphs that may run at the same time
  * need workspaces of their own.
  * ---------------------------------------------------------------------- */
+/* flags: do without the 16-bit copy of an 8-bit store's visible rows, which long chunks otherwise make in the workspace (most of its
+ * bytes, up to 1 GiB); slower, for a caller that is short of memory */
+enum { FG_CACHE_NO_COPY = 1 };
+
 typedef struct {
   fg_attn_params base;
   const float* k_scale; /* may be NULL */
@@ -446,7 +450,7 @@ typedef struct {
   int64_t sink_tokens;
   int64_t block_table_cols; /* entries of a block table row (paged form) */
   int32_t cache_dtype;
-  int32_t reserved;
+  int32_t flags; /* 0 or FG_CACHE_NO_COPY */
 } fg_attn_cache_params;
 FG_API int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream);
 FG_API int64_t fg_flash_attn_cache_workspace_bytes(const fg_attn_cache_params* p);

@@ -101,6 +101,47 @@ def test_workspace_goes_by_what_is_visible():
         assert 0 < windowed < long // 5 and windowed == need(max_seqlen_k=10 ** 6, window_left=2047, sink_tokens=4, **size)
 
 
+def test_long_chunks_without_the_widened_copy():
+    need = lambda **kw: _lib.load().fg_flash_attn_cache_workspace_bytes(ctypes.byref(params(**kw)))
+    path = lambda **kw: _lib.load().fg_flash_attn_cache_path(ctypes.byref(params(**kw)))
+    long = dict(max_seqlen_q=256, total_q=1000, max_seqlen_k=6400)
+    assert need(flags=1, **long) == need(cache_dtype=_lib.FG_BF16, **long) < need(**long) and path(flags=1, **long) == 1
+    long["head_dim"] = 64
+    assert path(**long) == 1 and path(flags=1, **long) == 0 and need(flags=1, **long) < need(**long)
+    with pytest.raises(RuntimeError, match="unknown flags"):
+        _lib.check(_lib.load().fg_flash_attn_cache(ctypes.byref(params(flags=6)), None))
+
+
+def test_no_memory_for_the_workspace(monkeypatch):
+    """What the call gets when the allocation fails: the form without the copy, then none."""
+    from flaggems_b200 import ops
+    lib = _lib.load()
+    block = bytes(params(max_seqlen_q=256, total_q=1000, max_seqlen_k=6400))
+    full = lib.fg_flash_attn_cache_workspace_bytes(block)
+    asked, limit = [], [0]
+    real = torch.empty
+
+    def empty(n, dtype, device):
+        asked.append(n)
+        if n > limit[0]:
+            raise torch.OutOfMemoryError("no memory")
+        return real(n, dtype=dtype, device="cpu")
+
+    monkeypatch.setattr(torch, "empty", empty)
+    for limit[0], sizes in ((full, 1), (full - 1, 2), (0, 2)):
+        asked.clear()
+        ws, got = ops._cache_workspace(lib, block, full, "cuda")
+        p = _lib.AttnCacheParams.from_buffer_copy(got)
+        assert len(asked) == sizes and asked[0] == full and p.flags == sizes - 1
+        small = lib.fg_flash_attn_cache_workspace_bytes(block[:-4] + _lib.CACHE_NO_COPY)
+        assert small < full and asked[1:] == [small][:sizes - 1]
+        if limit[0] == 0:
+            assert ws is None and not p.base.workspace and p.base.workspace_bytes == 0
+        else:
+            assert p.base.workspace == ws.data_ptr() and p.base.workspace_bytes == ws.numel() == asked[-1]
+        assert got[:80] == block[:80] and got[96:-4] == block[96:-4]
+
+
 def test_workspace_of_the_split_decode_form_is_bounded():
     """Soft-capping and odd head dims split by max_seqlen_k: large batches with a bound far above their contexts stay small."""
     need = lambda **kw: _lib.load().fg_flash_attn_cache_workspace_bytes(ctypes.byref(params(**kw)))

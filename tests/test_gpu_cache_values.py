@@ -226,3 +226,20 @@ def test_long_ranges_of_a_large_bound(fg, kw):
     kw = {"cache": E4M3, **kw}
     lens = [1 + (i * 977) % 3000 for i in range(44)] + [40000, 16384, 16385, 0]
     check(fg, [1] * 48, lens, 32, 8, page=16, dtype=BF16, bound=10 ** 6, **kw)
+
+
+@pytest.mark.parametrize("limit", [0, 96 << 20])
+@pytest.mark.parametrize("q_lens, dim", [([600, 1, 0, 130], 128), ([600, 1, 0, 130], 64), ([300, 1, 20, 7], 256), ([1, 1, 1, 1], 128)])
+def test_calls_that_find_no_memory_for_their_workspace(fg, monkeypatch, q_lens, dim, limit):
+    """The allocator is out of memory beyond `limit` bytes: the same results from the forms that need less."""
+    real, refused = torch.empty, []
+
+    def empty(*args, **kw):
+        if kw.get("dtype") == torch.uint8 and args[0] > limit:
+            refused.append(args[0])
+            raise torch.OutOfMemoryError("no memory")
+        return real(*args, **kw)
+
+    monkeypatch.setattr(torch, "empty", empty)
+    check(fg, q_lens, [900, 700, 33, 130], 8, 4, dim, 16, BF16, E4M3, bound=40000)
+    assert refused or (limit and max(q_lens) == 1)
