@@ -228,8 +228,9 @@ def stream_ptr(device: torch.device) -> int:
 
 
 _HERE = contextlib.nullcontext()
-# the stream handle without a torch.cuda.Stream object around it
-raw_stream = torch._C._cuda_getCurrentRawStream
+# the stream handle without a torch.cuda.Stream object around it, where this build of torch has the call
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def on_device(device: torch.device):

@@ -2,6 +2,8 @@
 and a restatement of the tile runs that the attention kernels walk."""
 import ctypes
 import re
+import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -258,3 +260,14 @@ def test_gather_stays_inside_the_cache():
                 assert got is None or (0 <= got[0] < 4 and 0 <= got[1] < 16)
     assert gathered_row(21, [0, 5, 40], [0, 3], [[9, 9], [2, 1]], 16, 4) == (1, 3)
     assert gathered_row(4, [0, 5, 5, 40], None, [[1], [2], [3]], 16, 4) == (1, 4)
+
+
+def test_import_without_the_private_stream_binding():
+    """A torch build without it still imports the package, and the stream comes from the public call."""
+    code = ("import torch; del torch._C._cuda_getCurrentRawStream\n"
+            "import flaggems_b200._lib as lib\n"
+            "torch.cuda.current_stream = lambda index: type('Stream', (), {'cuda_stream': 40 + index})\n"
+            "assert lib.raw_stream(2) == 42")
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
