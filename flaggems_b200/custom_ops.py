@@ -30,6 +30,7 @@ SCHEMAS = {
         "gather_cache_flash(Tensor key_cache, Tensor value_cache, Tensor(a!) key, Tensor(b!) value, "
         "Tensor block_table, Tensor cu_seqlens, str kv_cache_dtype, Tensor? k_scale=None, Tensor? v_scale=None, "
         "Tensor? seq_starts=None) -> ()",
+    # as in the reference's extension, and the argument of the windowed form behind its own
     "flash_attn_varlen_func":
         "flash_attn_varlen_func(Tensor q, Tensor k, Tensor v, SymInt max_seqlen_q, Tensor cu_seqlens_q, "
         "SymInt max_seqlen_k, Tensor? cu_seqlens_k=None, Tensor? seqused_k=None, Tensor? q_v=None, "
@@ -37,7 +38,7 @@ SCHEMAS = {
         "float softcap=0.0, Tensor? alibi_slopes=None, bool deterministic=False, bool return_attn_probs=False, "
         "Tensor? block_table=None, bool return_softmax_lse=False, Tensor? out=None, "
         "Tensor? scheduler_metadata=None, Tensor? q_descale=None, Tensor? k_descale=None, "
-        "Tensor? v_descale=None, SymInt fa_version=2) -> (Tensor, Tensor)",
+        "Tensor? v_descale=None, SymInt fa_version=2, SymInt sink_tokens=0) -> (Tensor, Tensor)",
     "mm": "mm(Tensor self, Tensor mat2) -> Tensor",
     "addmm": "addmm(Tensor self, Tensor mat1, Tensor mat2, *, Scalar beta=1, Scalar alpha=1) -> Tensor",
 }
@@ -76,11 +77,12 @@ def _flash_attn_varlen_func(q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, c
                             window_size=None, softcap=0.0, alibi_slopes=None, deterministic=False,
                             return_attn_probs=False, block_table=None, return_softmax_lse=False, out=None,
                             scheduler_metadata=None, q_descale=None, k_descale=None, v_descale=None,
-                            fa_version=2):
+                            fa_version=2, sink_tokens=0):
     return ops.flash_attn_varlen_func(
         q, k, v, max_seqlen_q, cu_seqlens_q, max_seqlen_k, cu_seqlens_k, seqused_k, q_v, dropout_p,
         softmax_scale, causal, window_size, softcap, alibi_slopes, deterministic, return_attn_probs,
-        block_table, True, out, scheduler_metadata, q_descale, k_descale, v_descale, 0, fa_version)
+        block_table, True, out, scheduler_metadata, q_descale, k_descale, v_descale, 0, fa_version,
+        sink_tokens)
 
 
 _IMPLS = {

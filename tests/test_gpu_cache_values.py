@@ -243,3 +243,21 @@ def test_calls_that_find_no_memory_for_their_workspace(fg, monkeypatch, q_lens, 
     monkeypatch.setattr(torch, "empty", empty)
     check(fg, q_lens, [900, 700, 33, 130], 8, 4, dim, 16, BF16, E4M3, bound=40000)
     assert refused or (limit and max(q_lens) == 1)
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [40, 3, 7]])
+def test_the_custom_op_takes_first_tokens(fg, cache, q_lens):
+    g = gen(3)
+    scale = torch.tensor([0.01], device=DEV) if cache in TOP else None
+    kc, vc, table = store(g, random_rows(g, 2, 128, cache, scale), cache)
+    cu = torch.tensor([0] + q_lens, device=DEV).cumsum(0, dtype=torch.int32)
+    lens = torch.tensor(LENS, dtype=torch.int32, device=DEV)
+    q = randn(g, sum(q_lens), 8, 128).to(BF16)
+    args, kw = (q, kc, vc, max(q_lens), cu, max(LENS)), dict(seqused_k=lens, causal=True, window_size=[50, 0], block_table=table,
+                                                            k_descale=scale, v_descale=scale)
+    out, lse = torch.ops.flag_gems.flash_attn_varlen_func(*args, sink_tokens=5, **kw)
+    want, want_lse = fg.flash_attn_varlen_func(*args, sink_tokens=5, return_softmax_lse=True, **kw)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    without = torch.ops.flag_gems.flash_attn_varlen_func(*args, **kw)[0]
+    assert not torch.equal(out, without)
