@@ -261,3 +261,14 @@ def test_the_custom_op_takes_first_tokens(fg, cache, q_lens):
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
     without = torch.ops.flag_gems.flash_attn_varlen_func(*args, **kw)[0]
     assert not torch.equal(out, without)
+
+
+@pytest.mark.parametrize("heads, hk", [(32, 32), (40, 40), (17, 17), (64, 32)])
+@pytest.mark.parametrize("cache, kw", [(E4M3, {}), (E4M3, dict(bound=10 ** 6)), (BF16, dict(window=(2500, 0), sinks=4)), (E5M2, dict(dim=256, bound=10 ** 5))])
+def test_more_kv_heads_than_a_team_of_ctas(fg, heads, hk, cache, kw):
+    """Decode walks KV heads in teams of CTAs, in rounds where there are more heads than a team has; unequal long sequences are cut
+    in later rounds and joined, short ones are whole."""
+    kw = {"dim": 128, **kw}
+    lens = [3000, 17, 5000, 129, 2900, 1, 4100, 640]
+    check(fg, [1] * 8, lens, heads, hk, page=16, dtype=BF16, cache=cache, scale_shape="heads", **kw)
+    check(fg, [1] * 8, [1 + n % 700 for n in lens], heads, hk, page=16, dtype=BF16, cache=cache, scale_shape="heads", **kw)
