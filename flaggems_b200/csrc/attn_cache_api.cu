@@ -97,7 +97,8 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
     plan.bytes = plan.whole ? 0 : attn_cache_decode_sm100_bytes(b.max_seqlen_q * group, b.head_dim, sms);
     return plan;
   }
-  if (b.max_seqlen_q * group > 16 && tma && !few && (b.head_dim == 64 || b.head_dim == 128 || b.head_dim == 256) && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 &&
+  const bool chunk_dim = b.head_dim == 64 || b.head_dim == 128 || b.head_dim == 256;
+  if (b.max_seqlen_q * group > 16 && tma && !few && chunk_dim && b.softcap == 0.0 && b.softmax_scale > 0.0 && group <= 128 &&
       b.q_head_stride > 0 && b.q_row_stride > 0) {
     plan.path = kPathChunk;            // cuts the keys itself, on the device
     plan.splits = plan.tiles_per_split = 1;
@@ -105,16 +106,18 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
     // An 8-bit store is widened once, ahead of the attention, when at least four items (of 256 query rows) read each key and
     // the copy takes at most 1 GiB.  The kernel's own widening is for head dim 128: at the others shorter chunks are too.
     int64_t rows = (b.max_seqlen_k + 63) / 64 * 64;
-    if (b.window_left >= 0 && b.window_left < b.max_seqlen_k && (b.causal || (b.window_right >= 0 && b.window_right < b.max_seqlen_k))) {
+    if (b.window_left >= 0 && b.window_left < b.max_seqlen_k &&
+        (b.causal || (b.window_right >= 0 && b.window_right < b.max_seqlen_k))) {
       const int64_t right = b.causal ? 0 : b.window_right;   // first tokens, then the keys of all new tokens' windows
       const int64_t seen = (p->sink_tokens + 63) / 64 * 64 + (b.window_left + right + b.max_seqlen_q + 2 * 63) / 64 * 64;
       if (seen < rows) rows = seen;
     }
-    if (!(p->flags & FG_CACHE_NO_COPY) && is_fp8(p->cache_dtype) && (b.max_seqlen_q * group >= 1024 || b.head_dim != 128) && rows > 0 &&
+    if (!(p->flags & FG_CACHE_NO_COPY) && is_fp8(p->cache_dtype) &&
+        (b.max_seqlen_q * group >= 1024 || b.head_dim != 128) && rows > 0 &&
         b.batch * rows <= (1ll << 30) / (4 * b.head_dim * b.num_heads_k))
       plan.dense = rows;
-    plan.bytes =
-        attn_cache_chunk_bytes(b.max_seqlen_q, group, b.batch, b.num_heads_k, b.head_dim, b.max_seqlen_k, plan.dense, plan.whole, sms);
+    plan.bytes = attn_cache_chunk_bytes(b.max_seqlen_q, group, b.batch, b.num_heads_k, b.head_dim, b.max_seqlen_k, plan.dense,
+                                        plan.whole, sms);
     if (plan.bytes >= 0 && (workspace || plan.bytes == 0) && (!is_fp8(p->cache_dtype) || b.head_dim == 128 || plan.dense > 0))
       return plan;
     plan.dense = plan.whole = 0;

@@ -2,10 +2,11 @@
 //
 // An item is one or two 128-row Q tiles of one (sequence, KV head).  A row is a (token, head of the group) pair, so a chunk of a
 // few tokens fills the tiles as well as a long one, and all query heads of the group share every K/V tile.  A tile holds
-// floor(128 / group) tokens (at head dim 256 an item is one tile).  The kernel is persistent, one CTA an SM: the K/V tiles (64 keys) of all items, laid end to end,
-// are cut into equal runs, one per CTA, so that few long items and many short ones fill the SMs alike (in whole items, 336
-// CTAs on 148 SMs would take three rounds for 2.27).  Short items are not cut (attn_cache_api.cu has the rule).  The parts of an item that runs cut are joined by a second kernel, in
-// order.  Nothing synchronises the CTA between items: the roles follow the barrier phases with running counters.
+// floor(128 / group) tokens (at head dim 256 an item is one tile).  The kernel is persistent, one CTA an SM: the K/V tiles (64
+// keys) of all items, laid end to end, are cut into equal runs, one per CTA, so that few long items and many short ones fill the
+// SMs alike (in whole items, 336 CTAs on 148 SMs would take three rounds for 2.27).  Short items are not cut (attn_cache_api.cu
+// has the rule).  The parts of an item that runs cut are joined by a second kernel, in order.  Nothing synchronises the CTA
+// between items: the roles follow the barrier phases with running counters.
 //
 //   warps 0-7    softmax, one warpgroup per Q tile, one thread per row (TMEM lane = row): scores of 64 keys from TMEM to
 //                registers, mask, running maximum (raised only when it grows by more than 8 in log2 units), exponentials,
@@ -32,8 +33,8 @@
 // Two 2048-token prompts at head dim 256 621 us, at 64 234 us (mma.sync: 1654 and 343).
 // Over 8-bit caches bf16 queries are brought to fp16, each row by a power of two, by the softmax warps before an item's first
 // step.
-// P is rounded once: to fp16 (2^-12 of itself, or 2^-32 of its row's largest), and over a bf16 cache to bf16 (2^-9): a second piece, which
-// the decode kernel has, would double the products P V, and those bound the step.
+// P is rounded once: to fp16 (2^-12 of itself, or 2^-32 of its row's largest), and over a bf16 cache to bf16 (2^-9): a second
+// piece, which the decode kernel has, would double the products P V, and those bound the step.
 // TMEM columns: tile t has its scores at t*128 (64 columns), two probability buffers at t*128+64 and +96, its output at
 // 256+t*128.  Every wait is an mbarrier wait with a limit.
 #include "attn_cache_common.cuh"
@@ -247,8 +248,10 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     for (int i = 0; i < 4; ++i) mbar_init(&o_done[i], 1);
     mbar_fence_init();
     prefetch_tmap(&tmap_q);
-    prefetch_tmap(&tmap_k);
-    prefetch_tmap(&tmap_v);
+    if constexpr (!kWiden) {
+      prefetch_tmap(&tmap_k);
+      prefetch_tmap(&tmap_v);
+    }
   }
   int total = mine;
   for (int p = tid + THREADS; p < pairs; p += THREADS) {
@@ -411,7 +414,8 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       bool ok = true;
       do {
         // (of every Q tile of this thread, whether it holds a token or not)
-        ok = wait1(kConvQ ? &q_ready[t0] : q_full, item & 1) && (!kConvQ || t0 + TILES > NT || TILES == 1 || wait1(&q_ready[1], item & 1));
+        ok = wait1(kConvQ ? &q_ready[t0] : q_full, item & 1) &&
+             (!kConvQ || t0 + TILES > NT || TILES == 1 || wait1(&q_ready[1], item & 1));
         ++item;
         for (int i = seg.lo; i < seg.hi && ok; ++i, ++kv) {
           const uint32_t stg = kv % STAGES;
@@ -467,7 +471,8 @@ attn_cache_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             if (t >= seg.nt || !ok) continue;
             const uint32_t par = g[t] & 1;
             // the first product of an item overwrites O: the previous item's must have been read out
-            if (!wait1(&p_ready[t * 2 + par], (g[t] >> 1) & 1) || (i == seg.lo && used[t] > 0 && !wait1(&o_free[t], (used[t] - 1) & 1))) {
+            if (!wait1(&p_ready[t * 2 + par], (g[t] >> 1) & 1) ||
+                (i == seg.lo && used[t] > 0 && !wait1(&o_free[t], (used[t] - 1) & 1))) {
               ok = false;
               continue;
             }
@@ -857,12 +862,11 @@ void chunk_shape(int64_t max_q, int64_t group, int64_t head_dim, int* tiles, int
 template <typename T, int KIND, typename M, int HD>
 int launch(ChunkArgs& pa, cudaStream_t st) {
   const AttnArgs& a = pa.c.a;
-  constexpr int ES = KIND == kCache16 ? 2 : 1;
   const bool pages = pa.c.pages();
   const int64_t stored = pa.c.dense > 0 ? a.batch * pa.c.dense : a.total_k;   // rows of a store without pages
   pa.page_rows = pages && a.block_size < BN ? a.block_size : BN;
   pa.pages_per_tile = BN / pa.page_rows;
-  CUtensorMap tq, maps[2];
+  CUtensorMap tq, maps[2] = {};        // of K and V: the widening form loads them without
   {
     const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)a.H, (uint64_t)a.total_q};
     const uint64_t strides[2] = {(uint64_t)a.q_hs * 2, (uint64_t)a.q_rs * 2};
@@ -870,16 +874,17 @@ int launch(ChunkArgs& pa, cudaStream_t st) {
     const int rc = encode_tmap_16bit(&tq, a.q, 3, dims, strides, box);
     if (rc != FG_OK) return rc;
   }
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t hs = (uint64_t)(i ? a.v_hs : a.k_hs) * ES, rs = (uint64_t)(i ? a.v_rs : a.k_rs) * ES;
-    const uint64_t bs = (uint64_t)(i ? a.v_bs : a.k_bs) * ES;
-    const uint64_t rows = pages ? (uint64_t)a.block_size : (uint64_t)(stored > 0 ? stored : 1);
-    const uint64_t dims[4] = {(uint64_t)HD, (uint64_t)a.Hk, rows, pages ? (uint64_t)a.num_blocks : 1};
-    const uint64_t strides[3] = {hs, rs, pages ? bs : rs * rows};
-    const uint32_t box[4] = {(uint32_t)(128 / ES), 1, (uint32_t)pa.page_rows, 1};
-    const int rc = ES == 2 ? encode_tmap_16bit(&maps[i], i ? a.v : a.k, 4, dims, strides, box)
-                           : encode_tmap_8bit(&maps[i], i ? a.v : a.k, 4, dims, strides, box);
-    if (rc != FG_OK) return rc;
+  if constexpr (KIND == kCache16) {
+    for (int i = 0; i < 2; ++i) {
+      const uint64_t hs = (uint64_t)(i ? a.v_hs : a.k_hs) * 2, rs = (uint64_t)(i ? a.v_rs : a.k_rs) * 2;
+      const uint64_t bs = (uint64_t)(i ? a.v_bs : a.k_bs) * 2;
+      const uint64_t rows = pages ? (uint64_t)a.block_size : (uint64_t)(stored > 0 ? stored : 1);
+      const uint64_t dims[4] = {(uint64_t)HD, (uint64_t)a.Hk, rows, pages ? (uint64_t)a.num_blocks : 1};
+      const uint64_t strides[3] = {hs, rs, pages ? bs : rs * rows};
+      const uint32_t box[4] = {64, 1, (uint32_t)pa.page_rows, 1};
+      const int rc = encode_tmap_16bit(&maps[i], i ? a.v : a.k, 4, dims, strides, box);
+      if (rc != FG_OK) return rc;
+    }
   }
   constexpr int smem = Shape<HD>::SMEM;
   static thread_local int attr_dev = -1;
@@ -948,7 +953,8 @@ __global__ void __launch_bounds__(256) attn_cache_widen_kernel(CacheAttnArgs c, 
       const int r = is_v ? row - kWidenRows : row;
       const int64_t at = s_row[is_v][r];
       if (at < 0) continue;
-      raw[u] = ldg16_stream(reinterpret_cast<const uint8_t*>(is_v ? a.v : a.k) + at + (int64_t)hk * (is_v ? a.v_hs : a.k_hs) + ch * 16);
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(is_v ? a.v : a.k);
+      raw[u] = ldg16_stream(from + at + (int64_t)hk * (is_v ? a.v_hs : a.k_hs) + ch * 16);
       dst[u] = (is_v ? v16 : k16) + (((int64_t)b * dense + row0 + r) * a.Hk + hk) * a.D + ch * 16;
     }
 #pragma unroll

@@ -1,6 +1,6 @@
 // Attention of a few query rows (at most 16 (token, head of the group) pairs of a sequence) over an 8-bit or windowed
-// cache, head dim 64, 128 or (8-bit) 256, on the tcgen05 tensor cores.  Memory bound: every cached byte is read once, and nothing else is
-// done with it -- the tensor cores read K and V from shared memory in the type and layout that TMA delivers.
+// cache, head dim 64, 128 or (8-bit) 256, on the tcgen05 tensor cores.  Memory bound: every cached byte is read once, and nothing
+// else is done with it -- the tensor cores read K and V from shared memory in the type and layout that TMA delivers.
 //
 // The products are turned round, so that the many keys fill the 128 rows of the instruction and the few query rows its
 // columns:
@@ -111,7 +111,9 @@ struct DecodeArgs {
   int team, rounds;     // CTAs of a team, a divisor of the KV heads; KV heads of each member
 };
 
-// Fewest tiles that a run is worth starting a CTA for.
+// Fewest tiles that a run is worth starting a CTA for.  8 sequences of up to 1328 keys, 8 KV heads (456 tiles), in runs of at least
+// 1, 2, 4 and 8 tiles: 18.7, 18.7, 17.6 and 23.9 us in a graph; 2 of up to 6000 keys 24.3, 24.4, 22.8 and 22.1: a part more to join
+// costs about what a tile does.
 constexpr int kMinRun = 4;
 
 // One item's part of a CTA's run.
@@ -237,8 +239,8 @@ __device__ __noinline__ void write_infinities(const DecodeArgs& da, const Segmen
       const float v = (up ? INFINITY : -INFINITY) * v_scale;
       const int tok = r / a.group;
       if (part < 0)
-        reinterpret_cast<T*>(a.out)[(int64_t)(g.s.q_begin + tok) * a.o_rs + (int64_t)(g.hk * a.group + r - tok * a.group) * a.o_hs + d] =
-            Cvt<T>::from_f32(v);
+        reinterpret_cast<T*>(a.out)[(int64_t)(g.s.q_begin + tok) * a.o_rs +
+                                    (int64_t)(g.hk * a.group + r - tok * a.group) * a.o_hs + d] = Cvt<T>::from_f32(v);
       else
         da.part_o[((int64_t)part * RP + r) * HD + d] = v;
     }
@@ -250,9 +252,11 @@ template <typename T, int KIND, int HD>
 __device__ __noinline__ float whole_score(const CacheAttnArgs& c, const Segment& g, int r, int key) {
   const AttnArgs& a = c.a;
   const int tok = r / a.group;
-  const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(g.s.q_begin + tok) * a.q_rs + (int64_t)(g.hk * a.group + r - tok * a.group) * a.q_hs;
+  const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(g.s.q_begin + tok) * a.q_rs +
+               (int64_t)(g.hk * a.group + r - tok * a.group) * a.q_hs;
   const int32_t* bt_row = a.paged ? a.block_table + (int64_t)g.b * a.bt_stride : nullptr;
-  const uint8_t* k = reinterpret_cast<const uint8_t*>(a.k) + cache_row(c, bt_row, g.s.k_begin, key, a.k_rs, a.k_bs) + (int64_t)g.hk * a.k_hs;
+  const uint8_t* k = reinterpret_cast<const uint8_t*>(a.k) + cache_row(c, bt_row, g.s.k_begin, key, a.k_rs, a.k_bs) +
+                     (int64_t)g.hk * a.k_hs;
   float sum = 0.f;
   for (int d = 0; d < HD; ++d) sum = fmaf(Cvt<T>::to_f32(q[d]), Pair<__half>::unpack(fp8x2_to_f16x2<KIND>(k[d])).x, sum);
   return sum * (cache_scale(c.k_scale, c.ks_batch, c.ks_head, g.b, g.hk) * a.scale_log2);
@@ -615,7 +619,8 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             x[4 * i + 2] = (x[4 * i + 2] - f1.x) * kQStep;
             x[4 * i + 3] = (x[4 * i + 3] - f1.y) * kQStep;
             if (q_row < RP)
-              *reinterpret_cast<uint32_t*>(buf + (d >> 7) * (C::QR * 128) + n * 128 + ((((d & 127) >> 4) ^ (n & 7)) << 4) + (d & 15)) =
+              *reinterpret_cast<uint32_t*>(buf + (d >> 7) * (C::QR * 128) + n * 128 +
+                                           ((((d & 127) >> 4) ^ (n & 7)) << 4) + (d & 15)) =
                   e0 | ((uint32_t)e1 << 16);
           }
         }
@@ -829,7 +834,8 @@ attn_cache_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_k, con
             for (int m = 0; m < C::OM; ++m) {
               float v = __uint_as_float(o[m * C::NP + (C::PP - 1) * RP + r]);
 #pragma unroll
-              for (int p = C::PP - 2; p >= 0; --p) v = fmaf(v, C::k8 ? 1.f / kPStep : 1.f, __uint_as_float(o[m * C::NP + p * RP + r]));
+              for (int p = C::PP - 2; p >= 0; --p)
+                v = fmaf(v, C::k8 ? 1.f / kPStep : 1.f, __uint_as_float(o[m * C::NP + p * RP + r]));
               // a NaN sum stays one: only a row that saw nothing is set to zero
               v = l == 0.f ? 0.f : v * (C::k8 ? 1.f / kPScale : 1.f) * (v_scale / l);
               const int d = m * 128 + tid;

@@ -264,7 +264,8 @@ def test_the_custom_op_takes_first_tokens(fg, cache, q_lens):
 
 
 @pytest.mark.parametrize("heads, hk", [(32, 32), (40, 40), (17, 17), (64, 32)])
-@pytest.mark.parametrize("cache, kw", [(E4M3, {}), (E4M3, dict(bound=10 ** 6)), (BF16, dict(window=(2500, 0), sinks=4)), (E5M2, dict(dim=256, bound=10 ** 5))])
+@pytest.mark.parametrize("cache, kw", [
+    (E4M3, {}), (E4M3, dict(bound=10 ** 6)), (BF16, dict(window=(2500, 0), sinks=4)), (E5M2, dict(dim=256, bound=10 ** 5))])
 def test_more_kv_heads_than_a_team_of_ctas(fg, heads, hk, cache, kw):
     """Decode walks KV heads in teams of CTAs, in rounds where there are more heads than a team has; unequal long sequences are cut
     in later rounds and joined, short ones are whole."""
