@@ -74,6 +74,11 @@ bool tma_ready(const fg_attn_cache_params* p) {
   return b.block_size >= 8 && (b.block_size & (b.block_size - 1)) == 0;
 }
 
+// Tokens that the split forms' partial results are for: `q` may have many more rows than its sequences.
+int64_t part_rows(const fg_attn_params& b) {
+  return b.max_seqlen_q < b.total_q && b.batch * b.max_seqlen_q < b.total_q ? b.batch * b.max_seqlen_q : b.total_q;
+}
+
 // `workspace`: whether the caller has any.
 Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
   const fg_attn_params& b = p->base;
@@ -130,7 +135,7 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
     const int64_t keys = most_keys(p, b.max_seqlen_q), ctas = b.num_heads_k * b.batch;
     int64_t chunk = 1024;
     while (chunk > 256 && ctas * ((keys + chunk - 1) / chunk) < (int64_t)sms * 2 * 8) chunk >>= 1;
-    const int64_t split_bytes = (b.total_q > 0 ? b.total_q : 1) * b.num_heads * (b.head_dim + 1) * 4;
+    const int64_t split_bytes = (b.total_q > 0 ? part_rows(b) : 1) * b.num_heads * (b.head_dim + 1) * 4;
     while (chunk < keys && (keys + chunk - 1) / chunk > kMostSplitBytes / split_bytes) chunk <<= 1;
     plan.tiles_per_split = (int)(chunk / bn);
     plan.splits = (int)((keys + chunk - 1) / chunk);
@@ -142,7 +147,7 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
     split_plan(mb * b.num_heads_k * b.batch, tiles, (int64_t)sms * 2, 4, &plan);
   }
   if (!workspace) plan.splits = 1;
-  plan.bytes = plan.splits > 1 ? (int64_t)plan.splits * b.total_q * b.num_heads * (b.head_dim + 1) * 4 : 0;
+  plan.bytes = plan.splits > 1 ? (int64_t)plan.splits * part_rows(b) * b.num_heads * (b.head_dim + 1) * 4 : 0;
   return plan;
 }
 
@@ -258,10 +263,11 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
                (long long)b.workspace_bytes, (long long)plan.bytes);
     FG_REQUIRE(aligned16(b.workspace), "flash_attn_cache: workspace must be 16-byte aligned");
     a.ws_o = reinterpret_cast<float*>(b.workspace);
-    a.ws_lse = a.ws_o + (int64_t)plan.splits * b.total_q * b.num_heads * b.head_dim;   // split forms only
+    a.ws_lse = a.ws_o + (int64_t)plan.splits * part_rows(b) * b.num_heads * b.head_dim;   // split forms only
   }
   a.num_splits = plan.splits;
   c.tiles_per_split = plan.tiles_per_split;
+  c.part_rows = part_rows(b);
   c.dense = plan.dense;
   c.whole = plan.whole;
   const int kind = p->cache_dtype == FG_E4M3 ? kCacheE4M3 : p->cache_dtype == FG_E5M2 ? kCacheE5M2 : kCache16;

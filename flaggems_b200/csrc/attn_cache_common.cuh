@@ -31,6 +31,7 @@ struct CacheAttnArgs {
   int sinks;
   int table_cols;                          // entries of a block table row
   int tiles_per_split;                     // K/V tiles of one split
+  int64_t part_rows;                       // tokens that the partial results of the split forms have room for
   int64_t dense;                           // chunk kernel: rows of each sequence in a 16-bit copy that k and v point at; 0: none
   int whole;                               // tensor-core kernels: runs are cut between items only, and nothing is joined
   __host__ __device__ bool pages() const { return a.paged && dense == 0; }
@@ -110,6 +111,13 @@ __device__ __forceinline__ RowMask row_mask(const CacheAttnArgs& c, int k_len, i
   m.lo = a.wl >= 0 ? max(0, p - a.wl) : 0;
   m.sinks = c.sinks;
   return m;
+}
+
+// Place of a token's partial results, which count from the first sequence's first token `q_first` on, so that rows of a padded q
+// take no room; -1 for tokens beyond what the sizes of the call allow.
+__device__ __forceinline__ int64_t part_row(const CacheAttnArgs& c, int q_first, int64_t qtok) {
+  const int64_t row = qtok - q_first;
+  return row >= 0 && row < c.part_rows ? row : -1;
 }
 
 // What an item of n K/V tiles counts where the tiles of all items are cut into runs.

@@ -74,6 +74,7 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
 
   const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const SeqInfo s = cache_seq_info(c, b);
+  const int q_first = a.num_splits > 1 ? a.cu_q[0] : 0;
   const int group = a.group;
   const int rows = min(s.q_len * group, 16);
   if (rows < 1) return;
@@ -95,7 +96,8 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int64_t qtok = q0 + tid / group;
       const int h = hk * group + tid % group;
       if (a.num_splits > 1) {
-        a.ws_lse[((int64_t)split * a.H + h) * a.total_q + qtok] = -INFINITY;
+        const int64_t at = part_row(c, q_first, qtok);
+        if (at >= 0) a.ws_lse[((int64_t)split * a.H + h) * c.part_rows + at] = -INFINITY;
       } else if (a.lse) {
         a.lse[(int64_t)h * a.total_q + qtok] = INFINITY;
       }
@@ -415,9 +417,11 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         const float inv = l == 0.f ? 0.f : vsc / l;   // a NaN sum stays one
         const int64_t qtok = q0 + r / group;
         const int h = hk * group + r % group;
+        const int64_t at = a.num_splits > 1 ? part_row(c, q_first, qtok) : 0;
+        if (at < 0) continue;
         if (d < a.D) {
           if (a.num_splits > 1)
-            *reinterpret_cast<float2*>(a.ws_o + (((int64_t)split * a.total_q + qtok) * a.H + h) * a.D + d) =
+            *reinterpret_cast<float2*>(a.ws_o + (((int64_t)split * c.part_rows + at) * a.H + h) * a.D + d) =
                 make_float2(x * inv, y * inv);
           else
             *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + qtok * a.o_rs + (int64_t)h * a.o_hs + d) =
@@ -426,7 +430,7 @@ attn_cache_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         if (d == 0) {
           const float lse2 = l == 0.f ? -INFINITY : m - kShift + log2f(l);
           if (a.num_splits > 1)
-            a.ws_lse[((int64_t)split * a.H + h) * a.total_q + qtok] = lse2;
+            a.ws_lse[((int64_t)split * a.H + h) * c.part_rows + at] = lse2;
           else if (a.lse)
             a.lse[(int64_t)h * a.total_q + qtok] = l == 0.f ? INFINITY : lse2 * 0.6931471805599453f;
         }

@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(NTHREADS) attn_cache_generic_kernel(CacheAttnA
   const int split = blockIdx.x % a.num_splits;
   const int hk = blockIdx.y, b = blockIdx.z;
   const SeqInfo s = cache_seq_info(c, b);
+  const int q_first = a.num_splits > 1 ? a.cu_q[0] : 0;
   const int rows = s.q_len * a.group;
   const int r0 = m_block * BM;
   if (r0 >= rows) return;
@@ -292,13 +293,15 @@ __global__ void __launch_bounds__(NTHREADS) attn_cache_generic_kernel(CacheAttnA
     const int64_t qtok = s.q_begin + tok;
     const float lse2 = l_run[r] == 0.f ? -INFINITY : m_run[r] - kShift + log2f(l_run[r]);
     if (a.num_splits > 1) {
-      float* out = a.ws_o + (((int64_t)split * a.total_q + qtok) * a.H + h) * a.D;
+      const int64_t at = part_row(c, q_first, qtok);
+      if (at < 0) continue;
+      float* out = a.ws_o + (((int64_t)split * c.part_rows + at) * a.H + h) * a.D;
 #pragma unroll
       for (int i = 0; i < DP / 8; ++i) {
         const int col = i * 8 + (lane & 3) * 2;
         if (col < a.D) *reinterpret_cast<float2*>(out + col) = make_float2(o[i][r * 2] * inv, o[i][r * 2 + 1] * inv);
       }
-      if ((lane & 3) == 0) a.ws_lse[((int64_t)split * a.H + h) * a.total_q + qtok] = lse2;
+      if ((lane & 3) == 0) a.ws_lse[((int64_t)split * a.H + h) * c.part_rows + at] = lse2;
     } else {
       T* out = reinterpret_cast<T*>(a.out) + qtok * a.o_rs + (int64_t)h * a.o_hs;
 #pragma unroll
@@ -352,11 +355,11 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attn_cache_combine_kernel(
   const AttnArgs& a = c.a;
   const int lane = threadIdx.x & 31;
   const int64_t pair = (int64_t)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);  // head fastest
-  const int64_t tok = pair / a.H;
-  if (tok < a.cu_q[0] || tok >= a.cu_q[a.batch] || tok >= a.total_q) return;
-  const int h = (int)(pair - tok * a.H);
-  const float* lse = a.ws_lse + (int64_t)h * a.total_q + tok;
-  const int64_t lse_step = (int64_t)a.H * a.total_q;
+  const int64_t row = pair / a.H, tok = row + a.cu_q[0];
+  if (row >= c.part_rows || tok < 0 || tok >= a.cu_q[a.batch] || tok >= a.total_q) return;
+  const int h = (int)(pair - row * a.H);
+  const float* lse = a.ws_lse + (int64_t)h * c.part_rows + row;
+  const int64_t lse_step = (int64_t)a.H * c.part_rows;
   float m = -INFINITY;
   for (int s = lane; s < a.num_splits; s += 32) m = fmaxf(m, lse[s * lse_step]);
   m = warp_max(m);
@@ -365,8 +368,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attn_cache_combine_kernel(
   for (int s = lane; s < a.num_splits; s += 32) wsum += exp2f(lse[s * lse_step] - msafe);
   wsum = warp_sum(wsum);
   const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
-  const float* part = a.ws_o + (tok * a.H + h) * (int64_t)a.D;
-  const int64_t part_step = a.total_q * (int64_t)a.H * a.D;
+  const float* part = a.ws_o + (row * a.H + h) * (int64_t)a.D;
+  const int64_t part_step = c.part_rows * (int64_t)a.H * a.D;
   T* out = reinterpret_cast<T*>(a.out) + tok * a.o_rs + (int64_t)h * a.o_hs;
   for (int d = lane * 4; d < a.D; d += 128) {   // D is a multiple of 8, the workspace and the rows are 16-byte aligned
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -396,7 +399,7 @@ int attn_cache_generic(const CacheAttnArgs& c, int dtype, int kind, cudaStream_t
 }
 
 int attn_cache_combine(const CacheAttnArgs& c, int dtype, cudaStream_t st) {
-  const unsigned grid = (unsigned)((c.a.total_q * (int64_t)c.a.H + kCombineWarps - 1) / kCombineWarps);
+  const unsigned grid = (unsigned)((c.part_rows * (int64_t)c.a.H + kCombineWarps - 1) / kCombineWarps);
   if (dtype == FG_BF16)
     attn_cache_combine_kernel<__nv_bfloat16><<<grid, kCombineWarps * 32, 0, st>>>(c);
   else

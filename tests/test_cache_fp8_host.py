@@ -159,6 +159,16 @@ def test_workspace_of_the_split_decode_form_is_bounded():
     assert need(total_q=0, softcap=50.0, max_seqlen_k=10 ** 6) == 0
 
 
+def test_rows_behind_the_sequences_take_no_workspace():
+    """A padded q: the split forms' partial results go by the tokens that the sequences can have, not by the rows of q."""
+    need = lambda **kw: _lib.load().fg_flash_attn_cache_workspace_bytes(ctypes.byref(params(**kw)))
+    for form in (dict(head_dim=96), dict(head_dim=200, softcap=30.0)):
+        for batch, max_q in ((1, 20), (3, 100), (2, 1), (64, 1)):
+            size = dict(batch=batch, max_seqlen_q=max_q, num_heads=32, num_heads_k=8, max_seqlen_k=16384, **form)
+            assert 0 < need(total_q=batch * max_q, **size) == need(total_q=65536, **size) <= 64 * 2 ** 20
+            assert need(total_q=batch * max_q - 1, **size) <= need(total_q=65536, **size)
+
+
 def test_path_by_sizes():
     path = lambda **kw: _lib.load().fg_flash_attn_cache_path(ctypes.byref(params(**{"max_seqlen_k": 10 ** 5, **kw})))
     assert path(max_seqlen_k=1000) == 2      # too few tiles of keys

@@ -273,3 +273,11 @@ def test_more_kv_heads_than_a_team_of_ctas(fg, heads, hk, cache, kw):
     lens = [3000, 17, 5000, 129, 2900, 1, 4100, 640]
     check(fg, [1] * 8, lens, heads, hk, page=16, dtype=BF16, cache=cache, scale_shape="heads", **kw)
     check(fg, [1] * 8, [1 + n % 700 for n in lens], heads, hk, page=16, dtype=BF16, cache=cache, scale_shape="heads", **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(dim=96), dict(dim=128, softcap=30.0), dict(dim=200, cache=E5M2), dict(dim=72, cache=BF16,
+                                                                                             window=(900, 0), sinks=4)])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1, 1], [20, 3, 0, 1], [200, 1, 64, 65]])
+def test_many_rows_behind_the_sequences(fg, kw, q_lens):
+    """A q padded far beyond its sequences: the rows behind them are left as they were, and take no room."""
+    check(fg, q_lens, [4000, 1300, 77, 700], 8, 2, page=16, dtype=BF16, behind=9000, **{"cache": E4M3, **kw})
