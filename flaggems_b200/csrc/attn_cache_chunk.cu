@@ -25,12 +25,13 @@
 // Widening inside the kernel makes a step half as long again, and every item widens the keys it reads anew.  Where the chunk is
 // long (several items read each key) and the store's 16-bit copy is not too large, a kernel before this one widens the visible
 // rows once into the workspace, and this one reads them as a 16-bit store (attn_cache_api.cu has the rule; two chunks of 2048
-// tokens 505 us, the copy included).  At head dims 64 and 256 that is the only form.
+// tokens 513 to 529 us, the copy included).  At head dims 64 and 256 that is the only form.
 // What bounds it: with two Q tiles of head dim 128 a step of 64 keys is 2 x 2 products of 128 x 64 x 128, 1024 clocks of the tensor
 // cores at 4096 multiply-adds a clock, and 16384 exponentials, 1024 clocks of the special function units at 16 a clock.  Long
-// chunks reach half of a large library product's rate, since each of the two waits for the other at times; short ones are bound
-// by the start and the joining of the items.
-// Two 2048-token prompts at head dim 256 621 us, at 64 234 us (mma.sync: 1654 and 343).
+// chunks reach half of a large library product's rate, since each of the two waits for the other at times (tensor pipe and
+// special-function unit 36 to 38 % busy); short ones over an 8-bit cache by the latency of the widening warps' loads, one tile on
+// its way behind its table entries (23 %; DRAM 15 %).
+// Two 2048-token prompts at head dim 256 607 us, at 64 202 us (mma.sync: 1654 and 343).
 // Over 8-bit caches bf16 queries are brought to fp16, each row by a power of two, by the softmax warps before an item's first
 // step.
 // P is rounded once: to fp16 (2^-12 of itself, or 2^-32 of its row's largest), and over a bf16 cache to bf16 (2^-9): a second

@@ -31,9 +31,10 @@
 //               rings the issue bounded the kernel (256 sequences: 521 us by one lane, 412 us by eight)
 //   warp 6      issues the products: scores of the next tile before P V of the current one when its keys are there
 //
-// Measured: 256 sequences of 512 to 8192 tokens, 32 heads over 8, 8-bit: 2.29 GB in 355 us, 6.4 TB/s; windowed, 64 sequences of up
-// to 16384, 16-bit 70 us, 8-bit 98 us.  A tile takes about 1 us (4 rows) to 1.6 us (16 rows) through the chain of score product, maximum,
-// probabilities and their pieces, which bounds short runs; mma.sync in smaller CTAs is faster there (attn_cache_api.cu).
+// Measured: 256 sequences of 512 to 8192 tokens, 32 heads over 8, 8-bit: 2.29 GB in 375 to 388 us, 5.9 to 6.1 TB/s (the
+// tensor pipe is 4 % busy); windowed, 64 sequences of up to 16384, 16-bit 74 us, 8-bit 104 us.  A tile takes about 1 us (4
+// rows) to 1.6 us (16 rows) through the chain of score product, maximum, probabilities and their pieces, which bounds short
+// runs; mma.sync in smaller CTAs is faster there (attn_cache_api.cu).
 //
 // The kernel is persistent.  An item is one (sequence, KV head).  A team of CTAs walks the same sequences, each for a KV head of
 // its own, so that the heads' pieces of a cached row, which lie side by side in memory, are fetched at about the same time.
