@@ -76,7 +76,7 @@ bool tma_ready(const fg_attn_cache_params* p) {
 
 // Tokens that the split forms' partial results are for: `q` may have many more rows than its sequences.
 int64_t part_rows(const fg_attn_params& b) {
-  return b.max_seqlen_q < b.total_q && b.batch * b.max_seqlen_q < b.total_q ? b.batch * b.max_seqlen_q : b.total_q;
+  return b.max_seqlen_q <= 0 || b.batch < b.total_q / b.max_seqlen_q ? b.batch * b.max_seqlen_q : b.total_q;
 }
 
 // `workspace`: whether the caller has any.
@@ -135,7 +135,7 @@ Plan make_plan(const fg_attn_cache_params* p, int sms, bool workspace) {
     const int64_t keys = most_keys(p, b.max_seqlen_q), ctas = b.num_heads_k * b.batch;
     int64_t chunk = 1024;
     while (chunk > 256 && ctas * ((keys + chunk - 1) / chunk) < (int64_t)sms * 2 * 8) chunk >>= 1;
-    const int64_t split_bytes = (b.total_q > 0 ? part_rows(b) : 1) * b.num_heads * (b.head_dim + 1) * 4;
+    const int64_t split_bytes = (part_rows(b) > 0 ? part_rows(b) : 1) * b.num_heads * (b.head_dim + 1) * 4;
     while (chunk < keys && (keys + chunk - 1) / chunk > kMostSplitBytes / split_bytes) chunk <<= 1;
     plan.tiles_per_split = (int)(chunk / bn);
     plan.splits = (int)((keys + chunk - 1) / chunk);
@@ -155,7 +155,8 @@ bool sizes_ok(const fg_attn_cache_params* p) {
   const fg_attn_params& b = p->base;
   return b.batch >= 0 && b.total_q >= 0 && b.num_heads > 0 && b.num_heads_k > 0 && b.num_heads % b.num_heads_k == 0 &&
          b.head_dim > 0 && b.head_dim <= 256 && b.head_dim % 8 == 0 && b.max_seqlen_q >= 0 && b.max_seqlen_k >= 0 &&
-         b.max_seqlen_q <= 2147483647LL / 64 && b.max_seqlen_k <= 2147483647LL / 64 && p->sink_tokens >= 0;
+         b.max_seqlen_q <= 2147483647LL / 64 && b.max_seqlen_k <= 2147483647LL / 64 && p->sink_tokens >= 0 &&
+         b.batch <= 2147483647LL && b.num_heads <= 2147483647LL && b.total_q <= 2147483647LL * 4 / b.num_heads;
 }
 
 }  // namespace
@@ -190,7 +191,7 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   FG_REQUIRE(b.head_dim % 8 == 0, "head_size must be a multiple of 8");
   FG_REQUIRE(p->sink_tokens >= 0, "flash_attn_cache: sink_tokens must not be negative");
   FG_REQUIRE(b.max_seqlen_q >= 0 && b.max_seqlen_k >= 0, "flash_attn_cache: negative max_seqlen");
-  FG_REQUIRE(sizes_ok(p) && b.total_q <= 2147483647LL, "flash_attn_cache: sequence too long");
+  FG_REQUIRE(sizes_ok(p) && b.total_q <= 2147483647LL, "flash_attn_cache: sequence too long, or too many rows");
   FG_REQUIRE(b.alibi_slopes == nullptr, "flash_attn_cache: ALiBi is not supported over an 8-bit cache or with sink_tokens");
   FG_REQUIRE((b.q_batch_stride | b.k_batch_stride | b.v_batch_stride | b.o_batch_stride) == 0,
              "flash_attn_cache: batch strides are not supported");
@@ -273,7 +274,6 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   const int kind = p->cache_dtype == FG_E4M3 ? kCacheE4M3 : p->cache_dtype == FG_E5M2 ? kCacheE5M2 : kCache16;
   cudaStream_t st = (cudaStream_t)stream;
   FG_REQUIRE((b.max_seqlen_q * a.group + 63) / 64 * plan.splits <= 2147483647LL, "flash_attn_cache: too many row tiles");
-  FG_REQUIRE(b.total_q * b.num_heads <= 2147483647LL * 4, "flash_attn_cache: too many rows");
   const int rc = plan.path == kPathDecodeSm100 ? attn_cache_decode_sm100(c, b.dtype, kind, st)
                  : plan.path == kPathDecode    ? attn_cache_decode(c, b.dtype, kind, st)
                  : plan.path == kPathChunk     ? attn_cache_chunk(c, b.dtype, kind, st)

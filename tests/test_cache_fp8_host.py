@@ -169,6 +169,19 @@ def test_rows_behind_the_sequences_take_no_workspace():
             assert need(total_q=batch * max_q - 1, **size) <= need(total_q=65536, **size)
 
 
+def test_sizes_of_nothing_and_out_of_range():
+    """The size queries come before any check of the call: no division by a size of zero, nor by a product that wrapped."""
+    need = lambda **kw: _lib.load().fg_flash_attn_cache_workspace_bytes(ctypes.byref(params(**kw)))
+    for form in (dict(), dict(head_dim=96), dict(softcap=3.0), dict(head_dim=64, max_seqlen_q=30), dict(max_seqlen_q=300)):
+        for kw in (dict(batch=0), dict(max_seqlen_q=0), dict(total_q=0), dict(max_seqlen_k=0), dict(batch=0, total_q=0)):
+            assert need(**{**form, **kw}) >= 0
+        for kw in (dict(total_q=2 ** 62), dict(batch=2 ** 40, total_q=2 ** 40), dict(num_heads=2 ** 40, num_heads_k=2 ** 40),
+                   dict(total_q=2 ** 31 - 1, num_heads=2 ** 20, num_heads_k=2 ** 10)):
+            assert need(**{**form, **kw}) == 0
+            with pytest.raises(RuntimeError, match="too long, or too many rows"):
+                _lib.check(_lib.load().fg_flash_attn_cache(ctypes.byref(params(**{**form, **kw})), None))
+
+
 def test_path_by_sizes():
     path = lambda **kw: _lib.load().fg_flash_attn_cache_path(ctypes.byref(params(**{"max_seqlen_k": 10 ** 5, **kw})))
     assert path(max_seqlen_k=1000) == 2      # too few tiles of keys
