@@ -239,8 +239,10 @@ extern "C" int fg_flash_attn_cache(const fg_attn_cache_params* p, void* stream) 
   a.causal = b.causal != 0;
   int64_t wl = b.window_left, wr = b.window_right;
   if (a.causal) wr = 0;
+  // Bounds that hide nothing: the last token is at k_len - 1, the first at k_len - q_len, which is negative where there are more new
+  // tokens than keys.
   if (wl >= b.max_seqlen_k) wl = -1;
-  if (wr >= b.max_seqlen_k) wr = -1;
+  if (wr >= b.max_seqlen_q - 1) wr = -1;
   a.wl = (int)(wl < 0 ? -1 : wl);
   a.wr = (int)(wr < 0 ? -1 : wr);
   a.local = a.wl >= 0 || (!a.causal && a.wr >= 0);

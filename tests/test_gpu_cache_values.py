@@ -281,3 +281,13 @@ def test_more_kv_heads_than_a_team_of_ctas(fg, heads, hk, cache, kw):
 def test_many_rows_behind_the_sequences(fg, kw, q_lens):
     """A q padded far beyond its sequences: the rows behind them are left as they were, and take no room."""
     check(fg, q_lens, [4000, 1300, 77, 700], 8, 2, page=16, dtype=BF16, behind=9000, **{"cache": E4M3, **kw})
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 96])
+@pytest.mark.parametrize("cache", [E4M3, BF16])
+@pytest.mark.parametrize("window", [(0, 100), (1023, 5), (3, 20), (8, 12), (2, 1)])
+@pytest.mark.parametrize("q_lens, bound", [([102, 25, 3], 0), ([102, 25, 3], 2000), ([4, 3, 1], 0), ([4, 3, 1], 10 ** 6)])
+def test_right_windows_over_fewer_keys_than_new_tokens(fg, q_lens, bound, window, cache, dim):
+    """Without the causal mask, the first of many new tokens are at negative positions: a right window longer than the sequence
+    still hides keys from them."""
+    check(fg, q_lens, [5, 9, 2], 8, 2, dim, 16, BF16, cache, causal=False, window=window, sinks=4, bound=bound)
