@@ -26,10 +26,10 @@ struct QuantArgs {
 // operator takes about three times as many.  The approximation is clamped far above both types' largest value: an
 // overflowing or infinite quotient then comes out as an infinity of its sign (saturated by the conversion) instead of
 // inf - inf, and NaN passes through the remainder.  Quotients that differ from the division's below 2^-20 are zero in
-// both types.
+// both types.  (The remainder is taken as q s - x: as x - q s its zero, which is +0, would turn a quotient of -0 into +0.)
 __device__ __forceinline__ float quotient(float x, float s, float r) {
   const float q = fminf(fmaxf(x * r, -1048576.f), 1048576.f);
-  return fmaf(fmaf(-q, s, x), r, q);
+  return fmaf(fmaf(q, s, -x), -r, q);
 }
 
 template <typename T, int KIND>

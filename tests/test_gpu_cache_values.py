@@ -291,3 +291,25 @@ def test_right_windows_over_fewer_keys_than_new_tokens(fg, q_lens, bound, window
     """Without the causal mask, the first of many new tokens are at negative positions: a right window longer than the sequence
     still hides keys from them."""
     check(fg, q_lens, [5, 9, 2], 8, 2, dim, 16, BF16, cache, causal=False, window=window, sinks=4, bound=bound)
+
+
+@pytest.mark.parametrize("scale", [None, 0.3, 114.0, 1e-20])
+@pytest.mark.parametrize("dim", [128, 40])
+@pytest.mark.parametrize("cache", [E4M3, E5M2])
+@pytest.mark.parametrize("dtype", [BF16, FP16, torch.float32])
+def test_write_keeps_the_sign_of_zero(fg, dtype, cache, dim, scale):
+    """Zeros, and quotients that round to zero, keep their sign as in a division, and come back with it."""
+    key = torch.zeros((4, 2, dim), device=DEV)
+    key[1] = -0.0
+    key[2], key[3] = 1e-7 * (scale or 1.0), -1e-7 * (scale or 1.0)      # below half of the smallest value of either type
+    key = key.to(dtype)
+    caches = [torch.full((1, 4, 2, dim), 0x55, dtype=torch.uint8, device=DEV).view(cache) for _ in range(2)]
+    s = None if scale is None else torch.tensor([scale], device=DEV)
+    name = "fp8_e4m3" if cache == E4M3 else "fp8_e5m2"
+    fg.reshape_and_cache_flash(key, -key, *caches, torch.arange(4, device=DEV), name, s, s)
+    for c, x in zip(caches, (key, -key)):
+        assert torch.equal(c.view(torch.uint8)[0], torch.signbit(x).to(torch.uint8) * 0x80)
+    k, v = torch.empty_like(key), torch.empty_like(key)
+    table, cu = torch.zeros((1, 1), dtype=torch.int32, device=DEV), torch.tensor([0, 4], dtype=torch.int32, device=DEV)
+    fg.gather_cache_flash(*caches, k, v, table, cu, name, s, s)
+    assert (k == 0).all() and torch.equal(torch.signbit(k), torch.signbit(key)) and torch.equal(torch.signbit(v), torch.signbit(-key))
